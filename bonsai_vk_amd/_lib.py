@@ -9,8 +9,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("BKV_LIBRARY") or os.path.join(HERE, "libbkv.so")
 
 BKV_F16, BKV_Q8_0 = 0, 1
-BKV_OP_DECODE, BKV_OP_PREFILL = 0, 1
+BKV_OP_DECODE, BKV_OP_PREFILL, BKV_OP_TREE = 0, 1, 2
 BKV_PREFILL_MAX_Q = 4096
+BKV_TREE_MAX_Q = 1024
+BKV_ROPE_HALF, BKV_ROPE_INTERLEAVED = 0, 1
+BKV_ROPE_PLAIN, BKV_ROPE_LINEAR, BKV_ROPE_NTK, BKV_ROPE_YARN = 0, 1, 2, 3
+BKV_OUT_F32, BKV_OUT_F16, BKV_OUT_BF16 = 0, 1, 2
 
 ERRORS = {
     0: "BKV_OK", -1: "BKV_EINVAL", -2: "BKV_ESHAPE", -3: "BKV_ECAP", -4: "BKV_EALIGN",
@@ -25,6 +29,7 @@ EXPORTS = [
     "bkv_kv_fill_synthetic", "bkv_attn_decode_qg", "bkv_decode_step_qg", "bkv_attn_prefill_chunk_qg", "bkv_prefill_step", "bkv_qk_norm_rope_append", "bkv_attn_decode_window",
     "bkv_workspace_error", "bkv_error_words", "bkv_decode_step_static", "bkv_static_scratch_bytes",
     "bkv_static_error", "bkv_static_reset", "bkv_static_debug_address",
+    "bkv_tree_mask", "bkv_attn_tree", "bkv_rope_init", "bkv_rope_append", "bkv_kv_read", "bkv_kv_commit",
 ]
 
 
@@ -40,6 +45,17 @@ class BkvCacheDesc(ctypes.Structure):
         ("layer_stride_bytes", ctypes.c_uint64 * 4),
         ("block_table", ctypes.c_void_p),
     ]
+
+
+class BkvRows(ctypes.Structure):
+    """Mirror of struct bkv_rows."""
+    _fields_ = [("p", ctypes.c_void_p), ("tok", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class BkvRope(ctypes.Structure):
+    """Mirror of struct bkv_rope."""
+    _fields_ = [("nrot", ctypes.c_int32), ("layout", ctypes.c_int32), ("mscale", ctypes.c_float),
+                ("reserved", ctypes.c_int32), ("turns", ctypes.c_double * 128)]
 
 
 class BkvError(RuntimeError):
@@ -64,6 +80,7 @@ def lib():
                           "(there is no CPU fallback for the KV-cache path)")
     L = ctypes.CDLL(LIB_PATH)
     P, D, i32, u32, sz = ctypes.c_void_p, ctypes.POINTER(BkvCacheDesc), ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t
+    R, O, i64, f64 = ctypes.POINTER(BkvRows), ctypes.POINTER(BkvRope), ctypes.c_int64, ctypes.c_double
     sig = {
         "bkv_geom_check": (i32, [D]),
         "bkv_slot_bytes": (ctypes.c_uint64, [D, i32]),
@@ -92,6 +109,12 @@ def lib():
         "bkv_static_error": (i32, [D, P]),
         "bkv_static_reset": (i32, [P]),
         "bkv_static_debug_address": (i32, [ctypes.POINTER(ctypes.c_void_p)]),
+        "bkv_tree_mask": (i32, [P, i32, P, P]),
+        "bkv_attn_tree": (i32, [D, i32, u32, i32, R, P, R, P, P, P, sz, P]),
+        "bkv_rope_init": (i32, [O, i32, i32, f64, i32, f64, f64, f64, f64]),
+        "bkv_rope_append": (i32, [D, i32, u32, i32, O, R, R, R, P, P, ctypes.c_float, P, P, P]),
+        "bkv_kv_read": (i32, [D, i32, u32, i32, i32, P, P, i64, i64, P]),
+        "bkv_kv_commit": (i32, [D, u32, i32, i32, P, P]),
         "bkv_qk_norm_rope_append": (i32, [D, i32, u32, i32, P, P, P, P, P, i32, ctypes.c_float,
                                           ctypes.c_float, P, P]),
     }

@@ -649,8 +649,207 @@ int bkv_attn_prefill_chunk_qg(const bkv_cache_desc *d, int layer, uint32_t pos0,
                         workspace, ws_bytes, stream, 2 * kHd, 2 * kHd);
 }
 
+// ------------------------------------------------------------------ drafted tokens
+// head_dim 256, any number of query heads per KV head
+static int check_hd(const bkv_cache_desc *d) { return d->hd == kHd ? BKV_OK : BKV_EUNSUPPORTED; }
+static int pool_pages(const bkv_cache_desc *d) { return d->page_tokens > 0 ? d->cap / d->page_tokens : 0; }
+
+static int check_rows(const bkv_rows *r) {
+  if (!r || !r->p || r->tok < 0 || r->head < 0) return BKV_EINVAL;
+  return aligned16(r->p) && r->tok % 4 == 0 && r->head % 4 == 0 ? BKV_OK : BKV_EALIGN;
+}
+static Rows rows_of(const bkv_rows *r) { return r ? Rows{r->p, r->tok, r->head} : Rows{nullptr, 0, 0}; }
+
+int bkv_tree_mask(const int32_t *parent, int n, uint64_t *mask, int32_t *depth) {
+  if (n < 0 || n > BKV_TREE_MAX_Q || (n > 0 && !parent)) return BKV_EINVAL;
+  for (int i = 0; i < n; ++i)
+    if (parent[i] < -1 || parent[i] >= i) return BKV_EINVAL;
+  const int words = (n + 63) / 64;
+  for (int i = 0; i < n; ++i) {
+    const int p = parent[i];
+    if (mask) {
+      uint64_t *row = mask + (size_t)i * words;
+      for (int w = 0; w < words; ++w) row[w] = p < 0 ? 0 : row[w + (std::ptrdiff_t)(p - i) * words];
+      row[i / 64] |= uint64_t(1) << (i % 64);
+    }
+  }
+  if (depth)
+    for (int i = 0; i < n; ++i) depth[i] = parent[i] < 0 ? 0 : depth[parent[i]] + 1;
+  return BKV_OK;
+}
+
+int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, const bkv_rows *q,
+                  const uint64_t *mask, const bkv_rows *gate, float *out, float *out_gated,
+                  void *workspace, size_t ws_bytes, hipStream_t stream) {
+  int rc = check(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (layer < 0 || layer >= d->n_layers || n_q < 0 || n_q > BKV_TREE_MAX_Q) return BKV_EINVAL;
+  if (n_q == 0) return BKV_OK;
+  if ((int64_t)pos0 + n_q > max_positions(d)) return BKV_ECAP;
+  if ((rc = check_rows(q))) return rc;
+  if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
+  if (gate && (rc = check_rows(gate))) return rc;
+  if (!aligned16(out) || (out_gated && !aligned16(out_gated)) || ((uintptr_t)mask & 7u) != 0) return BKV_EALIGN;
+  if (!workspace) return BKV_EWORKSPACE;
+  if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
+  const TreePlan p = plan_tree(d->nh, d->nkv, pos0, n_q, prefill_base(d));
+  if (ws_bytes < p.total) return BKV_EWORKSPACE;
+  char *w = (char *)workspace;
+  TreeArgs a{};
+  a.L = view(d, layer);
+  a.pool_pages = pool_pages(d);
+  a.nkv = d->nkv; a.nh = d->nh; a.grp = d->nh / d->nkv;
+  a.pos0 = pos0;
+  a.n_q = n_q;
+  a.scale2 = (float)((double)d->scale * 1.4426950408889634);
+  a.q = rows_of(q);
+  a.gate = rows_of(gate);
+  a.mask = mask;
+  a.words = (n_q + 63) / 64;
+  a.out = out;
+  a.out_gated = out_gated;
+  a.splits = p.splits;
+  a.ml = (float2 *)(w + p.off_ml);
+  a.part = (float *)(w + p.off_part);
+  return hip_fail(launch_tree(a, p, d->k_fmt, d->v_fmt, stream));
+}
+
+static bool positive(double x) { return std::isfinite(x) && x > 0.0; }
+
+int bkv_rope_init(bkv_rope *r, int nrot, int layout, double freq_base, int scaling, double factor,
+                  double trained_ctx, double beta_fast, double beta_slow) {
+  if (!r || nrot < 0 || nrot > kHd || (nrot & 1)) return BKV_EINVAL;
+  if (layout != BKV_ROPE_HALF && layout != BKV_ROPE_INTERLEAVED) return BKV_EINVAL;
+  if (scaling < BKV_ROPE_PLAIN || scaling > BKV_ROPE_YARN) return BKV_EINVAL;
+  if (!std::isfinite(freq_base) || freq_base <= 1.0) return BKV_EINVAL;
+  if (scaling != BKV_ROPE_PLAIN && !positive(factor)) return BKV_EINVAL;
+  if (scaling == BKV_ROPE_YARN && !(positive(trained_ctx) && positive(beta_slow) && std::isfinite(beta_fast) && beta_fast > beta_slow))
+    return BKV_EINVAL;
+  const double two_pi = 6.283185307179586476925;
+  double base = freq_base;
+  if (scaling == BKV_ROPE_NTK) {
+    if (nrot == 2) return BKV_EINVAL;              // (the exponent nrot / (nrot - 2))
+    if (nrot) base *= std::pow(factor, nrot / (nrot - 2.0));
+    if (!std::isfinite(base) || base <= 0.0) return BKV_EINVAL;
+  }
+  double lo = 0.0, hi = 0.0;
+  if (scaling == BKV_ROPE_YARN && nrot) {
+    // the pair, as a real number, that turns so often in trained_ctx positions
+    const double per = nrot / (2.0 * std::log(freq_base));
+    lo = std::max(0.0, std::floor(per * std::log(trained_ctx / (two_pi * beta_fast))));
+    hi = std::min(nrot - 1.0, std::ceil(per * std::log(trained_ctx / (two_pi * beta_slow))));
+  }
+  std::memset(r, 0, sizeof *r);
+  r->nrot = nrot;
+  r->layout = layout;
+  r->mscale = scaling == BKV_ROPE_YARN && factor > 1.0 ? (float)(1.0 + 0.1 * std::log(factor)) : 1.0f;
+  for (int p = 0; p < nrot / 2; ++p) {
+    double th = std::pow(base, -2.0 * p / nrot);
+    if (scaling == BKV_ROPE_LINEAR) th /= factor;
+    if (scaling == BKV_ROPE_YARN) {
+      const double ramp = std::min(1.0, std::max(0.0, (p - lo) / std::max(hi - lo, 1e-3)));
+      th = th * (1.0 - ramp) + th / factor * ramp;
+    }
+    r->turns[p] = th / two_pi;
+  }
+  return BKV_OK;
+}
+
+int bkv_rope_append(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok, const bkv_rope *rope,
+                    const bkv_rows *q, const bkv_rows *k, const bkv_rows *v, const float *qn_w,
+                    const float *kn_w, float eps, const int32_t *positions, float *q_out,
+                    hipStream_t stream) {
+  int rc = check(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (layer < 0 || layer >= d->n_layers || n_tok < 0 || !rope) return BKV_EINVAL;
+  if (rope->nrot < 0 || rope->nrot > kHd || (rope->nrot & 1) || !std::isfinite(rope->mscale)) return BKV_EINVAL;
+  if (rope->layout != BKV_ROPE_HALF && rope->layout != BKV_ROPE_INTERLEAVED) return BKV_EINVAL;
+  for (int p = 0; p < rope->nrot / 2; ++p)
+    if (!std::isfinite(rope->turns[p])) return BKV_EINVAL;
+  if ((qn_w == nullptr) != (kn_w == nullptr) || (qn_w && !(eps >= 0.0f))) return BKV_EINVAL;
+  if ((q == nullptr) != (q_out == nullptr)) return BKV_EINVAL;
+  if (n_tok == 0) return BKV_OK;
+  if ((int64_t)pos0 + n_tok > max_positions(d)) return BKV_ECAP;
+  if (q && (rc = check_rows(q))) return rc;
+  if ((rc = check_rows(k)) || (rc = check_rows(v))) return rc;
+  if ((q_out && !aligned16(q_out)) || (qn_w && (!aligned16(qn_w) || !aligned16(kn_w))) || ((uintptr_t)positions & 3u) != 0)
+    return BKV_EALIGN;
+  RopeArgs a{};
+  a.L = view(d, layer);
+  a.pool_pages = pool_pages(d);
+  a.nkv = d->nkv; a.nh = d->nh;
+  a.pos0 = pos0;
+  a.q = rows_of(q); a.k = rows_of(k); a.v = rows_of(v);
+  a.qn_w = qn_w; a.kn_w = kn_w;
+  a.eps = eps;
+  a.positions = positions;
+  a.q_out = q_out;
+  a.rope = *rope;
+  return hip_fail(launch_rope_append(a, d->k_fmt, d->v_fmt, n_tok, stream));
+}
+
+int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int out_type, void *k_out,
+                void *v_out, int64_t tok_stride, int64_t head_stride, hipStream_t stream) {
+  int rc = check(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (layer < 0 || layer >= d->n_layers || n < 0) return BKV_EINVAL;
+  if (out_type < BKV_OUT_F32 || out_type > BKV_OUT_BF16) return BKV_EINVAL;
+  if (n == 0) return BKV_OK;
+  if ((int64_t)pos0 + n > max_positions(d)) return BKV_ECAP;
+  if (!k_out && !v_out) return BKV_EINVAL;
+  // rows lie apart: whole tokens after one another, or whole heads
+  const bool tokens = tok_stride >= (__int128)(d->nkv - 1) * head_stride + kHd && head_stride >= kHd;
+  const bool heads = head_stride >= (__int128)(n - 1) * tok_stride + kHd && tok_stride >= kHd;
+  if (n > 1 && d->nkv > 1 ? !(tokens || heads) : (n > 1 && tok_stride < kHd) || (d->nkv > 1 && head_stride < kHd)) return BKV_EINVAL;
+  const int64_t unit = out_type == BKV_OUT_F32 ? 4 : 8;
+  if ((k_out && !aligned16(k_out)) || (v_out && !aligned16(v_out)) || (n > 1 && tok_stride % unit) || (d->nkv > 1 && head_stride % unit))
+    return BKV_EALIGN;
+  ReadArgs a{};
+  a.L = view(d, layer);
+  a.pool_pages = pool_pages(d);
+  a.nkv = d->nkv;
+  a.pos0 = pos0;
+  a.n = n;
+  a.k_out = k_out; a.v_out = v_out;
+  a.tok = tok_stride; a.head = head_stride;
+  return hip_fail(launch_kv_read(a, d->k_fmt, d->v_fmt, out_type, stream));
+}
+
+int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_keep, const int32_t *idx,
+                  hipStream_t stream) {
+  int rc = check(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (n_draft < 0 || n_draft > BKV_TREE_MAX_Q || n_keep < 0 || n_keep > n_draft) return BKV_EINVAL;
+  if (n_keep == 0) return BKV_OK;
+  if ((int64_t)pos0 + n_draft > max_positions(d)) return BKV_ECAP;
+  if (!idx) return BKV_EINVAL;
+  if (((uintptr_t)idx & 3u) != 0) return BKV_EALIGN;
+  CommitArgs a{};
+  void *bases[4] = {d->k_data, d->k_scales, d->v_data, d->v_scales};
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t sb = slot_bytes(d, i);
+    a.base[i] = sb ? (uint8_t *)bases[i] : nullptr;
+    a.stride[i] = d->layer_stride_bytes[i];
+    a.row[i] = (int)sb;
+    a.units[i] = (int)cdiv((int64_t)sb, 64);
+  }
+  a.bt = d->block_table;
+  a.max_pages = d->max_pages;
+  a.page = d->page_tokens;
+  a.pool_pages = pool_pages(d);
+  a.pos0 = pos0;
+  a.n_draft = n_draft; a.n_keep = n_keep;
+  a.idx = idx;
+  return hip_fail(launch_kv_commit(a, d->n_layers, stream));
+}
+
 size_t bkv_workspace_bytes(const bkv_cache_desc *d, int op, uint32_t max_ctx) {
   if (check(d) || max_ctx == 0) return 0;
+  if (op == BKV_OP_TREE) return tree_workspace_bound(d->nh, d->nkv, prefill_base(d));
   if (op == BKV_OP_PREFILL)
     return std::max(prefill_workspace_bound(d->nh, d->nkv, prefill_base(d)),
                     prefill_exact_workspace(d->nh, d->nkv, max_ctx, prefill_base(d)));

@@ -113,6 +113,14 @@ __device__ __forceinline__ int64_t slot_t(const LayerView &L, int64_t pos) {
   }
 }
 
+// slot_of with the block table's entries held against the pool: -1 where the position's page lies outside it
+__device__ __forceinline__ int slot_checked(const LayerView &L, int pool_pages, uint32_t pos) {
+  if (L.page == 0) return (int)pos;
+  const uint32_t pg = pos / (uint32_t)L.page;
+  const uint32_t b = (uint32_t)L.bt[pg];
+  return b < (uint32_t)pool_pages ? (int)(b * (uint32_t)L.page + (pos - pg * (uint32_t)L.page)) : -1;
+}
+
 // element oi = head*hd + d of an [nh][hd] output, in a gate array whose head rows are gs floats
 // apart (hd: contiguous; 2*hd: the q/gate interleave of the engine's attn_q output)
 __host__ __device__ __forceinline__ size_t gate_index(size_t oi, int gs) {

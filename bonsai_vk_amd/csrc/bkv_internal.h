@@ -226,6 +226,75 @@ struct NormRopeArgs {
 };
 hipError_t launch_norm_rope_append(const NormRopeArgs &a, int kf, int vf, int n_tok, hipStream_t st);
 
+// ------------------------------------------------------------------ drafted tokens
+// fp32 rows of head_dim values: token t's head h at p + t * tok + h * head
+struct Rows {
+  const float *p;
+  int64_t tok, head;
+  __host__ __device__ const float *at(int64_t t, int64_t h) const { return p + t * tok + h * head; }
+};
+
+struct TreeArgs {
+  LayerView L;
+  int pool_pages;                // pages of the pool (paged only): table entries from it on are not followed
+  int nkv, nh, grp;              // grp = nh / nkv query heads per KV head
+  uint32_t pos0;
+  int n_q;
+  float scale2;                  // softmax scale times log2(e)
+  Rows q, gate;                  // gate.p null: none
+  const uint64_t *mask;          // [n_q][words], or null: a chain
+  int words;
+  float *out, *out_gated;
+  int splits;                    // key ranges per row block
+  float *part;                   // [splits][n_q * nh][hd] unnormalised partial outputs
+  float2 *ml;                    // [splits][n_q * nh] their reference (log2) and sum
+};
+struct TreePlan {
+  int nrb, splits;               // row blocks per KV head, key ranges per row block
+  size_t off_ml, off_part, total;
+};
+TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base);
+size_t tree_workspace_bound(int nh, int nkv, size_t base);
+hipError_t launch_tree(const TreeArgs &a, const TreePlan &p, int kf, int vf, hipStream_t st);
+
+struct RopeArgs {
+  LayerView L;
+  int pool_pages;
+  int nkv, nh;
+  uint32_t pos0;
+  Rows q, k, v;                  // q.p null: K and V only
+  const float *qn_w, *kn_w;      // null: no norm
+  float eps;
+  const int32_t *positions;      // null: pos0 + t
+  float *q_out;
+  bkv_rope rope;
+};
+hipError_t launch_rope_append(const RopeArgs &a, int kf, int vf, int n_tok, hipStream_t st);
+
+struct ReadArgs {
+  LayerView L;
+  int pool_pages;
+  int nkv;
+  uint32_t pos0;
+  int n;
+  void *k_out, *v_out;           // (one may be null)
+  int64_t tok, head;             // strides in elements
+};
+hipError_t launch_kv_read(const ReadArgs &a, int kf, int vf, int out_type, hipStream_t st);
+
+struct CommitArgs {
+  uint8_t *base[4];              // layer 0's arrays (null: absent)
+  uint64_t stride[4];            // bytes from a layer to the next
+  int row[4];                    // bytes of a slot
+  int units[4];                  // 64-byte columns of a slot, rounded up
+  const int32_t *bt;             // layer 0's block-table row, or null
+  int max_pages, page, pool_pages;
+  uint32_t pos0;
+  int n_draft, n_keep;
+  const int32_t *idx;
+};
+hipError_t launch_kv_commit(const CommitArgs &a, int n_layers, hipStream_t st);
+
 #define BKV_FMT_SWITCH(KF, VF, ...)                                                    \
   do {                                                                                \
     if ((KF) == BKV_Q8_0 && (VF) == BKV_Q8_0) { constexpr int KF_ = 1, VF_ = 1; __VA_ARGS__; } \

@@ -52,7 +52,7 @@ enum bkv_err {
 };
 
 /* bkv_workspace_bytes() op codes */
-enum bkv_op { BKV_OP_DECODE = 0, BKV_OP_PREFILL = 1 };
+enum bkv_op { BKV_OP_DECODE = 0, BKV_OP_PREFILL = 1, BKV_OP_TREE = 2 };
 
 /* ------------------------------------------------------------------ the cache descriptor
  * One descriptor covers the attention layers of one model. Per layer there are four arrays (K data,
@@ -244,6 +244,94 @@ int bkv_static_reset(hipStream_t stream);
 /* Diagnostics (no counterpart in the reference; for tests): the device address of the current
  * GPU's static array in *out (NULL before the first static call or reset on this GPU). */
 int bkv_static_debug_address(void **out);
+
+/* ------------------------------------------------------------------ drafted tokens
+ * Checking several drafted tokens in one pass (speculative decoding; no counterpart in the reference,
+ * which runs one token at a time). The drafted tokens of a step are appended at positions pos0 ..
+ * pos0+n-1 (bkv_rope_append or bkv_kv_append), bkv_attn_tree lets each attend to the positions before
+ * pos0 and to the drafted tokens it follows, and bkv_kv_commit moves the accepted ones together.
+ * These calls take head_dim 256 and any nh that is a multiple of nkv. A block-table entry outside the
+ * pool is never followed: its positions are not written, read as zero, and no row sees them.      */
+#define BKV_TREE_MAX_Q 1024
+
+/* fp32 rows of 256 values in device memory: token t's head h at p + t*tok + h*head (strides in floats,
+ * multiples of 4, at least 0; p 16-byte aligned). Rows may lie in a fused projection's output. */
+typedef struct bkv_rows {
+  const float *p;
+  int64_t tok, head;
+} bkv_rows;
+
+/* Host side, no GPU: the masks and depths of a draft. parent[i] is the drafted token that token i
+ * follows, an earlier one (parent[i] < i), or -1 where it follows position pos0-1. mask, if not NULL,
+ * is [n][(n+63)/64]: bit j%64 of word j/64 of row i is set where j is i or one of the tokens that i
+ * follows. depth, if not NULL, is [n]: 0 for a token that follows pos0-1 (its rotary position is
+ * pos0 + depth). BKV_EINVAL: n outside 0 .. BKV_TREE_MAX_Q, or a parent that is no earlier token. */
+int bkv_tree_mask(const int32_t *parent, int n, uint64_t *mask, int32_t *depth);
+
+/* Attention of the n_q (0 .. BKV_TREE_MAX_Q) drafted tokens cached at pos0 .. pos0+n_q-1. Token i sees
+ * every position below pos0, and drafted token j where bit j of its mask row is set (bits from n_q on
+ * are ignored); mask: device, [n_q][(n_q+63)/64], or NULL for a chain (j <= i; n_q = 1: one token).
+ *   Per head row: score = scale * (q16 . k) with q rounded to fp16 as in bkv_attn_decode, p = softmax
+ *   over the visible positions, out = sum p * v. Probabilities are not rounded to fp16 here, and sums
+ *   run in fp32 in no stated order (the result does not change from call to call): rows agree with
+ *   bkv_attn_decode's to about the rounding of its fp16 probabilities.
+ *   A row that sees nothing gets 0. Positions that a row does not see have no effect on it, whatever
+ *   they hold (Inf and NaN included).
+ *   out: [n_q][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)).
+ * Workspace: bkv_workspace_bytes(d, BKV_OP_TREE, max_ctx), any max_ctx > 0; it needs no
+ * initialisation, and serves decodes too once bkv_workspace_init has run on it. */
+int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, const bkv_rows *q,
+                  const uint64_t *mask, const bkv_rows *gate, float *out, float *out_gated,
+                  void *workspace, size_t ws_bytes, hipStream_t stream);
+
+/* Rotary positions. The first nrot dims of a head row are rotated in pairs, pair p < nrot/2 by the
+ * angle 2*pi*pos*turns[p] (the product in fp64), both results times mscale; the other dims pass through. */
+enum bkv_rope_layout { BKV_ROPE_HALF = 0,          /* pair p: dims p and p + nrot/2              */
+                       BKV_ROPE_INTERLEAVED = 1 }; /* pair p: dims 2p and 2p + 1                 */
+enum bkv_rope_scaling {
+  BKV_ROPE_PLAIN = 0,    /* theta_p = base^(-2p/nrot) radians per position                       */
+  BKV_ROPE_LINEAR = 1,   /* theta_p / factor                                                     */
+  BKV_ROPE_NTK = 2,      /* base * factor^(nrot/(nrot-2)) in the place of base                   */
+  BKV_ROPE_YARN = 3      /* theta_p where a pair turns beta_fast times or more in trained_ctx
+                            positions, theta_p / factor where it turns beta_slow times or fewer,
+                            a ramp over p between; mscale = 1 + 0.1 ln(factor) (factor > 1)       */
+};
+typedef struct bkv_rope {
+  int32_t nrot, layout;
+  float mscale;
+  int32_t reserved;
+  double turns[128];     /* turns per position of each pair (theta_p / 2 pi)                      */
+} bkv_rope;
+
+/* Host side, no GPU: fill *r. nrot even, 0 .. 256; freq_base > 1; factor > 0 (ignored by PLAIN);
+ * trained_ctx > 0 and beta_fast > beta_slow > 0 (YARN only). A caller may fill the struct itself. */
+int bkv_rope_init(bkv_rope *r, int nrot, int layout, double freq_base, int scaling, double factor,
+                  double trained_ctx, double beta_fast, double beta_slow);
+
+/* n_tok projected tokens on their way into the cache at positions pos0 .. pos0+n_tok-1: optional
+ * per-head RMS norm (x * 1/sqrt(mean(x^2) + eps) * w; qn_w and kn_w [hd], both or neither), rotation
+ * of Q and K at positions[t] (device int32, any value; NULL: pos0 + t), K and the raw V written as
+ * bkv_kv_append writes them, the rotated Q rows to q_out [n_tok][nh][hd]. q with q_out may both be
+ * NULL. q_out may be q's own rows; it may not overlap the inputs otherwise. (bkv_qk_norm_rope_append
+ * is the reference's arithmetic bit for bit, for its half layout and consecutive positions; here the
+ * norm's sum is in no stated order and the angle is formed in fp64.) */
+int bkv_rope_append(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok, const bkv_rope *rope,
+                    const bkv_rows *q, const bkv_rows *k, const bkv_rows *v, const float *qn_w,
+                    const float *kn_w, float eps, const int32_t *positions, float *q_out,
+                    hipStream_t stream);
+
+/* Positions pos0 .. pos0+n-1 of a layer as values: fp16 entries, and f16(scale) * int8 of q8_0 ones,
+ * rounded to out_type. k_out and v_out (one may be NULL): position pos0+t's head h at
+ * t*tok_stride + h*head_stride elements (rows must not overlap; 16-byte aligned). */
+enum bkv_out_type { BKV_OUT_F32 = 0, BKV_OUT_F16 = 1, BKV_OUT_BF16 = 2 };
+int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int out_type, void *k_out,
+                void *v_out, int64_t tok_stride, int64_t head_stride, hipStream_t stream);
+
+/* Keep the accepted tokens of a draft: in every layer position pos0+i takes the bytes of position
+ * pos0+idx[i], i < n_keep, as if all were read before any is written. idx: device int32; an entry
+ * outside 0 .. n_draft-1 leaves its position as it is. n_keep <= n_draft <= BKV_TREE_MAX_Q. */
+int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_keep, const int32_t *idx,
+                  hipStream_t stream);
 
 /* Human-readable text of an enum bkv_err value (static storage). */
 const char *bkv_strerror(int err);
