@@ -250,6 +250,7 @@ struct TreeArgs {
   float2 *ml;                    // [splits][n_q * nh] their reference (log2) and sum
 };
 struct TreePlan {
+  int kind;                      // which kernel
   int nrb, splits;               // row blocks per KV head, key ranges per row block
   size_t off_ml, off_part, total;
 };

@@ -29,31 +29,28 @@ namespace bkv {
 constexpr float kLift = 6.0f;          // a score this far (in powers of two) above the reference lifts it
 constexpr float kPScale = 9.0f;        // log2 of the factor on p: 2^(kLift + kPScale) is within fp16
 constexpr int kTreeKeys = 32;          // keys of a step
-constexpr int kTreeFill = 512;         // workgroups that the key split aims for
 constexpr int kTreeMaxSplit = 128;     // (the merge holds a row's partial references two to a lane)
 
 // the 32 keys from kb on that row token i sees, one bit each; keys from nk on are not there
 __device__ __forceinline__ uint32_t tree_window(const TreeArgs &a, int i, int64_t kb) {
-  const int64_t rel = kb - a.pos0;                 // > -32: some of the keys are drafted ones
-  const int nq = a.n_q;
+  const int rel = (int)(kb - a.pos0);              // > -32: some of the keys are drafted ones
   uint32_t win;
   if (a.mask == nullptr) {
-    const int64_t last = i - rel;                  // bits 0 .. last
-    win = last < 0 ? 0u : last >= 31 ? ~0u : (2u << (int)last) - 1u;
+    const int last = i - rel;                      // bits 0 .. last
+    win = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1u;
   } else {
-    const uint64_t *row = a.mask + (int64_t)i * a.words;
+    const uint32_t row = (uint32_t)(i * a.words);
     if (rel < 0) {
-      const int c = (int)-rel;
-      win = ((uint32_t)row[0] << c) | ((1u << c) - 1u);
+      win = ((uint32_t)a.mask[row] << -rel) | ((1u << -rel) - 1u);
     } else {
-      const int w = (int)(rel >> 6), sh = (int)(rel & 63);
-      uint64_t v = row[w] >> sh;
-      if (sh > 32 && w + 1 < a.words) v |= row[w + 1] << (64 - sh);
+      const int w = rel >> 6, sh = rel & 63;
+      uint64_t v = a.mask[row + w] >> sh;
+      if (sh > 32 && w + 1 < a.words) v |= a.mask[row + w + 1] << (64 - sh);
       win = (uint32_t)v;
     }
   }
-  const int64_t there = nq - rel;                  // keys before nk
-  return there >= 32 ? win : win & ((1u << (int)there) - 1u);
+  const int there = a.n_q - rel;                   // keys before nk
+  return there >= 32 ? win : win & ((1u << there) - 1u);
 }
 
 // ------------------------------------------------------------------ joining the key ranges
@@ -185,10 +182,11 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   // (every wave holds the whole row: the decision is the workgroup's)
   const float big = fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
   bool fine = l > 0.0f && l < INFINITY && !__any(!(big < INFINITY) || o.x != o.x || o.y != o.y || o.z != o.z || o.w != o.w);
-  // fp16 V of subnormal size (kTiny is below 2^-14 by the averaging of a few keys): the matrix cores keep such a
-  // product to about 2^-37 of p's unit and not to 24 bits of itself (V of 1e-6: 7e-6 off; of 1e-4: 3e-7)
+  // V of subnormal fp16 size (kTiny is below 2^-14 by the averaging of a few keys): the matrix cores keep such a
+  // product to about 2^-37 of p's unit and not to 24 bits of itself (V of 1e-6: 7e-6 off; of 1e-4: 3e-7), and vl
+  // runs out of bits
   constexpr float kTiny = 0x1p-17f;
-  if (VF == BKV_F16 && fine) {
+  if (fine) {
     const float top = wave_max(big);
     fine = top == 0.0f || !(top < kTiny * l);
   }
@@ -484,34 +482,425 @@ __global__ __launch_bounds__(256, KF == BKV_F16 && VF == BKV_F16 ? 1 : 2) void t
   }
 }
 
+// ------------------------------------------------------------------ many rows: key tiles in LDS
+// A workgroup of NW waves holds 16 MT NW rows, each wave 16 MT of them with all 256 outputs in registers, and steps
+// through its key range 32 keys at a time. A step's K and V are brought into LDS once, already as the products'
+// operands: K's bytes as fp16 (their block scales as fp32 beside them, applied to each block's 32-term product), V
+// as vh (and vl for q8_0), transposed so that a lane's 8 keys of one dim are 16 bytes. The next step's bytes are
+// loaded while this one is computed. S^T and O^T are formed as in the kernel above, so P never leaves its lane.
+//
+// LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 8); V piece g of dim d (keys 4 g .. 4 g + 3
+// and 16 + 4 g .. 16 + 4 g + 3) at 8 (d / 2) + ((4 (d % 2) + g) ^ kx(d)), kx chosen so that both the 8 dims next to
+// one another that a read takes and the 8 dims 4 apart that a write takes lie in different banks.
+//
+// q8_0 scales: vh and vl keep 19 bits for scales up to 2^-1 and down to 2^-17 or so when they are taken times 2^9; a
+// step with a larger one in a wave's 64 dims takes 2^1 or 2^-7 there (its level), and the outputs are brought to the
+// step's unit. (Smaller values end as outputs below kTiny.)
+__device__ __forceinline__ constexpr int level_exp(int lv) { return 9 - 8 * lv; }
+// the level of the largest of fp16 scales (bits, sign cleared): above 2^-1, above 2^7
+__device__ __forceinline__ int scale_level(uint32_t top) { return (top > 0x3800u) + (top > 0x5800u); }
+
+__device__ __forceinline__ uint32_t v_piece(int d, int g) {
+  const int kx = ((d >> 4) & 1) << 2 | ((d >> 2) & 1) << 1 | (((d >> 1) ^ (d >> 3)) & 1);
+  return (uint32_t)(128 * (d >> 1) + 16 * ((4 * (d & 1) + g) ^ kx));
+}
+
+// PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
+// base for the whole workgroup); 2 any pages (a slot of its own for every key)
+template <int KF, int VF, int PG, int NW, int MT, int NBUF>
+__global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile_kernel(TreeArgs a, int nrb) {
+  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT * NW;
+  constexpr int kKB = kTreeKeys * 2 * kHd, kVB = kTreeKeys * 2 * kHd * (VF ? 2 : 1), kSB = KF ? 8 * kTreeKeys * 4 : 0;
+  constexpr int kBuf = kKB + kVB + kSB + 16;       // K, vh, vl, K's scales, the V levels
+  __shared__ __attribute__((aligned(128))) uint8_t sm[NBUF * kBuf];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
+  if (unit >= a.nkv * a.splits) return;
+  const int hk = unit / a.splits, split = unit - hk * a.splits;
+  const int R = a.n_q * a.grp, r0 = RB * rb + 16 * MT * w + n;
+  const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
+  const int64_t steps = (nk + kTreeKeys - 1) / kTreeKeys;
+  const int64_t t0 = steps * split / a.splits, t1 = steps * (split + 1) / a.splits;
+
+  // (the lane's number, opaque where addresses are formed from it: kept from step to step they would take the
+  // registers that the outputs need)
+  auto my_lane = [&]() {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto token_of = [&](int mt) { return min(RB * rb + 16 * MT * w + 16 * mt + (my_lane() & 15), R - 1) / a.grp; };
+  h8 qh[MT][8];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = min(r0 + 16 * mt, R - 1), tok = r / a.grp;
+    const float *q = a.q.at(tok, hk * a.grp + r - tok * a.grp) + 8 * g;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * b), y = *reinterpret_cast<const float4 *>(q + 32 * b + 4);
+      qh[mt][b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
+    }
+  }
+  f4 o[MT][16] = {};
+  float m[MT], l[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
+  uint32_t lv = 0;                                 // the outputs' levels, a byte per 64 dims
+
+  // ---- bringing a step in: waves 0 .. 3 V (64 dims each), the last four waves K (8 keys each)
+  const bool does_v = NW == 4 || w < 4, does_k = NW == 4 || w >= 4;
+  const int wk = w & 3;
+  const size_t krow = (size_t)a.nkv * KRB, vrow = (size_t)a.nkv * VRB, srow = (size_t)a.nkv * kScaleRowBytes;
+  const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
+  const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
+  // the bytes on their way; with 8 waves a wave holds K's or V's, in the same registers
+  constexpr int kKW = KF ? 8 : 16, kVW = VF ? 8 : 16, kV0 = NW == 8 ? 0 : kKW, kKS = NW == 8 ? 0 : 8;
+  uint32_t raw[NW == 8 ? (kKW > kVW ? kKW : kVW) : kKW + kVW], raws[9];   // data words; scales (V's 8, K's 1)
+  uint32_t there0 = ~0u, there1 = ~0u, there2 = ~0u;   // keys whose pages are in the pool: this step's, the next's, ..
+  auto request = [&](int64_t t) {
+    const int lane = my_lane(), n = lane & 15, g = lane >> 4;
+    const uint32_t kb = (uint32_t)t * kTreeKeys, last = min(nk - 1 - kb, (uint32_t)kTreeKeys - 1);
+    int sl = 0;
+    size_t s0 = kb;
+    if constexpr (PG == 1) {
+      const int first = slot_checked(a.L, a.pool_pages, kb);
+      there2 = first >= 0 ? ~0u : 0u;
+      s0 = (size_t)max(first, 0);
+    }
+    if constexpr (PG == 2) {
+      sl = slot_checked(a.L, a.pool_pages, kb + min((uint32_t)lane & 31, last));
+      there2 = (uint32_t)__ballot(sl >= 0);
+      s0 = 0;
+    }
+    const uint8_t *k0 = kd + s0 * krow, *v0 = vd + s0 * vrow, *ks0 = KF ? ksc + s0 * srow : nullptr, *vs0 = VF ? vsc + s0 * srow : nullptr;
+    // (offsets within a step are 32 bits: 31 rows)
+    auto at = [&](const uint8_t *base, int j, size_t row, int col) -> const uint8_t * {
+      if constexpr (PG == 2) return base + (size_t)max(__shfl(sl, j), 0) * row + col;
+      else return base + (min((uint32_t)j, last) * (uint32_t)row + (uint32_t)col);
+    };
+    if (does_k) {
+      constexpr int LR = KF ? 16 : 32;             // lanes of a row
+#pragma unroll
+      for (int u = 0; u < (KF ? 2 : 4); ++u) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(at(k0, 8 * wk + (64 / LR) * u + lane / LR, krow, 16 * (lane % LR)));
+        raw[4 * u] = x.x; raw[4 * u + 1] = x.y; raw[4 * u + 2] = x.z; raw[4 * u + 3] = x.w;
+      }
+      if constexpr (KF) raws[kKS] = *reinterpret_cast<const uint16_t *>(at(ks0, 8 * wk + (lane >> 3), srow, 2 * (lane & 7)));
+    }
+    if (does_v) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = (j & 4) * 4 + 4 * g + (j & 3);
+        if constexpr (VF) {
+          raw[kV0 + j] = *reinterpret_cast<const uint32_t *>(at(v0, key, vrow, 64 * wk + 4 * n));
+          raws[j] = *reinterpret_cast<const uint16_t *>(at(vs0, key, srow, 2 * (2 * wk + (n >> 3))));
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2 *>(at(v0, key, vrow, 128 * wk + 8 * n));
+          raw[kV0 + (VF ? 0 : 2 * j)] = x.x;
+          raw[kV0 + (VF ? 0 : 2 * j + 1)] = x.y;
+        }
+      }
+    }
+  };
+  auto store = [&](uint8_t *buf) {
+    const int lane = my_lane(), n = lane & 15, g = lane >> 4;
+    if (does_k) {
+      if constexpr (KF) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int key = 8 * wk + 4 * u + (lane >> 4), c = 2 * (lane & 15);
+          const uint32_t x[4] = {raw[4 * u] ^ 0x80808080u, raw[4 * u + 1] ^ 0x80808080u, raw[4 * u + 2] ^ 0x80808080u, raw[4 * u + 3] ^ 0x80808080u};
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<uint4 *>(buf + 512 * key + 16 * ((c + e) ^ (key & 7))) =
+                make_uint4(as_u(bytes_h2<0x04010400u>(x[2 * e])), as_u(bytes_h2<0x04030402u>(x[2 * e])),
+                           as_u(bytes_h2<0x04010400u>(x[2 * e + 1])), as_u(bytes_h2<0x04030402u>(x[2 * e + 1])));
+        }
+        reinterpret_cast<float *>(buf + kKB + kVB)[kTreeKeys * (lane & 7) + 8 * wk + (lane >> 3)] = f16_to_f32(raws[kKS]) * a.scale2;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int key = 8 * wk + 2 * u + (lane >> 5), c = lane & 31;
+          *reinterpret_cast<uint4 *>(buf + 512 * key + 16 * (c ^ (key & 7))) = make_uint4(raw[4 * u], raw[4 * u + 1], raw[4 * u + 2], raw[4 * u + 3]);
+        }
+      }
+    }
+    if (does_v) {
+      uint8_t *vb = buf + kKB;
+      if constexpr (VF) {
+        uint32_t top = 0;
+        h2 d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, max(raws[2 * j] & 0x7FFFu, raws[2 * j + 1] & 0x7FFFu));
+        const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
+        const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
+        if (lane == 0) (buf + kKB + kVB + kSB)[wk] = (uint8_t)level;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = as_h2(raws[2 * j] | (raws[2 * j + 1] << 16)) * h2{f, f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t ah[4], al[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = raw[kV0 + 2 * j], hi = raw[kV0 + 2 * j + 1];
+            const uint32_t pb = e == 0 ? pair_bytes<0>(lo, hi) : e == 1 ? pair_bytes<1>(lo, hi) : e == 2 ? pair_bytes<2>(lo, hi) : pair_bytes<3>(lo, hi);
+            h2 h, lw;
+            split_prod(as_h2(pb ^ 0x64806480u) - h2{(_Float16)1152.0f, (_Float16)1152.0f}, d[j], h, lw);
+            ah[j] = as_u(h);
+            al[j] = as_u(lw);
+          }
+          const uint32_t at = v_piece(64 * wk + 4 * n + e, g);
+          *reinterpret_cast<uint4 *>(vb + at) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+          *reinterpret_cast<uint4 *>(vb + kKB + at) = make_uint4(al[0], al[1], al[2], al[3]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t ah[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            ah[j] = __builtin_amdgcn_perm(raw[kV0 + (VF ? 0 : 4 * j + 2 + (e >> 1))], raw[kV0 + (VF ? 0 : 4 * j + (e >> 1))],
+                                          e & 1 ? 0x07060302u : 0x05040100u);
+          *reinterpret_cast<uint4 *>(vb + v_piece(64 * wk + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+        }
+      }
+    }
+  };
+
+  auto compute = [&](const uint8_t *buf, int64_t kb, int64_t next) {
+    // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
+    const int g4 = 4 * (my_lane() >> 4);
+    const bool whole = kb + kTreeKeys <= a.pos0 && (!PG || there0 == ~0u);
+    uint32_t win[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) win[mt] = ~0u;
+    if (!whole) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) win[mt] = (kb + kTreeKeys > a.pos0 ? there0 & tree_window(a, token_of(mt), kb) : there0) >> g4;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- scores (q8_0: times the softmax scale and log2(e) already); the next product's operands are asked for
+    // before this one's are used, and no further ahead (the registers hold no more)
+    f4 s[MT][2] = {};
+    const int lane = my_lane(), n = lane & 15, g = lane >> 4;
+    const uint8_t *kp[2] = {buf + 512 * n + 16 * (g ^ (n & 7)), buf + 512 * n + 16 * ((4 + g) ^ (n & 7))};
+    const uint8_t *sp = buf + kKB + kVB + 16 * g;
+    h8 kf = *reinterpret_cast<const h8 *>(kp[0]);
+    f4 sc = {}, p[MT] = {};                        // q8_0: the last block's scales and products, still to be added
+#pragma unroll
+    for (int ub = 0; ub < 16; ++ub) {
+      const int u = ub >> 3, b = ub & 7, un = (ub + 1) >> 3, bn = (ub + 1) & 7;
+      h8 kn = kf;
+      if (ub < 15) kn = *reinterpret_cast<const h8 *>(kp[bn & 1] + 8192 * un + 128 * (bn >> 1));
+      if constexpr (KF) {
+        const f4 now = *reinterpret_cast<const f4 *>(sp + 4 * (kTreeKeys * b + 16 * u));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const f4 z = mfma16(kf, qh[mt][b], f4{});
+          if (ub > 0)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[mt][(ub - 1) >> 3][i] = __builtin_fmaf(p[mt][i], sc[i], s[mt][(ub - 1) >> 3][i]);
+          p[mt] = z;
+        }
+        sc = now;
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][u] = mfma16(kf, qh[mt][b], s[mt][u]);
+      }
+      kf = kn;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (KF)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[mt][1][i] = __builtin_fmaf(p[mt][i], sc[i], s[mt][1][i]);
+    // (here, and not where the second row tile's are first used, with every block's product kept until then)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));
+    // ---- probabilities
+    h8 ph[MT], pl[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float x[8], top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = KF ? s[mt][j >> 2][j & 3] : s[mt][j >> 2][j & 3] * a.scale2;
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) x[j] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+      if (__any(top > m[mt] + (kLift + kPScale))) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float mn = fmaxf(m[mt], top - kPScale);
+        const float f = mn == m[mt] ? 1.0f : exp2f(m[mt] - mn);
+        m[mt] = mn;
+        l[mt] *= f;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) o[mt][dt] *= f;
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(x[j] - m[mt]);
+      if (!whole) {                                // (where nothing was seen yet, -Inf - -Inf)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) p[j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        l[mt] += p[j];
+        ph[mt][j] = (_Float16)p[j];
+        pl[mt][j] = (_Float16)(p[j] - (float)ph[mt][j]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    request(next);                                 // (here, where the scores' registers are free)
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- P V
+    if constexpr (VF) {
+      const uint32_t now = *reinterpret_cast<const uint32_t *>(buf + kKB + kVB + kSB);
+      if (now != lv) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float f = __builtin_ldexpf(1.0f, 8 * ((int)((lv >> (8 * c)) & 3u) - (int)((now >> (8 * c)) & 3u)));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) o[mt][4 * c + dt] *= f;
+        }
+        lv = now;
+      }
+    }
+    const uint8_t *vb = buf + kKB;
+    const uint32_t vp[2] = {v_piece(n, g), v_piece(16 + n, g) - 1024u};
+    h8 vh = *reinterpret_cast<const h8 *>(vb + vp[0]), vl = vh;
+    if constexpr (VF) vl = *reinterpret_cast<const h8 *>(vb + kKB + vp[0]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt) {
+      h8 hn = vh, ln = vl;
+      if (dt < 15) {
+        hn = *reinterpret_cast<const h8 *>(vb + vp[(dt + 1) & 1] + 1024 * (dt + 1));
+        if constexpr (VF) ln = *reinterpret_cast<const h8 *>(vb + kKB + vp[(dt + 1) & 1] + 1024 * (dt + 1));
+      }
+      if constexpr (VF) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vl, ph[mt], o[mt][dt]);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, pl[mt], o[mt][dt]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, ph[mt], o[mt][dt]);
+      vh = hn;
+      vl = ln;
+      if (dt & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (t0 < t1) {                                   // (the same for the whole workgroup)
+    request(t0);
+    there0 = there1 = there2;
+    if constexpr (NBUF == 2) {
+      store(sm);
+      request(min(t0 + 1, t1 - 1));
+      there1 = there2;
+      lds_barrier();
+    }
+#pragma unroll 1
+    for (int64_t t = t0; t < t1; ++t) {
+      if constexpr (NBUF == 2) {
+        const int at = (int)(t - t0) & 1;
+        store(sm + (at ^ 1) * kBuf);               // step t + 1 (after the last one: once more the last, unused)
+        __builtin_amdgcn_sched_barrier(0);
+        compute(sm + at * kBuf, t * kTreeKeys, min(t + 2, t1 - 1));
+        lds_barrier();
+        there0 = there1;
+        there1 = there2;
+      } else {
+        store(sm);
+        lds_barrier();
+        compute(sm, t * kTreeKeys, min(t + 1, t1 - 1));
+        lds_barrier();
+        there0 = there2;
+      }
+    }
+  }
+
+  // ---- one partial result per row
+  const int64_t rows = (int64_t)a.n_q * a.nh;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = RB * rb + 16 * MT * w + 16 * mt + n, tok = min(r, R - 1) / a.grp;
+    float sum = l[mt];
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (r < R) {
+      const int64_t at = (int64_t)split * rows + (int64_t)tok * a.nh + hk * a.grp + r - tok * a.grp;
+#pragma unroll
+      for (int dt = 0; dt < 16; ++dt) {
+        const float f = VF ? __builtin_ldexpf(1.0f, 8 * (int)((lv >> (8 * (dt >> 2))) & 3u) - 9) : 1.0f;
+        const f4 v = o[mt][dt] * f;
+        *reinterpret_cast<f4 *>(a.part + at * kHd + 16 * dt + 4 * g) = v;
+      }
+      if (g == 0) a.ml[at] = make_float2(m[mt], sum);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ host side
 static inline int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// Which kernel a call takes, by the rows of one KV head: up to 32 the stream kernel in blocks of 16, then tiles of 64,
+// 128 and 256 rows (what each measured: see the kernels).
+enum { kTreeStream, kTree64, kTree128, kTree256 };
+static int tree_kind(int64_t rows) { return rows <= 32 ? kTreeStream : rows <= 64 ? kTree64 : rows <= 128 ? kTree128 : kTree256; }
+static int tree_rows(int kind) { return kind == kTreeStream ? 16 : kind == kTree64 ? 64 : kind == kTree128 ? 128 : 256; }
+// workgroups that the key split aims for: as many as run at once
+static int tree_fill(int kind) { return kind == kTreeStream ? 512 : kind == kTree64 ? 768 : kind == kTree128 ? 512 : 256; }
+
 TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   TreePlan p{};
   const int64_t rows = (int64_t)n_q * (nh / nkv), steps = cdiv(pos0 + n_q, kTreeKeys);
-  p.nrb = (int)cdiv(rows, 16);
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, kTreeFill / ((int64_t)nkv * p.nrb)));
+  p.kind = tree_kind(rows);
+  p.nrb = (int)cdiv(rows, tree_rows(p.kind));
+  // at least 4 steps to a workgroup
+  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, tree_fill(p.kind) / ((int64_t)nkv * p.nrb)));
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
   return p;
 }
 
-// the largest plan of any call: split row blocks are at most kTreeFill of 16 rows, others write every row once
+// the largest plan of any call: 65536 rows where the keys are split (256 workgroups of 256 rows, 512 of 128, ..),
+// otherwise every row once
 size_t tree_workspace_bound(int nh, int nkv, size_t base) {
-  const size_t rows = std::max<size_t>((size_t)kTreeFill * 16, (size_t)BKV_TREE_MAX_Q * nh);
   (void)nkv;
+  const size_t rows = std::max<size_t>(65536, (size_t)BKV_TREE_MAX_Q * nh);
   return base + up256(rows * sizeof(float2)) + up256(rows * kHd * sizeof(float)) + 256;
 }
 
+template <int KF, int VF, int PG>
+static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStream_t st) {
+  const dim3 grid((unsigned)(cdiv((int64_t)a.nkv * a.splits, 8) * 8 * p.nrb));
+  switch (p.kind) {
+    case kTreeStream: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG != 0>), grid, dim3(256), 0, st, a, p.nrb); break;
+    case kTree64: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 4, 1, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
+    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 4, 2, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
+    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 8, 2, 2>), grid, dim3(512), 0, st, a, p.nrb); break;
+  }
+  return hipGetLastError();
+}
+
 hipError_t launch_tree(const TreeArgs &a, const TreePlan &p, int kf, int vf, hipStream_t st) {
-  const unsigned grid = (unsigned)(cdiv((int64_t)a.nkv * a.splits, 8) * 8 * p.nrb);
   BKV_FMT_SWITCH(kf, vf, {
-    if (a.L.page) hipLaunchKernelGGL((tree_stream_kernel<KF_, VF_, true>), dim3(grid), dim3(256), 0, st, a, p.nrb);
-    else hipLaunchKernelGGL((tree_stream_kernel<KF_, VF_, false>), dim3(grid), dim3(256), 0, st, a, p.nrb);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = a.L.page == 0 ? launch_tree_main<KF_, VF_, 0>(a, p, st)
+                         : a.L.page % kTreeKeys == 0 ? launch_tree_main<KF_, VF_, 1>(a, p, st)
+                                                     : launch_tree_main<KF_, VF_, 2>(a, p, st);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((tree_merge_kernel<KF_, VF_>), dim3((unsigned)((int64_t)a.n_q * a.nh)), dim3(256), 0, st, a);
   });
