@@ -206,6 +206,18 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   }
 }
 
+// 8 probabilities as ph + pl: ph cut to fp16 (two in one instruction), pl the rest, rounded (one instruction each)
+__device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const auto c = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
+    ph[j] = (_Float16)c[0];
+    ph[j + 1] = (_Float16)c[1];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) pl[j] = (_Float16)__builtin_fmaf((float)ph[j], -1.0f, p[j]);
+}
+
 // ------------------------------------------------------------------ few rows: keys straight into registers
 // A workgroup holds 16 rows; each of its 4 waves streams a key range of its own, 32 keys a step, without LDS or
 // barriers until the ranges are joined. Bound by the memory: a wave has a step's K and V (17 KB in q8_0) in flight.
@@ -483,11 +495,11 @@ __global__ __launch_bounds__(256, KF == BKV_F16 && VF == BKV_F16 ? 1 : 2) void t
 }
 
 // ------------------------------------------------------------------ many rows: key tiles in LDS
-// A workgroup of NW waves holds 16 MT NW rows, each wave 16 MT of them with all 256 outputs in registers, and steps
-// through its key range 32 keys at a time. A step's K and V are brought into LDS once, already as the products'
-// operands: K's bytes as fp16 (their block scales as fp32 beside them, applied to each block's 32-term product), V
-// as vh (and vl for q8_0), transposed so that a lane's 8 keys of one dim are 16 bytes. The next step's bytes are
-// loaded while this one is computed. S^T and O^T are formed as in the kernel above, so P never leaves its lane.
+// A workgroup of 4 waves holds 64 MT rows, each wave 16 MT of them with all 256 outputs in registers, and steps
+// through its key range 32 keys at a time. A step's cache bytes are loaded straight into LDS while the step before it
+// is computed, and turned once into the products' operands for all of the workgroup's rows: K's bytes into fp16
+// (fp16 K needs nothing: its pieces land where they are wanted), V transposed, so that a lane's 8 keys of one dim are
+// 16 bytes, as vh (and vl for q8_0). S^T and O^T are formed as in the kernel above, so P never leaves its lane.
 //
 // LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 8); V piece g of dim d (keys 4 g .. 4 g + 3
 // and 16 + 4 g .. 16 + 4 g + 3) at 8 (d / 2) + ((4 (d % 2) + g) ^ kx(d)), kx chosen so that both the 8 dims next to
@@ -505,22 +517,33 @@ __device__ __forceinline__ uint32_t v_piece(int d, int g) {
   return (uint32_t)(128 * (d >> 1) + 16 * ((4 * (d & 1) + g) ^ kx));
 }
 
+// 16 bytes per lane from base + off into LDS at dst + 16 * lane (dst the same in all lanes), not waited for
+__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(const uint8_t *src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+
 // PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
 // base for the whole workgroup); 2 any pages (a slot of its own for every key)
-template <int KF, int VF, int PG, int NW, int MT, int NBUF>
-__global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile_kernel(TreeArgs a, int nrb) {
-  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT * NW;
-  constexpr int kKB = kTreeKeys * 2 * kHd, kVB = kTreeKeys * 2 * kHd * (VF ? 2 : 1), kSB = KF ? 8 * kTreeKeys * 4 : 0;
-  constexpr int kBuf = kKB + kVB + kSB + 16;       // K, vh, vl, K's scales, the V levels
-  __shared__ __attribute__((aligned(128))) uint8_t sm[NBUF * kBuf];
+template <int KF, int VF, int PG, int MT>
+__global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) {
+  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 64 * MT;
+  constexpr uint32_t kOp = kTreeKeys * 2 * kHd;    // an operand: 32 keys of 256 fp16
+  // V's operands (vh, vl), K's (two for fp16, which is loaded in place), the bytes as they came, scales, V's levels
+  constexpr uint32_t oV = 0, oK = oV + kOp * (VF ? 2 : 1), oRV = oK + kOp * (KF ? 1 : 2), oRK = oRV + kTreeKeys * VRB;
+  constexpr uint32_t oSV = oRK + (KF ? kTreeKeys * KRB : 0), oSK = oSV + (VF ? 512 : 0), oSC = oSK + (KF ? 512 : 0), oLV = oSC + (KF ? 512 : 0);
+  __shared__ __attribute__((aligned(128))) uint8_t sm[oLV + 16];
+  const uint32_t sm0 = lds_addr(sm);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
   if (unit >= a.nkv * a.splits) return;
   const int hk = unit / a.splits, split = unit - hk * a.splits;
-  const int R = a.n_q * a.grp, r0 = RB * rb + 16 * MT * w + n;
+  const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
-  const int64_t steps = (nk + kTreeKeys - 1) / kTreeKeys;
-  const int64_t t0 = steps * split / a.splits, t1 = steps * (split + 1) / a.splits;
+  const int steps = (int)((nk + kTreeKeys - 1) / kTreeKeys);
+  const int t0 = (int)((int64_t)steps * split / a.splits), t1 = (int)((int64_t)steps * (split + 1) / a.splits);
 
   // (the lane's number, opaque where addresses are formed from it: kept from step to step they would take the
   // registers that the outputs need)
@@ -529,11 +552,57 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile
     asm volatile("" : "+v"(x));
     return x;
   };
-  auto token_of = [&](int mt) { return min(RB * rb + 16 * MT * w + 16 * mt + (my_lane() & 15), R - 1) / a.grp; };
+  const uint32_t krow = (uint32_t)a.nkv * KRB, vrow = (uint32_t)a.nkv * VRB, srow = (uint32_t)a.nkv * kScaleRowBytes;
+  const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
+  const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
+
+  // ---- a step's bytes on their way: wave w takes keys 8 w .. 8 w + 7 of K and of V, waves 0 and 1 the scales
+  uint32_t there = ~0u, there_next = ~0u;          // keys whose pages are in the pool: this step's, the next's
+  int sl = 0;                                      // PG 2: the slot of the next step's key lane % 32
+  auto look_up = [&](int t) {
+    if constexpr (PG == 2) sl = slot_checked(a.L, a.pool_pages, min((uint32_t)t * kTreeKeys + ((uint32_t)lane & 31), nk - 1));
+  };
+  auto request = [&](int t, int kbuf) {
+    const int lane = my_lane();
+    const uint32_t kb = (uint32_t)t * kTreeKeys, last = min(nk - 1 - kb, (uint32_t)kTreeKeys - 1);
+    size_t s0 = kb;
+    if constexpr (PG == 1) {
+      const int first = __builtin_amdgcn_readfirstlane(slot_checked(a.L, a.pool_pages, kb));
+      there_next = first >= 0 ? ~0u : 0u;
+      s0 = (size_t)max(first, 0);
+    }
+    if constexpr (PG == 2) there_next = (uint32_t)__ballot(sl >= 0);
+    // (offsets within a step are 32 bits: 31 rows)
+    auto take = [&](const uint8_t *base, int key, uint32_t row, uint32_t col, uint32_t dst) {
+      if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, dst);
+      else load_to_lds(base + s0 * row, min((uint32_t)key, last) * row + col, dst);
+    };
+#pragma unroll
+    for (int u = 0; u < (KF ? 2 : 4); ++u) {
+      constexpr int LR = KF ? 16 : 32;             // lanes of a row
+      const int first = 8 * w + (64 / LR) * u, key = first + lane / LR, c = lane % LR;
+      if constexpr (KF) take(kd, key, krow, 16 * c, sm0 + oRK + KRB * first);
+      else take(kd, key, krow, 16 * (c ^ (key & 7)), sm0 + oK + kOp * kbuf + KRB * first);
+    }
+#pragma unroll
+    for (int u = 0; u < (VF ? 2 : 4); ++u) {
+      constexpr int LR = VF ? 16 : 32;
+      const int first = 8 * w + (64 / LR) * u;
+      take(vd, first + lane / LR, vrow, 16 * (lane % LR), sm0 + oRV + VRB * first);
+    }
+    if (KF && w == 0 && lane < 32) take(ksc, lane, srow, 0, sm0 + oSK);
+    if (VF && w == 1 && lane < 32) take(vsc, lane, srow, 0, sm0 + oSV);
+  };
+
+  if (t0 < t1) {
+    look_up(t0);
+    request(t0, 0);
+  }
   h8 qh[MT][8];
+  auto token_of = [&](int mt) { return min(RB * rb + 16 * MT * w + 16 * mt + (my_lane() & 15), R - 1) / a.grp; };
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int r = min(r0 + 16 * mt, R - 1), tok = r / a.grp;
+    const int r = min(RB * rb + 16 * MT * w + 16 * mt + n, R - 1), tok = r / a.grp;
     const float *q = a.q.at(tok, hk * a.grp + r - tok * a.grp) + 8 * g;
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
@@ -547,174 +616,126 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile
   for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
   uint32_t lv = 0;                                 // the outputs' levels, a byte per 64 dims
 
-  // ---- bringing a step in: waves 0 .. 3 V (64 dims each), the last four waves K (8 keys each)
-  const bool does_v = NW == 4 || w < 4, does_k = NW == 4 || w >= 4;
-  const int wk = w & 3;
-  const size_t krow = (size_t)a.nkv * KRB, vrow = (size_t)a.nkv * VRB, srow = (size_t)a.nkv * kScaleRowBytes;
-  const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
-  const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
-  // the bytes on their way; with 8 waves a wave holds K's or V's, in the same registers
-  constexpr int kKW = KF ? 8 : 16, kVW = VF ? 8 : 16, kV0 = NW == 8 ? 0 : kKW, kKS = NW == 8 ? 0 : 8;
-  uint32_t raw[NW == 8 ? (kKW > kVW ? kKW : kVW) : kKW + kVW], raws[9];   // data words; scales (V's 8, K's 1)
-  uint32_t there0 = ~0u, there1 = ~0u, there2 = ~0u;   // keys whose pages are in the pool: this step's, the next's, ..
-  auto request = [&](int64_t t) {
+  // ---- the bytes that have landed, made into operands: wave w takes K of keys 8 w .. 8 w + 7 and V of dims 64 w ..
+  auto convert = [&]() {
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
-    const uint32_t kb = (uint32_t)t * kTreeKeys, last = min(nk - 1 - kb, (uint32_t)kTreeKeys - 1);
-    int sl = 0;
-    size_t s0 = kb;
-    if constexpr (PG == 1) {
-      const int first = slot_checked(a.L, a.pool_pages, kb);
-      there2 = first >= 0 ? ~0u : 0u;
-      s0 = (size_t)max(first, 0);
-    }
-    if constexpr (PG == 2) {
-      sl = slot_checked(a.L, a.pool_pages, kb + min((uint32_t)lane & 31, last));
-      there2 = (uint32_t)__ballot(sl >= 0);
-      s0 = 0;
-    }
-    const uint8_t *k0 = kd + s0 * krow, *v0 = vd + s0 * vrow, *ks0 = KF ? ksc + s0 * srow : nullptr, *vs0 = VF ? vsc + s0 * srow : nullptr;
-    // (offsets within a step are 32 bits: 31 rows)
-    auto at = [&](const uint8_t *base, int j, size_t row, int col) -> const uint8_t * {
-      if constexpr (PG == 2) return base + (size_t)max(__shfl(sl, j), 0) * row + col;
-      else return base + (min((uint32_t)j, last) * (uint32_t)row + (uint32_t)col);
-    };
-    if (does_k) {
-      constexpr int LR = KF ? 16 : 32;             // lanes of a row
+    if constexpr (KF) {
 #pragma unroll
-      for (int u = 0; u < (KF ? 2 : 4); ++u) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(at(k0, 8 * wk + (64 / LR) * u + lane / LR, krow, 16 * (lane % LR)));
-        raw[4 * u] = x.x; raw[4 * u + 1] = x.y; raw[4 * u + 2] = x.z; raw[4 * u + 3] = x.w;
+      for (int u = 0; u < 2; ++u) {
+        const int key = 8 * w + 4 * u + g, c = 2 * n;
+        const uint4 r = *reinterpret_cast<const uint4 *>(sm + oRK + KRB * (8 * w + 4 * u) + 16 * lane);
+        const uint32_t x[4] = {r.x ^ 0x80808080u, r.y ^ 0x80808080u, r.z ^ 0x80808080u, r.w ^ 0x80808080u};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<uint4 *>(sm + oK + 512 * key + 16 * ((c + e) ^ (key & 7))) =
+              make_uint4(as_u(bytes_h2<0x04010400u>(x[2 * e])), as_u(bytes_h2<0x04030402u>(x[2 * e])),
+                         as_u(bytes_h2<0x04010400u>(x[2 * e + 1])), as_u(bytes_h2<0x04030402u>(x[2 * e + 1])));
       }
-      if constexpr (KF) raws[kKS] = *reinterpret_cast<const uint16_t *>(at(ks0, 8 * wk + (lane >> 3), srow, 2 * (lane & 7)));
+      const int key = 8 * w + (lane >> 3);         // scales: [key / 4][block][key % 4]
+      reinterpret_cast<uint16_t *>(sm + oSC)[32 * (key >> 2) + 4 * (lane & 7) + (key & 3)] =
+          reinterpret_cast<const uint16_t *>(sm + oSK)[64 * w + lane];
     }
-    if (does_v) {
+    if constexpr (VF) {
+      uint32_t r[8], sc[8], top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int key = (j & 4) * 4 + 4 * g + (j & 3);
-        if constexpr (VF) {
-          raw[kV0 + j] = *reinterpret_cast<const uint32_t *>(at(v0, key, vrow, 64 * wk + 4 * n));
-          raws[j] = *reinterpret_cast<const uint16_t *>(at(vs0, key, srow, 2 * (2 * wk + (n >> 3))));
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2 *>(at(v0, key, vrow, 128 * wk + 8 * n));
-          raw[kV0 + (VF ? 0 : 2 * j)] = x.x;
-          raw[kV0 + (VF ? 0 : 2 * j + 1)] = x.y;
-        }
+        r[j] = *reinterpret_cast<const uint32_t *>(sm + oRV + VRB * key + 64 * w + 4 * n);
+        sc[j] = *reinterpret_cast<const uint16_t *>(sm + oSV + 16 * key + 4 * w + 2 * (n >> 3));
+        top = max(top, sc[j] & 0x7FFFu);
       }
-    }
-  };
-  auto store = [&](uint8_t *buf) {
-    const int lane = my_lane(), n = lane & 15, g = lane >> 4;
-    if (does_k) {
-      if constexpr (KF) {
+      const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
+      const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
+      if (lane == 0) sm[oLV + w] = (uint8_t)level;
+      h2 d[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int key = 8 * wk + 4 * u + (lane >> 4), c = 2 * (lane & 15);
-          const uint32_t x[4] = {raw[4 * u] ^ 0x80808080u, raw[4 * u + 1] ^ 0x80808080u, raw[4 * u + 2] ^ 0x80808080u, raw[4 * u + 3] ^ 0x80808080u};
+      for (int j = 0; j < 4; ++j) d[j] = as_h2(sc[2 * j] | (sc[2 * j + 1] << 16)) * h2{f, f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<uint4 *>(buf + 512 * key + 16 * ((c + e) ^ (key & 7))) =
-                make_uint4(as_u(bytes_h2<0x04010400u>(x[2 * e])), as_u(bytes_h2<0x04030402u>(x[2 * e])),
-                           as_u(bytes_h2<0x04010400u>(x[2 * e + 1])), as_u(bytes_h2<0x04030402u>(x[2 * e + 1])));
+      for (int e = 0; e < 4; ++e) {
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = r[2 * j], hi = r[2 * j + 1];
+          const uint32_t pb = e == 0 ? pair_bytes<0>(lo, hi) : e == 1 ? pair_bytes<1>(lo, hi) : e == 2 ? pair_bytes<2>(lo, hi) : pair_bytes<3>(lo, hi);
+          h2 h, lw;
+          split_prod(as_h2(pb ^ 0x64806480u) - h2{(_Float16)1152.0f, (_Float16)1152.0f}, d[j], h, lw);
+          ah[j] = as_u(h);
+          al[j] = as_u(lw);
         }
-        reinterpret_cast<float *>(buf + kKB + kVB)[kTreeKeys * (lane & 7) + 8 * wk + (lane >> 3)] = f16_to_f32(raws[kKS]) * a.scale2;
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int key = 8 * wk + 2 * u + (lane >> 5), c = lane & 31;
-          *reinterpret_cast<uint4 *>(buf + 512 * key + 16 * (c ^ (key & 7))) = make_uint4(raw[4 * u], raw[4 * u + 1], raw[4 * u + 2], raw[4 * u + 3]);
-        }
+        const uint32_t at = v_piece(64 * w + 4 * n + e, g);
+        *reinterpret_cast<uint4 *>(sm + oV + at) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+        *reinterpret_cast<uint4 *>(sm + oV + (VF ? kOp : 0u) + at) = make_uint4(al[0], al[1], al[2], al[3]);
       }
-    }
-    if (does_v) {
-      uint8_t *vb = buf + kKB;
-      if constexpr (VF) {
-        uint32_t top = 0;
-        h2 d[4];
+    } else {
+      uint2 r[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, max(raws[2 * j] & 0x7FFFu, raws[2 * j + 1] & 0x7FFFu));
-        const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
-        const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
-        if (lane == 0) (buf + kKB + kVB + kSB)[wk] = (uint8_t)level;
+      for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const uint2 *>(sm + oRV + VRB * ((j & 4) * 4 + 4 * g + (j & 3)) + 128 * w + 8 * n);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] = as_h2(raws[2 * j] | (raws[2 * j + 1] << 16)) * h2{f, f};
+      for (int e = 0; e < 4; ++e) {
+        uint32_t ah[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t ah[4], al[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = raw[kV0 + 2 * j], hi = raw[kV0 + 2 * j + 1];
-            const uint32_t pb = e == 0 ? pair_bytes<0>(lo, hi) : e == 1 ? pair_bytes<1>(lo, hi) : e == 2 ? pair_bytes<2>(lo, hi) : pair_bytes<3>(lo, hi);
-            h2 h, lw;
-            split_prod(as_h2(pb ^ 0x64806480u) - h2{(_Float16)1152.0f, (_Float16)1152.0f}, d[j], h, lw);
-            ah[j] = as_u(h);
-            al[j] = as_u(lw);
-          }
-          const uint32_t at = v_piece(64 * wk + 4 * n + e, g);
-          *reinterpret_cast<uint4 *>(vb + at) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
-          *reinterpret_cast<uint4 *>(vb + kKB + at) = make_uint4(al[0], al[1], al[2], al[3]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t ah[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            ah[j] = __builtin_amdgcn_perm(raw[kV0 + (VF ? 0 : 4 * j + 2 + (e >> 1))], raw[kV0 + (VF ? 0 : 4 * j + (e >> 1))],
-                                          e & 1 ? 0x07060302u : 0x05040100u);
-          *reinterpret_cast<uint4 *>(vb + v_piece(64 * wk + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
-        }
+        for (int j = 0; j < 4; ++j)
+          ah[j] = __builtin_amdgcn_perm(e & 2 ? r[2 * j + 1].y : r[2 * j + 1].x, e & 2 ? r[2 * j].y : r[2 * j].x, e & 1 ? 0x07060302u : 0x05040100u);
+        *reinterpret_cast<uint4 *>(sm + oV + v_piece(64 * w + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
       }
     }
   };
 
-  auto compute = [&](const uint8_t *buf, int64_t kb, int64_t next) {
+  auto compute = [&](int t, int kbuf) {
+    const int64_t kb = (int64_t)t * kTreeKeys;
     // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
     const int g4 = 4 * (my_lane() >> 4);
-    const bool whole = kb + kTreeKeys <= a.pos0 && (!PG || there0 == ~0u);
+    const bool whole = kb + kTreeKeys <= a.pos0 && (!PG || there == ~0u);
     uint32_t win[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) win[mt] = ~0u;
     if (!whole) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) win[mt] = (kb + kTreeKeys > a.pos0 ? there0 & tree_window(a, token_of(mt), kb) : there0) >> g4;
+      for (int mt = 0; mt < MT; ++mt) win[mt] = (kb + kTreeKeys > a.pos0 ? there & tree_window(a, token_of(mt), kb) : there) >> g4;
     }
     __builtin_amdgcn_sched_barrier(0);
-    // ---- scores (q8_0: times the softmax scale and log2(e) already); the next product's operands are asked for
-    // before this one's are used, and no further ahead (the registers hold no more)
+    // ---- scores; the operands of product ub + AK are asked for before product ub, and no further ahead (the
+    // registers hold no more)
+    constexpr int AH = 2, AK = KF && MT == 2 ? 1 : 2;
     f4 s[MT][2] = {};
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
-    const uint8_t *kp[2] = {buf + 512 * n + 16 * (g ^ (n & 7)), buf + 512 * n + 16 * ((4 + g) ^ (n & 7))};
-    const uint8_t *sp = buf + kKB + kVB + 16 * g;
-    h8 kf = *reinterpret_cast<const h8 *>(kp[0]);
-    f4 sc = {}, p[MT] = {};                        // q8_0: the last block's scales and products, still to be added
+    const uint8_t *kop = sm + oK + (KF ? 0 : kOp * kbuf) + 512 * n;
+    const uint8_t *kp[2] = {kop + 16 * (g ^ (n & 7)), kop + 16 * ((4 + g) ^ (n & 7))};
+    const uint8_t *sp = sm + oSC + 64 * g;
+    auto k_at = [&](int ub) { return *reinterpret_cast<const h8 *>(kp[ub & 1] + 8192 * (ub >> 3) + 128 * ((ub & 7) >> 1)); };
+    auto s_at = [&](int ub) { return *reinterpret_cast<const h8 *>(sp + 256 * (ub >> 3) + 16 * ((ub & 7) >> 1)); };   // two blocks
+    h8 kf[AK + 1], sc = {}, sn = {};
+    f4 p[MT] = {};                                 // q8_0: the last block's products, still to be scaled and added
+    if constexpr (KF) sn = s_at(0);
 #pragma unroll
-    for (int ub = 0; ub < 16; ++ub) {
-      const int u = ub >> 3, b = ub & 7, un = (ub + 1) >> 3, bn = (ub + 1) & 7;
-      h8 kn = kf;
-      if (ub < 15) kn = *reinterpret_cast<const h8 *>(kp[bn & 1] + 8192 * un + 128 * (bn >> 1));
-      if constexpr (KF) {
-        const f4 now = *reinterpret_cast<const f4 *>(sp + 4 * (kTreeKeys * b + 16 * u));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const f4 z = mfma16(kf, qh[mt][b], f4{});
-          if (ub > 0)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[mt][(ub - 1) >> 3][i] = __builtin_fmaf(p[mt][i], sc[i], s[mt][(ub - 1) >> 3][i]);
-          p[mt] = z;
-        }
-        sc = now;
-      } else {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt][u] = mfma16(kf, qh[mt][b], s[mt][u]);
-      }
-      kf = kn;
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (KF)
+    for (int j = 0; j < AK; ++j) kf[j] = k_at(j);
+    auto add = [&](int ub) {                       // block ub's products (its pair's scales are in sc)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[mt][1][i] = __builtin_fmaf(p[mt][i], sc[i], s[mt][1][i]);
+        for (int i = 0; i < 4; ++i) s[mt][ub >> 3][i] = __builtin_fmaf(p[mt][i], (float)sc[4 * (ub & 1) + i], s[mt][ub >> 3][i]);
+    };
+#pragma unroll
+    for (int ub = 0; ub < 16; ++ub) {
+      if (ub + AK < 16) kf[(ub + AK) % (AK + 1)] = k_at(ub + AK);
+      if constexpr (KF) {
+        f4 z[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) z[mt] = mfma16(kf[ub % (AK + 1)], qh[mt][ub & 7], f4{});
+        if (ub > 0) add(ub - 1);
+        if (!(ub & 1)) {
+          sc = sn;
+          if (ub < 14) sn = s_at(ub + 2);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) p[mt] = z[mt];
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][ub >> 3] = mfma16(kf[ub % (AK + 1)], qh[mt][ub & 7], s[mt][ub >> 3]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (KF) add(15);
     // (here, and not where the second row tile's are first used, with every block's product kept until then)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));
@@ -722,16 +743,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile
     h8 ph[MT], pl[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float x[8], top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = KF ? s[mt][j >> 2][j & 3] : s[mt][j >> 2][j & 3] * a.scale2;
       if (!whole) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) x[j] = -INFINITY;
+          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) s[mt][j >> 2][j & 3] = -INFINITY;
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+      float top = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
+                        fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3]))) * a.scale2;
       if (__any(top > m[mt] + (kLift + kPScale))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
@@ -744,25 +762,19 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile
       }
       float p[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(x[j] - m[mt]);
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][j >> 2][j & 3], a.scale2, -m[mt]));
       if (!whole) {                                // (where nothing was seen yet, -Inf - -Inf)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) p[j] = 0.0f;
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        l[mt] += p[j];
-        ph[mt][j] = (_Float16)p[j];
-        pl[mt][j] = (_Float16)(p[j] - (float)ph[mt][j]);
-      }
+      l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      split_p(p, ph[mt], pl[mt]);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    request(next);                                 // (here, where the scores' registers are free)
     __builtin_amdgcn_sched_barrier(0);
     // ---- P V
     if constexpr (VF) {
-      const uint32_t now = *reinterpret_cast<const uint32_t *>(buf + kKB + kVB + kSB);
+      const uint32_t now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(sm + oLV));
       if (now != lv) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -775,59 +787,47 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile
         lv = now;
       }
     }
-    const uint8_t *vb = buf + kKB;
+    const uint8_t *vb = sm + oV;
     const uint32_t vp[2] = {v_piece(n, g), v_piece(16 + n, g) - 1024u};
-    h8 vh = *reinterpret_cast<const h8 *>(vb + vp[0]), vl = vh;
-    if constexpr (VF) vl = *reinterpret_cast<const h8 *>(vb + kKB + vp[0]);
+    auto v_at = [&](int dt, int lo) { return *reinterpret_cast<const h8 *>(vb + lo * kOp + vp[dt & 1] + 1024 * dt); };
+    h8 vh[AH + 1], vl[VF ? AH + 1 : 1];
+#pragma unroll
+    for (int j = 0; j < AH; ++j) {
+      vh[j] = v_at(j, 0);
+      if constexpr (VF) vl[j] = v_at(j, 1);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int dt = 0; dt < 16; ++dt) {
-      h8 hn = vh, ln = vl;
-      if (dt < 15) {
-        hn = *reinterpret_cast<const h8 *>(vb + vp[(dt + 1) & 1] + 1024 * (dt + 1));
-        if constexpr (VF) ln = *reinterpret_cast<const h8 *>(vb + kKB + vp[(dt + 1) & 1] + 1024 * (dt + 1));
+      const int c = dt % (AH + 1), f = (dt + AH) % (AH + 1);
+      if (dt + AH < 16) {
+        vh[f] = v_at(dt + AH, 0);
+        if constexpr (VF) vl[f] = v_at(dt + AH, 1);
       }
       if constexpr (VF) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vl, ph[mt], o[mt][dt]);
+        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vl[c], ph[mt], o[mt][dt]);
       }
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, pl[mt], o[mt][dt]);
+      for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh[c], pl[mt], o[mt][dt]);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, ph[mt], o[mt][dt]);
-      vh = hn;
-      vl = ln;
-      if (dt & 1) __builtin_amdgcn_sched_barrier(0);
+      for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh[c], ph[mt], o[mt][dt]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  if (t0 < t1) {                                   // (the same for the whole workgroup)
-    request(t0);
-    there0 = there1 = there2;
-    if constexpr (NBUF == 2) {
-      store(sm);
-      request(min(t0 + 1, t1 - 1));
-      there1 = there2;
-      lds_barrier();
-    }
-#pragma unroll 1
-    for (int64_t t = t0; t < t1; ++t) {
-      if constexpr (NBUF == 2) {
-        const int at = (int)(t - t0) & 1;
-        store(sm + (at ^ 1) * kBuf);               // step t + 1 (after the last one: once more the last, unused)
-        __builtin_amdgcn_sched_barrier(0);
-        compute(sm + at * kBuf, t * kTreeKeys, min(t + 2, t1 - 1));
-        lds_barrier();
-        there0 = there1;
-        there1 = there2;
-      } else {
-        store(sm);
-        lds_barrier();
-        compute(sm, t * kTreeKeys, min(t + 1, t1 - 1));
-        lds_barrier();
-        there0 = there2;
-      }
-    }
+  for (int t = t0; t < t1; ++t) {                  // (the same count in the whole workgroup)
+    const int kbuf = (t - t0) & 1;
+    // this step's bytes have landed, and no wave reads the last one's operands any more
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    there = there_next;
+    convert();
+    look_up(min(t + 1, t1 - 1));
+    lds_barrier();
+    if (t + 1 < t1) request(t + 1, kbuf ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    compute(t, kbuf);
   }
 
   // ---- one partial result per row
@@ -855,13 +855,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && MT == 1 ? 3 : 2) void tree_tile
 static inline int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Which kernel a call takes, by the rows of one KV head: up to 32 the stream kernel in blocks of 16, then tiles of 64,
-// 128 and 256 rows (what each measured: see the kernels).
-enum { kTreeStream, kTree64, kTree128, kTree256 };
-static int tree_kind(int64_t rows) { return rows <= 32 ? kTreeStream : rows <= 64 ? kTree64 : rows <= 128 ? kTree128 : kTree256; }
-static int tree_rows(int kind) { return kind == kTreeStream ? 16 : kind == kTree64 ? 64 : kind == kTree128 ? 128 : 256; }
+// Which kernel a call takes, by the rows of one KV head: up to 32 the stream kernel in blocks of 16, up to 64 one tile
+// of 64 rows, beyond that tiles of 128 (what each measured: see the kernels).
+enum { kTreeStream, kTree64, kTree128 };
+static int tree_kind(int64_t rows) { return rows <= 32 ? kTreeStream : rows <= 64 ? kTree64 : kTree128; }
+static int tree_rows(int kind) { return kind == kTreeStream ? 16 : kind == kTree64 ? 64 : 128; }
 // workgroups that the key split aims for: as many as run at once
-static int tree_fill(int kind) { return kind == kTreeStream ? 512 : kind == kTree64 ? 768 : kind == kTree128 ? 512 : 256; }
+constexpr int kTreeFill = 512;
 
 TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   TreePlan p{};
@@ -869,14 +869,14 @@ TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   p.kind = tree_kind(rows);
   p.nrb = (int)cdiv(rows, tree_rows(p.kind));
   // at least 4 steps to a workgroup
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, tree_fill(p.kind) / ((int64_t)nkv * p.nrb)));
+  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, kTreeFill / ((int64_t)nkv * p.nrb)));
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
   return p;
 }
 
-// the largest plan of any call: 65536 rows where the keys are split (256 workgroups of 256 rows, 512 of 128, ..),
+// the largest plan of any call: 65536 rows where the keys are split (512 workgroups of 128),
 // otherwise every row once
 size_t tree_workspace_bound(int nh, int nkv, size_t base) {
   (void)nkv;
@@ -889,9 +889,8 @@ static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStre
   const dim3 grid((unsigned)(cdiv((int64_t)a.nkv * a.splits, 8) * 8 * p.nrb));
   switch (p.kind) {
     case kTreeStream: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG != 0>), grid, dim3(256), 0, st, a, p.nrb); break;
-    case kTree64: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 4, 1, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
-    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 4, 2, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
-    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 8, 2, 2>), grid, dim3(512), 0, st, a, p.nrb); break;
+    case kTree64: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
+    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a, p.nrb); break;
   }
   return hipGetLastError();
 }
