@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256, KF == BKV_F16 && VF == BKV_F16 ? 1 : 2) void t
 // (fp16 K needs nothing: its pieces land where they are wanted), V transposed, so that a lane's 8 keys of one dim are
 // 16 bytes, as vh (and vl for q8_0). S^T and O^T are formed as in the kernel above, so P never leaves its lane.
 //
-// LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 8); V piece g of dim d (keys 4 g .. 4 g + 3
+// LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
 // and 16 + 4 g .. 16 + 4 g + 3) at 8 (d / 2) + ((4 (d % 2) + g) ^ kx(d)), kx chosen so that both the 8 dims next to
 // one another that a read takes and the 8 dims 4 apart that a write takes lie in different banks.
 //
@@ -525,16 +525,21 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
 }
 
+__device__ __forceinline__ void load4_to_lds(const uint8_t *src, uint32_t dst) {   // 4 bytes per lane
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+
 // PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
 // base for the whole workgroup); 2 any pages (a slot of its own for every key)
 template <int KF, int VF, int PG, int MT>
-__global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) {
-  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 64 * MT;
+__global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) {
+  constexpr int NW = 8, KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT * NW;
   constexpr uint32_t kOp = kTreeKeys * 2 * kHd;    // an operand: 32 keys of 256 fp16
-  // V's operands (vh, vl), K's (two for fp16, which is loaded in place), the bytes as they came, scales, V's levels
-  constexpr uint32_t oV = 0, oK = oV + kOp * (VF ? 2 : 1), oRV = oK + kOp * (KF ? 1 : 2), oRK = oRV + kTreeKeys * VRB;
-  constexpr uint32_t oSV = oRK + (KF ? kTreeKeys * KRB : 0), oSK = oSV + (VF ? 512 : 0), oSC = oSK + (KF ? 512 : 0), oLV = oSC + (KF ? 512 : 0);
-  __shared__ __attribute__((aligned(128))) uint8_t sm[oLV + 16];
+  // three steps' V operands (vh, vl, their levels) and two steps' of K (with its scales); behind them the bytes as
+  // they came, a wave's own
+  constexpr uint32_t kVB = kOp * (VF ? 2 : 1) + 128, kKB = kOp + (KF ? 512 : 0), oLV = kVB - 128;
+  constexpr uint32_t oK = 3 * kVB, oRV = oK + 2 * kKB, oRK = oRV + kTreeKeys * VRB, oSV = oRK + (KF ? kTreeKeys * KRB : 0), oSK = oSV + (VF ? 512 : 0);
+  __shared__ __attribute__((aligned(128))) uint8_t sm[oSK + (KF ? 512 : 0)];
   const uint32_t sm0 = lds_addr(sm);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
@@ -556,47 +561,63 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
   const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
   const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
 
-  // ---- a step's bytes on their way: wave w takes keys 8 w .. 8 w + 7 of K and of V, waves 0 and 1 the scales
-  uint32_t there = ~0u, there_next = ~0u;          // keys whose pages are in the pool: this step's, the next's
-  int sl = 0;                                      // PG 2: the slot of the next step's key lane % 32
+  // ---- a step's bytes on their way: waves 0 .. 3 take V (64 dims each), waves 4 .. 7 K (8 keys each), what they will
+  // make into operands themselves, so that a wave waits for its own loads only
+  const bool does_v = w < 4;
+  const int wk = w & 3;
+  uint32_t there = ~0u, there_next = ~0u, there_after = ~0u;   // keys whose pages are in the pool: this step's, the next's, ..
+  int sl = 0;                                      // PG 2: the slot of the key lane % 32 of the step asked for next
   auto look_up = [&](int t) {
     if constexpr (PG == 2) sl = slot_checked(a.L, a.pool_pages, min((uint32_t)t * kTreeKeys + ((uint32_t)lane & 31), nk - 1));
   };
-  auto request = [&](int t, int kbuf) {
+  auto request = [&](int t, int buf) {
     const int lane = my_lane();
     const uint32_t kb = (uint32_t)t * kTreeKeys, last = min(nk - 1 - kb, (uint32_t)kTreeKeys - 1);
     size_t s0 = kb;
     if constexpr (PG == 1) {
       const int first = __builtin_amdgcn_readfirstlane(slot_checked(a.L, a.pool_pages, kb));
-      there_next = first >= 0 ? ~0u : 0u;
+      there_after = first >= 0 ? ~0u : 0u;
       s0 = (size_t)max(first, 0);
     }
-    if constexpr (PG == 2) there_next = (uint32_t)__ballot(sl >= 0);
+    if constexpr (PG == 2) there_after = (uint32_t)__ballot(sl >= 0);
     // (offsets within a step are 32 bits: 31 rows)
     auto take = [&](const uint8_t *base, int key, uint32_t row, uint32_t col, uint32_t dst) {
       if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, dst);
       else load_to_lds(base + s0 * row, min((uint32_t)key, last) * row + col, dst);
     };
+    if (does_v) {
+      // [place][64 dims], 4 or 8 lanes of 16 bytes per key; place 4 j + g is key slot (g, j) of the contraction, so that
+      // the 4 groups' reads of one j are neighbours
+      constexpr int LR = VF ? 4 : 8;
+      auto key_of = [](int p) { return (p & 16) + 4 * (p & 3) + ((p >> 2) & 3); };
 #pragma unroll
-    for (int u = 0; u < (KF ? 2 : 4); ++u) {
+      for (int u = 0; u < (VF ? 2 : 4); ++u)
+        take(vd, key_of((64 / LR) * u + lane / LR), vrow, 16 * (LR * wk + lane % LR), sm0 + oRV + 32 * 16 * LR * wk + 1024 * u);
+      if constexpr (VF) {                          // its two blocks' scales: 4 bytes of each key's row
+        const int key = key_of(lane & 31);
+        const uint8_t *src = PG == 2 ? vsc + (size_t)max(__shfl(sl, key), 0) * srow : vsc + s0 * srow + min((uint32_t)key, last) * srow;
+        if (lane < 32) load4_to_lds(src + 4 * wk, sm0 + oSV + 128 * wk);
+      }
+    } else {
       constexpr int LR = KF ? 16 : 32;             // lanes of a row
-      const int first = 8 * w + (64 / LR) * u, key = first + lane / LR, c = lane % LR;
-      if constexpr (KF) take(kd, key, krow, 16 * c, sm0 + oRK + KRB * first);
-      else take(kd, key, krow, 16 * (c ^ (key & 7)), sm0 + oK + kOp * kbuf + KRB * first);
-    }
 #pragma unroll
-    for (int u = 0; u < (VF ? 2 : 4); ++u) {
-      constexpr int LR = VF ? 16 : 32;
-      const int first = 8 * w + (64 / LR) * u;
-      take(vd, first + lane / LR, vrow, 16 * (lane % LR), sm0 + oRV + VRB * first);
+      for (int u = 0; u < (KF ? 2 : 4); ++u) {
+        const int first = 8 * wk + (64 / LR) * u, key = first + lane / LR, c = lane % LR;
+        if constexpr (KF) take(kd, key, krow, 16 * c, sm0 + oRK + KRB * first);
+        else take(kd, key, krow, 16 * (c ^ (key & 15)), sm0 + oK + kKB * buf + KRB * first);
+      }
+      if constexpr (KF) {                          // (the shuffle with every lane there, the load with 8)
+        const int key = (8 * wk + lane) & 31;
+        const uint8_t *src = PG == 2 ? ksc + (size_t)max(__shfl(sl, key), 0) * srow : ksc + s0 * srow + min((uint32_t)key, last) * srow;
+        if (lane < 8) load_to_lds(src, sm0 + oSK + 128 * wk);
+      }
     }
-    if (KF && w == 0 && lane < 32) take(ksc, lane, srow, 0, sm0 + oSK);
-    if (VF && w == 1 && lane < 32) take(vsc, lane, srow, 0, sm0 + oSV);
   };
 
   if (t0 < t1) {
     look_up(t0);
     request(t0, 0);
+    there = there_after;
   }
   h8 qh[MT][8];
   auto token_of = [&](int mt) { return min(RB * rb + 16 * MT * w + 16 * mt + (my_lane() & 15), R - 1) / a.grp; };
@@ -616,37 +637,40 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
   for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
   uint32_t lv = 0;                                 // the outputs' levels, a byte per 64 dims
 
-  // ---- the bytes that have landed, made into operands: wave w takes K of keys 8 w .. 8 w + 7 and V of dims 64 w ..
-  auto convert = [&]() {
+  // ---- the wave's bytes, landed, made into operands
+  auto convert = [&](uint8_t *kto, uint8_t *vto) {
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
-    if constexpr (KF) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!does_v) {
+      if constexpr (KF) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = 8 * w + 4 * u + g, c = 2 * n;
-        const uint4 r = *reinterpret_cast<const uint4 *>(sm + oRK + KRB * (8 * w + 4 * u) + 16 * lane);
-        const uint32_t x[4] = {r.x ^ 0x80808080u, r.y ^ 0x80808080u, r.z ^ 0x80808080u, r.w ^ 0x80808080u};
+        for (int u = 0; u < 2; ++u) {
+          const int key = 8 * wk + 4 * u + g;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<uint4 *>(sm + oK + 512 * key + 16 * ((c + e) ^ (key & 7))) =
-              make_uint4(as_u(bytes_h2<0x04010400u>(x[2 * e])), as_u(bytes_h2<0x04030402u>(x[2 * e])),
-                         as_u(bytes_h2<0x04010400u>(x[2 * e + 1])), as_u(bytes_h2<0x04030402u>(x[2 * e + 1])));
+          for (int e = 0; e < 2; ++e) {            // pieces n and 16 + n: 16 lanes write 16 banks' worth
+            const uint2 r = *reinterpret_cast<const uint2 *>(sm + oRK + KRB * key + 8 * n + 128 * e);
+            const uint32_t x = r.x ^ 0x80808080u, y = r.y ^ 0x80808080u;
+            *reinterpret_cast<uint4 *>(kto + 512 * key + 16 * ((n ^ (key & 15)) + 16 * e)) =
+                make_uint4(as_u(bytes_h2<0x04010400u>(x)), as_u(bytes_h2<0x04030402u>(x)), as_u(bytes_h2<0x04010400u>(y)), as_u(bytes_h2<0x04030402u>(y)));
+          }
+        }
+        const int key = 8 * wk + (lane >> 3);      // scales: [key / 4][block][key % 4]
+        reinterpret_cast<uint16_t *>(kto + kOp)[32 * (key >> 2) + 4 * (lane & 7) + (key & 3)] =
+            reinterpret_cast<const uint16_t *>(sm + oSK)[64 * wk + lane];
       }
-      const int key = 8 * w + (lane >> 3);         // scales: [key / 4][block][key % 4]
-      reinterpret_cast<uint16_t *>(sm + oSC)[32 * (key >> 2) + 4 * (lane & 7) + (key & 3)] =
-          reinterpret_cast<const uint16_t *>(sm + oSK)[64 * w + lane];
+      return;
     }
     if constexpr (VF) {
       uint32_t r[8], sc[8], top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int key = (j & 4) * 4 + 4 * g + (j & 3);
-        r[j] = *reinterpret_cast<const uint32_t *>(sm + oRV + VRB * key + 64 * w + 4 * n);
-        sc[j] = *reinterpret_cast<const uint16_t *>(sm + oSV + 16 * key + 4 * w + 2 * (n >> 3));
+        r[j] = *reinterpret_cast<const uint32_t *>(sm + oRV + 2048 * wk + 64 * (4 * j + g) + 4 * n);
+        sc[j] = *reinterpret_cast<const uint16_t *>(sm + oSV + 128 * wk + 4 * (4 * j + g) + 2 * (n >> 3));
         top = max(top, sc[j] & 0x7FFFu);
       }
       const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
       const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
-      if (lane == 0) sm[oLV + w] = (uint8_t)level;
+      if (lane == 0) vto[oLV + wk] = (uint8_t)level;
       h2 d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = as_h2(sc[2 * j] | (sc[2 * j + 1] << 16)) * h2{f, f};
@@ -662,26 +686,27 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
           ah[j] = as_u(h);
           al[j] = as_u(lw);
         }
-        const uint32_t at = v_piece(64 * w + 4 * n + e, g);
-        *reinterpret_cast<uint4 *>(sm + oV + at) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
-        *reinterpret_cast<uint4 *>(sm + oV + (VF ? kOp : 0u) + at) = make_uint4(al[0], al[1], al[2], al[3]);
+        const uint32_t at = v_piece(64 * wk + 4 * n + e, g);
+        *reinterpret_cast<uint4 *>(vto + at) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+        *reinterpret_cast<uint4 *>(vto + (VF ? kOp : 0u) + at) = make_uint4(al[0], al[1], al[2], al[3]);
       }
     } else {
       uint2 r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const uint2 *>(sm + oRV + VRB * ((j & 4) * 4 + 4 * g + (j & 3)) + 128 * w + 8 * n);
+      for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const uint2 *>(sm + oRV + 4096 * wk + 128 * (4 * j + g) + 8 * n);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t ah[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           ah[j] = __builtin_amdgcn_perm(e & 2 ? r[2 * j + 1].y : r[2 * j + 1].x, e & 2 ? r[2 * j].y : r[2 * j].x, e & 1 ? 0x07060302u : 0x05040100u);
-        *reinterpret_cast<uint4 *>(sm + oV + v_piece(64 * w + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+        *reinterpret_cast<uint4 *>(vto + v_piece(64 * wk + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
       }
     }
   };
 
-  auto compute = [&](int t, int kbuf) {
+  h8 ph[MT], pl[MT];
+  auto scores = [&](int t, const uint8_t *kbuf) {
     const int64_t kb = (int64_t)t * kTreeKeys;
     // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
     const int g4 = 4 * (my_lane() >> 4);
@@ -696,13 +721,13 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
     __builtin_amdgcn_sched_barrier(0);
     // ---- scores; the operands of product ub + AK are asked for before product ub, and no further ahead (the
     // registers hold no more)
-    constexpr int AH = 2, AK = KF && MT == 2 ? 1 : 2;
+    constexpr int AK = KF ? (MT == 2 ? 1 : 2) : 2;
     f4 s[MT][2] = {};
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
-    const uint8_t *kop = sm + oK + (KF ? 0 : kOp * kbuf) + 512 * n;
-    const uint8_t *kp[2] = {kop + 16 * (g ^ (n & 7)), kop + 16 * ((4 + g) ^ (n & 7))};
-    const uint8_t *sp = sm + oSC + 64 * g;
-    auto k_at = [&](int ub) { return *reinterpret_cast<const h8 *>(kp[ub & 1] + 8192 * (ub >> 3) + 128 * ((ub & 7) >> 1)); };
+    const uint8_t *kop = kbuf + 512 * n;
+    const uint32_t kx = 16 * (g ^ n);              // piece 4 b + g at (4 b + g) ^ n
+    const uint8_t *sp = kbuf + kOp + 64 * g;
+    auto k_at = [&](int ub) { return *reinterpret_cast<const h8 *>(kop + (kx ^ (64u * (ub & 3))) + 8192 * (ub >> 3) + 256 * ((ub & 7) >> 2)); };
     auto s_at = [&](int ub) { return *reinterpret_cast<const h8 *>(sp + 256 * (ub >> 3) + 16 * ((ub & 7) >> 1)); };   // two blocks
     h8 kf[AK + 1], sc = {}, sn = {};
     f4 p[MT] = {};                                 // q8_0: the last block's products, still to be scaled and added
@@ -740,7 +765,6 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));
     // ---- probabilities
-    h8 ph[MT], pl[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       if (!whole) {
@@ -771,10 +795,12 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
       l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       split_p(p, ph[mt], pl[mt]);
     }
+  };
+  auto products = [&](const uint8_t *vb) {
+    const int lane = my_lane(), n = lane & 15, g = lane >> 4;
     __builtin_amdgcn_sched_barrier(0);
-    // ---- P V
     if constexpr (VF) {
-      const uint32_t now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(sm + oLV));
+      const uint32_t now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(vb + oLV));
       if (now != lv) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -787,9 +813,9 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
         lv = now;
       }
     }
-    const uint8_t *vb = sm + oV;
     const uint32_t vp[2] = {v_piece(n, g), v_piece(16 + n, g) - 1024u};
     auto v_at = [&](int dt, int lo) { return *reinterpret_cast<const h8 *>(vb + lo * kOp + vp[dt & 1] + 1024 * dt); };
+    constexpr int AH = 2;
     h8 vh[AH + 1], vl[VF ? AH + 1 : 1];
 #pragma unroll
     for (int j = 0; j < AH; ++j) {
@@ -816,19 +842,52 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
     }
   };
 
-  for (int t = t0; t < t1; ++t) {                  // (the same count in the whole workgroup)
-    const int kbuf = (t - t0) & 1;
-    // this step's bytes have landed, and no wave reads the last one's operands any more
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // Waves 4 .. 7, which share their SIMDs with waves 0 .. 3, take P V of a step at the beginning of the next one: while
+  // one wave's scores and probabilities keep the vector unit busy, the other's products keep the matrix cores busy.
+  const bool late = w >= 4;
+  if (t0 < t1) {
+    convert(sm + oK, sm);
+    look_up(min(t0 + 1, t1 - 1));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t0 + 1 < t1) request(t0 + 1, 1);
+    there_next = there_after;
     lds_barrier();
-    there = there_next;
-    convert();
-    look_up(min(t + 1, t1 - 1));
-    lds_barrier();
-    if (t + 1 < t1) request(t + 1, kbuf ^ 1);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(t, kbuf);
   }
+  uint32_t v_last = 0, v_now = 0, v_next = kVB;    // V's operands of the last step, of this one, of the next
+  for (int t = t0; t < t1; ++t) {                  // (the same count in the whole workgroup)
+    const int b = (t - t0) & 1;
+    // (the products, a stream of matrix instructions, go on where the other wave leaves room)
+    __builtin_amdgcn_s_setprio(0);
+    if (late && t > t0) products(sm + v_last);
+    __builtin_amdgcn_s_setprio(2);
+    __builtin_amdgcn_sched_barrier(0);
+    scores(t, sm + oK + kKB * b);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    if (!late) products(sm + v_now);
+    __builtin_amdgcn_s_setprio(2);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 1 < t1) {
+      // the next step's operands, in places whose readers have passed the barrier; then, with the wave's bytes used,
+      // those of the step after it
+      convert(sm + oK + kKB * (b ^ 1), sm + v_next);
+      look_up(min(t + 2, t1 - 1));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if constexpr (KF) {
+        if (t + 2 < t1) request(t + 2, 0);
+      }
+    }
+    lds_barrier();
+    if constexpr (!KF) {                           // (fp16 K lands where this step's was read)
+      if (t + 2 < t1) request(t + 2, b);
+    }
+    there = there_next;
+    there_next = there_after;
+    v_last = v_now;
+    v_now = v_next;
+    v_next = v_next == 2 * kVB ? 0 : v_next + kVB;
+  }
+  if (late && t0 < t1) products(sm + v_last);
 
   // ---- one partial result per row
   const int64_t rows = (int64_t)a.n_q * a.nh;
@@ -855,13 +914,13 @@ __global__ __launch_bounds__(256, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 static inline int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Which kernel a call takes, by the rows of one KV head: up to 32 the stream kernel in blocks of 16, up to 64 one tile
-// of 64 rows, beyond that tiles of 128 (what each measured: see the kernels).
-enum { kTreeStream, kTree64, kTree128 };
-static int tree_kind(int64_t rows) { return rows <= 32 ? kTreeStream : rows <= 64 ? kTree64 : kTree128; }
-static int tree_rows(int kind) { return kind == kTreeStream ? 16 : kind == kTree64 ? 64 : 128; }
+// Which kernel a call takes, by the rows of one KV head: up to 32 the stream kernel in blocks of 16, up to 128 one tile
+// of 128 rows, beyond that tiles of 256 (what each measured: see the kernels).
+enum { kTreeStream, kTree128, kTree256 };
+static int tree_kind(int64_t rows) { return rows <= 32 ? kTreeStream : rows <= 128 ? kTree128 : kTree256; }
+static int tree_rows(int kind) { return kind == kTreeStream ? 16 : kind == kTree128 ? 128 : 256; }
 // workgroups that the key split aims for: as many as run at once
-constexpr int kTreeFill = 512;
+static int tree_fill(int kind) { return kind == kTreeStream ? 512 : 256; }
 
 TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   TreePlan p{};
@@ -869,14 +928,14 @@ TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   p.kind = tree_kind(rows);
   p.nrb = (int)cdiv(rows, tree_rows(p.kind));
   // at least 4 steps to a workgroup
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, kTreeFill / ((int64_t)nkv * p.nrb)));
+  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, tree_fill(p.kind) / ((int64_t)nkv * p.nrb)));
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
   return p;
 }
 
-// the largest plan of any call: 65536 rows where the keys are split (512 workgroups of 128),
+// the largest plan of any call: 65536 rows where the keys are split (256 workgroups of 256),
 // otherwise every row once
 size_t tree_workspace_bound(int nh, int nkv, size_t base) {
   (void)nkv;
@@ -889,8 +948,8 @@ static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStre
   const dim3 grid((unsigned)(cdiv((int64_t)a.nkv * a.splits, 8) * 8 * p.nrb));
   switch (p.kind) {
     case kTreeStream: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG != 0>), grid, dim3(256), 0, st, a, p.nrb); break;
-    case kTree64: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
-    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a, p.nrb); break;
+    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(512), 0, st, a, p.nrb); break;
+    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(512), 0, st, a, p.nrb); break;
   }
   return hipGetLastError();
 }
