@@ -54,9 +54,9 @@ __device__ __forceinline__ uint32_t tree_window(const TreeArgs &a, int i, int64_
 }
 
 // ------------------------------------------------------------------ joining the key ranges
-// Row r = i * nh + h by itself: 4 waves take every fourth key, a lane 4 dims. Only reached for rows whose partial
-// results are not finite, so its time (about 1 us per 30 keys) is not that of ordinary calls.
-template <int KF, int VF>
+// Row r = i * nh + h by itself: each wave takes every NWV-th key, a lane 4 dims. Only reached for rows whose partial
+// results are not finite, so its time (about 1 us per 30 keys and 4 waves) is not that of ordinary calls.
+template <int KF, int VF, int NWV>
 __device__ void tree_careful_row(const TreeArgs &a, int i, int h, float *s_o, float *s_ml, float4 &o, float &l) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hk = h / a.grp;
   const float4 qv = reinterpret_cast<const float4 *>(a.q.at(i, h))[lane];
@@ -76,7 +76,7 @@ __device__ void tree_careful_row(const TreeArgs &a, int i, int h, float *s_o, fl
       x[2] = f16_to_f32(b.y & 0xFFFFu); x[3] = f16_to_f32(b.y >> 16);
     }
   };
-  for (uint32_t k = (uint32_t)w; k < nk; k += 4) {
+  for (uint32_t k = (uint32_t)w; k < nk; k += NWV) {
     if (k >= a.pos0 && !(tree_window(a, i, k) & 1u)) continue;
     const int slot = slot_checked(a.L, a.pool_pages, k);
     if (slot < 0) continue;
@@ -110,10 +110,11 @@ __device__ void tree_careful_row(const TreeArgs &a, int i, int h, float *s_o, fl
   reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   if (lane == 0) { s_ml[2 * w] = m; s_ml[2 * w + 1] = l; }
   __syncthreads();
-  float mm = fmaxf(fmaxf(s_ml[0], s_ml[2]), fmaxf(s_ml[4], s_ml[6]));
+  float mm = -INFINITY;
+  for (int j = 0; j < NWV; ++j) mm = fmaxf(mm, s_ml[2 * j]);
   l = 0.0f;
   o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < NWV; ++j) {
     const float mj = s_ml[2 * j], lj = s_ml[2 * j + 1];
     const float f = mj == mm ? 1.0f : exp2f(mj - mm);
     const float4 t = reinterpret_cast<const float4 *>(s_o + j * kHd)[lane];
@@ -140,43 +141,51 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs &a, int i) {
   return false;
 }
 
-// One workgroup per row: wave w sums the ranges w, w + 4, .. (a lane 4 dims, kB ranges requested together), then
-// the waves' sums meet in LDS.
-template <int KF, int VF>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+// One workgroup of NWV waves per row: wave w sums the ranges w, w + NWV, .. (a lane 4 dims, 8 ranges requested
+// together), then the waves' sums meet in LDS. The launch takes as many waves as leave each 8 ranges: one row's 128
+// ranges on 4 waves took 12.4 us, a latency after the other.
+template <int KF, int VF, int NWV>
+__global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rows = (int64_t)a.n_q * a.nh, r = blockIdx.x;
   const int i = (int)(r / a.nh), h = (int)(r - (int64_t)i * a.nh);
-  __shared__ __attribute__((aligned(16))) float s_o[4 * kHd];
-  __shared__ float s_ml[8];
+  __shared__ __attribute__((aligned(16))) float s_o[NWV * kHd];
+  __shared__ float s_ml[2 * NWV];
   const float2 none = make_float2(-INFINITY, 0.0f);
   const float2 m0 = lane < a.splits ? a.ml[(int64_t)lane * rows + r] : none;
   const float2 m1 = lane + 64 < a.splits ? a.ml[(int64_t)(lane + 64) * rows + r] : none;
-  const float mm = wave_max(fmaxf(m0.x, m1.x));
-  const float f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - mm), f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - mm);
-  float l = wave_sum(m0.y * f0 + m1.y * f1);
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  constexpr int kB = 8;
-  for (int s0 = w; s0 < a.splits; s0 += 4 * kB) {
-    float4 t[kB];
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f), t[8];
+  float mm = 0.0f, f0 = 0.0f, f1 = 0.0f, l = 0.0f;
+  for (int s0 = w; s0 < a.splits; s0 += 8 * NWV) {
 #pragma unroll
-    for (int j = 0; j < kB; ++j)
-      t[j] = reinterpret_cast<const float4 *>(a.part + ((int64_t)min(s0 + 4 * j, a.splits - 1) * rows + r) * kHd)[lane];
+    for (int j = 0; j < 8; ++j)
+      if (s0 + j * NWV < a.splits) t[j] = reinterpret_cast<const float4 *>(a.part + ((int64_t)(s0 + j * NWV) * rows + r) * kHd)[lane];
+    if (s0 == w) {
+      mm = wave_max(fmaxf(m0.x, m1.x));
+      f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - mm);
+      f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - mm);
+    }
 #pragma unroll
-    for (int j = 0; j < kB; ++j) {
-      const int s = s0 + 4 * j;
+    for (int j = 0; j < 8; ++j) {
+      const int s = s0 + j * NWV;
       if (s >= a.splits) break;
       const float f = __shfl(s < 64 ? f0 : f1, s & 63);
       o.x = fmaf(t[j].x, f, o.x); o.y = fmaf(t[j].y, f, o.y); o.z = fmaf(t[j].z, f, o.z); o.w = fmaf(t[j].w, f, o.w);
     }
   }
+  if (w >= a.splits) {                             // (a wave without ranges: the row's sum all the same)
+    mm = wave_max(fmaxf(m0.x, m1.x));
+    f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - mm);
+    f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - mm);
+  }
+  l = wave_sum(m0.y * f0 + m1.y * f1);
   reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = o;
   __syncthreads();
   o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float4 t = reinterpret_cast<const float4 *>(s_o + j * kHd)[lane];
-    o.x += t.x; o.y += t.y; o.z += t.z; o.w += t.w;
+  for (int j = 0; j < NWV; ++j) {
+    const float4 x = reinterpret_cast<const float4 *>(s_o + j * kHd)[lane];
+    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
   }
   __syncthreads();
   // (every wave holds the whole row: the decision is the workgroup's)
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   bool empty = false;
   if (!fine) {
     empty = !tree_sees(a, i);
-    if (!empty) tree_careful_row<KF, VF>(a, i, h, s_o, s_ml, o, l);
+    if (!empty) tree_careful_row<KF, VF, NWV>(a, i, h, s_o, s_ml, o, l);
   }
   if (w == 0) {
     const float4 v = empty ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
@@ -218,304 +227,11 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
   for (int j = 0; j < 8; ++j) pl[j] = (_Float16)__builtin_fmaf((float)ph[j], -1.0f, p[j]);
 }
 
-// ------------------------------------------------------------------ few rows: keys straight into registers
-// A workgroup holds 16 rows; each of its 4 waves streams a key range of its own, 32 keys a step, without LDS or
-// barriers until the ranges are joined. Bound by the memory: a wave has a step's K and V (17 KB in q8_0) in flight.
-//
-// Scores are computed transposed, S^T = K Q^T: lane (n, g) = (lane % 16, lane / 16) then holds keys 4 g .. 4 g + 3 of
-// a 16-key tile for row n, which is P^T's operand of O^T = V^T P^T as it stands if slot (g, j) of the 32-key
-// contraction stands for key 4 g + j (j < 4) or 16 + 4 g + j - 4, for both operands. V's operand wants one dim of 8
-// keys per lane: lane (m, g) loads its 8 keys' bytes of dims 16 m .. 16 m + 15 (whole 256-byte rows per 16 lanes), and
-// product dt takes byte dt of each, so that row m of product dt is dim 16 m + dt (fp16 V: 8 dims per load, dim
-// 128 (dt / 8) + 8 m + dt % 8). No transposition goes through LDS.
-template <int VF>
-__device__ __forceinline__ int tree_dim(int dt, int m) {
-  return VF == BKV_Q8_0 ? 16 * m + dt : 128 * (dt >> 3) + 8 * m + (dt & 7);
-}
-
-// fp16 pair (low half of a's selected half or byte, then b's)
-template <int SEL>
-__device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
-  return __builtin_amdgcn_perm(hi, lo, 0x0C000C00u | (uint32_t)SEL | ((uint32_t)(SEL + 4) << 16));
-}
-
-// keys 4 g + i of the tile for all lanes of row group g: lane (r, g) holds the scales of key 4 g + r % 4
-template <int I>
-__device__ __forceinline__ uint32_t row_lane(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x150 + I, 0xF, 0xF, false);
-}
-
-template <int KF, int VF, bool PG>
-__global__ __launch_bounds__(256, KF == BKV_F16 && VF == BKV_F16 ? 1 : 2) void tree_stream_kernel(TreeArgs a, int nrb) {
-  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF);
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  // workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there
-  const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
-  if (unit >= a.nkv * a.splits) return;
-  const int hk = unit / a.splits, split = unit - hk * a.splits;
-  const int R = a.n_q * a.grp, r = min(16 * rb + n, R - 1), tok = r / a.grp, hq = hk * a.grp + r - tok * a.grp;
-  const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
-  const int64_t steps = (nk + kTreeKeys - 1) / kTreeKeys, wi = split * 4 + w, nw = a.splits * 4;
-  const int64_t t0 = steps * wi / nw, t1 = steps * (wi + 1) / nw;
-
-  h8 qh[8];                                        // row n, dims 32 b + 8 g ..
-  {
-    const float *q = a.q.at(tok, hq) + 8 * g;
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * b), y = *reinterpret_cast<const float4 *>(q + 32 * b + 4);
-      qh[b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
-    }
-  }
-  f4 o[16] = {};
-  float m = -INFINITY, l = 0.0f;                   // m: the reference less kPScale
-  int ve = 100;                                    // q8_0 V: the outputs are in units of 2^-ve (100: none yet)
-  uint4 kr[2][KF ? 4 : 8], ks[2], vr[8][VF ? 1 : 2];
-  uint32_t vs[4];
-  const size_t krow = (size_t)a.nkv * KRB, vrow = (size_t)a.nkv * VRB, srow = (size_t)a.nkv * kScaleRowBytes;
-  const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
-  const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
-
-  // lane l's slot of key kb + l % 32 (keys from nk on: the last one's), -1 outside the pool
-  auto slots = [&](int64_t kb) { return slot_checked(a.L, a.pool_pages, (uint32_t)min(kb + (lane & 31), (int64_t)nk - 1)); };
-  auto slot = [&](int sl, int64_t kb, int j) -> int64_t {
-    if constexpr (PG) return max(__shfl(sl, j), 0);
-    else return min(kb + j, (int64_t)nk - 1);
-  };
-  auto load_k = [&](int64_t kb, int sl) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint8_t *p = kd + (size_t)slot(sl, kb, 16 * t + n) * krow;
-      if constexpr (KF) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint2 x = *reinterpret_cast<const uint2 *>(p + 64 * b + 8 * g), y = *reinterpret_cast<const uint2 *>(p + 64 * b + 32 + 8 * g);
-          kr[t][b] = make_uint4(x.x, x.y, y.x, y.y);
-        }
-        ks[t] = *reinterpret_cast<const uint4 *>(ksc + (size_t)slot(sl, kb, 16 * t + 4 * g + (n & 3)) * srow);
-      } else {
-#pragma unroll
-        for (int b = 0; b < 8; ++b) kr[t][b] = *reinterpret_cast<const uint4 *>(p + 64 * b + 16 * g);
-      }
-    }
-  };
-  auto load_v = [&](int64_t kb, int sl) {
-    uint32_t s[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const size_t at = (size_t)slot(sl, kb, (j & 4) * 4 + 4 * g + (j & 3));
-      const uint8_t *p = vd + at * vrow + 16 * n;
-      vr[j][0] = *reinterpret_cast<const uint4 *>(p);
-      if constexpr (VF) s[j] = *reinterpret_cast<const uint16_t *>(vsc + at * srow + 2 * (n >> 1));
-      else vr[j][VF ? 0 : 1] = *reinterpret_cast<const uint4 *>(p + 256);
-    }
-    if constexpr (VF)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vs[j] = s[2 * j] | (s[2 * j + 1] << 16);
-  };
-
-  int sl = 0;
-  if (t0 < t1) {
-    if constexpr (PG) sl = slots(t0 * kTreeKeys);
-    load_k(t0 * kTreeKeys, sl);
-    load_v(t0 * kTreeKeys, sl);
-  }
-#pragma unroll 1
-  for (int64_t t = t0; t < t1; ++t) {
-    const int64_t kb = t * kTreeKeys;
-    const int64_t kn = min(t + 1, t1 - 1) * kTreeKeys;
-    // ---- scores
-    f4 s[2] = {};
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if constexpr (KF) {
-        const uint32_t sw[4] = {ks[u].x, ks[u].y, ks[u].z, ks[u].w};
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint32_t x[4] = {kr[u][b].x ^ 0x80808080u, kr[u][b].y ^ 0x80808080u, kr[u][b].z ^ 0x80808080u, kr[u][b].w ^ 0x80808080u};
-          const uint32_t d[4] = {row_lane<0>(sw[b]), row_lane<1>(sw[b]), row_lane<2>(sw[b]), row_lane<3>(sw[b])};
-#pragma unroll
-          for (int hb = 0; hb < 2; ++hb) {
-            uint4 kv;
-            kv.x = as_u(bytes_h2<0x04010400u>(x[2 * hb])); kv.y = as_u(bytes_h2<0x04030402u>(x[2 * hb]));
-            kv.z = as_u(bytes_h2<0x04010400u>(x[2 * hb + 1])); kv.w = as_u(bytes_h2<0x04030402u>(x[2 * hb + 1]));
-            const f4 p = mfma16(__builtin_bit_cast(h8, kv), qh[2 * b + hb], f4{});
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[u][i] = __builtin_fmaf(p[i], (float)__builtin_bit_cast(_Float16, (uint16_t)(d[i] >> (16 * hb))), s[u][i]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int b = 0; b < 8; ++b) s[u] = mfma16(__builtin_bit_cast(h8, kr[u][b]), qh[b], s[u]);
-      }
-    }
-    uint32_t there = ~0u;                          // keys whose page is in the pool
-    if constexpr (PG) there = (uint32_t)__ballot(sl >= 0);
-    int sn = 0;
-    if constexpr (PG) sn = slots(kn);
-    load_k(kn, sn);
-    // ---- probabilities
-    uint32_t win = there;
-    if (kb + kTreeKeys > a.pos0) win &= tree_window(a, tok, kb);
-    win >>= 4 * g;                                 // bit i: key 4 g + i of tile 0, bit 16 + i: of tile 1
-    float x[8], top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = s[j >> 2][j & 3] * a.scale2;
-      if (!((win >> ((j & 4) * 4 + (j & 3))) & 1u)) x[j] = -INFINITY;
-      top = fmaxf(top, x[j]);
-    }
-    if (__any(top > m + (kLift + kPScale))) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top - kPScale);
-      const float f = mn == m ? 1.0f : exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int dt = 0; dt < 16; ++dt) o[dt] *= f;
-    }
-    h8 ph, pl;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool seen = (win >> ((j & 4) * 4 + (j & 3))) & 1u;
-      const float p = seen ? __builtin_amdgcn_exp2f(x[j] - m) : 0.0f;
-      l += p;
-      ph[j] = (_Float16)p;
-      pl[j] = (_Float16)(p - (float)ph[j]);
-    }
-    // ---- V
-    if constexpr (VF) {
-      // the factor 2^ve that brings the largest scale to [2^7, 2^8) of the keys so far
-      uint32_t b = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b = max(b, max(vs[j] & 0x7FFFu, (vs[j] >> 16) & 0x7FFFu));
-      const int e = b ? 7 + 15 - (int)max(b >> 10, 1u) : 15;
-      if (__any(e < ve)) {
-        int en = min(e, 15);
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) en = min(en, __shfl_xor(en, k));
-        if (ve != 100) {
-          const float f = __builtin_ldexpf(1.0f, en - ve);
-#pragma unroll
-          for (int dt = 0; dt < 16; ++dt) o[dt] *= f;
-        }
-        ve = en;
-      }
-      const _Float16 vf = (_Float16)__builtin_ldexpf(1.0f, ve);
-      h2 d[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] = as_h2(vs[j]) * h2{vf, vf};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t wv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) wv[j] = (&vr[j][0].x)[c];
-#pragma unroll
-        for (int by = 0; by < 4; ++by) {
-          uint32_t ah[4], al[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = wv[2 * j], hi = wv[2 * j + 1];
-            const uint32_t pb = by == 0 ? pair_bytes<0>(lo, hi) : by == 1 ? pair_bytes<1>(lo, hi) : by == 2 ? pair_bytes<2>(lo, hi) : pair_bytes<3>(lo, hi);
-            h2 h, lw;
-            split_prod(as_h2(pb ^ 0x64806480u) - h2{(_Float16)1152.0f, (_Float16)1152.0f}, d[j], h, lw);
-            ah[j] = as_u(h);
-            al[j] = as_u(lw);
-          }
-          const h8 vh = __builtin_bit_cast(h8, make_uint4(ah[0], ah[1], ah[2], ah[3]));
-          const h8 vl = __builtin_bit_cast(h8, make_uint4(al[0], al[1], al[2], al[3]));
-          f4 &z = o[4 * c + by];
-          z = mfma16(vl, ph, z);
-          z = mfma16(vh, pl, z);
-          z = mfma16(vh, ph, z);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t wv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) wv[j] = (&vr[j][VF ? 0 : c >> 2].x)[c & 3];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t av[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) av[j] = __builtin_amdgcn_perm(wv[2 * j + 1], wv[2 * j], hf ? 0x07060302u : 0x05040100u);
-          const h8 vh = __builtin_bit_cast(h8, make_uint4(av[0], av[1], av[2], av[3]));
-          f4 &z = o[2 * c + hf];
-          z = mfma16(vh, pl, z);
-          z = mfma16(vh, ph, z);
-        }
-      }
-    }
-    load_v(kn, sn);
-    sl = sn;
-  }
-
-  // ---- the 4 ranges joined, one partial result per row and workgroup
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  constexpr int kOS = kHd + 4;
-  __shared__ __attribute__((aligned(16))) float s_o[4][16][kOS];
-  __shared__ float s_m[4][16], s_l[4][16];
-  if (g == 0) { s_m[w][n] = m; s_l[w][n] = l; }
-  __syncthreads();
-  const float mm = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
-  const float f = m == -INFINITY ? 0.0f : exp2f(m - mm), fo = VF && ve != 100 ? __builtin_ldexpf(f, -ve) : f;
-#pragma unroll
-  for (int dt = 0; dt < 16; ++dt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s_o[w][n][tree_dim<VF>(dt, 4 * g + i)] = o[dt][i] * fo;
-  __syncthreads();
-  const int row = threadIdx.x >> 4, c = threadIdx.x & 15, rr = 16 * rb + row;
-  if (rr < R) {
-    const int64_t rows = (int64_t)a.n_q * a.nh;
-    const int ti = rr / a.grp;
-    const int64_t at = (int64_t)split * rows + (int64_t)ti * a.nh + hk * a.grp + rr - ti * a.grp;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 t = *reinterpret_cast<const float4 *>(&s_o[j][row][4 * c + 64 * k]);
-        v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
-      }
-      *reinterpret_cast<float4 *>(a.part + at * kHd + 4 * c + 64 * k) = v;
-    }
-    if (c == 0) {
-      const float mr = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-      float lr = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) lr += s_m[j][row] == -INFINITY ? s_l[j][row] : s_l[j][row] * exp2f(s_m[j][row] - mr);
-      a.ml[at] = make_float2(mr, lr);
-    }
-  }
-}
-
-// ------------------------------------------------------------------ many rows: key tiles in LDS
-// A workgroup of 4 waves holds 64 MT rows, each wave 16 MT of them with all 256 outputs in registers, and steps
-// through its key range 32 keys at a time. A step's cache bytes are loaded straight into LDS while the step before it
-// is computed, and turned once into the products' operands for all of the workgroup's rows: K's bytes into fp16
-// (fp16 K needs nothing: its pieces land where they are wanted), V transposed, so that a lane's 8 keys of one dim are
-// 16 bytes, as vh (and vl for q8_0). S^T and O^T are formed as in the kernel above, so P never leaves its lane.
-//
-// LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
-// and 16 + 4 g .. 16 + 4 g + 3) at 8 (d / 2) + ((4 (d % 2) + g) ^ kx(d)), kx chosen so that both the 8 dims next to
-// one another that a read takes and the 8 dims 4 apart that a write takes lie in different banks.
-//
 // q8_0 scales: vh and vl keep 19 bits for scales up to 2^-1 and down to 2^-17 or so when they are taken times 2^9; a
-// step with a larger one in a wave's 64 dims takes 2^1 or 2^-7 there (its level), and the outputs are brought to the
-// step's unit. (Smaller values end as outputs below kTiny.)
-__device__ __forceinline__ constexpr int level_exp(int lv) { return 9 - 8 * lv; }
+// step with a larger one takes 2^1 or 2^-7 (its level), and the outputs are brought to the step's unit. (Smaller
+// values end as outputs below kTiny.)
 // the level of the largest of fp16 scales (bits, sign cleared): above 2^-1, above 2^7
 __device__ __forceinline__ int scale_level(uint32_t top) { return (top > 0x3800u) + (top > 0x5800u); }
-
-__device__ __forceinline__ uint32_t v_piece(int d, int g) {
-  const int kx = ((d >> 4) & 1) << 2 | ((d >> 2) & 1) << 1 | (((d >> 1) ^ (d >> 3)) & 1);
-  return (uint32_t)(128 * (d >> 1) + 16 * ((4 * (d & 1) + g) ^ kx));
-}
 
 // 16 bytes per lane from base + off into LDS at dst + 16 * lane (dst the same in all lanes), not waited for
 __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t dst) {
@@ -531,6 +247,329 @@ __device__ __forceinline__ void load4_to_lds(const uint8_t *src, uint32_t dst) {
 
 // PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
 // base for the whole workgroup); 2 any pages (a slot of its own for every key)
+// fp16 pair: the SEL-th byte of lo in the low half and of hi in the high one
+template <int SEL>
+__device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x0C000C00u | (uint32_t)SEL | ((uint32_t)(SEL + 4) << 16));
+}
+
+// ------------------------------------------------------------------ few rows: every wave a key range of its own
+// A workgroup holds 16 MT rows; each of its 4 waves streams a key range, 32 keys a step, without barriers until the
+// ranges are joined. Bound by the memory: a step's K is asked for as soon as the last one's has been read, its V
+// likewise, so that a wave has nearly a whole step (17 KB in q8_0) on its way into its own part of LDS at all times.
+//
+// Scores are computed transposed, S^T = K Q^T: lane (n, g) = (lane % 16, lane / 16) then holds keys 4 g .. 4 g + 3 of
+// a 16-key tile for row n, which is P^T's operand of O^T = V^T P^T as it stands if slot (g, j) of the 32-key
+// contraction stands for key 4 g + j (j < 4) or 16 + 4 g + j - 4, for both operands. V's operand wants one dim of 8
+// keys per lane: lane (m, g) reads its 8 keys' bytes of dims 16 m .. 16 m + 15, and product dt takes byte dt of each,
+// so that row m of product dt is dim 16 m + dt (fp16 V: 8 dims per read, dim 128 (dt / 8) + 8 m + dt % 8).
+// LDS: V rows as they are; 16-byte piece c of K's row k at place c ^ k % 16, so that 16 rows' pieces lie in 16 banks'
+// widths (the lanes of the load ask for the pieces in that order).
+template <int VF>
+__device__ __forceinline__ int tree_dim(int dt, int m) {
+  return VF == BKV_Q8_0 ? 16 * m + dt : 128 * (dt >> 3) + 8 * m + (dt & 7);
+}
+
+template <int KF, int VF, int PG, int MT>
+__global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 2 : 1) void tree_stream_kernel(TreeArgs a, int nrb) {
+  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT;
+  constexpr uint32_t oV = kTreeKeys * KRB, oSK = oV + kTreeKeys * VRB, oSV = oSK + (KF ? 512 : 0), kWave = oSV + (VF ? 512 : 0);
+  constexpr int kOS = kHd + 4;                     // a row of the join
+  constexpr uint32_t kJoin = 4 * 16 * kOS * 4;
+  __shared__ __attribute__((aligned(128))) uint8_t sm[4 * kWave > kJoin ? 4 * kWave : kJoin];
+  __shared__ float s_m[4][16], s_l[4][16];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  // workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there
+  const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
+  if (unit >= a.nkv * a.splits) return;
+  const int hk = unit / a.splits, split = unit - hk * a.splits;
+  const int R = a.n_q * a.grp;
+  const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
+  const int steps = (int)((nk + kTreeKeys - 1) / kTreeKeys), wi = split * 4 + w, nw = a.splits * 4;
+  const int t0 = (int)((int64_t)steps * wi / nw), t1 = (int)((int64_t)steps * (wi + 1) / nw);
+  const uint32_t krow = (uint32_t)a.nkv * KRB, vrow = (uint32_t)a.nkv * VRB, srow = (uint32_t)a.nkv * kScaleRowBytes;
+  const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
+  const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
+  uint8_t *const my = sm + kWave * w;
+  const uint32_t my0 = lds_addr(sm) + kWave * w;
+
+  // ---- a step's bytes on their way
+  uint32_t there = ~0u, there_next = ~0u;          // keys whose pages are in the pool: this step's, the next's
+  int sl = 0;                                      // PG 2: the slot of key lane % 32 of the step asked for
+  size_t s0 = 0;
+  auto look_up = [&](int t) {
+    const uint32_t kb = (uint32_t)t * kTreeKeys;
+    s0 = kb;
+    if constexpr (PG == 1) {
+      const int first = __builtin_amdgcn_readfirstlane(slot_checked(a.L, a.pool_pages, kb));
+      there_next = first >= 0 ? ~0u : 0u;
+      s0 = (size_t)max(first, 0);
+    }
+    if constexpr (PG == 2) {
+      sl = slot_checked(a.L, a.pool_pages, min(kb + ((uint32_t)lane & 31), nk - 1));
+      there_next = (uint32_t)__ballot(sl >= 0);
+    }
+  };
+  // (offsets within a step are 32 bits: 31 rows)
+  auto take = [&](int t, const uint8_t *base, int key, uint32_t row, uint32_t col, uint32_t dst) {
+    if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, dst);
+    else load_to_lds(base + s0 * row, min((uint32_t)key, nk - 1 - (uint32_t)t * kTreeKeys) * row + col, dst);
+  };
+  constexpr int NK = KF ? 9 : 16, NV = VF ? 9 : 16;   // loads of a step's K, of its V
+  auto scales = [&](int t, const uint8_t *base, uint32_t dst) {
+    const uint32_t key = (uint32_t)lane & 31;
+    const uint8_t *src = PG == 2 ? base + (size_t)max(__shfl(sl, (int)key), 0) * srow : base + s0 * srow + min(key, nk - 1 - (uint32_t)t * kTreeKeys) * srow;
+    if (lane < 32) load_to_lds(src, dst);
+  };
+  auto request_k = [&](int t) {
+    constexpr int LR = KF ? 16 : 32;               // lanes of a row
+#pragma unroll
+    for (int u = 0; u < 32 * LR / 64; ++u) {
+      const int key = (64 / LR) * u + lane / LR;
+      take(t, kd, key, krow, 16 * ((lane % LR) ^ (key & 15)), my0 + 1024 * u);
+    }
+    if constexpr (KF) scales(t, ksc, my0 + oSK);
+  };
+  auto request_v = [&](int t) {
+    constexpr int LR = VF ? 16 : 32;
+#pragma unroll
+    for (int u = 0; u < 32 * LR / 64; ++u) take(t, vd, (64 / LR) * u + lane / LR, vrow, 16 * (lane % LR), my0 + oV + 1024 * u);
+    if constexpr (VF) scales(t, vsc, my0 + oSV);
+  };
+  if (t0 < t1) {
+    look_up(t0);
+    request_k(t0);
+    request_v(t0);
+  }
+
+  int tok[MT];
+  h8 qh[MT][8];                                    // row 16 mt + n, dims 32 b + 8 g ..
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = min(RB * rb + 16 * mt + n, R - 1);
+    tok[mt] = r / a.grp;
+    const float *q = a.q.at(tok[mt], hk * a.grp + r - tok[mt] * a.grp) + 8 * g;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * b), y = *reinterpret_cast<const float4 *>(q + 32 * b + 4);
+      qh[mt][b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
+    }
+  }
+  f4 o[MT][16] = {};
+  float m[MT], l[MT];                              // m: the reference less kPScale
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
+  int lv = 0;                                      // the outputs' level
+
+#pragma unroll 1
+  for (int t = t0; t < t1; ++t) {
+    const int64_t kb = (int64_t)t * kTreeKeys;
+    there = there_next;
+    // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
+    const bool whole = kb + kTreeKeys <= a.pos0 && (!PG || there == ~0u);
+    uint32_t win[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) win[mt] = (whole ? ~0u : kb + kTreeKeys > a.pos0 ? there & tree_window(a, tok[mt], kb) : there) >> (4 * g);
+    // ---- scores
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV) : "memory");   // (this step's V may still be on its way)
+    f4 s[MT][2] = {};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (KF) {
+        uint4 sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] = *reinterpret_cast<const uint4 *>(my + oSK + 16 * (16 * u + 4 * g + i));
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const uint2 r = *reinterpret_cast<const uint2 *>(my + KRB * (16 * u + n) + 16 * ((2 * b + (g >> 1)) ^ n) + 8 * (g & 1));
+          const uint32_t x = r.x ^ 0x80808080u, y = r.y ^ 0x80808080u;
+          const uint4 kv = make_uint4(as_u(bytes_h2<0x04010400u>(x)), as_u(bytes_h2<0x04030402u>(x)), as_u(bytes_h2<0x04010400u>(y)), as_u(bytes_h2<0x04030402u>(y)));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const f4 z = mfma16(__builtin_bit_cast(h8, kv), qh[mt][b], f4{});
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[mt][u][i] = __builtin_fmaf(z[i], (float)__builtin_bit_cast(_Float16, (uint16_t)((&sc[i].x)[b >> 1] >> (16 * (b & 1)))), s[mt][u][i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const h8 kf = *reinterpret_cast<const h8 *>(my + KRB * (16 * u + n) + 16 * ((4 * b + g) ^ n));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) s[mt][u] = mfma16(kf, qh[mt][b], s[mt][u]);
+        }
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + 1 < t1) {
+      look_up(t + 1);
+      request_k(t + 1);
+    }
+    // ---- probabilities
+    h8 ph[MT], pl[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) s[mt][j >> 2][j & 3] = -INFINITY;
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
+                        fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3]))) * a.scale2;
+      if (__any(top > m[mt] + (kLift + kPScale))) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float mn = fmaxf(m[mt], top - kPScale);
+        const float f = mn == m[mt] ? 1.0f : exp2f(m[mt] - mn);
+        m[mt] = mn;
+        l[mt] *= f;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) o[mt][dt] *= f;
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][j >> 2][j & 3], a.scale2, -m[mt]));
+      if (!whole) {                                // (where nothing was seen yet, -Inf - -Inf)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) p[j] = 0.0f;
+      }
+      l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      split_p(p, ph[mt], pl[mt]);
+    }
+    // ---- P V
+    if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK) : "memory");   // (the next step's K may still be on its way)
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint8_t *vp = my + oV + 16 * n;
+    auto key_of = [&](int j) { return (j & 4) * 4 + 4 * g + (j & 3); };
+    if constexpr (VF) {
+      uint32_t sc[8], top = 0;
+      uint4 r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sc[j] = *reinterpret_cast<const uint16_t *>(my + oSV + 16 * key_of(j) + 2 * (n >> 1));
+        r[j] = *reinterpret_cast<const uint4 *>(vp + VRB * key_of(j));
+        top = max(top, sc[j] & 0x7FFFu);
+      }
+      const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
+      const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
+      if (level != lv) {
+        const float x = __builtin_ldexpf(1.0f, 8 * (lv - level));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int dt = 0; dt < 16; ++dt) o[mt][dt] *= x;
+        lv = level;
+      }
+      h2 d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = as_h2(sc[2 * j] | (sc[2 * j + 1] << 16)) * h2{f, f};
+#pragma unroll
+      for (int dt = 0; dt < 16; ++dt) {
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = (&r[2 * j].x)[dt >> 2], hi = (&r[2 * j + 1].x)[dt >> 2];
+          const uint32_t pb = (dt & 3) == 0 ? pair_bytes<0>(lo, hi) : (dt & 3) == 1 ? pair_bytes<1>(lo, hi) : (dt & 3) == 2 ? pair_bytes<2>(lo, hi) : pair_bytes<3>(lo, hi);
+          h2 h, lw;
+          split_prod(as_h2(pb ^ 0x64806480u) - h2{(_Float16)1152.0f, (_Float16)1152.0f}, d[j], h, lw);
+          ah[j] = as_u(h);
+          al[j] = as_u(lw);
+        }
+        const h8 vh = __builtin_bit_cast(h8, make_uint4(ah[0], ah[1], ah[2], ah[3]));
+        const h8 vl = __builtin_bit_cast(h8, make_uint4(al[0], al[1], al[2], al[3]));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vl, ph[mt], o[mt][dt]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, pl[mt], o[mt][dt]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, ph[mt], o[mt][dt]);
+      }
+    } else {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint4 r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const uint4 *>(vp + VRB * key_of(j) + 256 * hf);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint32_t av[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            av[j] = __builtin_amdgcn_perm((&r[2 * j + 1].x)[e >> 1], (&r[2 * j].x)[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+          const h8 vh = __builtin_bit_cast(h8, make_uint4(av[0], av[1], av[2], av[3]));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) o[mt][8 * hf + e] = mfma16(vh, pl[mt], o[mt][8 * hf + e]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) o[mt][8 * hf + e] = mfma16(vh, ph[mt], o[mt][8 * hf + e]);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + 1 < t1) request_v(t + 1);
+  }
+
+  // ---- the 4 ranges joined, one partial result per row and workgroup
+  float *s_o = reinterpret_cast<float *>(sm);
+  const int64_t rows = (int64_t)a.n_q * a.nh;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    l[mt] += __shfl_xor(l[mt], 16);
+    l[mt] += __shfl_xor(l[mt], 32);
+    __syncthreads();                               // (the waves' own parts, or the last row tile's sums, have been read)
+    if (g == 0) { s_m[w][n] = m[mt]; s_l[w][n] = l[mt]; }
+    __syncthreads();
+    const float mm = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+    const float f = m[mt] == -INFINITY ? 0.0f : exp2f(m[mt] - mm), fo = VF ? __builtin_ldexpf(f, 8 * lv - 9) : f;
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s_o[(16 * w + n) * kOS + tree_dim<VF>(dt, 4 * g + i)] = o[mt][dt][i] * fo;
+    __syncthreads();
+    const int row = threadIdx.x >> 4, c = threadIdx.x & 15, r = RB * rb + 16 * mt + row;
+    if (r < R) {
+      const int ti = r / a.grp;
+      const int64_t at = (int64_t)split * rows + (int64_t)ti * a.nh + hk * a.grp + r - ti * a.grp;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 x = *reinterpret_cast<const float4 *>(&s_o[(16 * j + row) * kOS + 4 * c + 64 * k]);
+          v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        *reinterpret_cast<float4 *>(a.part + at * kHd + 4 * c + 64 * k) = v;
+      }
+      if (c == 0) {
+        const float mr = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+        float lr = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lr += s_m[j][row] == -INFINITY ? s_l[j][row] : s_l[j][row] * exp2f(s_m[j][row] - mr);
+        a.ml[at] = make_float2(mr, lr);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ many rows: key tiles in LDS
+// A workgroup of 4 waves holds 64 MT rows, each wave 16 MT of them with all 256 outputs in registers, and steps
+// through its key range 32 keys at a time. A step's cache bytes are loaded straight into LDS while the step before it
+// is computed, and turned once into the products' operands for all of the workgroup's rows: K's bytes into fp16
+// (fp16 K needs nothing: its pieces land where they are wanted), V transposed, so that a lane's 8 keys of one dim are
+// 16 bytes, as vh (and vl for q8_0). S^T and O^T are formed as in the kernel above, so P never leaves its lane.
+//
+// LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
+// and 16 + 4 g .. 16 + 4 g + 3) at 8 (d / 2) + ((4 (d % 2) + g) ^ kx(d)), kx chosen so that both the 8 dims next to
+// one another that a read takes and the 8 dims 4 apart that a write takes lie in different banks.
+//
+__device__ __forceinline__ uint32_t v_piece(int d, int g) {
+  const int kx = ((d >> 4) & 1) << 2 | ((d >> 2) & 1) << 1 | (((d >> 1) ^ (d >> 3)) & 1);
+  return (uint32_t)(128 * (d >> 1) + 16 * ((4 * (d & 1) + g) ^ kx));
+}
+
 template <int KF, int VF, int PG, int MT>
 __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) {
   constexpr int NW = 8, KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT * NW;
@@ -616,20 +655,31 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 
   if (t0 < t1) {
     look_up(t0);
-    request(t0, 0);
+    request(t0, 1);
     there = there_after;
   }
   h8 qh[MT][8];
   auto token_of = [&](int mt) { return min(RB * rb + 16 * MT * w + 16 * mt + (my_lane() & 15), R - 1) / a.grp; };
+  // the rows of Q, whole rows at a time (a row's pieces lane by lane would ask for each line four times), to fp16 and
+  // through LDS, 8 KB of the operands' place per wave, to the lanes that want them; pieces as K's
+  static_assert(oRV >= 8 * 8192 && (KF || oK + kKB >= 8 * 8192), "the rows end before the bytes that are on their way");
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int r = min(RB * rb + 16 * MT * w + 16 * mt + n, R - 1), tok = r / a.grp;
-    const float *q = a.q.at(tok, hk * a.grp + r - tok * a.grp) + 8 * g;
+    float4 x[16];
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * b), y = *reinterpret_cast<const float4 *>(q + 32 * b + 4);
-      qh[mt][b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
+    for (int j = 0; j < 16; ++j) {
+      const int r = min(RB * rb + 16 * MT * w + 16 * mt + j, R - 1), tok = r / a.grp;      // (the same in all lanes)
+      x[j] = reinterpret_cast<const float4 *>(a.q.at(tok, hk * a.grp + r - tok * a.grp))[lane];
     }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const h2 lo = {(_Float16)x[j].x, (_Float16)x[j].y}, hi = {(_Float16)x[j].z, (_Float16)x[j].w};
+      *reinterpret_cast<uint2 *>(sm + 8192 * w + 512 * j + 16 * ((lane >> 1) ^ j) + 8 * (lane & 1)) = make_uint2(as_u(lo), as_u(hi));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int b = 0; b < 8; ++b) qh[mt][b] = *reinterpret_cast<const h8 *>(sm + 8192 * w + 512 * n + 16 * ((4 * b + g) ^ n));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   f4 o[MT][16] = {};
   float m[MT], l[MT];
@@ -844,27 +894,28 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 
   // Waves 4 .. 7, which share their SIMDs with waves 0 .. 3, take P V of a step at the beginning of the next one: while
   // one wave's scores and probabilities keep the vector unit busy, the other's products keep the matrix cores busy.
-  const bool late = w >= 4;
+  const bool late = w >= 4, works = RB * rb + 16 * MT * w < R;   // (a wave whose rows are all past the last only brings bytes)
+  lds_barrier();                                   // (every wave has its rows)
   if (t0 < t1) {
-    convert(sm + oK, sm);
+    convert(sm + oK + kKB, sm);
     look_up(min(t0 + 1, t1 - 1));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (t0 + 1 < t1) request(t0 + 1, 1);
+    if (t0 + 1 < t1) request(t0 + 1, 0);
     there_next = there_after;
     lds_barrier();
   }
   uint32_t v_last = 0, v_now = 0, v_next = kVB;    // V's operands of the last step, of this one, of the next
   for (int t = t0; t < t1; ++t) {                  // (the same count in the whole workgroup)
-    const int b = (t - t0) & 1;
+    const int b = (t - t0 + 1) & 1;              // (the first step's K lies in the second place, clear of the rows)
     // (the products, a stream of matrix instructions, go on where the other wave leaves room)
     __builtin_amdgcn_s_setprio(0);
-    if (late && t > t0) products(sm + v_last);
+    if (works && late && t > t0) products(sm + v_last);
     __builtin_amdgcn_s_setprio(2);
     __builtin_amdgcn_sched_barrier(0);
-    scores(t, sm + oK + kKB * b);
+    if (works) scores(t, sm + oK + kKB * b);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
-    if (!late) products(sm + v_now);
+    if (works && !late) products(sm + v_now);
     __builtin_amdgcn_s_setprio(2);
     __builtin_amdgcn_sched_barrier(0);
     if (t + 1 < t1) {
@@ -887,7 +938,7 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
     v_now = v_next;
     v_next = v_next == 2 * kVB ? 0 : v_next + kVB;
   }
-  if (late && t0 < t1) products(sm + v_last);
+  if (works && late && t0 < t1) products(sm + v_last);
 
   // ---- one partial result per row
   const int64_t rows = (int64_t)a.n_q * a.nh;
@@ -914,21 +965,21 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 static inline int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Which kernel a call takes, by the rows of one KV head: up to 32 the stream kernel in blocks of 16, up to 128 one tile
-// of 128 rows, beyond that tiles of 256 (what each measured: see the kernels).
-enum { kTreeStream, kTree128, kTree256 };
-static int tree_kind(int64_t rows) { return rows <= 32 ? kTreeStream : rows <= 128 ? kTree128 : kTree256; }
-static int tree_rows(int kind) { return kind == kTreeStream ? 16 : kind == kTree128 ? 128 : 256; }
+// Which kernel a call takes, by the rows of one KV head: the stream kernel with 16 or 32 rows, up to 128 one tile of
+// 128 rows, beyond that tiles of 256 (what each measured: see the kernels).
+enum { kTree16, kTree32, kTree128, kTree256 };
+static int tree_kind(int64_t rows) { return rows <= 16 ? kTree16 : rows <= 32 ? kTree32 : rows <= 128 ? kTree128 : kTree256; }
+static int tree_rows(int kind) { return kind == kTree16 ? 16 : kind == kTree32 ? 32 : kind == kTree128 ? 128 : 256; }
 // workgroups that the key split aims for: as many as run at once
-static int tree_fill(int kind) { return kind == kTreeStream ? 512 : 256; }
+static int tree_fill(int kind, int kfmt, int vfmt) { return kind == kTree16 && kfmt == BKV_Q8_0 && vfmt == BKV_Q8_0 ? 512 : 256; }
 
-TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
+TreePlan plan_tree(int nh, int nkv, int kfmt, int vfmt, int64_t pos0, int n_q, size_t base) {
   TreePlan p{};
   const int64_t rows = (int64_t)n_q * (nh / nkv), steps = cdiv(pos0 + n_q, kTreeKeys);
   p.kind = tree_kind(rows);
   p.nrb = (int)cdiv(rows, tree_rows(p.kind));
-  // at least 4 steps to a workgroup
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, cdiv(steps, 4)), std::max<int64_t>(1, tree_fill(p.kind) / ((int64_t)nkv * p.nrb)));
+  // a wave of the stream kernel takes a step at least, a workgroup of the tiles too
+  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, p.kind <= kTree32 ? cdiv(steps, 4) : steps), std::max<int64_t>(1, tree_fill(p.kind, kfmt, vfmt) / ((int64_t)nkv * p.nrb)));
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
@@ -947,7 +998,8 @@ template <int KF, int VF, int PG>
 static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStream_t st) {
   const dim3 grid((unsigned)(cdiv((int64_t)a.nkv * a.splits, 8) * 8 * p.nrb));
   switch (p.kind) {
-    case kTreeStream: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG != 0>), grid, dim3(256), 0, st, a, p.nrb); break;
+    case kTree16: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
+    case kTree32: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a, p.nrb); break;
     case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(512), 0, st, a, p.nrb); break;
     default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(512), 0, st, a, p.nrb); break;
   }
@@ -960,7 +1012,11 @@ hipError_t launch_tree(const TreeArgs &a, const TreePlan &p, int kf, int vf, hip
                          : a.L.page % kTreeKeys == 0 ? launch_tree_main<KF_, VF_, 1>(a, p, st)
                                                      : launch_tree_main<KF_, VF_, 2>(a, p, st);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((tree_merge_kernel<KF_, VF_>), dim3((unsigned)((int64_t)a.n_q * a.nh)), dim3(256), 0, st, a);
+    const dim3 rows((unsigned)((int64_t)a.n_q * a.nh));
+    if (a.splits <= 8) hipLaunchKernelGGL((tree_merge_kernel<KF_, VF_, 1>), rows, dim3(64), 0, st, a);
+    else if (a.splits <= 32) hipLaunchKernelGGL((tree_merge_kernel<KF_, VF_, 4>), rows, dim3(256), 0, st, a);
+    else if (a.splits <= 64) hipLaunchKernelGGL((tree_merge_kernel<KF_, VF_, 8>), rows, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((tree_merge_kernel<KF_, VF_, 16>), rows, dim3(1024), 0, st, a);
   });
   return hipGetLastError();
 }
