@@ -6,7 +6,6 @@ the K, V-data and V-scale sub-arenas and the three divisibility rules. KvCache o
 bkv_attn_decode / bkv_decode_step / bkv_attn_prefill_chunk on the current torch stream, the way the
 engine's attn_block (runtime_vk/bonsai_forward.h:581-645) records its three attention dispatches.
 """
-import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -18,7 +17,6 @@ from ._lib import (BKV_F16, BKV_OP_DECODE, BKV_OP_PREFILL, BKV_OP_TREE, BKV_OUT_
 
 # (private to torch, so not taken for granted)
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_NOOP = contextlib.nullcontext()
 
 
 @dataclass
@@ -269,28 +267,36 @@ class KvCache:
         return out, out_gated
 
     # ---------------------------------------------------------------- drafted tokens
-    def _here(self):
-        """The cache's device as the current one, for a call; its current stream is taken inside."""
-        return _NOOP if torch.cuda.current_device() == self._dev.index else torch.cuda.device(self._dev)
+    # These calls are a few us of a kernel, so what the host does for each is kept short: a tensor that is as the call
+    # needs it is taken with one look at each of its properties.
+    def _elsewhere(self):
+        """Whether another device than the cache's is current (its calls then run under torch.cuda.device)."""
+        return torch.cuda.current_device() != self._dev.index
+
+    def _my_stream(self):
+        """The current stream of the cache's device."""
+        if _RAW_STREAM is not None:
+            return _RAW_STREAM(self._dev.index)
+        return torch.cuda.current_stream(self._dev).cuda_stream
 
     def _rows(self, t, heads, keep):
         """fp32 [n][heads][hd] on the cache's device as a BkvRows, in place where its rows are whole (element stride 1,
         token and head strides multiples of 4 floats); anything else is copied, and `keep` holds the copy."""
-        if type(t) is not torch.Tensor or t.device != self._dev or t.dtype is not torch.float32:
-            t = torch.as_tensor(t, dtype=torch.float32, device=self._dev)
+        if type(t) is torch.Tensor and t.dtype is torch.float32 and t.device == self._dev and t.dim() == 3:
+            (n, h, d), (tok, head, one), p = t.shape, t.stride(), t.data_ptr()
+            if h == heads and d == self.hd and one == 1 and not (tok | head) & 3 and not p & 15:
+                return BkvRows(p, tok, head)
+        t = torch.as_tensor(t, dtype=torch.float32, device=self._dev)
         if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.hd:
             raise ValueError(f"rows of shape [n][{heads}][{self.hd}] are wanted, got {tuple(t.shape)}")
-        tok, head, one = t.stride()
-        if one != 1 or (tok | head) & 3 or t.data_ptr() & 15:
-            t = t.contiguous()
-            if t.data_ptr() & 15:
-                t = t.clone()
-            tok, head, one = t.stride()
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
         keep.append(t)
-        return BkvRows(t.data_ptr(), tok, head)
+        return BkvRows(t.data_ptr(), t.stride(0), t.stride(1))
 
     def _on_device(self, t, dtype, shape):
-        if t.device != self._dev or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        if t.dtype is not dtype or t.device != self._dev or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"a contiguous {dtype} tensor of shape {tuple(shape)} on {self._dev} is wanted, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
         return t
@@ -307,80 +313,98 @@ class KvCache:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call tree_workspace() before the capture: memory of a graph's own pool would not outlive it")
             need = lib().bkv_workspace_bytes(ctypes.byref(self.desc), BKV_OP_TREE, self.max_ctx)
-            self._tws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+            self._tws, self._tws_bytes = torch.empty(need, dtype=torch.uint8, device=self._dev), need
         return self._tws
 
     def attn_tree(self, layer, pos0, q, mask=None, gate=None, out=None, out_gated=None):
         """bkv_attn_tree: attention of the n drafted tokens cached at pos0.. (q [n][nh][hd]), each over the positions
         before pos0 and the drafted tokens of its mask row (int64 [n][ceil(n/64)] on the cache's device, see tree_mask;
         None: a chain). q and gate may be strided rows. Returns (out, out_gated); out_gated is None without a gate."""
-        with self._here():
-            n, keep = q.shape[0], []
-            qr = self._rows(q, self.nh, keep)
-            gr = None
-            if gate is not None:
-                gr = self._rows(gate, self.nh, keep)
-                if gate.shape[0] != n:
-                    raise ValueError(f"a gate of {n} tokens is wanted, got {gate.shape[0]}")
-                out_gated = self._out(out_gated, n)
-            elif out_gated is not None:
-                raise ValueError("out_gated without a gate")
-            out = self._out(out, n)
-            if mask is not None:
-                self._on_device(mask, torch.int64, (n, -(-n // 64)))
-            ws = self.tree_workspace()
-            check(lib().bkv_attn_tree(self.desc, layer, pos0, n, qr, self._ptr(mask), gr, out.data_ptr(), self._ptr(out_gated),
-                                      ws.data_ptr(), ws.numel(), self._stream()), "bkv_attn_tree")
+        if self._elsewhere():
+            with torch.cuda.device(self._dev):
+                return self.attn_tree(layer, pos0, q, mask, gate, out, out_gated)
+        n, keep = q.shape[0], []
+        qr, gr = self._rows(q, self.nh, keep), None
+        if gate is not None:
+            gr = self._rows(gate, self.nh, keep)
+            if gate.shape[0] != n:
+                raise ValueError(f"a gate of {n} tokens is wanted, got {gate.shape[0]}")
+            out_gated = self._out(out_gated, n)
+        elif out_gated is not None:
+            raise ValueError("out_gated without a gate")
+        out = self._out(out, n)
+        if mask is not None:
+            self._on_device(mask, torch.int64, (n, -(-n // 64)))
+        ws = self.tree_workspace()
+        rc = lib().bkv_attn_tree(self.desc, layer, pos0, n, qr, self._ptr(mask), gr, out.data_ptr(), self._ptr(out_gated),
+                                 ws.data_ptr(), self._tws_bytes, self._my_stream())
+        if rc:
+            check(rc, "bkv_attn_tree")
         return out, out_gated
 
     def rope_append(self, layer, pos0, q, k, v, rope, positions=None, qn_w=None, kn_w=None, eps=1e-6, q_out=None):
         """bkv_rope_append: q [n][nh][hd], k and v [n][nkv][hd] as the projections left them (strided rows are taken in
         place; q may be None), normed where qn_w and kn_w are given, rotated by `rope` at positions (int32 [n] on the
         cache's device; None: pos0..); K and the raw V appended at pos0... Returns the rotated Q."""
-        with self._here():
-            n, keep = k.shape[0], []
-            kr, vr = self._rows(k, self.nkv, keep), self._rows(v, self.nkv, keep)
-            qr = None
-            if q is not None:
-                qr = self._rows(q, self.nh, keep)
-                q_out = self._out(q_out, n)
-            elif q_out is not None:
-                raise ValueError("q_out without q")
-            if v.shape[0] != n or (q is not None and q.shape[0] != n):
-                raise ValueError("q, k and v of as many tokens are wanted")
-            if qn_w is not None:
-                qn_w = self._f32(qn_w, (self.hd,))
-            if kn_w is not None:
-                kn_w = self._f32(kn_w, (self.hd,))
-            if positions is not None:
-                self._on_device(positions, torch.int32, (n,))
-            check(lib().bkv_rope_append(self.desc, layer, pos0, n, rope.params, qr, kr, vr, self._ptr(qn_w), self._ptr(kn_w),
-                                        eps, self._ptr(positions), self._ptr(q_out), self._stream()), "bkv_rope_append")
+        if self._elsewhere():
+            with torch.cuda.device(self._dev):
+                return self.rope_append(layer, pos0, q, k, v, rope, positions, qn_w, kn_w, eps, q_out)
+        n, keep = k.shape[0], []
+        kr, vr, qr, qo = self._rows(k, self.nkv, keep), self._rows(v, self.nkv, keep), None, None
+        if v.shape[0] != n or (q is not None and q.shape[0] != n):
+            raise ValueError("q, k and v of as many tokens are wanted")
+        if q is not None:
+            qr = self._rows(q, self.nh, keep)
+            q_out = self._out(q_out, n)
+            qo = q_out.data_ptr()
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        qw = None if qn_w is None else self._f32(qn_w, (self.hd,))
+        kw = None if kn_w is None else self._f32(kn_w, (self.hd,))
+        if positions is not None:
+            self._on_device(positions, torch.int32, (n,))
+        rc = lib().bkv_rope_append(self.desc, layer, pos0, n, rope.params, qr, kr, vr, self._ptr(qw), self._ptr(kw), eps,
+                                   self._ptr(positions), qo, self._my_stream())
+        if rc:
+            check(rc, "bkv_rope_append")
         return q_out
 
     def read(self, layer, pos0, n, dtype=torch.float32, k_out=None, v_out=None):
         """bkv_kv_read: (K, V) of positions pos0 .. pos0 + n - 1 as values, [n][nkv][hd] of dtype (float32, float16 or
         bfloat16). k_out, v_out: tensors of that shape to write instead, of any strides that both share (a transposed
         [nkv][n][hd], say)."""
-        with self._here():
-            if k_out is None and v_out is None:
-                k_out, v_out = torch.empty((2, n, self.nkv, self.hd), dtype=dtype, device=self._dev).unbind(0)
+        if self._elsewhere():
+            with torch.cuda.device(self._dev):
+                return self.read(layer, pos0, n, dtype, k_out, v_out)
+        if k_out is None and v_out is None:
+            if dtype not in _OUT_TYPES:
+                raise ValueError(f"{dtype} is none of {list(_OUT_TYPES)}")
+            k_out, v_out = torch.empty((2, n, self.nkv, self.hd), dtype=dtype, device=self._dev).unbind(0)
+            tok, head = self.nkv * self.hd, self.hd
+        else:
             given = [t for t in (k_out, v_out) if t is not None]
-            strides = given[0].stride()
+            dtype, (tok, head, one) = given[0].dtype, given[0].stride()
             for t in given:
-                if t.device != self._dev or t.dtype not in _OUT_TYPES or t.dtype != given[0].dtype or \
-                        tuple(t.shape) != (n, self.nkv, self.hd) or t.stride() != strides or strides[2] != 1:
+                if t.device != self._dev or t.dtype not in _OUT_TYPES or t.dtype != dtype or \
+                        t.shape != (n, self.nkv, self.hd) or t.stride() != (tok, head, one) or one != 1:
                     raise ValueError(f"{n} x {self.nkv} x {self.hd} values of one type and one layout on {self._dev} are wanted")
-            check(lib().bkv_kv_read(self.desc, layer, pos0, n, _OUT_TYPES[given[0].dtype], self._ptr(k_out), self._ptr(v_out),
-                                    strides[0], strides[1], self._stream()), "bkv_kv_read")
+        rc = lib().bkv_kv_read(self.desc, layer, pos0, n, _OUT_TYPES[dtype], self._ptr(k_out), self._ptr(v_out), tok, head,
+                               self._my_stream())
+        if rc:
+            check(rc, "bkv_kv_read")
         return k_out, v_out
 
     def commit(self, pos0, n_draft, idx):
         """bkv_kv_commit: in every layer position pos0 + i takes what position pos0 + idx[i] holds (idx int32 on the
         cache's device, entries outside 0 .. n_draft - 1 leave theirs), as if all were read before any is written."""
-        with self._here():
-            self._on_device(idx, torch.int32, (idx.numel(),))
-            check(lib().bkv_kv_commit(self.desc, pos0, n_draft, idx.numel(), idx.data_ptr(), self._stream()), "bkv_kv_commit")
+        if self._elsewhere():
+            with torch.cuda.device(self._dev):
+                return self.commit(pos0, n_draft, idx)
+        n = idx.numel()
+        self._on_device(idx, torch.int32, (n,))
+        rc = lib().bkv_kv_commit(self.desc, pos0, n_draft, n, idx.data_ptr(), self._my_stream())
+        if rc:
+            check(rc, "bkv_kv_commit")
 
     def prefill_workspace(self, max_ctx):
         need = lib().bkv_workspace_bytes(ctypes.byref(self.desc), BKV_OP_PREFILL, max_ctx)

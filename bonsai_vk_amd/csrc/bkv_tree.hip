@@ -215,6 +215,12 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   }
 }
 
+// where the i-th of n nearly equal parts of x things begins (the same in all lanes)
+__device__ __forceinline__ int share(int x, int i, int n) {
+  const int q = x / n, rest = x - q * n;
+  return __builtin_amdgcn_readfirstlane(i * q + min(i, rest));
+}
+
 // 8 probabilities as ph + pl: ph cut to fp16 (two in one instruction), pl the rest, rounded (one instruction each)
 __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
 #pragma unroll
@@ -235,14 +241,14 @@ __device__ __forceinline__ int scale_level(uint32_t top) { return (top > 0x3800u
 
 // 16 bytes per lane from base + off into LDS at dst + 16 * lane (dst the same in all lanes), not waited for
 __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds(const uint8_t *src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
 
 __device__ __forceinline__ void load4_to_lds(const uint8_t *src, uint32_t dst) {   // 4 bytes per lane
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
 
 // PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
@@ -275,9 +281,9 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT;
   constexpr uint32_t oV = kTreeKeys * KRB, oSK = oV + kTreeKeys * VRB, oSV = oSK + (KF ? 512 : 0), kWave = oSV + (VF ? 512 : 0);
   constexpr int kOS = kHd + 4;                     // a row of the join
-  constexpr uint32_t kJoin = 4 * 16 * kOS * 4;
+  constexpr uint32_t kJoin = 4 * RB * kOS * 4;
   __shared__ __attribute__((aligned(128))) uint8_t sm[4 * kWave > kJoin ? 4 * kWave : kJoin];
-  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ float s_m[4][RB], s_l[4][RB];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   // workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there
   const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
@@ -286,7 +292,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
   const int steps = (int)((nk + kTreeKeys - 1) / kTreeKeys), wi = split * 4 + w, nw = a.splits * 4;
-  const int t0 = (int)((int64_t)steps * wi / nw), t1 = (int)((int64_t)steps * (wi + 1) / nw);
+  const int t0 = share(steps, wi, nw), t1 = share(steps, wi + 1, nw);
   const uint32_t krow = (uint32_t)a.nkv * KRB, vrow = (uint32_t)a.nkv * VRB, srow = (uint32_t)a.nkv * kScaleRowBytes;
   const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
   const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
@@ -336,11 +342,21 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
     for (int u = 0; u < 32 * LR / 64; ++u) take(t, vd, (64 / LR) * u + lane / LR, vrow, 16 * (lane % LR), my0 + oV + 1024 * u);
     if constexpr (VF) scales(t, vsc, my0 + oSV);
   };
+  // the workgroup's rows of Q first, 4 MT of them by each wave into the place of its V (piece c of row r at c ^ r % 16),
+  // then K; V once the rows have been read
+#pragma unroll
+  for (int j = 0; j < 4 * MT; ++j) {
+    const int row = 4 * MT * w + j, r = min(RB * rb + row, R - 1), ti = r / a.grp;
+    load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(ti, hk * a.grp + r - ti * a.grp)) + 16 * (lane ^ (row & 15)), my0 + oV + 1024 * j);
+  }
   if (t0 < t1) {
     look_up(t0);
     request_k(t0);
-    request_v(t0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
+  lds_barrier();
 
   int tok[MT];
   h8 qh[MT][8];                                    // row 16 mt + n, dims 32 b + 8 g ..
@@ -348,13 +364,16 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   for (int mt = 0; mt < MT; ++mt) {
     const int r = min(RB * rb + 16 * mt + n, R - 1);
     tok[mt] = r / a.grp;
-    const float *q = a.q.at(tok[mt], hk * a.grp + r - tok[mt] * a.grp) + 8 * g;
+    const int row = 16 * mt + n;
+    const uint8_t *q = sm + kWave * (row / (4 * MT)) + oV + 1024 * (row % (4 * MT));
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
-      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * b), y = *reinterpret_cast<const float4 *>(q + 32 * b + 4);
+      const float4 x = *reinterpret_cast<const float4 *>(q + 16 * ((8 * b + 2 * g) ^ n)), y = *reinterpret_cast<const float4 *>(q + 16 * ((8 * b + 2 * g + 1) ^ n));
       qh[mt][b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
     }
   }
+  lds_barrier();
+  if (t0 < t1) request_v(t0);
   f4 o[MT][16] = {};
   float m[MT], l[MT];                              // m: the reference less kPScale
 #pragma unroll
@@ -519,17 +538,25 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   for (int mt = 0; mt < MT; ++mt) {
     l[mt] += __shfl_xor(l[mt], 16);
     l[mt] += __shfl_xor(l[mt], 32);
-    __syncthreads();                               // (the waves' own parts, or the last row tile's sums, have been read)
-    if (g == 0) { s_m[w][n] = m[mt]; s_l[w][n] = l[mt]; }
-    __syncthreads();
-    const float mm = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+    if (g == 0) { s_m[w][16 * mt + n] = m[mt]; s_l[w][16 * mt + n] = l[mt]; }
+  }
+  __syncthreads();                                 // (and the waves' own parts have been read)
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = 16 * mt + n;
+    const float mm = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
     const float f = m[mt] == -INFINITY ? 0.0f : exp2f(m[mt] - mm), fo = VF ? __builtin_ldexpf(f, 8 * lv - 9) : f;
 #pragma unroll
-    for (int dt = 0; dt < 16; ++dt)
+    for (int dt = 0; dt < 16; dt += 4)             // (4 products' dims are neighbours)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s_o[(16 * w + n) * kOS + tree_dim<VF>(dt, 4 * g + i)] = o[mt][dt][i] * fo;
-    __syncthreads();
-    const int row = threadIdx.x >> 4, c = threadIdx.x & 15, r = RB * rb + 16 * mt + row;
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4 *>(&s_o[(RB * w + row) * kOS + tree_dim<VF>(dt, 4 * g + i)]) =
+            make_float4(o[mt][dt][i] * fo, o[mt][dt + 1][i] * fo, o[mt][dt + 2][i] * fo, o[mt][dt + 3][i] * fo);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = 16 * mt + (threadIdx.x >> 4), c = threadIdx.x & 15, r = RB * rb + row;
     if (r < R) {
       const int ti = r / a.grp;
       const int64_t at = (int64_t)split * rows + (int64_t)ti * a.nh + hk * a.grp + r - ti * a.grp;
@@ -538,7 +565,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float4 x = *reinterpret_cast<const float4 *>(&s_o[(16 * j + row) * kOS + 4 * c + 64 * k]);
+          const float4 x = *reinterpret_cast<const float4 *>(&s_o[(RB * j + row) * kOS + 4 * c + 64 * k]);
           v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
         }
         *reinterpret_cast<float4 *>(a.part + at * kHd + 4 * c + 64 * k) = v;
@@ -587,7 +614,7 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
   const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
   const int steps = (int)((nk + kTreeKeys - 1) / kTreeKeys);
-  const int t0 = (int)((int64_t)steps * split / a.splits), t1 = (int)((int64_t)steps * (split + 1) / a.splits);
+  const int t0 = share(steps, split, a.splits), t1 = share(steps, split + 1, a.splits);
 
   // (the lane's number, opaque where addresses are formed from it: kept from step to step they would take the
   // registers that the outputs need)
