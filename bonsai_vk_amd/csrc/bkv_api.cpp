@@ -693,7 +693,7 @@ int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, co
   if (!aligned16(out) || (out_gated && !aligned16(out_gated)) || ((uintptr_t)mask & 7u) != 0) return BKV_EALIGN;
   if (!workspace) return BKV_EWORKSPACE;
   if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
-  const TreePlan p = plan_tree(d->nh, d->nkv, d->k_fmt, d->v_fmt, pos0, n_q, prefill_base(d));
+  const TreePlan p = plan_tree(d->nh, d->nkv, pos0, n_q, prefill_base(d));
   if (ws_bytes < p.total) return BKV_EWORKSPACE;
   char *w = (char *)workspace;
   TreeArgs a{};

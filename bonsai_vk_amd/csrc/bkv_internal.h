@@ -254,7 +254,7 @@ struct TreePlan {
   int nrb, splits;               // row blocks per KV head, key ranges per row block
   size_t off_ml, off_part, total;
 };
-TreePlan plan_tree(int nh, int nkv, int kfmt, int vfmt, int64_t pos0, int n_q, size_t base);
+TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base);
 size_t tree_workspace_bound(int nh, int nkv, size_t base);
 hipError_t launch_tree(const TreeArgs &a, const TreePlan &p, int kf, int vf, hipStream_t st);
 

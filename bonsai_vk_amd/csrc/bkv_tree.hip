@@ -19,6 +19,7 @@
 // finite at the end is computed again by tree_careful_row, key by key, in fp32, without the keys that are not seen.
 
 #include <algorithm>
+#include <cmath>
 
 #include "bkv_device.h"
 #include "bkv_internal.h"
@@ -597,8 +598,11 @@ __device__ __forceinline__ uint32_t v_piece(int d, int g) {
   return (uint32_t)(128 * (d >> 1) + 16 * ((4 * (d & 1) + g) ^ kx));
 }
 
+// 8 waves with rows, and 4 more where the registers allow them
+constexpr int tree_tile_threads(int mt) { return mt == 1 ? 768 : 512; }
+
 template <int KF, int VF, int PG, int MT>
-__global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) {
+__global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_tile_kernel(TreeArgs a, int nrb) {
   constexpr int NW = 8, KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT * NW;
   constexpr uint32_t kOp = kTreeKeys * 2 * kHd;    // an operand: 32 keys of 256 fp16
   // three steps' V operands (vh, vl, their levels) and two steps' of K (with its scales); behind them the bytes as
@@ -627,10 +631,12 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
   const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
   const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
 
-  // ---- a step's bytes on their way: waves 0 .. 3 take V (64 dims each), waves 4 .. 7 K (8 keys each), what they will
-  // make into operands themselves, so that a wave waits for its own loads only
-  const bool does_v = w < 4;
+  // ---- a step's bytes on their way, and later into operands: 4 waves V (64 dims each), 4 waves K (8 keys each). A wave
+  // brings what it will make into operands itself, so it waits for its own loads only. With 256 rows waves 0 .. 3 take
+  // V and waves 4 .. 7 K beside their rows; with 128 the registers leave room for 4 more waves, which take both and have
+  // no rows.
   const int wk = w & 3;
+  const bool does_v = MT == 1 ? w >= NW : w < 4, does_k = MT == 1 ? w >= NW : w >= 4;
   uint32_t there = ~0u, there_next = ~0u, there_after = ~0u;   // keys whose pages are in the pool: this step's, the next's, ..
   int sl = 0;                                      // PG 2: the slot of the key lane % 32 of the step asked for next
   auto look_up = [&](int t) {
@@ -664,7 +670,8 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
         const uint8_t *src = PG == 2 ? vsc + (size_t)max(__shfl(sl, key), 0) * srow : vsc + s0 * srow + min((uint32_t)key, last) * srow;
         if (lane < 32) load4_to_lds(src + 4 * wk, sm0 + oSV + 128 * wk);
       }
-    } else {
+    }
+    if (does_k) {
       constexpr int LR = KF ? 16 : 32;             // lanes of a row
 #pragma unroll
       for (int u = 0; u < (KF ? 2 : 4); ++u) {
@@ -685,11 +692,13 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
     request(t0, 1);
     there = there_after;
   }
+  const bool has_rows = w < NW;
   h8 qh[MT][8];
   auto token_of = [&](int mt) { return min(RB * rb + 16 * MT * w + 16 * mt + (my_lane() & 15), R - 1) / a.grp; };
   // the rows of Q, whole rows at a time (a row's pieces lane by lane would ask for each line four times), to fp16 and
   // through LDS, 8 KB of the operands' place per wave, to the lanes that want them; pieces as K's
   static_assert(oRV >= 8 * 8192 && (KF || oK + kKB >= 8 * 8192), "the rows end before the bytes that are on their way");
+  if (has_rows)
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float4 x[16];
@@ -718,7 +727,7 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
   auto convert = [&](uint8_t *kto, uint8_t *vto) {
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (!does_v) {
+    if (does_k) {
       if constexpr (KF) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -735,8 +744,8 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
         reinterpret_cast<uint16_t *>(kto + kOp)[32 * (key >> 2) + 4 * (lane & 7) + (key & 3)] =
             reinterpret_cast<const uint16_t *>(sm + oSK)[64 * wk + lane];
       }
-      return;
     }
+    if (!does_v) return;
     if constexpr (VF) {
       uint32_t r[8], sc[8], top = 0;
 #pragma unroll
@@ -921,7 +930,7 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 
   // Waves 4 .. 7, which share their SIMDs with waves 0 .. 3, take P V of a step at the beginning of the next one: while
   // one wave's scores and probabilities keep the vector unit busy, the other's products keep the matrix cores busy.
-  const bool late = w >= 4, works = RB * rb + 16 * MT * w < R;   // (a wave whose rows are all past the last only brings bytes)
+  const bool late = w >= 4, works = has_rows && RB * rb + 16 * MT * w < R;   // (a wave whose rows are all past the last only brings bytes)
   lds_barrier();                                   // (every wave has its rows)
   if (t0 < t1) {
     convert(sm + oK + kKB, sm);
@@ -967,7 +976,8 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
   }
   if (works && late && t0 < t1) products(sm + v_last);
 
-  // ---- one partial result per row
+  // ---- one partial result per row (through LDS, so that whole rows are written at once, took 2 us more)
+  if (!works) return;
   const int64_t rows = (int64_t)a.n_q * a.nh;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -980,8 +990,7 @@ __global__ __launch_bounds__(512, 2) void tree_tile_kernel(TreeArgs a, int nrb) 
 #pragma unroll
       for (int dt = 0; dt < 16; ++dt) {
         const float f = VF ? __builtin_ldexpf(1.0f, 8 * (int)((lv >> (8 * (dt >> 2))) & 3u) - 9) : 1.0f;
-        const f4 v = o[mt][dt] * f;
-        *reinterpret_cast<f4 *>(a.part + at * kHd + 16 * dt + 4 * g) = v;
+        *reinterpret_cast<f4 *>(a.part + at * kHd + 16 * dt + 4 * g) = o[mt][dt] * f;
       }
       if (g == 0) a.ml[at] = make_float2(m[mt], sum);
     }
@@ -997,16 +1006,21 @@ static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 enum { kTree16, kTree32, kTree128, kTree256 };
 static int tree_kind(int64_t rows) { return rows <= 16 ? kTree16 : rows <= 32 ? kTree32 : rows <= 128 ? kTree128 : kTree256; }
 static int tree_rows(int kind) { return kind == kTree16 ? 16 : kind == kTree32 ? 32 : kind == kTree128 ? 128 : 256; }
-// workgroups that the key split aims for: as many as run at once
-static int tree_fill(int kind, int kfmt, int vfmt) { return kind == kTree16 && kfmt == BKV_Q8_0 && vfmt == BKV_Q8_0 ? 512 : 256; }
+// workgroups that the key split aims for: one per CU (two of the stream kernel's would fit in q8_0, and leave twice the
+// ranges to join: 1 token onto 32768 keys 18.7 + 7.6 us against 18.2 + 5.6, onto 131072 56.0 + 7.5 against 48.4 + 5.4)
+constexpr int kTreeFill = 256;
 
-TreePlan plan_tree(int nh, int nkv, int kfmt, int vfmt, int64_t pos0, int n_q, size_t base) {
+TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   TreePlan p{};
   const int64_t rows = (int64_t)n_q * (nh / nkv), steps = cdiv(pos0 + n_q, kTreeKeys);
   p.kind = tree_kind(rows);
   p.nrb = (int)cdiv(rows, tree_rows(p.kind));
-  // a wave of the stream kernel takes a step at least, a workgroup of the tiles too
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, p.kind <= kTree32 ? cdiv(steps, 4) : steps), std::max<int64_t>(1, tree_fill(p.kind, kfmt, vfmt) / ((int64_t)nkv * p.nrb)));
+  // A wave of the stream kernel takes a step at least. The tiles: a step fewer per workgroup saves 2 us (4 with 256 rows),
+  // a key range more costs 0.2 us per 1024 rows of partial results to write and join; the least of their sum, measured:
+  // 25 tokens onto 500 keys 18.5 us in 17 ranges, 23.5 in 5; onto 2000 28.1 in 63, 24.4 in 24; 64 onto 2000 41.4 in 64,
+  // 39.3 in 24.
+  const int64_t most = p.kind <= kTree32 ? cdiv(steps, 4) : std::max<int64_t>(1, (int64_t)std::sqrt(80.0 * tree_rows(p.kind) * (double)steps / ((double)n_q * nh)));
+  p.splits = (int)std::min<int64_t>(std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, steps), most), std::max<int64_t>(1, kTreeFill / ((int64_t)nkv * p.nrb)));
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
@@ -1027,8 +1041,8 @@ static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStre
   switch (p.kind) {
     case kTree16: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
     case kTree32: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a, p.nrb); break;
-    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(512), 0, st, a, p.nrb); break;
-    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(512), 0, st, a, p.nrb); break;
+    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(tree_tile_threads(1)), 0, st, a, p.nrb); break;
+    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(tree_tile_threads(2)), 0, st, a, p.nrb); break;
   }
   return hipGetLastError();
 }
