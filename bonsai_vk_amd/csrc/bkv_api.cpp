@@ -652,6 +652,10 @@ int bkv_attn_prefill_chunk_qg(const bkv_cache_desc *d, int layer, uint32_t pos0,
 // ------------------------------------------------------------------ drafted tokens
 // head_dim 256, any number of query heads per KV head
 static int check_hd(const bkv_cache_desc *d) { return d->hd == kHd ? BKV_OK : BKV_EUNSUPPORTED; }
+// whether positions pos0 .. pos0 + n - 1 leave the cache (or the 32 bits of a position: a block table may span more)
+static bool outside(const bkv_cache_desc *d, uint32_t pos0, int n) {
+  return (int64_t)pos0 + n > std::min<int64_t>(max_positions(d), (int64_t(1) << 32) - 64);
+}
 static int pool_pages(const bkv_cache_desc *d) { return d->page_tokens > 0 ? d->cap / d->page_tokens : 0; }
 
 static int check_rows(const bkv_rows *r) {
@@ -686,7 +690,7 @@ int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, co
   if ((rc = check_hd(d))) return rc;
   if (layer < 0 || layer >= d->n_layers || n_q < 0 || n_q > BKV_TREE_MAX_Q) return BKV_EINVAL;
   if (n_q == 0) return BKV_OK;
-  if ((int64_t)pos0 + n_q > max_positions(d)) return BKV_ECAP;
+  if (outside(d, pos0, n_q)) return BKV_ECAP;
   if ((rc = check_rows(q))) return rc;
   if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
   if (gate && (rc = check_rows(gate))) return rc;
@@ -710,6 +714,8 @@ int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, co
   a.out = out;
   a.out_gated = out_gated;
   a.splits = p.splits;
+  a.share = p.share;
+  a.spare = p.spare;
   a.ml = (float2 *)(w + p.off_ml);
   a.part = (float *)(w + p.off_part);
   return hip_fail(launch_tree(a, p, d->k_fmt, d->v_fmt, stream));
@@ -771,7 +777,7 @@ int bkv_rope_append(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok
   if ((qn_w == nullptr) != (kn_w == nullptr) || (qn_w && !(eps >= 0.0f))) return BKV_EINVAL;
   if ((q == nullptr) != (q_out == nullptr)) return BKV_EINVAL;
   if (n_tok == 0) return BKV_OK;
-  if ((int64_t)pos0 + n_tok > max_positions(d)) return BKV_ECAP;
+  if (outside(d, pos0, n_tok)) return BKV_ECAP;
   if (q && (rc = check_rows(q))) return rc;
   if ((rc = check_rows(k)) || (rc = check_rows(v))) return rc;
   if ((q_out && !aligned16(q_out)) || (qn_w && (!aligned16(qn_w) || !aligned16(kn_w))) || ((uintptr_t)positions & 3u) != 0)
@@ -798,7 +804,7 @@ int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int ou
   if (layer < 0 || layer >= d->n_layers || n < 0) return BKV_EINVAL;
   if (out_type < BKV_OUT_F32 || out_type > BKV_OUT_BF16) return BKV_EINVAL;
   if (n == 0) return BKV_OK;
-  if ((int64_t)pos0 + n > max_positions(d)) return BKV_ECAP;
+  if (outside(d, pos0, n)) return BKV_ECAP;
   if (!k_out && !v_out) return BKV_EINVAL;
   // rows lie apart: whole tokens after one another, or whole heads
   const bool tokens = tok_stride >= (__int128)(d->nkv - 1) * head_stride + kHd && head_stride >= kHd;
@@ -825,7 +831,7 @@ int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_kee
   if ((rc = check_hd(d))) return rc;
   if (n_draft < 0 || n_draft > BKV_TREE_MAX_Q || n_keep < 0 || n_keep > n_draft) return BKV_EINVAL;
   if (n_keep == 0) return BKV_OK;
-  if ((int64_t)pos0 + n_draft > max_positions(d)) return BKV_ECAP;
+  if (outside(d, pos0, n_draft)) return BKV_ECAP;
   if (!idx) return BKV_EINVAL;
   if (((uintptr_t)idx & 3u) != 0) return BKV_EALIGN;
   CommitArgs a{};

@@ -246,12 +246,15 @@ struct TreeArgs {
   int words;
   float *out, *out_gated;
   int splits;                    // key ranges per row block
+  int share, spare;              // 32-key steps of a range (of a wave's, in the stream kernel), and how many ranges take
+                                 // one more
   float *part;                   // [splits][n_q * nh][hd] unnormalised partial outputs
   float2 *ml;                    // [splits][n_q * nh] their reference (log2) and sum
 };
 struct TreePlan {
   int kind;                      // which kernel
   int nrb, splits;               // row blocks per KV head, key ranges per row block
+  int share, spare;
   size_t off_ml, off_part, total;
 };
 TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base);

@@ -216,11 +216,17 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   }
 }
 
-// where the i-th of n nearly equal parts of x things begins (the same in all lanes)
-__device__ __forceinline__ int share(int x, int i, int n) {
-  const int q = x / n, rest = x - q * n;
-  return __builtin_amdgcn_readfirstlane(i * q + min(i, rest));
-}
+// where the i-th key range begins, in steps (the host has divided: a division here is 200 cycles before the first load)
+__device__ __forceinline__ int range_begin(const TreeArgs &a, int i) { return __builtin_amdgcn_readfirstlane(i * a.share + min(i, a.spare)); }
+
+// The rows r, r + 1, .. of a KV head as (token, query head of the group), r < rows
+struct RowWalk {
+  int tok, h;
+  __device__ __forceinline__ RowWalk(int r, int grp) : tok(r / grp), h(r - tok * grp) {}
+  __device__ __forceinline__ void next(int grp) {
+    if (++h == grp) { h = 0; ++tok; }
+  }
+};
 
 // 8 probabilities as ph + pl: ph cut to fp16 (two in one instruction), pl the rest, rounded (one instruction each)
 __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
@@ -278,7 +284,7 @@ __device__ __forceinline__ int tree_dim(int dt, int m) {
 }
 
 template <int KF, int VF, int PG, int MT>
-__global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 2 : 1) void tree_stream_kernel(TreeArgs a, int nrb) {
+__global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 2 : 1) void tree_stream_kernel(TreeArgs a) {
   constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT;
   constexpr uint32_t oV = kTreeKeys * KRB, oSK = oV + kTreeKeys * VRB, oSV = oSK + (KF ? 512 : 0), kWave = oSV + (VF ? 512 : 0);
   constexpr int kOS = kHd + 4;                     // a row of the join
@@ -286,14 +292,13 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   __shared__ __attribute__((aligned(128))) uint8_t sm[4 * kWave > kJoin ? 4 * kWave : kJoin];
   __shared__ float s_m[4][RB], s_l[4][RB];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  // workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there
-  const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
+  // (workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there)
+  const int unit = (int)(8 * blockIdx.z + blockIdx.x), rb = blockIdx.y;
   if (unit >= a.nkv * a.splits) return;
   const int hk = unit / a.splits, split = unit - hk * a.splits;
   const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
-  const int steps = (int)((nk + kTreeKeys - 1) / kTreeKeys), wi = split * 4 + w, nw = a.splits * 4;
-  const int t0 = share(steps, wi, nw), t1 = share(steps, wi + 1, nw);
+  const int t0 = range_begin(a, split * 4 + w), t1 = range_begin(a, split * 4 + w + 1);
   const uint32_t krow = (uint32_t)a.nkv * KRB, vrow = (uint32_t)a.nkv * VRB, srow = (uint32_t)a.nkv * kScaleRowBytes;
   const uint8_t *kd = a.L.kd + (size_t)hk * KRB, *vd = a.L.vd + (size_t)hk * VRB;
   const uint8_t *ksc = KF ? a.L.ks + (size_t)hk * kScaleRowBytes : nullptr, *vsc = VF ? a.L.vs + (size_t)hk * kScaleRowBytes : nullptr;
@@ -345,10 +350,14 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   };
   // the workgroup's rows of Q first, 4 MT of them by each wave into the place of its V (piece c of row r at c ^ r % 16),
   // then K; V once the rows have been read
+  {
+    RowWalk at(min(RB * rb + 4 * MT * w, R - 1), a.grp);
 #pragma unroll
-  for (int j = 0; j < 4 * MT; ++j) {
-    const int row = 4 * MT * w + j, r = min(RB * rb + row, R - 1), ti = r / a.grp;
-    load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(ti, hk * a.grp + r - ti * a.grp)) + 16 * (lane ^ (row & 15)), my0 + oV + 1024 * j);
+    for (int j = 0; j < 4 * MT; ++j) {
+      const int row = 4 * MT * w + j;
+      load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(at.tok, hk * a.grp + at.h)) + 16 * (lane ^ (row & 15)), my0 + oV + 1024 * j);
+      if (RB * rb + row + 1 < R) at.next(a.grp);
+    }
   }
   if (t0 < t1) {
     look_up(t0);
@@ -602,7 +611,7 @@ __device__ __forceinline__ uint32_t v_piece(int d, int g) {
 constexpr int tree_tile_threads(int mt) { return mt == 1 ? 768 : 512; }
 
 template <int KF, int VF, int PG, int MT>
-__global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_tile_kernel(TreeArgs a, int nrb) {
+__global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_tile_kernel(TreeArgs a) {
   constexpr int NW = 8, KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT * NW;
   constexpr uint32_t kOp = kTreeKeys * 2 * kHd;    // an operand: 32 keys of 256 fp16
   // three steps' V operands (vh, vl, their levels) and two steps' of K (with its scales); behind them the bytes as
@@ -612,13 +621,12 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   __shared__ __attribute__((aligned(128))) uint8_t sm[oSK + (KF ? 512 : 0)];
   const uint32_t sm0 = lds_addr(sm);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  const int unit = (int)(blockIdx.x / (8 * nrb)) * 8 + (blockIdx.x & 7), rb = (blockIdx.x >> 3) % nrb;
+  const int unit = (int)(8 * blockIdx.z + blockIdx.x), rb = blockIdx.y;
   if (unit >= a.nkv * a.splits) return;
   const int hk = unit / a.splits, split = unit - hk * a.splits;
   const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
-  const int steps = (int)((nk + kTreeKeys - 1) / kTreeKeys);
-  const int t0 = share(steps, split, a.splits), t1 = share(steps, split + 1, a.splits);
+  const int t0 = range_begin(a, split), t1 = range_begin(a, split + 1);
 
   // (the lane's number, opaque where addresses are formed from it: kept from step to step they would take the
   // registers that the outputs need)
@@ -698,14 +706,15 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   // the rows of Q, whole rows at a time (a row's pieces lane by lane would ask for each line four times), to fp16 and
   // through LDS, 8 KB of the operands' place per wave, to the lanes that want them; pieces as K's
   static_assert(oRV >= 8 * 8192 && (KF || oK + kKB >= 8 * 8192), "the rows end before the bytes that are on their way");
+  RowWalk at(min(RB * rb + 16 * MT * w, R - 1), a.grp);   // (the same in all lanes)
   if (has_rows)
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float4 x[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const int r = min(RB * rb + 16 * MT * w + 16 * mt + j, R - 1), tok = r / a.grp;      // (the same in all lanes)
-      x[j] = reinterpret_cast<const float4 *>(a.q.at(tok, hk * a.grp + r - tok * a.grp))[lane];
+      x[j] = reinterpret_cast<const float4 *>(a.q.at(at.tok, hk * a.grp + at.h))[lane];
+      if (RB * rb + 16 * (MT * w + mt) + j + 1 < R) at.next(a.grp);
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -987,12 +996,27 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
     sum += __shfl_xor(sum, 32);
     if (r < R) {
       const int64_t at = (int64_t)split * rows + (int64_t)tok * a.nh + hk * a.grp + r - tok * a.grp;
-#pragma unroll
-      for (int dt = 0; dt < 16; ++dt) {
-        const float f = VF ? __builtin_ldexpf(1.0f, 8 * (int)((lv >> (8 * (dt >> 2))) & 3u) - 9) : 1.0f;
-        *reinterpret_cast<f4 *>(a.part + at * kHd + 16 * dt + 4 * g) = o[mt][dt] * f;
-      }
       if (g == 0) a.ml[at] = make_float2(m[mt], sum);
+    }
+    // A store of one product's outputs would reach 16 rows' 64 bytes, half a line each, at a third of the rate of whole
+    // lines: so lanes n and n ^ 1 exchange halves of two products, and a store reaches 8 rows' 128 bytes.
+    const int64_t mine = r < R ? (int64_t)split * rows + (int64_t)tok * a.nh + hk * a.grp + r - tok * a.grp : -1;
+    const int64_t other = __shfl_xor(mine, 1);
+    const bool odd = n & 1;
+    const int64_t even_row = odd ? other : mine, odd_row = odd ? mine : other;
+#pragma unroll
+    for (int dt = 0; dt < 16; dt += 2) {
+      const float f = VF ? __builtin_ldexpf(1.0f, 8 * (int)((lv >> (8 * (dt >> 2))) & 3u) - 9) : 1.0f;
+      f4 a0 = o[mt][dt] * f, a1 = o[mt][dt + 1] * f, e, d;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = dpp<0xB1>(odd ? a0[i] : a1[i]);          // the other row's half
+        e[i] = odd ? x : a0[i];
+        d[i] = odd ? a1[i] : x;
+      }
+      const int col = 16 * (dt + (odd ? 1 : 0)) + 4 * g;
+      if (even_row >= 0) *reinterpret_cast<f4 *>(a.part + even_row * kHd + col) = e;
+      if (odd_row >= 0) *reinterpret_cast<f4 *>(a.part + odd_row * kHd + col) = d;
     }
   }
 }
@@ -1021,6 +1045,9 @@ TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
   // 39.3 in 24.
   const int64_t most = p.kind <= kTree32 ? cdiv(steps, 4) : std::max<int64_t>(1, (int64_t)std::sqrt(80.0 * tree_rows(p.kind) * (double)steps / ((double)n_q * nh)));
   p.splits = (int)std::min<int64_t>(std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, steps), most), std::max<int64_t>(1, kTreeFill / ((int64_t)nkv * p.nrb)));
+  const int64_t ranges = p.splits * (p.kind <= kTree32 ? 4 : 1);
+  p.share = (int)(steps / ranges);
+  p.spare = (int)(steps % ranges);
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
@@ -1037,12 +1064,12 @@ size_t tree_workspace_bound(int nh, int nkv, size_t base) {
 
 template <int KF, int VF, int PG>
 static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStream_t st) {
-  const dim3 grid((unsigned)(cdiv((int64_t)a.nkv * a.splits, 8) * 8 * p.nrb));
+  const dim3 grid(8, p.nrb, (unsigned)cdiv((int64_t)a.nkv * a.splits, 8));
   switch (p.kind) {
-    case kTree16: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a, p.nrb); break;
-    case kTree32: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a, p.nrb); break;
-    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(tree_tile_threads(1)), 0, st, a, p.nrb); break;
-    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(tree_tile_threads(2)), 0, st, a, p.nrb); break;
+    case kTree16: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a); break;
+    case kTree32: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a); break;
+    case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(tree_tile_threads(1)), 0, st, a); break;
+    default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(tree_tile_threads(2)), 0, st, a); break;
   }
   return hipGetLastError();
 }

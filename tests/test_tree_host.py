@@ -122,6 +122,12 @@ def test_attn_tree_refusals():
     assert tree(d, ws=None) == EWORKSPACE and tree(d, ws=Z + 16) == EALIGN
     paged = desc(page_tokens=64, max_pages=3, block_table=0x500000)
     assert tree(paged, pos0=185) == ECAP
+    # a block table of more positions than 32 bits hold
+    wide = desc(page_tokens=4096, max_pages=1 << 21, block_table=0x500000)
+    assert call("bkv_max_positions", wide) == 1 << 33
+    assert tree(wide, pos0=2**32 - 64, n=8) == ECAP and tree(wide, pos0=2**32 - 200, n=8, ws=None) == EWORKSPACE
+    assert rope_call(wide, pos0=2**32 - 4) == ECAP and read(wide, pos0=2**32 - 8) == ECAP
+    assert call("bkv_kv_commit", wide, 2**32 - 8, 8, 4, Z, None) == ECAP
 
 
 def test_tree_workspace_does_not_depend_on_the_context():
