@@ -293,7 +293,12 @@ class KvCache:
         if t.data_ptr() & 15:
             t = t.clone()
         keep.append(t)
-        return BkvRows(t.data_ptr(), t.stride(0), t.stride(1))
+        return BkvRows(t.data_ptr(), heads * self.hd, self.hd)   # (torch leaves the stride of an axis of 1 as it was)
+
+    @staticmethod
+    def _pos(pos0):
+        if not 0 <= pos0 <= 0xFFFFFFFF:
+            raise ValueError(f"positions are 32 bits, got {pos0}")
 
     def _on_device(self, t, dtype, shape):
         if t.dtype is not dtype or t.device != self._dev or t.shape != shape or not t.is_contiguous():
@@ -308,7 +313,8 @@ class KvCache:
 
     def tree_workspace(self):
         """The workspace of attn_tree, made at its first call; a program that captures that call into a graph asks for
-        it before."""
+        it before. All of this cache's attn_tree calls share it: like its decodes they run one after another, on one
+        stream or on streams that wait for one another."""
         if getattr(self, "_tws", None) is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call tree_workspace() before the capture: memory of a graph's own pool would not outlive it")
@@ -323,6 +329,7 @@ class KvCache:
         if self._elsewhere():
             with torch.cuda.device(self._dev):
                 return self.attn_tree(layer, pos0, q, mask, gate, out, out_gated)
+        self._pos(pos0)
         n, keep = q.shape[0], []
         qr, gr = self._rows(q, self.nh, keep), None
         if gate is not None:
@@ -349,6 +356,7 @@ class KvCache:
         if self._elsewhere():
             with torch.cuda.device(self._dev):
                 return self.rope_append(layer, pos0, q, k, v, rope, positions, qn_w, kn_w, eps, q_out)
+        self._pos(pos0)
         n, keep = k.shape[0], []
         kr, vr, qr, qo = self._rows(k, self.nkv, keep), self._rows(v, self.nkv, keep), None, None
         if v.shape[0] != n or (q is not None and q.shape[0] != n):
@@ -376,6 +384,7 @@ class KvCache:
         if self._elsewhere():
             with torch.cuda.device(self._dev):
                 return self.read(layer, pos0, n, dtype, k_out, v_out)
+        self._pos(pos0)
         if k_out is None and v_out is None:
             if dtype not in _OUT_TYPES:
                 raise ValueError(f"{dtype} is none of {list(_OUT_TYPES)}")
@@ -400,6 +409,7 @@ class KvCache:
         if self._elsewhere():
             with torch.cuda.device(self._dev):
                 return self.commit(pos0, n_draft, idx)
+        self._pos(pos0)
         n = idx.numel()
         self._on_device(idx, torch.int32, (n,))
         rc = lib().bkv_kv_commit(self.desc, pos0, n_draft, n, idx.data_ptr(), self._my_stream())

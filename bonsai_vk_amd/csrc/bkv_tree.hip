@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   const float2 m0 = lane < a.splits ? a.ml[(int64_t)lane * rows + r] : none;
   const float2 m1 = lane + 64 < a.splits ? a.ml[(int64_t)(lane + 64) * rows + r] : none;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f), t[8];
-  float mm = 0.0f, f0 = 0.0f, f1 = 0.0f, l = 0.0f;
+  float mm = 0.0f, f0 = 0.0f, f1 = 0.0f;
   for (int s0 = w; s0 < a.splits; s0 += 8 * NWV) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -179,7 +179,8 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
     f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - mm);
     f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - mm);
   }
-  l = wave_sum(m0.y * f0 + m1.y * f1);
+  const float l0 = fabsf(m0.y) * f0, l1 = fabsf(m1.y) * f1;   // (the sign: see marked_sum)
+  float l = wave_sum(l0 + l1);
   reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = o;
   __syncthreads();
   o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -192,13 +193,13 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   // (every wave holds the whole row: the decision is the workgroup's)
   const float big = fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
   bool fine = l > 0.0f && l < INFINITY && !__any(!(big < INFINITY) || o.x != o.x || o.y != o.y || o.z != o.z || o.w != o.w);
-  // V of subnormal fp16 size (kTiny is below 2^-14 by the averaging of a few keys): the matrix cores keep such a
-  // product to about 2^-37 of p's unit and not to 24 bits of itself (V of 1e-6: 7e-6 off; of 1e-4: 3e-7), and vl
-  // runs out of bits
-  constexpr float kTiny = 0x1p-17f;
+  // Products below 2^-28 are lost in the matrix cores: of fp16 V, of subnormal size for this to matter, what is below
+  // 2^-37 (V of 1e-6 was 7e-6 off, V of 1e-4 3e-7); of q8_0 V, taken times 2^9 or 2^1, less; of a step of level 2, taken
+  // times 2^-7, what is below 2^-30. Rows whose outputs come near that are formed again.
   if (fine) {
     const float top = wave_max(big);
-    fine = top == 0.0f || !(top < kTiny * l);
+    const bool high = __any((m0.y < 0.0f && f0 > 0.0f) || (m1.y < 0.0f && f1 > 0.0f));
+    fine = top == 0.0f ? !high : top >= l * (high ? 0x1p-9f : 0x1p-17f);
   }
   bool empty = false;
   if (!fine) {
@@ -240,11 +241,25 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
   for (int j = 0; j < 8; ++j) pl[j] = (_Float16)__builtin_fmaf((float)ph[j], -1.0f, p[j]);
 }
 
-// q8_0 scales: vh and vl keep 19 bits for scales up to 2^-1 and down to 2^-17 or so when they are taken times 2^9; a
-// step with a larger one takes 2^1 or 2^-7 (its level), and the outputs are brought to the step's unit. (Smaller
-// values end as outputs below kTiny.)
+// q8_0 scales are taken times 2^9, so that vl of the smallest is no subnormal product; a step with one above 2^-1 takes
+// all of its times 2^1, with one above 2^7 times 2^-7 (its level: 0, 1, 2), which keeps vh within fp16, and the outputs
+// are brought to the step's unit. vh and vl hold d * b exactly where the scaled d is exact: always at levels 0 and 1,
+// at level 2 from d = 2^-7 on. Smaller ones beside such large ones (16256 beside 1, in 32 neighbouring keys) leave NaN
+// in place of the range's sum, so that its rows are computed key by key.
 // the level of the largest of fp16 scales (bits, sign cleared): above 2^-1, above 2^7
 __device__ __forceinline__ int scale_level(uint32_t top) { return (top > 0x3800u) + (top > 0x5800u); }
+// whether a step of level 2 loses bits of one of the scales
+__device__ __forceinline__ bool scale_lost(const uint32_t (&sc)[8]) {
+  bool lost = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) lost |= ((sc[j] & 0x7FFFu) - 1u) < 0x1FFFu;
+  return __any(lost);
+}
+constexpr int kLostBits = 4;                       // (beside the level)
+// a range's sum of p as it is left for the join: below zero where a step had level 2
+__device__ __forceinline__ float marked_sum(float l, uint32_t levels) {
+  return levels & kLostBits ? __builtin_nanf("") : levels & 2 ? -l : l;
+}
 
 // 16 bytes per lane from base + off into LDS at dst + 16 * lane (dst the same in all lanes), not waited for
 __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t dst) {
@@ -291,6 +306,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   constexpr uint32_t kJoin = 4 * RB * kOS * 4;
   __shared__ __attribute__((aligned(128))) uint8_t sm[4 * kWave > kJoin ? 4 * kWave : kJoin];
   __shared__ float s_m[4][RB], s_l[4][RB];
+  __shared__ uint32_t s_lv[4];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   // (workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there)
   const int unit = (int)(8 * blockIdx.z + blockIdx.x), rb = blockIdx.y;
@@ -389,6 +405,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
   int lv = 0;                                      // the outputs' level
+  uint32_t lv_any = 0;                             // all that were taken, or-ed
 
 #pragma unroll 1
   for (int t = t0; t < t1; ++t) {
@@ -485,6 +502,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
       }
       const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
       const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
+      if (level == 2) lv_any |= 2u | (scale_lost(sc) ? kLostBits : 0);
       if (level != lv) {
         const float x = __builtin_ldexpf(1.0f, 8 * (lv - level));
 #pragma unroll
@@ -550,6 +568,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
     l[mt] += __shfl_xor(l[mt], 32);
     if (g == 0) { s_m[w][16 * mt + n] = m[mt]; s_l[w][16 * mt + n] = l[mt]; }
   }
+  if (lane == 0) s_lv[w] = lv_any;
   __syncthreads();                                 // (and the waves' own parts have been read)
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -585,7 +604,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
         float lr = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) lr += s_m[j][row] == -INFINITY ? s_l[j][row] : s_l[j][row] * exp2f(s_m[j][row] - mr);
-        a.ml[at] = make_float2(mr, lr);
+        a.ml[at] = make_float2(mr, marked_sum(lr, s_lv[0] | s_lv[1] | s_lv[2] | s_lv[3]));
       }
     }
   }
@@ -730,7 +749,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   float m[MT], l[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
-  uint32_t lv = 0;                                 // the outputs' levels, a byte per 64 dims
+  uint32_t lv = 0, lv_any = 0;                     // the outputs' levels, a byte per 64 dims; all that were taken, or-ed
 
   // ---- the wave's bytes, landed, made into operands
   auto convert = [&](uint8_t *kto, uint8_t *vto) {
@@ -765,7 +784,8 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
       }
       const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
       const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
-      if (lane == 0) vto[oLV + wk] = (uint8_t)level;
+      const int lost = level == 2 && scale_lost(sc) ? kLostBits : 0;
+      if (lane == 0) vto[oLV + wk] = (uint8_t)(level | lost);
       h2 d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = as_h2(sc[2 * j] | (sc[2 * j + 1] << 16)) * h2{f, f};
@@ -906,6 +926,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
             for (int dt = 0; dt < 4; ++dt) o[mt][4 * c + dt] *= f;
         }
         lv = now;
+        lv_any |= now;
       }
     }
     const uint32_t vp[2] = {v_piece(n, g), v_piece(16 + n, g) - 1024u};
@@ -996,7 +1017,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
     sum += __shfl_xor(sum, 32);
     if (r < R) {
       const int64_t at = (int64_t)split * rows + (int64_t)tok * a.nh + hk * a.grp + r - tok * a.grp;
-      if (g == 0) a.ml[at] = make_float2(m[mt], sum);
+      if (g == 0) a.ml[at] = make_float2(m[mt], marked_sum(sum, lv_any | lv_any >> 16 | (lv_any | lv_any >> 16) >> 8));
     }
     // A store of one product's outputs would reach 16 rows' 64 bytes, half a line each, at a third of the rate of whole
     // lines: so lanes n and n ^ 1 exchange halves of two products, and a store reaches 8 rows' 128 bytes.

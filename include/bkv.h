@@ -277,9 +277,11 @@ int bkv_tree_mask(const int32_t *parent, int n, uint64_t *mask, int32_t *depth);
  *   bkv_attn_decode's to about the rounding of its fp16 probabilities.
  *   A row that sees nothing gets 0. Positions that a row does not see have no effect on it, whatever
  *   they hold (Inf and NaN included).
- *   out: [n_q][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)).
+ *   out: [n_q][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)). Neither
+ *   may overlap the inputs or the other.
  * Workspace: bkv_workspace_bytes(d, BKV_OP_TREE, max_ctx), any max_ctx > 0; it needs no
- * initialisation, and serves decodes too once bkv_workspace_init has run on it. */
+ * initialisation, and serves decodes too once bkv_workspace_init has run on it. Calls (and replays of
+ * captured ones) that share a workspace must not overlap in time. */
 int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, const bkv_rows *q,
                   const uint64_t *mask, const bkv_rows *gate, float *out, float *out_gated,
                   void *workspace, size_t ws_bytes, hipStream_t stream);

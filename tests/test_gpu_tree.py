@@ -159,6 +159,44 @@ def test_v_scales_over_their_whole_range(kf, scale):
     check(c, pos0, n, "tree", accurate=False)
 
 
+@pytest.mark.parametrize("n", [3, 8, 30, 70])
+@pytest.mark.parametrize("usual,big", [(1e-3, 100.0), (2e-2, 100.0), (1e-3, 2e4), (1.0, 2e4), (0.05, 1e6), (0.05, 6e6)])
+def test_a_far_larger_v_among_ordinary_ones(n, usual, big):
+    """A drafted token's q8_0 V, and one of the context with hardly any weight, 10^4 to 10^8 times the others': the
+    rows that do not see it keep their precision. Scores are small, so that tolerance() is about 2^-19 of sum p |v|; the
+    2-norm's bound is check()'s."""
+    pos0 = 300
+    c = filled(pos0 + n, Q8, Q8)
+    v = torch.randn(pos0 + n, 4, HD, generator=gen(4), device="cuda") * usual
+    v[pos0 + 1] *= big / usual
+    c.append(0, 0, torch.randn(pos0 + n, 4, HD, generator=gen(5), device="cuda"), v)
+    q, _ = rows(n, c.nh, 6, 0.01)
+    mask = some_mask("tree", n, 9)
+    mask[torch.arange(n, device="cuda") != 1, 0] &= ~2                 # (only token 1 sees token 1)
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    want, _, size = attention(c, 0, pos0, q, mask)
+    others = torch.arange(n, device="cuda") != 1
+    say(f"usual {usual} big {big}: rel {rel(out[others], want[others]):.2e}")
+    check_rows(out, want, tolerance(size, pos0 + n))
+    assert rel(out[others], want[others]) < 4e-6
+    # the same in the context, where every row sees it with next to no weight: the 2^-34 of sum |v| is the bound then
+    k = torch.randn(pos0 + n, 4, HD, generator=gen(5), device="cuda")
+    k[7] = -40.0
+    v[pos0 + 1] *= usual / big
+    v[7] *= big / usual
+    c.append(0, 0, k, v)
+    q = q.abs() * 100
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    want, _, size = attention(c, 0, pos0, q, mask)
+    # (6e6: most blocks' scales are above fp16's largest, Inf. The weight of e^-500 is not 0 in 64 bits, so Inf is the
+    # sum there; it is far below 2^-149, fp32's smallest, and 0 * Inf is NaN)
+    fin = torch.isfinite(want)
+    assert not bool(torch.isfinite(out[~fin]).any()) and (big > 1e6 or bool(fin.all()))
+    tol = tolerance(size, pos0 + n)
+    check_rows(out[fin], want[fin], tol[fin])
+    assert rel(out[fin], want[fin]) < 4e-6
+
+
 def test_fp16_values_over_their_whole_range():
     pos0, n = 130, 5
     for mul in (6e-8, 1e-6, 1e-4, 1.0, 6e4):
@@ -210,6 +248,32 @@ def test_scores_that_are_not_finite():
     good = torch.isfinite(want)
     t = (want.abs() + 1.0) * 1e-4                  # (this test is about which rows are finite)
     check_rows(out[good], want[good], t[good])
+
+
+def test_axes_of_one_may_have_any_stride():
+    """One token, or one head, whose stride is whatever a view left there."""
+    for nkv, group, n in ((4, 4, 1), (1, 1, 5)):
+        c = filled(64, Q8, Q8, nkv=nkv, group=group)
+        q, g = rows(n, c.nh, 4)
+        want = c.attn_tree(0, 50, q, None, g)
+        odd = [x.as_strided(x.shape, (1, HD, 1) if n == 1 else (HD, 3, 1)) for x in (q, g)]
+        got = c.attn_tree(0, 50, odd[0], None, odd[1])
+        assert all(same(a, b) for a, b in zip(want, got))
+
+
+def test_positions_of_more_than_32_bits_are_refused():
+    """They would be taken modulo 2^32."""
+    c = filled(64, Q8, Q8)
+    q, _ = rows(2, c.nh, 4)
+    kv = torch.zeros(2, 4, HD, device="cuda")
+    from bonsai_vk_amd import Rope
+    before = [x.clone() for x in (c.k_data, c.v_data)]
+    for pos0 in (2 ** 32, 2 ** 32 + 5, -2 ** 32 + 5, -1):
+        for call in (lambda: c.attn_tree(0, pos0, q), lambda: c.read(0, pos0, 2), lambda: c.rope_append(0, pos0, None, kv, kv, Rope(0)),
+                     lambda: c.commit(pos0, 2, torch.zeros(1, dtype=torch.int32, device="cuda"))):
+            with pytest.raises(ValueError):
+                call()
+    assert same(before[0], c.k_data) and same(before[1], c.v_data)
 
 
 def test_strided_rows():
