@@ -691,13 +691,14 @@ int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, co
   if (layer < 0 || layer >= d->n_layers || n_q < 0 || n_q > BKV_TREE_MAX_Q) return BKV_EINVAL;
   if (n_q == 0) return BKV_OK;
   if (outside(d, pos0, n_q)) return BKV_ECAP;
+  if ((int64_t)n_q * d->nh > INT32_MAX / 2) return BKV_EUNSUPPORTED;   // (rows are counted in 32 bits)
   if ((rc = check_rows(q))) return rc;
   if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
   if (gate && (rc = check_rows(gate))) return rc;
   if (!aligned16(out) || (out_gated && !aligned16(out_gated)) || ((uintptr_t)mask & 7u) != 0) return BKV_EALIGN;
   if (!workspace) return BKV_EWORKSPACE;
   if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
-  const TreePlan p = plan_tree(d->nh, d->nkv, pos0, n_q, prefill_base(d));
+  const TreePlan p = plan_tree(d->nh, d->nkv, d->k_fmt, d->v_fmt, d->page_tokens > 0, pos0, n_q, prefill_base(d));
   if (ws_bytes < p.total) return BKV_EWORKSPACE;
   char *w = (char *)workspace;
   TreeArgs a{};
@@ -713,7 +714,11 @@ int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, co
   a.words = (n_q + 63) / 64;
   a.out = out;
   a.out_gated = out_gated;
+  a.nrb = p.nrb;
   a.splits = p.splits;
+  a.whole = d->nkv * p.splits / 8 * p.nrb;
+  a.left = d->nkv * p.splits % 8 * p.nrb;
+  a.share_out = (a.left + 7) / 8;
   a.share = p.share;
   a.spare = p.spare;
   a.ml = (float2 *)(w + p.off_ml);

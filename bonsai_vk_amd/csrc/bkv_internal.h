@@ -245,7 +245,8 @@ struct TreeArgs {
   const uint64_t *mask;          // [n_q][words], or null: a chain
   int words;
   float *out, *out_gated;
-  int splits;                    // key ranges per row block
+  int nrb, splits;               // row blocks per KV head, key ranges per row block
+  int whole, left, share_out;    // workgroups of an XCD's own ranges; of the ranges left over; an eighth of those
   int share, spare;              // 32-key steps of a range (of a wave's, in the stream kernel), and how many ranges take
                                  // one more
   float *part;                   // [splits][n_q * nh][hd] unnormalised partial outputs
@@ -257,7 +258,7 @@ struct TreePlan {
   int share, spare;
   size_t off_ml, off_part, total;
 };
-TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base);
+TreePlan plan_tree(int nh, int nkv, int kf, int vf, bool paged, int64_t pos0, int n_q, size_t base);
 size_t tree_workspace_bound(int nh, int nkv, size_t base);
 hipError_t launch_tree(const TreeArgs &a, const TreePlan &p, int kf, int vf, hipStream_t st);
 

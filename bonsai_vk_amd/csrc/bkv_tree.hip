@@ -11,12 +11,15 @@
 // P V on the fp16 matrix cores keeps fp32's precision by splitting both factors: 2^(x - m) * 2^9 = ph + pl, two
 // fp16 (22 bits; the factor keeps pl normal down to p = 2^-14 of the largest), and q8_0's d * b = vh + vl, two fp16
 // (exact: 19 bits); out = ph vh + pl vh + ph vl, what is left out is below 2^-22 of the result. A single fp16 per
-// factor would leave 1e-4. q8_0 scales are brought near 2^7 by a power of two that a wave keeps for its keys, so
-// that neither a large scale leaves fp16 nor a small one loses vl.
+// factor would leave 1e-4; against the formula in 64 bits the results are 3e-7 to 6e-7 off (2-norm). scale_level says
+// how q8_0 scales of any size stay within fp16.
 //
 // Keys that a row does not see enter the products with p = 0. Where such a key's V is Inf or NaN the product is NaN,
 // and so are Inf V under a visible key (ph and pl may have opposite signs) and non-finite scores: whatever is not
 // finite at the end is computed again by tree_careful_row, key by key, in fp32, without the keys that are not seen.
+//
+// Two launches whatever the sizes: by the rows of a KV head tree_stream_kernel (16 or 32) or tree_tile_kernel (128 or
+// 256 a workgroup), then the join.
 
 #include <algorithm>
 #include <cmath>
@@ -55,7 +58,7 @@ __device__ __forceinline__ uint32_t tree_window(const TreeArgs &a, int i, int64_
 }
 
 // ------------------------------------------------------------------ joining the key ranges
-// Row r = i * nh + h by itself: each wave takes every NWV-th key, a lane 4 dims. Only reached for rows whose partial
+// Row (i, h) by itself: each wave takes every NWV-th key, a lane 4 dims. Only reached for rows whose partial
 // results are not finite, so its time (about 1 us per 30 keys and 4 waves) is not that of ordinary calls.
 template <int KF, int VF, int NWV>
 __device__ void tree_careful_row(const TreeArgs &a, int i, int h, float *s_o, float *s_ml, float4 &o, float &l) {
@@ -144,7 +147,8 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs &a, int i) {
 
 // One workgroup of NWV waves per row: wave w sums the ranges w, w + NWV, .. (a lane 4 dims, 8 ranges requested
 // together), then the waves' sums meet in LDS. The launch takes as many waves as leave each 8 ranges: one row's 128
-// ranges on 4 waves took 12.4 us, a latency after the other.
+// ranges on 4 waves took 12.4 us, a latency after the other. 4 us for a few rows, a launch and two latencies; 15 us for
+// 1024 rows of 64 ranges, whose 67 MB it reads at 4.5 TB/s.
 template <int KF, int VF, int NWV>
 __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -220,6 +224,27 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
 // where the i-th key range begins, in steps (the host has divided: a division here is 200 cycles before the first load)
 __device__ __forceinline__ int range_begin(const TreeArgs &a, int i) { return __builtin_amdgcn_readfirstlane(i * a.share + min(i, a.spare)); }
 
+// Which KV head, key range and row block a workgroup takes. Workgroups 8 apart run on the same XCD, whose L2 reads a
+// range once for its row blocks: range u of all KV heads' goes to XCD u % 8 with every row block, and the row blocks of
+// the last nkv * splits % 8 ranges are shared out evenly. (Those by whole ranges as well: 3 row blocks of 84 ranges put 33
+// workgroups on 4 XCDs' 32 CUs, 66 us in place of 33. Every XCD a run of neighbouring ranges instead: 131072 keys took
+// 52 us in place of 48.)
+__device__ __forceinline__ bool tree_place(const TreeArgs &a, int &hk, int &split, int &rb) {
+  const int xcd = (int)(blockIdx.x & 7);
+  int at = (int)(blockIdx.x >> 3), unit;
+  const bool whole = at < a.whole;
+  if (!whole) {
+    at = xcd * a.share_out + at - a.whole;
+    if (at >= a.left) return false;
+  }
+  unit = a.nrb == 1 ? at : at / a.nrb;
+  rb = at - unit * a.nrb;
+  unit = whole ? 8 * unit + xcd : a.nkv * a.splits / 8 * 8 + unit;
+  hk = unit / a.splits;
+  split = unit - hk * a.splits;
+  return true;
+}
+
 // The rows r, r + 1, .. of a KV head as (token, query head of the group), r < rows
 struct RowWalk {
   int tok, h;
@@ -282,9 +307,12 @@ __device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
 }
 
 // ------------------------------------------------------------------ few rows: every wave a key range of its own
-// A workgroup holds 16 MT rows; each of its 4 waves streams a key range, 32 keys a step, without barriers until the
-// ranges are joined. Bound by the memory: a step's K is asked for as soon as the last one's has been read, its V
-// likewise, so that a wave has nearly a whole step (17 KB in q8_0) on its way into its own part of LDS at all times.
+// A workgroup holds 16 rows; each of its 4 waves streams a key range, 32 keys a step, without barriers until the
+// ranges are joined. A step's K is asked for as soon as the last one's has been read, its V likewise, so that a wave has
+// nearly a whole step (17 KB in q8_0) on its way into its own part of LDS at all times. Bound by the memory over long
+// contexts (4 rows of q8_0: 131072 keys 48 us, 5.9 TB/s; 32768 17.5 us, 4.1) and by latencies over short ones (600
+// keys: 7 us with 4 rows, 12 with 28, most of it the first step's). Loads into registers took 27.9 us where this takes
+// 17.5; 8 waves a workgroup, for half the ranges to join, 18.9 (53 against 48 at 131072 keys).
 //
 // Scores are computed transposed, S^T = K Q^T: lane (n, g) = (lane % 16, lane / 16) then holds keys 4 g .. 4 g + 3 of
 // a 16-key tile for row n, which is P^T's operand of O^T = V^T P^T as it stands if slot (g, j) of the 32-key
@@ -298,9 +326,9 @@ __device__ __forceinline__ int tree_dim(int dt, int m) {
   return VF == BKV_Q8_0 ? 16 * m + dt : 128 * (dt >> 3) + 8 * m + (dt & 7);
 }
 
-template <int KF, int VF, int PG, int MT>
-__global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 2 : 1) void tree_stream_kernel(TreeArgs a) {
-  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16 * MT;
+template <int KF, int VF, int PG>
+__global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void tree_stream_kernel(TreeArgs a) {
+  constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16;
   constexpr uint32_t oV = kTreeKeys * KRB, oSK = oV + kTreeKeys * VRB, oSV = oSK + (KF ? 512 : 0), kWave = oSV + (VF ? 512 : 0);
   constexpr int kOS = kHd + 4;                     // a row of the join
   constexpr uint32_t kJoin = 4 * RB * kOS * 4;
@@ -308,10 +336,8 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   __shared__ float s_m[4][RB], s_l[4][RB];
   __shared__ uint32_t s_lv[4];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  // (workgroups 8 apart run on the same XCD: the row blocks of one key range are neighbours there)
-  const int unit = (int)(8 * blockIdx.z + blockIdx.x), rb = blockIdx.y;
-  if (unit >= a.nkv * a.splits) return;
-  const int hk = unit / a.splits, split = unit - hk * a.splits;
+  int hk, split, rb;
+  if (!tree_place(a, hk, split, rb)) return;
   const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
   const int t0 = range_begin(a, split * 4 + w), t1 = range_begin(a, split * 4 + w + 1);
@@ -364,13 +390,13 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
     for (int u = 0; u < 32 * LR / 64; ++u) take(t, vd, (64 / LR) * u + lane / LR, vrow, 16 * (lane % LR), my0 + oV + 1024 * u);
     if constexpr (VF) scales(t, vsc, my0 + oSV);
   };
-  // the workgroup's rows of Q first, 4 MT of them by each wave into the place of its V (piece c of row r at c ^ r % 16),
+  // the workgroup's rows of Q first, 4 of them by each wave into the place of its V (piece c of row r at c ^ r % 16),
   // then K; V once the rows have been read
   {
-    RowWalk at(min(RB * rb + 4 * MT * w, R - 1), a.grp);
+    RowWalk at(min(RB * rb + 4 * w, R - 1), a.grp);
 #pragma unroll
-    for (int j = 0; j < 4 * MT; ++j) {
-      const int row = 4 * MT * w + j;
+    for (int j = 0; j < 4; ++j) {
+      const int row = 4 * w + j;
       load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(at.tok, hk * a.grp + at.h)) + 16 * (lane ^ (row & 15)), my0 + oV + 1024 * j);
       if (RB * rb + row + 1 < R) at.next(a.grp);
     }
@@ -384,26 +410,18 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   }
   lds_barrier();
 
-  int tok[MT];
-  h8 qh[MT][8];                                    // row 16 mt + n, dims 32 b + 8 g ..
+  const int tok = min(RB * rb + n, R - 1) / a.grp;
+  h8 qh[8];                                        // row n, dims 32 b + 8 g ..
+  const uint8_t *q = sm + kWave * (n / 4) + oV + 1024 * (n % 4);
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = min(RB * rb + 16 * mt + n, R - 1);
-    tok[mt] = r / a.grp;
-    const int row = 16 * mt + n;
-    const uint8_t *q = sm + kWave * (row / (4 * MT)) + oV + 1024 * (row % (4 * MT));
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const float4 x = *reinterpret_cast<const float4 *>(q + 16 * ((8 * b + 2 * g) ^ n)), y = *reinterpret_cast<const float4 *>(q + 16 * ((8 * b + 2 * g + 1) ^ n));
-      qh[mt][b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
-    }
+  for (int b = 0; b < 8; ++b) {
+    const float4 x = *reinterpret_cast<const float4 *>(q + 16 * ((8 * b + 2 * g) ^ n)), y = *reinterpret_cast<const float4 *>(q + 16 * ((8 * b + 2 * g + 1) ^ n));
+    qh[b] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
   }
   lds_barrier();
   if (t0 < t1) request_v(t0);
-  f4 o[MT][16] = {};
-  float m[MT], l[MT];                              // m: the reference less kPScale
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) { m[mt] = -INFINITY; l[mt] = 0.0f; }
+  f4 o[16] = {};
+  float m = -INFINITY, l = 0.0f;                   // m: the reference less kPScale
   int lv = 0;                                      // the outputs' level
   uint32_t lv_any = 0;                             // all that were taken, or-ed
 
@@ -413,12 +431,10 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
     there = there_next;
     // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
     const bool whole = kb + kTreeKeys <= a.pos0 && (!PG || there == ~0u);
-    uint32_t win[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) win[mt] = (whole ? ~0u : kb + kTreeKeys > a.pos0 ? there & tree_window(a, tok[mt], kb) : there) >> (4 * g);
+    const uint32_t win = (whole ? ~0u : kb + kTreeKeys > a.pos0 ? there & tree_window(a, tok, kb) : there) >> (4 * g);
     // ---- scores
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NV) : "memory");   // (this step's V may still be on its way)
-    f4 s[MT][2] = {};
+    f4 s[2] = {};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if constexpr (KF) {
@@ -430,62 +446,54 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
           const uint2 r = *reinterpret_cast<const uint2 *>(my + KRB * (16 * u + n) + 16 * ((2 * b + (g >> 1)) ^ n) + 8 * (g & 1));
           const uint32_t x = r.x ^ 0x80808080u, y = r.y ^ 0x80808080u;
           const uint4 kv = make_uint4(as_u(bytes_h2<0x04010400u>(x)), as_u(bytes_h2<0x04030402u>(x)), as_u(bytes_h2<0x04010400u>(y)), as_u(bytes_h2<0x04030402u>(y)));
+          const f4 z = mfma16(__builtin_bit_cast(h8, kv), qh[b], f4{});
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const f4 z = mfma16(__builtin_bit_cast(h8, kv), qh[mt][b], f4{});
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              s[mt][u][i] = __builtin_fmaf(z[i], (float)__builtin_bit_cast(_Float16, (uint16_t)((&sc[i].x)[b >> 1] >> (16 * (b & 1)))), s[mt][u][i]);
-          }
+          for (int i = 0; i < 4; ++i)
+            s[u][i] = __builtin_fmaf(z[i], (float)__builtin_bit_cast(_Float16, (uint16_t)((&sc[i].x)[b >> 1] >> (16 * (b & 1)))), s[u][i]);
         }
       } else {
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
           const h8 kf = *reinterpret_cast<const h8 *>(my + KRB * (16 * u + n) + 16 * ((4 * b + g) ^ n));
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) s[mt][u] = mfma16(kf, qh[mt][b], s[mt][u]);
+          s[u] = mfma16(kf, qh[b], s[u]);
         }
       }
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (t + 1 < t1) {
       look_up(t + 1);
       request_k(t + 1);
     }
     // ---- probabilities
-    h8 ph[MT], pl[MT];
+    h8 ph, pl;
+    if (!whole) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) s[mt][j >> 2][j & 3] = -INFINITY;
-      }
-      float top = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
-                        fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3]))) * a.scale2;
-      if (__any(top > m[mt] + (kLift + kPScale))) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m[mt], top - kPScale);
-        const float f = mn == m[mt] ? 1.0f : exp2f(m[mt] - mn);
-        m[mt] = mn;
-        l[mt] *= f;
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt) o[mt][dt] *= f;
-      }
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][j >> 2][j & 3], a.scale2, -m[mt]));
-      if (!whole) {                                // (where nothing was seen yet, -Inf - -Inf)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!((win[mt] >> ((j & 4) * 4 + (j & 3))) & 1u)) p[j] = 0.0f;
-      }
-      l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-      split_p(p, ph[mt], pl[mt]);
+      for (int j = 0; j < 8; ++j)
+        if (!((win >> ((j & 4) * 4 + (j & 3))) & 1u)) s[j >> 2][j & 3] = -INFINITY;
     }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * a.scale2;
+    if (__any(top > m + (kLift + kPScale))) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top - kPScale);
+      const float f = mn == m ? 1.0f : exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < 16; ++dt) o[dt] *= f;
+    }
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], a.scale2, -m));
+    if (!whole) {                                  // (where nothing was seen yet, -Inf - -Inf)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!((win >> ((j & 4) * 4 + (j & 3))) & 1u)) p[j] = 0.0f;
+    }
+    l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    split_p(p, ph, pl);
     // ---- P V
     if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK) : "memory");   // (the next step's K may still be on its way)
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -506,9 +514,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
       if (level != lv) {
         const float x = __builtin_ldexpf(1.0f, 8 * (lv - level));
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int dt = 0; dt < 16; ++dt) o[mt][dt] *= x;
+        for (int dt = 0; dt < 16; ++dt) o[dt] *= x;
         lv = level;
       }
       h2 d[4];
@@ -528,12 +534,9 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
         }
         const h8 vh = __builtin_bit_cast(h8, make_uint4(ah[0], ah[1], ah[2], ah[3]));
         const h8 vl = __builtin_bit_cast(h8, make_uint4(al[0], al[1], al[2], al[3]));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vl, ph[mt], o[mt][dt]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, pl[mt], o[mt][dt]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][dt] = mfma16(vh, ph[mt], o[mt][dt]);
+        o[dt] = mfma16(vl, ph, o[dt]);
+        o[dt] = mfma16(vh, pl, o[dt]);
+        o[dt] = mfma16(vh, ph, o[dt]);
       }
     } else {
 #pragma unroll
@@ -548,10 +551,8 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
           for (int j = 0; j < 4; ++j)
             av[j] = __builtin_amdgcn_perm((&r[2 * j + 1].x)[e >> 1], (&r[2 * j].x)[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
           const h8 vh = __builtin_bit_cast(h8, make_uint4(av[0], av[1], av[2], av[3]));
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) o[mt][8 * hf + e] = mfma16(vh, pl[mt], o[mt][8 * hf + e]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) o[mt][8 * hf + e] = mfma16(vh, ph[mt], o[mt][8 * hf + e]);
+          o[8 * hf + e] = mfma16(vh, pl, o[8 * hf + e]);
+          o[8 * hf + e] = mfma16(vh, ph, o[8 * hf + e]);
         }
       }
     }
@@ -562,60 +563,58 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 && MT == 1 ? 
   // ---- the 4 ranges joined, one partial result per row and workgroup
   float *s_o = reinterpret_cast<float *>(sm);
   const int64_t rows = (int64_t)a.n_q * a.nh;
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    l[mt] += __shfl_xor(l[mt], 16);
-    l[mt] += __shfl_xor(l[mt], 32);
-    if (g == 0) { s_m[w][16 * mt + n] = m[mt]; s_l[w][16 * mt + n] = l[mt]; }
-  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) { s_m[w][n] = m; s_l[w][n] = l; }
   if (lane == 0) s_lv[w] = lv_any;
   __syncthreads();                                 // (and the waves' own parts have been read)
+  const float mm = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+  const float f = m == -INFINITY ? 0.0f : exp2f(m - mm), fo = VF ? __builtin_ldexpf(f, 8 * lv - 9) : f;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int row = 16 * mt + n;
-    const float mm = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-    const float f = m[mt] == -INFINITY ? 0.0f : exp2f(m[mt] - mm), fo = VF ? __builtin_ldexpf(f, 8 * lv - 9) : f;
+  for (int dt = 0; dt < 16; dt += 4)               // (4 products' dims are neighbours)
 #pragma unroll
-    for (int dt = 0; dt < 16; dt += 4)             // (4 products' dims are neighbours)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4 *>(&s_o[(RB * w + row) * kOS + tree_dim<VF>(dt, 4 * g + i)]) =
-            make_float4(o[mt][dt][i] * fo, o[mt][dt + 1][i] * fo, o[mt][dt + 2][i] * fo, o[mt][dt + 3][i] * fo);
-  }
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<float4 *>(&s_o[(RB * w + n) * kOS + tree_dim<VF>(dt, 4 * g + i)]) =
+          make_float4(o[dt][i] * fo, o[dt + 1][i] * fo, o[dt + 2][i] * fo, o[dt + 3][i] * fo);
   __syncthreads();
+  const int row = threadIdx.x >> 4, c = threadIdx.x & 15, r = RB * rb + row;
+  if (r < R) {
+    const int ti = r / a.grp;
+    const int64_t at = (int64_t)split * rows + (int64_t)ti * a.nh + hk * a.grp + r - ti * a.grp;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int row = 16 * mt + (threadIdx.x >> 4), c = threadIdx.x & 15, r = RB * rb + row;
-    if (r < R) {
-      const int ti = r / a.grp;
-      const int64_t at = (int64_t)split * rows + (int64_t)ti * a.nh + hk * a.grp + r - ti * a.grp;
+    for (int k = 0; k < 4; ++k) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 x = *reinterpret_cast<const float4 *>(&s_o[(RB * j + row) * kOS + 4 * c + 64 * k]);
-          v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-        }
-        *reinterpret_cast<float4 *>(a.part + at * kHd + 4 * c + 64 * k) = v;
+      for (int j = 0; j < 4; ++j) {
+        const float4 x = *reinterpret_cast<const float4 *>(&s_o[(RB * j + row) * kOS + 4 * c + 64 * k]);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
       }
-      if (c == 0) {
-        const float mr = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-        float lr = 0.0f;
+      *reinterpret_cast<float4 *>(a.part + at * kHd + 4 * c + 64 * k) = v;
+    }
+    if (c == 0) {
+      const float mr = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+      float lr = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) lr += s_m[j][row] == -INFINITY ? s_l[j][row] : s_l[j][row] * exp2f(s_m[j][row] - mr);
-        a.ml[at] = make_float2(mr, marked_sum(lr, s_lv[0] | s_lv[1] | s_lv[2] | s_lv[3]));
-      }
+      for (int j = 0; j < 4; ++j) lr += s_m[j][row] == -INFINITY ? s_l[j][row] : s_l[j][row] * exp2f(s_m[j][row] - mr);
+      a.ml[at] = make_float2(mr, marked_sum(lr, s_lv[0] | s_lv[1] | s_lv[2] | s_lv[3]));
     }
   }
 }
 
 // ------------------------------------------------------------------ many rows: key tiles in LDS
-// A workgroup of 4 waves holds 64 MT rows, each wave 16 MT of them with all 256 outputs in registers, and steps
-// through its key range 32 keys at a time. A step's cache bytes are loaded straight into LDS while the step before it
-// is computed, and turned once into the products' operands for all of the workgroup's rows: K's bytes into fp16
-// (fp16 K needs nothing: its pieces land where they are wanted), V transposed, so that a lane's 8 keys of one dim are
-// 16 bytes, as vh (and vl for q8_0). S^T and O^T are formed as in the kernel above, so P never leaves its lane.
+// 8 waves hold 16 MT rows each with all 256 outputs in registers, and step through the workgroup's key range 32 keys at
+// a time. A step's cache bytes are loaded straight into LDS while the step before it is computed, and turned once into
+// the products' operands for all of the workgroup's rows: K's bytes into fp16 (fp16 K needs nothing: its pieces land
+// where they are wanted), V transposed, so that a lane's 8 keys of one dim are 16 bytes, as vh (and vl for q8_0). S^T and
+// O^T are formed as in the kernel above, so P never leaves its lane. Two waves share a SIMD, and the second one's P V
+// runs a step late, beside the first one's scores: hence two steps' operands of K and three of V. With 128 rows the
+// registers leave room for 4 more waves, which bring and turn the bytes.
+//
+// Bound by what two waves a SIMD can overlap: of a step's 7500 cycles (256 rows, q8_0) the matrix cores work 4096, the
+// vector unit (softmax, the scales of K's blocks, the operands) 4200, LDS about as many. q8_0 takes 4 products and fp16
+// 3 where the formula has 2. 1024 rows onto 32768 keys: 82 us (34 GFLOP, 0.42 PFLOP/s), 8192 onto 8192 164 us (71
+// GFLOP, 0.43), 1008 onto 65536 in fp16 110 us (68 GFLOP, 0.61). Of 82 us 25 are the rows' first bytes and the partial
+// results (67 MB written).
 //
 // LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
 // and 16 + 4 g .. 16 + 4 g + 3) at 8 (d / 2) + ((4 (d % 2) + g) ^ kx(d)), kx chosen so that both the 8 dims next to
@@ -640,9 +639,8 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   __shared__ __attribute__((aligned(128))) uint8_t sm[oSK + (KF ? 512 : 0)];
   const uint32_t sm0 = lds_addr(sm);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  const int unit = (int)(8 * blockIdx.z + blockIdx.x), rb = blockIdx.y;
-  if (unit >= a.nkv * a.splits) return;
-  const int hk = unit / a.splits, split = unit - hk * a.splits;
+  int hk, split, rb;
+  if (!tree_place(a, hk, split, rb)) return;
   const int R = a.n_q * a.grp;
   const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
   const int t0 = range_begin(a, split), t1 = range_begin(a, split + 1);
@@ -1046,29 +1044,52 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
 static inline int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Which kernel a call takes, by the rows of one KV head: the stream kernel with 16 or 32 rows, up to 128 one tile of
-// 128 rows, beyond that tiles of 256 (what each measured: see the kernels).
-enum { kTree16, kTree32, kTree128, kTree256 };
-static int tree_kind(int64_t rows) { return rows <= 16 ? kTree16 : rows <= 32 ? kTree32 : rows <= 128 ? kTree128 : kTree256; }
-static int tree_rows(int kind) { return kind == kTree16 ? 16 : kind == kTree32 ? 32 : kind == kTree128 ? 128 : 256; }
+// Which kernel a call takes: the one with the least estimate of its time in us. The estimates' constants are this card's,
+// and choose what was faster wherever two kernels differ by more than 2 us of (kernel + join), among them, 4 KV heads of
+// q8_0, blocks of 16 / tiles of 128 / of 256:
+//   onto 600 keys      8 tokens 11.9 / 13.0,  25 tokens 13.2 / 17.9 / 19.6
+//   onto 2000         33 tokens 19.4 / 25.7 / 30.6,  128 tokens 35.5 / 35.9 / 43.9
+//   onto 8192          8 tokens 17.6 / 20.8,  25 tokens 31.6 / 30.1 / 33.1,  64 tokens .. / 42.2 / 50.2,  300 .. / 134 / 119
+//   onto 32768         8 tokens 32.8 / 40.1,  12 tokens 42.9 / 42.4,  33 tokens .. / 93 / 79,  64 tokens .. / 101 / 93
+// (of fp16, whose tiles have 3 products a step and no scales: 64 tokens onto 32768 68 in tiles of 128, 76 in 256; onto
+// 65536 124 / 119, in pages 137 / 127.)
+enum { kTree16, kTree128, kTree256 };
 // workgroups that the key split aims for: one per CU (two of the stream kernel's would fit in q8_0, and leave twice the
 // ranges to join: 1 token onto 32768 keys 18.7 + 7.6 us against 18.2 + 5.6, onto 131072 56.0 + 7.5 against 48.4 + 5.4)
 constexpr int kTreeFill = 256;
 
-TreePlan plan_tree(int nh, int nkv, int64_t pos0, int n_q, size_t base) {
+TreePlan plan_tree(int nh, int nkv, int kf, int vf, bool paged, int64_t pos0, int n_q, size_t base) {
   TreePlan p{};
   const int64_t rows = (int64_t)n_q * (nh / nkv), steps = cdiv(pos0 + n_q, kTreeKeys);
-  p.kind = tree_kind(rows);
-  p.nrb = (int)cdiv(rows, tree_rows(p.kind));
-  // A wave of the stream kernel takes a step at least. The tiles: a step fewer per workgroup saves 2 us (4 with 256 rows),
-  // a key range more costs 0.2 us per 1024 rows of partial results to write and join; the least of their sum, measured:
-  // 25 tokens onto 500 keys 18.5 us in 17 ranges, 23.5 in 5; onto 2000 28.1 in 63, 24.4 in 24; 64 onto 2000 41.4 in 64,
-  // 39.3 in 24.
-  const int64_t most = p.kind <= kTree32 ? cdiv(steps, 4) : std::max<int64_t>(1, (int64_t)std::sqrt(80.0 * tree_rows(p.kind) * (double)steps / ((double)n_q * nh)));
-  p.splits = (int)std::min<int64_t>(std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, steps), most), std::max<int64_t>(1, kTreeFill / ((int64_t)nkv * p.nrb)));
-  const int64_t ranges = p.splits * (p.kind <= kTree32 ? 4 : 1);
-  p.share = (int)(steps / ranges);
-  p.spare = (int)(steps % ranges);
+  const int kq = kf == BKV_Q8_0, vq = vf == BKV_Q8_0;
+  const double mb = (double)n_q * nh / 1024.0;       // of partial results, for a key range
+  const double read = (double)(pos0 + n_q) * nkv * ((kq ? 272 : 512) + (vq ? 272 : 512)) / 5.5e6;
+  double least = 0.0;
+  for (int kind = kTree16; kind <= kTree256; ++kind) {
+    const int rb = kind == kTree16 ? 16 : kind == kTree128 ? 128 : 256, waves = kind == kTree16 ? 4 : 1;
+    const int64_t nrb = cdiv(rows, rb), full = std::min<int64_t>(rows, rb);
+    // A step of a wave (stream kernel) or of a workgroup, and what is there without any. q8_0 adds the scales and the
+    // products of vl, pages their look-up; 64 rows leave every SIMD of the tile of 128 one wave.
+    const double step = (paged ? 0.2 : 0.0) +
+                        (kind == kTree16    ? 2.2 + 0.5 * vq
+                         : kind == kTree128 ? (1.55 + 0.35 * kq + 0.5 * vq) * (full <= 64 ? 2.0 / 3.0 : 1.0)
+                                            : 2.6 + 0.8 * kq + 0.9 * vq - 0.6 * kq * vq);
+    const double start = kind == kTree16 ? 5.0 : kind == kTree128 ? 6.0 + 7.0 * (double)full / 128.0 : 12.0 + 8.0 * (double)full / 256.0;
+    // A wave of the stream kernel takes a step at least. The tiles: a step fewer per workgroup saves `step`, a key range
+    // more costs 0.2 us per MB of partial results to write and join; the least of their sum.
+    const int64_t most = kind == kTree16 ? cdiv(steps, waves) : std::max<int64_t>(1, (int64_t)std::sqrt(step * (double)steps / (0.2 * mb)));
+    const int64_t splits = std::min(std::min<int64_t>(std::min<int64_t>(kTreeMaxSplit, steps), most), std::max<int64_t>(1, kTreeFill / (nkv * nrb)));
+    const double rounds = (double)cdiv(nkv * nrb * splits, kTreeFill);
+    const double n_steps = kind == kTree16 ? (double)cdiv(steps, splits * waves) : (double)steps / (double)splits;
+    const double cost = std::max(rounds * (start + step * n_steps), 3.0 + read) + 0.2 * mb * (double)splits;
+    if (kind > kTree16 && cost >= least) continue;
+    least = cost;
+    p.kind = kind;
+    p.nrb = (int)nrb;
+    p.splits = (int)splits;
+    p.share = (int)(steps / (splits * waves));
+    p.spare = (int)(steps % (splits * waves));
+  }
   p.off_ml = base;
   p.off_part = up256(base + (size_t)p.splits * n_q * nh * sizeof(float2));
   p.total = up256(p.off_part + (size_t)p.splits * n_q * nh * kHd * sizeof(float));
@@ -1085,10 +1106,9 @@ size_t tree_workspace_bound(int nh, int nkv, size_t base) {
 
 template <int KF, int VF, int PG>
 static hipError_t launch_tree_main(const TreeArgs &a, const TreePlan &p, hipStream_t st) {
-  const dim3 grid(8, p.nrb, (unsigned)cdiv((int64_t)a.nkv * a.splits, 8));
+  const dim3 grid(8 * (unsigned)(a.whole + a.share_out));
   switch (p.kind) {
-    case kTree16: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 1>), grid, dim3(256), 0, st, a); break;
-    case kTree32: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG, 2>), grid, dim3(256), 0, st, a); break;
+    case kTree16: hipLaunchKernelGGL((tree_stream_kernel<KF, VF, PG>), grid, dim3(256), 0, st, a); break;
     case kTree128: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 1>), grid, dim3(tree_tile_threads(1)), 0, st, a); break;
     default: hipLaunchKernelGGL((tree_tile_kernel<KF, VF, PG, 2>), grid, dim3(tree_tile_threads(2)), 0, st, a); break;
   }
