@@ -9,7 +9,8 @@ namespace bkv {
 // ------------------------------------------------------------------ read
 // A head row is 256 values; 32 lanes take one, 8 values each, so that loads are 8 bytes (q8_0) or 16 (fp16) per
 // lane and stores 16 or 32, all whole lines per row. Rows of one tensor run head first, then position. Bound by
-// the memory; each thread asks for kReadRows rows before it stores the first.
+// the memory; each thread asks for kReadRows rows before it stores the first. 32768 positions of q8_0 as bf16: 31.9 us,
+// 206 MB at 6.4 TB/s; 777 of fp16 as fp32 5.4 us, 9.5 MB; a few positions 2.2 us, a launch.
 constexpr int kReadRows = 4;
 
 template <int OT>
@@ -93,7 +94,8 @@ hipError_t launch_kv_read(const ReadArgs &a, int kf, int vf, int out_type, hipSt
 // A workgroup owns one 64-byte column of one array of one layer and all of the kept tokens: it reads every source
 // into registers, and writes after a barrier, so that a source which another token's write covers has been read
 // (positions of different columns, arrays and layers never meet). 4 lanes take the column's 16-byte pieces of a
-// token, 64 tokens at a time, PT times.
+// token, 64 tokens at a time, PT times. 5 tokens of 8 layers 2.9 us, 300 tokens of 8 fp16 layers 4.0 us: a launch and
+// three latencies (the index, the page, the bytes); the 20 MB of the latter stay in the caches.
 template <int PT>
 __global__ __launch_bounds__(256) void kv_commit_kernel(CommitArgs a) {
   int u = blockIdx.x, arr = 0;

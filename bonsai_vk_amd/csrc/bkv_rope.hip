@@ -12,7 +12,9 @@
 namespace bkv {
 
 // One wave per row, 4 dims per lane; a workgroup takes 8 rows of one token (Q heads, then K, then V), so that a
-// single token's 24 rows run on 3 workgroups and the token's sines are formed once for 8 rows.
+// single token's 24 rows run on 3 workgroups and the token's sines are formed once for 8 rows. 1 token 4.4 us (a
+// launch, the rows' latency and the fp64 sines), 501 tokens 6.1 us (22 MB read and written, 3.6 TB/s: the same chain,
+// with the memory at two thirds of a copy's rate).
 constexpr int kRopeRows = 8;
 
 // the maximum over the 8 lanes that hold a q8_0 block

@@ -18,8 +18,8 @@
 // and so are Inf V under a visible key (ph and pl may have opposite signs) and non-finite scores: whatever is not
 // finite at the end is computed again by tree_careful_row, key by key, in fp32, without the keys that are not seen.
 //
-// Two launches whatever the sizes: by the rows of a KV head tree_stream_kernel (16 or 32) or tree_tile_kernel (128 or
-// 256 a workgroup), then the join.
+// Two launches whatever the sizes: tree_stream_kernel (16 rows a workgroup) or tree_tile_kernel (128 or 256), whichever
+// plan_tree expects to take less time, then the join.
 
 #include <algorithm>
 #include <cmath>
@@ -310,9 +310,10 @@ __device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
 // A workgroup holds 16 rows; each of its 4 waves streams a key range, 32 keys a step, without barriers until the
 // ranges are joined. A step's K is asked for as soon as the last one's has been read, its V likewise, so that a wave has
 // nearly a whole step (17 KB in q8_0) on its way into its own part of LDS at all times. Bound by the memory over long
-// contexts (4 rows of q8_0: 131072 keys 48 us, 5.9 TB/s; 32768 17.5 us, 4.1) and by latencies over short ones (600
-// keys: 7 us with 4 rows, 12 with 28, most of it the first step's). Loads into registers took 27.9 us where this takes
-// 17.5; 8 waves a workgroup, for half the ranges to join, 18.9 (53 against 48 at 131072 keys).
+// contexts (4 rows of q8_0: 131072 keys 49 us, 5.8 TB/s; 32768 17.8 us, 4.0) and by latencies over short ones (600
+// keys: 7 us with 4 rows, 8.3 with 28, most of it the first step's). Loads into registers took 27.9 us where this takes
+// 17.8; 8 waves a workgroup, for half the ranges to join, 18.9 (53 against 48 at 131072 keys); 32 rows a workgroup, which
+// read the cache once, 31.4 where two blocks of 16 take 28.4 and the second reads L2.
 //
 // Scores are computed transposed, S^T = K Q^T: lane (n, g) = (lane % 16, lane / 16) then holds keys 4 g .. 4 g + 3 of
 // a 16-key tile for row n, which is P^T's operand of O^T = V^T P^T as it stands if slot (g, j) of the 32-key
@@ -612,8 +613,8 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
 //
 // Bound by what two waves a SIMD can overlap: of a step's 7500 cycles (256 rows, q8_0) the matrix cores work 4096, the
 // vector unit (softmax, the scales of K's blocks, the operands) 4200, LDS about as many. q8_0 takes 4 products and fp16
-// 3 where the formula has 2. 1024 rows onto 32768 keys: 82 us (34 GFLOP, 0.42 PFLOP/s), 8192 onto 8192 164 us (71
-// GFLOP, 0.43), 1008 onto 65536 in fp16 110 us (68 GFLOP, 0.61). Of 82 us 25 are the rows' first bytes and the partial
+// 3 where the formula has 2. 1024 rows onto 32768 keys: 80 us (34 GFLOP, 0.43 PFLOP/s), 8192 onto 8192 163 us (71
+// GFLOP, 0.43), 1008 onto 65536 in fp16 108 us (68 GFLOP, 0.63). Of 80 us 25 are the rows' first bytes and the partial
 // results (67 MB written).
 //
 // LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
@@ -1096,7 +1097,7 @@ TreePlan plan_tree(int nh, int nkv, int kf, int vf, bool paged, int64_t pos0, in
   return p;
 }
 
-// the largest plan of any call: 65536 rows where the keys are split (256 workgroups of 256),
+// the largest plan of any call: 65536 rows where the keys are split (at most 256 workgroups of at most 256 rows),
 // otherwise every row once
 size_t tree_workspace_bound(int nh, int nkv, size_t base) {
   (void)nkv;
