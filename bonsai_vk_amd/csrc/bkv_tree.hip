@@ -129,20 +129,17 @@ __device__ void tree_careful_row(const TreeArgs &a, int i, int h, float *s_o, fl
   __syncthreads();
 }
 
-// whether row i's token sees any key
+// whether row i's token sees any key (a lane a page, then a lane a drafted token)
 __device__ __forceinline__ bool tree_sees(const TreeArgs &a, int i) {
-  const uint32_t nk = a.pos0 + (uint32_t)a.n_q;
-  if (a.L.page == 0) {
-    if (a.pos0 > 0 || a.mask == nullptr) return true;
-    for (int j = 0; j < a.n_q; j += 32)
-      if (tree_window(a, i, j)) return true;
-    return false;
-  }
-  for (uint32_t k = 0; k < nk; ++k) {
-    if (k >= a.pos0 && !(tree_window(a, i, k) & 1u)) continue;
-    if (slot_checked(a.L, a.pool_pages, k) >= 0) return true;
-  }
-  return false;
+  const int lane = threadIdx.x & 63;
+  if (a.L.page == 0 && a.pos0 > 0) return true;
+  bool some = false;
+  if (a.L.page > 0)
+    for (uint64_t k = (uint64_t)lane * (uint32_t)a.L.page; k < a.pos0; k += 64ull * (uint32_t)a.L.page)
+      some |= slot_checked(a.L, a.pool_pages, (uint32_t)k) >= 0;
+  for (int j = lane; j < a.n_q; j += 64)
+    some |= (tree_window(a, i, (int64_t)a.pos0 + j) & 1u) && slot_checked(a.L, a.pool_pages, a.pos0 + (uint32_t)j) >= 0;
+  return __any(some);
 }
 
 // One workgroup of NWV waves per row: wave w sums the ranges w, w + NWV, .. (a lane 4 dims, 8 ranges requested

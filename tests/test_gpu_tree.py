@@ -11,6 +11,8 @@ from tests.tree_util import (F16, HD, Q8, attention, check_rows, gen, make_cache
 
 pytestmark = pytest.mark.gpu
 FORMATS = [(Q8, Q8), (F16, Q8), (Q8, F16), (F16, F16)]
+# drafts that 16 rows, 128 rows (of them 60, and more than two tiles) and 256 rows a workgroup are chosen for
+KERNELS = [(9, 801), (15, 20000), (70, 6001), (1000, 4011)]
 
 
 def filled(n, kf, vf, seed=1, **kw):
@@ -77,6 +79,64 @@ def test_head_counts(nkv, group, kf, vf):
 def test_longer(kf, vf, n, pos0):
     say(f"tree kf {kf} vf {vf}")
     check(filled(pos0 + n, kf, vf), pos0, n, "tree", gate=False)
+
+
+@pytest.mark.parametrize("kf,vf", FORMATS)
+@pytest.mark.parametrize("page", [0, 48, 64])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_each_kernel(kf, vf, page, n, pos0):
+    say(f"tree kf {kf} vf {vf} page {page}")
+    check(filled(pos0 + n, kf, vf, page=page), pos0, n, "padded")
+
+
+@pytest.mark.parametrize("vf", [Q8, F16])
+@pytest.mark.parametrize("page", [0, 48, 64])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_each_kernel_with_values_that_are_not_finite(vf, page, n, pos0):
+    """NaN in a drafted token's V that most rows do not see, and Inf in its K."""
+    c = filled(pos0 + n, F16, vf, page=page)
+    q, _ = rows(n, c.nh, 5, 0.1)
+    mask = some_mask("tree", n, 9)
+    mask[torch.arange(n, device="cuda") != 1, 0] &= ~2                 # (only token 1 sees token 1)
+    want, _, size = attention(c, 0, pos0, q, mask)
+    others = torch.arange(n, device="cuda") != 1
+    for bad in (math.inf, math.nan):
+        x = torch.full((4, HD), bad, device="cuda")
+        put(c, "v", 0, pos0 + 1, x if vf == F16 else (torch.full((4, HD), 3, device="cuda"), torch.full((4, 8), bad, device="cuda")))
+        put(c, "k", 0, pos0 + 1, x)
+        out, _ = c.attn_tree(0, pos0, q, mask)
+        check_rows(out[others], want[others], tolerance(size, pos0 + n)[others])
+        assert bool(torch.isnan(out[1]).any())
+
+
+@pytest.mark.parametrize("page", [48, 64])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_each_kernel_with_bad_pages(page, n, pos0):
+    """As if the positions of a page outside the pool were absent, in the context and among the drafted tokens."""
+    c = make_cache(pos0 + n, Q8, Q8, page=page)
+    k, v = (torch.randn(pos0 + n, 4, HD, generator=gen(2 + i), device="cuda") for i in range(2))
+    c.append(0, 0, k, v)
+    q, _ = rows(n, c.nh, 4, 0.1)
+    mask = some_mask("tree", n, 2)
+    c.block_table[0, 3], c.block_table[0, 5] = -1, c.cap // page
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    keep = torch.ones(pos0 + n, dtype=torch.bool, device="cuda")
+    keep[3 * page:4 * page] = keep[5 * page:6 * page] = False
+    d = make_cache(int(keep.sum()), Q8, Q8)
+    d.append(0, 0, k[keep], v[keep])
+    want, _, size = attention(d, 0, int(keep[:pos0].sum()), q, mask)
+    check_rows(out, want, tolerance(size, pos0 + n))
+    # nothing but the drafted tokens' own pages, and no page at all
+    first = pos0 // page
+    keep[:first * page], keep[first * page:] = False, True
+    c.block_table[0, :first] = -1
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    d = make_cache(int(keep.sum()), Q8, Q8)
+    d.append(0, 0, k[keep], v[keep])
+    want, _, size = attention(d, 0, pos0 - first * page, q, mask)
+    check_rows(out, want, tolerance(size, pos0 + n))
+    c.block_table[0, :] = -1
+    assert not bool(c.attn_tree(0, pos0, q, mask)[0].any())
 
 
 @pytest.mark.parametrize("kf,vf", [(Q8, Q8), (F16, F16)])
@@ -159,13 +219,7 @@ def test_v_scales_over_their_whole_range(kf, scale):
     check(c, pos0, n, "tree", accurate=False)
 
 
-@pytest.mark.parametrize("n", [3, 8, 30, 70])
-@pytest.mark.parametrize("usual,big", [(1e-3, 100.0), (2e-2, 100.0), (1e-3, 2e4), (1.0, 2e4), (0.05, 1e6), (0.05, 6e6)])
-def test_a_far_larger_v_among_ordinary_ones(n, usual, big):
-    """A drafted token's q8_0 V, and one of the context with hardly any weight, 10^4 to 10^8 times the others': the
-    rows that do not see it keep their precision. Scores are small, so that tolerance() is about 2^-19 of sum p |v|; the
-    2-norm's bound is check()'s."""
-    pos0 = 300
+def far_larger(n, pos0, usual, big):
     c = filled(pos0 + n, Q8, Q8)
     v = torch.randn(pos0 + n, 4, HD, generator=gen(4), device="cuda") * usual
     v[pos0 + 1] *= big / usual
@@ -195,6 +249,21 @@ def test_a_far_larger_v_among_ordinary_ones(n, usual, big):
     tol = tolerance(size, pos0 + n)
     check_rows(out[fin], want[fin], tol[fin])
     assert rel(out[fin], want[fin]) < 4e-6
+
+
+@pytest.mark.parametrize("n", [3, 8, 30, 70])
+@pytest.mark.parametrize("usual,big", [(1e-3, 100.0), (2e-2, 100.0), (1e-3, 2e4), (1.0, 2e4), (0.05, 1e6), (0.05, 6e6)])
+def test_a_far_larger_v_among_ordinary_ones(n, usual, big):
+    """A drafted token's q8_0 V, and one of the context with hardly any weight, 10^4 to 10^8 times the others': the
+    rows that do not see it keep their precision. Scores are small, so that tolerance() is about 2^-19 of sum p |v|; the
+    2-norm's bound is check()'s."""
+    far_larger(n, 300, usual, big)
+
+
+@pytest.mark.parametrize("usual,big", [(2e-2, 100.0), (1e-3, 2e4), (0.05, 1e6)])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_a_far_larger_v_in_each_kernel(n, pos0, usual, big):
+    far_larger(n, pos0, usual, big)
 
 
 def test_fp16_values_over_their_whole_range():

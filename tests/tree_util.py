@@ -123,6 +123,10 @@ def attention(c, layer, pos0, q, mask, gate=None):
         top = max(top, float(fin[torch.isfinite(fin)].max()))
         some = see.any(1)
         p = torch.softmax(s[some], 1)
+        if bool(torch.isfinite(vh).all()):
+            out[some, h], size[some, h] = p @ vh, p @ vh.abs()
+            every[some, h] = see[some].double() @ vh.abs()
+            continue
         for i, row in zip(torch.nonzero(some).flatten().tolist(), p):
             m = see[i]
             out[i, h] = row[m] @ vh[m]
