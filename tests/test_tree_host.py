@@ -109,6 +109,7 @@ def test_attn_tree_refusals():
     d = desc()
     assert tree(desc(hd=128)) == EUNSUPPORTED
     assert tree(desc(nh=15)) == -2
+    assert tree(desc(nh=1 << 22), n=1024) == EUNSUPPORTED          # (rows are counted in 32 bits)
     assert tree(d, layer=8) == EINVAL and tree(d, layer=-1) == EINVAL
     assert tree(d, n=-1) == EINVAL and tree(d, n=1025) == EINVAL
     assert tree(d, n=0, q=None, out=None, ws=None) == OK
