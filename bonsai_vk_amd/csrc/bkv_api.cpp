@@ -860,7 +860,7 @@ int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_kee
 
 size_t bkv_workspace_bytes(const bkv_cache_desc *d, int op, uint32_t max_ctx) {
   if (check(d) || max_ctx == 0) return 0;
-  if (op == BKV_OP_TREE) return tree_workspace_bound(d->nh, d->nkv, prefill_base(d));
+  if (op == BKV_OP_TREE) return tree_workspace_bound(d->nh, prefill_base(d));
   if (op == BKV_OP_PREFILL)
     return std::max(prefill_workspace_bound(d->nh, d->nkv, prefill_base(d)),
                     prefill_exact_workspace(d->nh, d->nkv, max_ctx, prefill_base(d)));

@@ -259,7 +259,7 @@ struct TreePlan {
   size_t off_ml, off_part, total;
 };
 TreePlan plan_tree(int nh, int nkv, int kf, int vf, bool paged, int64_t pos0, int n_q, size_t base);
-size_t tree_workspace_bound(int nh, int nkv, size_t base);
+size_t tree_workspace_bound(int nh, size_t base);
 hipError_t launch_tree(const TreeArgs &a, const TreePlan &p, int kf, int vf, hipStream_t st);
 
 struct RopeArgs {

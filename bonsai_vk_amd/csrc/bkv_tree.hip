@@ -1096,8 +1096,7 @@ TreePlan plan_tree(int nh, int nkv, int kf, int vf, bool paged, int64_t pos0, in
 
 // the largest plan of any call: 65536 rows where the keys are split (at most 256 workgroups of at most 256 rows),
 // otherwise every row once
-size_t tree_workspace_bound(int nh, int nkv, size_t base) {
-  (void)nkv;
+size_t tree_workspace_bound(int nh, size_t base) {
   const size_t rows = std::max<size_t>(65536, (size_t)BKV_TREE_MAX_Q * nh);
   return base + up256(rows * sizeof(float2)) + up256(rows * kHd * sizeof(float)) + 256;
 }

@@ -89,6 +89,23 @@ def test_each_kernel(kf, vf, page, n, pos0):
     check(filled(pos0 + n, kf, vf, page=page), pos0, n, "padded")
 
 
+@pytest.mark.parametrize("kf,vf", [(Q8, Q8), (F16, F16)])
+@pytest.mark.parametrize("nkv", [1, 2, 3])
+@pytest.mark.parametrize("n,pos0", [(1, 20000), (40, 30000)])
+def test_few_heads_many_ranges(kf, vf, nkv, n, pos0):
+    """Up to 128 ranges of the keys, and numbers of ranges and row blocks that 8 does not divide."""
+    say(f"tree heads {nkv} kf {kf}")
+    check(filled(pos0 + n, kf, vf, nkv=nkv), pos0, n, "tree")
+
+
+@pytest.mark.parametrize("kf,vf", [(Q8, Q8), (F16, F16)])
+@pytest.mark.parametrize("nkv,group,n", [(3, 5, 41), (5, 3, 43), (16, 4, 65), (1, 33, 31), (16, 8, 600), (8, 8, 1024)])
+def test_places(kf, vf, nkv, group, n):
+    """Row blocks shared out over the XCDs, and more workgroups than one round of them."""
+    say(f"tree heads {nkv} x {group} n {n}")
+    check(filled(700 + n, kf, vf, nkv=nkv, group=group), 700, n, "tree", gate=False)
+
+
 @pytest.mark.parametrize("vf", [Q8, F16])
 @pytest.mark.parametrize("page", [0, 48, 64])
 @pytest.mark.parametrize("n,pos0", KERNELS)
