@@ -113,6 +113,19 @@ __device__ __forceinline__ int64_t slot_t(const LayerView &L, int64_t pos) {
   }
 }
 
+// Loads straight into LDS, not waited for: 16 (4) bytes per lane from src, or from base + off, to dst + 16 (4) * lane;
+// dst is the same in all lanes. A scalar write of M0 and the load that uses it need a wait state between them, which
+// the hardware does not insert (nor the compiler, inside an asm string).
+__device__ __forceinline__ void load_to_lds(const void *src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(const void *base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ void load4_to_lds(const void *src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+
 // slot_of with the block table's entries held against the pool: -1 where the position's page lies outside it
 __device__ __forceinline__ int slot_checked(const LayerView &L, int pool_pages, uint32_t pos) {
   if (L.page == 0) return (int)pos;

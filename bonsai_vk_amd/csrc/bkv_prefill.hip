@@ -1075,9 +1075,7 @@ __global__ __launch_bounds__(512, 1) void prefill_pv64_kernel(PrefillXArgs a) {
       const int sw = VF ? (i & 3) : 2 * ((i >> 1) & 3);
       const uint8_t *src = a.L.vd + (slot_t<PG>(a.L, key) * a.nkv + g) * row_bytes(VF ? BKV_Q8_0 : BKV_F16) +
                            256 * (u >> 1) + 16 * ((lane >> 2) ^ sw);
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
-                   "s"(__builtin_amdgcn_readfirstlane(vbase + (uint32_t)VB * (uint32_t)(tt % 3) + 1024u * (i + 16 * (u >> 1))))
-                   : "memory", "m0");
+      load_to_lds(src, __builtin_amdgcn_readfirstlane(vbase + (uint32_t)VB * (uint32_t)(tt % 3) + 1024u * (i + 16 * (u >> 1))));
     }
   };
   // tile t's p16 into the P buffer pb, its block scales into vsk

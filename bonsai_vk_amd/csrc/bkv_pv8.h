@@ -123,11 +123,9 @@ __device__ __forceinline__ void pv8_dma_region(uint32_t region, RowF rows, SclF 
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const uint8_t *src = rows(4 * i + r) + 16 * (sl ^ (i & 3));
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(region + 1024u * i)
-                 : "memory", "m0");
+    load_to_lds(src, region + 1024u * i);
   }
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(scl(lane)), "s"(region + (uint32_t)kPv8Scales)
-               : "memory", "m0");
+  load_to_lds(scl(lane), region + (uint32_t)kPv8Scales);
 }
 
 // the region from registers: vd[i] = chunk lane % 16 of key 4 i + lane / 16, vs[i] = that key's

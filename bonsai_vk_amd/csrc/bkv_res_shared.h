@@ -105,8 +105,7 @@ __device__ __forceinline__ void stage_k_wave(uint4 *kt, const SlotMap &sm, int n
     const uint8_t *src = (KF == BKV_Q8_0 && col == 16)
                              ? sm.L->ks + (sl * nkv + g) * kScaleRowBytes
                              : sm.L->kd + (sl * nkv + g) * RB + (ch * 16 + (col & 15)) * 16;
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
-                 :: "v"(src), "s"(base + 1024u * i) : "memory", "m0");
+    load_to_lds(src, base + 1024u * i);
   }
 }
 template <int N>
@@ -428,7 +427,7 @@ __device__ __forceinline__ void stage_k16_quarter(uint4 *kt, const SlotMap &sm, 
   for (int i = 0; i < 8; ++i) {
     const int64_t sl = slot_k<PG>(sm, k0 + min(8 * i + (lane >> 3), n - 1));
     const uint8_t *src = sm.L->kd + (sl * nkv + g) * row_bytes(BKV_F16) + 128 * Q + 16 * (lane & 7);
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(base + 1024u * i) : "memory", "m0");
+    load_to_lds(src, base + 1024u * i);
   }
 }
 

@@ -352,17 +352,14 @@ __global__ __launch_bounds__(kShNT, 1) void short_kernel(ShortArgs a) {
       const int i = 2 * w + (u & 1);
       const int sw = VF ? (i & 3) : 2 * ((i >> 1) & 3);
       const uint8_t *src = a.L.vd + krow(64 * t + 4 * i + (lane & 3)) * VRB + 256 * (u >> 1) + 16 * ((lane >> 2) ^ sw);
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
-                   "s"(__builtin_amdgcn_readfirstlane(vbase + (uint32_t)VB * (uint32_t)(t % NB) + 1024u * (i + 16 * (u >> 1))))
-                   : "memory", "m0");
+      load_to_lds(src, __builtin_amdgcn_readfirstlane(vbase + (uint32_t)VB * (uint32_t)(t % NB) + 1024u * (i + 16 * (u >> 1))));
     }
   };
   const int sw = (w + 7) & 7;                      // the tile whose scale rows this wave takes (wave 0: the eighth)
   if constexpr (VF) {
     if (sw < nt) {
       const uint8_t *src = a.L.vs + krow(64 * sw + lane) * kScaleRowBytes;
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
-                   "s"(__builtin_amdgcn_readfirstlane(lds_addr(s_vs) + 1024u * (uint32_t)sw)) : "memory", "m0");
+      load_to_lds(src, __builtin_amdgcn_readfirstlane(lds_addr(s_vs) + 1024u * (uint32_t)sw));
     }
   }
   for (int t = 0; t < min(nt, NB); ++t) dma_tile(t);

@@ -57,9 +57,7 @@ __device__ __forceinline__ void stage_tail(uint4 *tt, const SlotMap &sm, int nkv
     const int64_t sl = slot_k<PG>(sm, k0 + min(row, n - 1));
     const uint8_t *src = col == 16 ? sm.L->ks + (sl * nkv + g) * kScaleRowBytes
                                    : sm.L->kd + (sl * nkv + g) * kHd + col * 16;
-    if (slotx < kResTail * kUPR)
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base + 1024u * i)
-                   : "memory", "m0");
+    if (slotx < kResTail * kUPR) load_to_lds(src, base + 1024u * i);
   }
 }
 
@@ -326,14 +324,11 @@ __global__ __launch_bounds__(kResNT, 1) void stream_kernel(ResArgs a) {
     const float *qsrc = a.q + (size_t)g * kGqa * a.qs;
 #pragma unroll
     for (int i = 0; i < kGqa; ++i)             // head i's 256 floats: 64 lanes x 16 B
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(qsrc + (size_t)i * a.qs + 4 * lane),
-                   "s"(qb + 1024u * i) : "memory", "m0");
+      load_to_lds(qsrc + (size_t)i * a.qs + 4 * lane, qb + 1024u * i);
     if (appender) {
       const uint32_t xbs = __builtin_amdgcn_readfirstlane(lds_addr(s_x));
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(a.ap.k + (size_t)g * kHd + 4 * lane),
-                   "s"(xbs) : "memory", "m0");
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(a.ap.v + (size_t)g * kHd + 4 * lane),
-                   "s"(xbs + 1024u) : "memory", "m0");
+      load_to_lds(a.ap.k + (size_t)g * kHd + 4 * lane, xbs);
+      load_to_lds(a.ap.v + (size_t)g * kHd + 4 * lane, xbs + 1024u);
     }
   }
   // (fp16 K: half row ch, dims 128 ch .., of each key; column 16 an unused copy. Full plans: quarter
@@ -356,8 +351,7 @@ __global__ __launch_bounds__(kResNT, 1) void stream_kernel(ResArgs a) {
       const int64_t sl = slot_k<PG>(sm, NP + 2 * wave + min(row, tr - 1));
       const uint8_t *src = K16 ? L.kd + (sl * nkv + g) * row_bytes(KF) + (ch * 16 + (col & 15)) * 16
                          : col == 16 ? L.ks + (sl * nkv + g) * kScaleRowBytes : L.kd + (sl * nkv + g) * kHd + col * 16;
-      if (lane < 2 * kUPR)
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(tb) : "memory", "m0");
+      if (lane < 2 * kUPR) load_to_lds(src, tb);
     }
   };
   stage_tile(0);
@@ -631,8 +625,7 @@ __global__ __launch_bounds__(kResNT, 1) void stream_kernel(ResArgs a) {
     {
       const uint32_t sb = __builtin_amdgcn_readfirstlane(lds_addr(vsc + wave * 64));
       const int64_t sl = slot_k<PG>(sm, min(kw0 + (lane & (NKW - 1)), nk - 1));
-      asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(L.vs + (sl * nkv + g) * kScaleRowBytes),
-                   "s"(sb) : "memory", "m0");
+      load_to_lds(L.vs + (sl * nkv + g) * kScaleRowBytes, sb);
     }
 #pragma unroll
     for (int s = 0; s < NS1; ++s) {

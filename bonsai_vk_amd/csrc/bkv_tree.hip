@@ -283,18 +283,6 @@ __device__ __forceinline__ float marked_sum(float l, uint32_t levels) {
   return levels & kLostBits ? __builtin_nanf("") : levels & 2 ? -l : l;
 }
 
-// 16 bytes per lane from base + off into LDS at dst + 16 * lane (dst the same in all lanes), not waited for
-__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
-}
-__device__ __forceinline__ void load_to_lds(const uint8_t *src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
-}
-
-__device__ __forceinline__ void load4_to_lds(const uint8_t *src, uint32_t dst) {   // 4 bytes per lane
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
-}
-
 // PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
 // base for the whole workgroup); 2 any pages (a slot of its own for every key)
 // fp16 pair: the SEL-th byte of lo in the low half and of hi in the high one
@@ -364,14 +352,14 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
   };
   // (offsets within a step are 32 bits: 31 rows)
   auto take = [&](int t, const uint8_t *base, int key, uint32_t row, uint32_t col, uint32_t dst) {
-    if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, dst);
-    else load_to_lds(base + s0 * row, min((uint32_t)key, nk - 1 - (uint32_t)t * kTreeKeys) * row + col, dst);
+    if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, __builtin_amdgcn_readfirstlane(dst));
+    else load_to_lds(base + s0 * row, min((uint32_t)key, nk - 1 - (uint32_t)t * kTreeKeys) * row + col, __builtin_amdgcn_readfirstlane(dst));
   };
   constexpr int NK = KF ? 9 : 16, NV = VF ? 9 : 16;   // loads of a step's K, of its V
   auto scales = [&](int t, const uint8_t *base, uint32_t dst) {
     const uint32_t key = (uint32_t)lane & 31;
     const uint8_t *src = PG == 2 ? base + (size_t)max(__shfl(sl, (int)key), 0) * srow : base + s0 * srow + min(key, nk - 1 - (uint32_t)t * kTreeKeys) * srow;
-    if (lane < 32) load_to_lds(src, dst);
+    if (lane < 32) load_to_lds(src, __builtin_amdgcn_readfirstlane(dst));
   };
   auto request_k = [&](int t) {
     constexpr int LR = KF ? 16 : 32;               // lanes of a row
@@ -395,7 +383,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = 4 * w + j;
-      load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(at.tok, hk * a.grp + at.h)) + 16 * (lane ^ (row & 15)), my0 + oV + 1024 * j);
+      load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(at.tok, hk * a.grp + at.h)) + 16 * (lane ^ (row & 15)), __builtin_amdgcn_readfirstlane(my0 + oV + 1024 * j));
       if (RB * rb + row + 1 < R) at.next(a.grp);
     }
   }
@@ -677,8 +665,8 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
     if constexpr (PG == 2) there_after = (uint32_t)__ballot(sl >= 0);
     // (offsets within a step are 32 bits: 31 rows)
     auto take = [&](const uint8_t *base, int key, uint32_t row, uint32_t col, uint32_t dst) {
-      if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, dst);
-      else load_to_lds(base + s0 * row, min((uint32_t)key, last) * row + col, dst);
+      if constexpr (PG == 2) load_to_lds(base + (size_t)max(__shfl(sl, key), 0) * row + col, __builtin_amdgcn_readfirstlane(dst));
+      else load_to_lds(base + s0 * row, min((uint32_t)key, last) * row + col, __builtin_amdgcn_readfirstlane(dst));
     };
     if (does_v) {
       // [place][64 dims], 4 or 8 lanes of 16 bytes per key; place 4 j + g is key slot (g, j) of the contraction, so that
@@ -691,7 +679,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
       if constexpr (VF) {                          // its two blocks' scales: 4 bytes of each key's row
         const int key = key_of(lane & 31);
         const uint8_t *src = PG == 2 ? vsc + (size_t)max(__shfl(sl, key), 0) * srow : vsc + s0 * srow + min((uint32_t)key, last) * srow;
-        if (lane < 32) load4_to_lds(src + 4 * wk, sm0 + oSV + 128 * wk);
+        if (lane < 32) load4_to_lds(src + 4 * wk, __builtin_amdgcn_readfirstlane(sm0 + oSV + 128 * wk));
       }
     }
     if (does_k) {
@@ -705,7 +693,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
       if constexpr (KF) {                          // (the shuffle with every lane there, the load with 8)
         const int key = (8 * wk + lane) & 31;
         const uint8_t *src = PG == 2 ? ksc + (size_t)max(__shfl(sl, key), 0) * srow : ksc + s0 * srow + min((uint32_t)key, last) * srow;
-        if (lane < 8) load_to_lds(src, sm0 + oSK + 128 * wk);
+        if (lane < 8) load_to_lds(src, __builtin_amdgcn_readfirstlane(sm0 + oSK + 128 * wk));
       }
     }
   };
