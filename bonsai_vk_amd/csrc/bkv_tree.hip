@@ -194,10 +194,9 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   // (every wave holds the whole row: the decision is the workgroup's)
   const float big = fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
   bool fine = l > 0.0f && l < INFINITY && !__any(!(big < INFINITY) || o.x != o.x || o.y != o.y || o.z != o.z || o.w != o.w);
-  // Products below 2^-28 are lost in the matrix cores: of fp16 V, of subnormal size for this to matter, what is below
-  // 2^-37 (V of 1e-6 was 7e-6 off, V of 1e-4 3e-7); of q8_0 V, taken times 2^9 or 2^1, less; of a step of level 2, taken
-  // times 2^-7, what is below 2^-30. Rows whose outputs come near that are formed again.
-  if (fine) {
+  // Products below 2^-28 are lost in the matrix cores: of q8_0 V, taken times 2^9 or 2^1, what is below 2^-29; of a step of
+  // level 2, taken times 2^-7, what is below 2^-21. Rows whose outputs come near that are formed again.
+  if (VF == BKV_Q8_0 && fine) {
     const float top = wave_max(big);
     const bool high = __any((m0.y < 0.0f && f0 > 0.0f) || (m1.y < 0.0f && f1 > 0.0f));
     fine = top == 0.0f ? !high : top >= l * (high ? 0x1p-9f : 0x1p-17f);
@@ -268,6 +267,13 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
 // are brought to the step's unit. vh and vl hold d * b exactly where the scaled d is exact: always at levels 0 and 1,
 // at level 2 from d = 2^-7 on. Smaller ones beside such large ones (16256 beside 1, in 32 neighbouring keys) leave NaN
 // in place of the range's sum, so that its rows are computed key by key.
+// fp16 V is taken as it is, but for steps in which a lane's 8 keys have nothing but subnormals (and zeros) in some dim:
+// those are taken times 2^10 (level 1). The matrix cores align the products of a sum by their exponents, a subnormal's
+// taken as 2^-14, and lose what is 2^-22 below the largest: dims of 1e-7 beside ordinary ones came out 1e-4 off. Beside
+// values of 64 or more, which the factor would take past fp16, such a dim leaves NaN as a lost scale does. (A subnormal
+// beside a larger value in its own dim and 8 keys loses 2^-36 of the largest weight.) Looking for these dims takes 0 to
+// 2 % of the kernels' time, 4 % onto q8_0 K in blocks of 16 rows that read L2; all steps times 2^10 if their values
+// allow it took 2 to 14 %.
 // the level of the largest of fp16 scales (bits, sign cleared): above 2^-1, above 2^7
 __device__ __forceinline__ int scale_level(uint32_t top) { return (top > 0x3800u) + (top > 0x5800u); }
 // whether a step of level 2 loses bits of one of the scales
@@ -278,6 +284,44 @@ __device__ __forceinline__ bool scale_lost(const uint32_t (&sc)[8]) {
   return __any(lost);
 }
 constexpr int kLostBits = 4;                       // (beside the level)
+// V's operands are V * 2^(unit - step * level)
+constexpr int v_unit(int vf) { return vf ? 9 : 0; }
+constexpr int v_step(int vf) { return vf ? 8 : -10; }
+// the level of fp16 V of 8 keys and 2 W dims per lane, and kLostBits
+template <int W>
+__device__ __forceinline__ int f16_level(const uint32_t (&r)[8][W]) {
+  typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+  // (3 of the keys first: a dim whose or-ed exponent is not 0 has a value that is not subnormal)
+  uint32_t x[W];
+  u2 least = {0xFFFF, 0xFFFF};
+#pragma unroll
+  for (int c = 0; c < W; ++c) {
+    x[c] = (r[0][c] | r[1][c] | r[2][c]) & 0x7FFF7FFFu;
+    least = __builtin_elementwise_min(least, __builtin_bit_cast(u2, x[c]));
+  }
+  if (!__any(least[0] < 0x400 || least[1] < 0x400)) return 0;
+  bool some = false;                               // (dims of zeros need nothing)
+#pragma unroll
+  for (int c = 0; c < W; ++c) {
+#pragma unroll
+    for (int j = 3; j < 8; ++j) x[c] |= r[j][c];
+    some |= (x[c] & 0x7FFFu) - 1u < 0x3FFu || (x[c] >> 16 & 0x7FFFu) - 1u < 0x3FFu;
+  }
+  if (!__any(some)) return 0;
+  float sq = 0.0f;                                 // (64^2 or more, or NaN, where a value is 64 or more)
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int c = 0; c < W; ++c) sq = __builtin_amdgcn_fdot2(as_h2(r[j][c]), as_h2(r[j][c]), sq, false);
+  return __any(!(sq < 4096.0f)) ? kLostBits : 1;
+}
+template <int W>
+__device__ __forceinline__ void f16_lift(uint32_t (&r)[8][W]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int c = 0; c < W; ++c) r[j][c] = as_u(as_h2(r[j][c]) * h2{(_Float16)0x1p10f, (_Float16)0x1p10f});
+}
 // a range's sum of p as it is left for the join: below zero where a step had level 2
 __device__ __forceinline__ float marked_sum(float l, uint32_t levels) {
   return levels & kLostBits ? __builtin_nanf("") : levels & 2 ? -l : l;
@@ -525,17 +569,30 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
         o[dt] = mfma16(vh, ph, o[dt]);
       }
     } else {
+      uint32_t r[8][8];                            // dims 8 n .. and 128 + 8 n ..
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(vp + VRB * key_of(j & 7) + 256 * (j >> 3));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r[j & 7][4 * (j >> 3) + c] = (&x.x)[c];
+      }
+      const int level = f16_level(r);
+      if (level | lv) {
+        lv_any |= level & kLostBits;
+        const float x = __builtin_ldexpf(1.0f, v_step(VF) * (lv - (level & 1)));
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) o[dt] *= x;
+        lv = level & 1;
+        if (lv) f16_lift(r);
+      }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        uint4 r[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const uint4 *>(vp + VRB * key_of(j) + 256 * hf);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           uint32_t av[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            av[j] = __builtin_amdgcn_perm((&r[2 * j + 1].x)[e >> 1], (&r[2 * j].x)[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+            av[j] = __builtin_amdgcn_perm(r[2 * j + 1][4 * hf + (e >> 1)], r[2 * j][4 * hf + (e >> 1)], e & 1 ? 0x07060302u : 0x05040100u);
           const h8 vh = __builtin_bit_cast(h8, make_uint4(av[0], av[1], av[2], av[3]));
           o[8 * hf + e] = mfma16(vh, pl, o[8 * hf + e]);
           o[8 * hf + e] = mfma16(vh, ph, o[8 * hf + e]);
@@ -555,7 +612,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
   if (lane == 0) s_lv[w] = lv_any;
   __syncthreads();                                 // (and the waves' own parts have been read)
   const float mm = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
-  const float f = m == -INFINITY ? 0.0f : exp2f(m - mm), fo = VF ? __builtin_ldexpf(f, 8 * lv - 9) : f;
+  const float f = m == -INFINITY ? 0.0f : exp2f(m - mm), fo = __builtin_ldexpf(f, v_step(VF) * lv - v_unit(VF));
 #pragma unroll
   for (int dt = 0; dt < 16; dt += 4)               // (4 products' dims are neighbours)
 #pragma unroll
@@ -790,15 +847,22 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
         *reinterpret_cast<uint4 *>(vto + (VF ? kOp : 0u) + at) = make_uint4(al[0], al[1], al[2], al[3]);
       }
     } else {
-      uint2 r[8];
+      uint32_t r[8][2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = *reinterpret_cast<const uint2 *>(sm + oRV + 4096 * wk + 128 * (4 * j + g) + 8 * n);
+      for (int j = 0; j < 8; ++j) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(sm + oRV + 4096 * wk + 128 * (4 * j + g) + 8 * n);
+        r[j][0] = x.x;
+        r[j][1] = x.y;
+      }
+      const int level = f16_level(r);
+      if (lane == 0) vto[oLV + wk] = (uint8_t)level;
+      if (level & 1) f16_lift(r);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t ah[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          ah[j] = __builtin_amdgcn_perm(e & 2 ? r[2 * j + 1].y : r[2 * j + 1].x, e & 2 ? r[2 * j].y : r[2 * j].x, e & 1 ? 0x07060302u : 0x05040100u);
+          ah[j] = __builtin_amdgcn_perm(r[2 * j + 1][e >> 1], r[2 * j][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
         *reinterpret_cast<uint4 *>(vto + v_piece(64 * wk + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
       }
     }
@@ -898,20 +962,18 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   auto products = [&](const uint8_t *vb) {
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (VF) {
-      const uint32_t now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(vb + oLV));
-      if (now != lv) {
+    const uint32_t now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(vb + oLV));
+    if (now != lv) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float f = __builtin_ldexpf(1.0f, 8 * ((int)((lv >> (8 * c)) & 3u) - (int)((now >> (8 * c)) & 3u)));
+      for (int c = 0; c < 4; ++c) {
+        const float f = __builtin_ldexpf(1.0f, v_step(VF) * ((int)((lv >> (8 * c)) & 3u) - (int)((now >> (8 * c)) & 3u)));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) o[mt][4 * c + dt] *= f;
-        }
-        lv = now;
-        lv_any |= now;
+          for (int dt = 0; dt < 4; ++dt) o[mt][4 * c + dt] *= f;
       }
+      lv = now;
+      lv_any |= now;
     }
     const uint32_t vp[2] = {v_piece(n, g), v_piece(16 + n, g) - 1024u};
     auto v_at = [&](int dt, int lo) { return *reinterpret_cast<const h8 *>(vb + lo * kOp + vp[dt & 1] + 1024 * dt); };
@@ -1011,7 +1073,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
     const int64_t even_row = odd ? other : mine, odd_row = odd ? mine : other;
 #pragma unroll
     for (int dt = 0; dt < 16; dt += 2) {
-      const float f = VF ? __builtin_ldexpf(1.0f, 8 * (int)((lv >> (8 * (dt >> 2))) & 3u) - 9) : 1.0f;
+      const float f = __builtin_ldexpf(1.0f, v_step(VF) * (int)((lv >> (8 * (dt >> 2))) & 3u) - v_unit(VF));
       f4 a0 = o[mt][dt] * f, a1 = o[mt][dt + 1] * f, e, d;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -1,0 +1,105 @@
+"""bkv_attn_tree with V of very different sizes in different dims, held to the formula in 64 bits dim by dim: a row's
+large outputs say nothing about its small ones."""
+import pytest
+import torch
+
+from tests.gpu_util import say
+from tests.test_gpu_tree import KERNELS, filled, rows
+from tests.tree_util import F16, HD, Q8, attention, check_rows, gen, rel, some_mask, tolerance
+
+pytestmark = pytest.mark.gpu
+SMALL = {0: 1e-5, 9: 1e-6, 66: 1e-6, 130: 1e-7, 131: 2.0 ** -24, 250: 1e-7}   # dims and the size of their V
+
+
+def put_v(c, v):
+    """v [n][nkv][HD] as the fp16 V of the first n positions, unrounded by any append."""
+    c.v_data[0, :v.shape[0]] = v.half().view(torch.uint8).reshape(v.shape[0], -1)
+
+
+def small_dims(v):
+    for d, size in SMALL.items():
+        v[..., d] *= size / 0.5
+    return v
+
+
+def check_dims(c, pos0, n, q, mask, dims):
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    want, _, size = attention(c, 0, pos0, q, mask)
+    worst = max(rel(out[..., d], want[..., d]) for d in dims)
+    say(f"  n {n} pos0 {pos0}: worst dim {worst:.2e}")
+    check_rows(out, want, tolerance(size, pos0 + n))
+    # A dim's outputs are as precise as a whole row's: its products and sums are its own. 4e-6 as for whole rows, the
+    # scores being smaller here.
+    assert worst < 4e-6
+    return out, want
+
+
+@pytest.mark.parametrize("kf", [Q8, F16])
+@pytest.mark.parametrize("page", [0, 48, 64])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_dims_of_small_fp16_values(kf, page, n, pos0):
+    """V of 1e-5 to fp16's smallest in a few dims, ordinary in the others."""
+    c = filled(pos0 + n, kf, F16, page=page)
+    v = small_dims(torch.randn(pos0 + n, 4, HD, generator=gen(6), device="cuda") * 0.5)
+    c.append(0, 0, torch.randn(pos0 + n, 4, HD, generator=gen(7), device="cuda"), v)
+    q, _ = rows(n, 16, 3, 0.5)
+    check_dims(c, pos0, n, q, some_mask("tree", n, 3), SMALL)
+
+
+@pytest.mark.parametrize("kf", [Q8, F16])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_dims_of_small_fp16_values_beside_large_ones(kf, n, pos0):
+    """The same with values of 100 and more: in two dims of every key, and in all of two keys."""
+    for where in ("dims", "keys"):
+        c = filled(pos0 + n, kf, F16)
+        v = torch.randn(pos0 + n, 4, HD, generator=gen(6), device="cuda") * 0.5
+        if where == "dims":
+            v[..., 7] *= 400.0
+            v[..., 200] *= 60000.0
+        else:
+            v[5] *= 1000.0
+            v[pos0 - 3] *= 30000.0
+        small_dims(v)
+        put_v(c, v.clamp(-6e4, 6e4))
+        q, _ = rows(n, 16, 3, 0.5)
+        check_dims(c, pos0, n, q, some_mask("tree", n, 3), [d for d in SMALL])
+
+
+@pytest.mark.parametrize("kf", [Q8, F16])
+def test_steps_with_and_without_large_values(kf):
+    """Large values in some keys of many: the outputs change their unit back and forth, in each half of the dims."""
+    for n, pos0 in KERNELS:
+        c = filled(pos0 + n, kf, F16)
+        v = torch.randn(pos0 + n, 4, HD, generator=gen(6), device="cuda") * 0.5
+        v[::77, :, :100] *= 300.0
+        v[::50, :, 150:] *= 500.0
+        put_v(c, v)
+        q, _ = rows(n, 16, 3, 0.5)
+        check_dims(c, pos0, n, q, some_mask("padded", n, 3), range(0, HD, 15))
+
+
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_small_values_behind_a_zero_of_a_large_weight(n, pos0):
+    """One key with nearly all of the weight has V = 0, the others fp16's smallest: the result is theirs, not 0."""
+    c = filled(pos0 + n, F16, F16)
+    k = torch.randn(pos0 + n, 4, HD, generator=gen(7), device="cuda") * 0.01
+    v = torch.full((pos0 + n, 4, HD), 2.0 ** -24, device="cuda")
+    q = torch.randn(n, 16, HD, generator=gen(8), device="cuda") * 0.01
+    q[..., 0] = 1.0
+    k[3, :, 0] = 16 * 9.7                          # a score of 9.7, e^9.7 = 2^14
+    v[3] = 0.0
+    c.append(0, 0, k, v)
+    mask = some_mask("tree", n, 3)
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    want, _, size = attention(c, 0, pos0, q, mask)
+    check_rows(out, want, tolerance(size, pos0 + n))
+    assert float(want.min()) > 0 and rel(out, want) < 4e-6
+
+
+def test_v_of_zeros_is_zero():
+    for vf in (F16, Q8):
+        for n, pos0 in KERNELS:
+            c = filled(pos0 + n, F16, vf)
+            c.v_data.zero_()
+            out, _ = c.attn_tree(0, pos0, rows(n, 16, 3)[0], some_mask("tree", n, 3))
+            assert not bool(out.any())
