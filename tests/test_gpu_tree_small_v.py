@@ -78,10 +78,11 @@ def test_steps_with_and_without_large_values(kf):
         check_dims(c, pos0, n, q, some_mask("padded", n, 3), range(0, HD, 15))
 
 
+@pytest.mark.parametrize("vf", [F16, Q8])
 @pytest.mark.parametrize("n,pos0", KERNELS)
-def test_small_values_behind_a_zero_of_a_large_weight(n, pos0):
-    """One key with nearly all of the weight has V = 0, the others fp16's smallest: the result is theirs, not 0."""
-    c = filled(pos0 + n, F16, F16)
+def test_small_values_behind_a_zero_of_a_large_weight(vf, n, pos0):
+    """One key with nearly all of the weight has V = 0, the others the type's smallest: the result is theirs, not 0."""
+    c = filled(pos0 + n, F16, vf)
     k = torch.randn(pos0 + n, 4, HD, generator=gen(7), device="cuda") * 0.01
     v = torch.full((pos0 + n, 4, HD), 2.0 ** -24, device="cuda")
     q = torch.randn(n, 16, HD, generator=gen(8), device="cuda") * 0.01
@@ -89,11 +90,52 @@ def test_small_values_behind_a_zero_of_a_large_weight(n, pos0):
     k[3, :, 0] = 16 * 9.7                          # a score of 9.7, e^9.7 = 2^14
     v[3] = 0.0
     c.append(0, 0, k, v)
+    if vf == F16:
+        put_v(c, v)
+    else:                                          # (bytes of 1 with fp16's smallest scale)
+        c.v_data.fill_(1)
+        c.v_scales.copy_(torch.full((c.v_scales.numel() // 2,), 2.0 ** -24, device="cuda").half().view(torch.uint8).view(c.v_scales.shape))
+        c.v_data[0, 3] = 0
     mask = some_mask("tree", n, 3)
     out, _ = c.attn_tree(0, pos0, q, mask)
     want, _, size = attention(c, 0, pos0, q, mask)
     check_rows(out, want, tolerance(size, pos0 + n))
     assert float(want.min()) > 0 and rel(out, want) < 4e-6
+
+
+def q8_rows(c, n, scales):
+    """Small whole numbers in every dim, under scales [n][4][8]."""
+    b = torch.randint(-2, 3, (n, 4, HD), generator=gen(11), device="cuda")
+    c.v_data[0, :n] = b.to(torch.int8).view(torch.uint8).reshape(n, -1)
+    c.v_scales[0, :n] = scales.half().view(torch.uint8).reshape(n, -1)
+
+
+@pytest.mark.parametrize("kf", [Q8, F16])
+@pytest.mark.parametrize("big", [0.3, 1.0, 100.0, 300.0, 6e4])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_blocks_of_small_q8_0_scales_beside_large_ones(kf, big, n, pos0):
+    """q8_0 blocks whose values are fp16's smallest beside blocks of ordinary and of large ones, in every key; and as
+    much of each in some keys only, beside others whose blocks in the same place are large."""
+    for some in (False, True):
+        c = filled(pos0 + n, kf, Q8)
+        g = gen(9)
+        sc = torch.full((pos0 + n, 4, 8), 0.01, device="cuda")
+        small = 2.0 ** -24 * torch.randint(1, 4, (pos0 + n, 4, 2), generator=g, device="cuda")
+        sc[..., 1::4] = small
+        sc[..., 2] = big
+        if some:
+            sc[::3, :, 1::4] = 0.02
+            sc[1::5, :, 2] = 0.01
+        q8_rows(c, pos0 + n, sc)
+        q, _ = rows(n, 16, 3, 0.5)
+        mask = some_mask("tree", n, 3)
+        if some:
+            out, _ = c.attn_tree(0, pos0, q, mask)
+            want, _, size = attention(c, 0, pos0, q, mask)
+            check_rows(out, want, tolerance(size, pos0 + n))
+            assert rel(out, want) < 4e-6
+        else:
+            check_dims(c, pos0, n, q, mask, list(range(32, 64, 5)) + list(range(160, 192, 5)) + [0, 70])
 
 
 def test_v_of_zeros_is_zero():
