@@ -391,12 +391,18 @@ class KvCache:
             k_out, v_out = torch.empty((2, n, self.nkv, self.hd), dtype=dtype, device=self._dev).unbind(0)
             tok, head = self.nkv * self.hd, self.hd
         else:
-            given = [t for t in (k_out, v_out) if t is not None]
-            dtype, (tok, head, one) = given[0].dtype, given[0].stride()
-            for t in given:
-                if t.device != self._dev or t.dtype not in _OUT_TYPES or t.dtype != dtype or \
-                        t.shape != (n, self.nkv, self.hd) or t.stride() != (tok, head, one) or one != 1:
-                    raise ValueError(f"{n} x {self.nkv} x {self.hd} values of one type and one layout on {self._dev} are wanted")
+            kind, shape = None, (n, self.nkv, self.hd)
+            for t in (k_out, v_out):
+                if t is None:
+                    continue
+                if t.device != self._dev or t.dtype not in _OUT_TYPES or t.shape != shape or t.stride(2) != 1:
+                    raise ValueError(f"{n} x {self.nkv} x {self.hd} values in whole rows on {self._dev} are wanted")
+                # (the stride of an axis of one means nothing)
+                mine = (t.dtype, t.stride(0) if n > 1 else self.nkv * self.hd, t.stride(1) if self.nkv > 1 else self.hd)
+                if kind is not None and mine != kind:
+                    raise ValueError("k_out and v_out of one type and one layout are wanted")
+                kind = mine
+            dtype, tok, head = kind
         rc = lib().bkv_kv_read(self.desc, layer, pos0, n, _OUT_TYPES[dtype], self._ptr(k_out), self._ptr(v_out), tok, head,
                                self._my_stream())
         if rc:
