@@ -692,6 +692,10 @@ int bkv_attn_tree(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_q, co
   if (n_q == 0) return BKV_OK;
   if (outside(d, pos0, n_q)) return BKV_ECAP;
   if ((int64_t)n_q * d->nh > INT32_MAX / 2) return BKV_EUNSUPPORTED;   // (rows are counted in 32 bits)
+  for (int i = 0; i < 4; i += 2) {                 // (and so are the bytes of a step: 31 slots and a row)
+    const uint64_t sb = slot_bytes(d, i);
+    if (31 * sb + sb / d->nkv > UINT32_MAX) return BKV_EUNSUPPORTED;
+  }
   if ((rc = check_rows(q))) return rc;
   if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
   if (gate && (rc = check_rows(gate))) return rc;
@@ -837,6 +841,7 @@ int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_kee
   if (n_draft < 0 || n_draft > BKV_TREE_MAX_Q || n_keep < 0 || n_keep > n_draft) return BKV_EINVAL;
   if (n_keep == 0) return BKV_OK;
   if (outside(d, pos0, n_draft)) return BKV_ECAP;
+  if (slot_bytes(d, 0) > INT32_MAX || slot_bytes(d, 2) > INT32_MAX) return BKV_EUNSUPPORTED;   // (columns in 31 bits)
   if (!idx) return BKV_EINVAL;
   if (((uintptr_t)idx & 3u) != 0) return BKV_EALIGN;
   CommitArgs a{};

@@ -250,7 +250,8 @@ int bkv_static_debug_address(void **out);
  * which runs one token at a time). The drafted tokens of a step are appended at positions pos0 ..
  * pos0+n-1 (bkv_rope_append or bkv_kv_append), bkv_attn_tree lets each attend to the positions before
  * pos0 and to the drafted tokens it follows, and bkv_kv_commit moves the accepted ones together.
- * These calls take head_dim 256 and any nh that is a multiple of nkv. A block-table entry outside the
+ * These calls take head_dim 256, any nh that is a multiple of nkv, and up to 128 MiB of K and of V per
+ * position and layer (BKV_EUNSUPPORTED where more would not fit their numbers). A block-table entry outside the
  * pool is never followed: its positions are not written, read as zero, and no row sees them.      */
 #define BKV_TREE_MAX_Q 1024
 
