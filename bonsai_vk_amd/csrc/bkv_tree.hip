@@ -59,7 +59,9 @@ __device__ __forceinline__ uint32_t tree_window(const TreeArgs &a, int i, int64_
 
 // ------------------------------------------------------------------ joining the key ranges
 // Row (i, h) by itself: each wave takes every NWV-th key, a lane 4 dims. Only reached for rows whose partial
-// results are not finite, so its time (about 1 us per 30 keys and 4 waves) is not that of ordinary calls.
+// results are not finite, so its time is not that of ordinary calls: a latency after the other, 1.1 us per key of a wave.
+// 8 tokens, one of whose V is NaN, onto 8192 and 32768 keys take 1.2 and 4.6 ms (22 and 38 us without), on 8 waves a row;
+// 1024 tokens, which have one wave a row, 17 and 66 ms (0.37 and 1.1).
 template <int KF, int VF, int NWV>
 __device__ void tree_careful_row(const TreeArgs &a, int i, int h, float *s_o, float *s_ml, float4 &o, float &l) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hk = h / a.grp;
@@ -322,8 +324,6 @@ __device__ __forceinline__ void f16_lift(uint32_t (&r)[8][W]) {
 // a range's sum of p as it is left for the join
 __device__ __forceinline__ float marked_sum(float l, uint32_t levels) { return levels & kLostBits ? __builtin_nanf("") : l; }
 
-// PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours, at one
-// base for the whole workgroup); 2 any pages (a slot of its own for every key)
 // fp16 pair: the SEL-th byte of lo in the low half and of hi in the high one
 template <int SEL>
 __device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
@@ -334,8 +334,8 @@ __device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
 // A workgroup holds 16 rows; each of its 4 waves streams a key range, 32 keys a step, without barriers until the
 // ranges are joined. A step's K is asked for as soon as the last one's has been read, its V likewise, so that a wave has
 // nearly a whole step (17 KB in q8_0) on its way into its own part of LDS at all times. Bound by the memory over long
-// contexts (4 rows of q8_0: 131072 keys 49 us, 5.8 TB/s; 32768 17.8 us, 4.0) and by latencies over short ones (600
-// keys: 7 us with 4 rows, 8.3 with 28, most of it the first step's). Loads into registers took 27.9 us where this takes
+// contexts (4 rows of q8_0: 131072 keys 49 us, 5.8 TB/s; 32768 17.3 us, 4.1) and by latencies over short ones (600
+// keys: 7 us with 4 rows, 8.2 with 28, most of it the first step's). Loads into registers took 27.9 us where this took
 // 17.8; 8 waves a workgroup, for half the ranges to join, 18.9 (53 against 48 at 131072 keys); 32 rows a workgroup, which
 // read the cache once, 31.4 where two blocks of 16 take 28.4 and the second reads L2.
 //
@@ -351,6 +351,8 @@ __device__ __forceinline__ int tree_dim(int dt, int m) {
   return VF == BKV_Q8_0 ? 16 * m + dt : 128 * (dt >> 3) + 8 * m + (dt & 7);
 }
 
+// PG, here and below: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens: a step's keys are neighbours,
+// at one base for the whole workgroup); 2 any pages (a slot of its own for every key)
 template <int KF, int VF, int PG>
 __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void tree_stream_kernel(TreeArgs a) {
   constexpr int KRB = row_bytes(KF), VRB = row_bytes(VF), RB = 16;
@@ -650,8 +652,8 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
 //
 // Bound by what two waves a SIMD can overlap: of a step's 7500 cycles (256 rows, q8_0) the matrix cores work 4096, the
 // vector unit (softmax, the scales of K's blocks, the operands) 4200, LDS about as many. q8_0 takes 4 products and fp16
-// 3 where the formula has 2. 1024 rows onto 32768 keys: 80 us (34 GFLOP, 0.43 PFLOP/s), 8192 onto 8192 163 us (71
-// GFLOP, 0.43), 1008 onto 65536 in fp16 108 us (68 GFLOP, 0.63). Of 80 us 25 are the rows' first bytes and the partial
+// 3 where the formula has 2. 1024 rows onto 32768 keys: 81 us (34 GFLOP, 0.42 PFLOP/s), 8192 onto 8192 164 us (71
+// GFLOP, 0.43), 1008 onto 65536 in fp16 113 us (68 GFLOP, 0.60). Of 81 us 25 are the rows' first bytes and the partial
 // results (67 MB written).
 //
 // LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
@@ -1088,8 +1090,9 @@ static inline int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Which kernel a call takes: the one with the least estimate of its time in us. The estimates' constants are this card's,
-// and choose what was faster wherever two kernels differ by more than 2 us of (kernel + join), among them, 4 KV heads of
-// q8_0, blocks of 16 / tiles of 128 / of 256:
+// and choose what was faster wherever two kernels differ by more than 2 us of (kernel + join), as a profiler times them
+// (0 to 4 us more than the same call takes among others). Among them, 4 KV heads of q8_0, blocks of 16 / tiles of 128 / of
+// 256:
 //   onto 600 keys      8 tokens 11.9 / 13.0,  25 tokens 13.2 / 17.9 / 19.6
 //   onto 2000         33 tokens 19.4 / 25.7 / 30.6,  128 tokens 35.5 / 35.9 / 43.9
 //   onto 8192          8 tokens 17.6 / 20.8,  25 tokens 31.6 / 30.1 / 33.1,  64 tokens .. / 42.2 / 50.2,  300 .. / 134 / 119
