@@ -182,7 +182,8 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
     f0 = m0.x == -INFINITY ? 0.0f : exp2f(m0.x - mm);
     f1 = m1.x == -INFINITY ? 0.0f : exp2f(m1.x - mm);
   }
-  float l = wave_sum(m0.y * f0 + m1.y * f1);
+  const float l0 = fabsf(m0.y) * f0, l1 = fabsf(m1.y) * f1;   // (the sign: see marked_sum)
+  float l = wave_sum(l0 + l1);
   reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = o;
   __syncthreads();
   o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -194,7 +195,14 @@ __global__ __launch_bounds__(64 * NWV) void tree_merge_kernel(TreeArgs a) {
   __syncthreads();
   // (every wave holds the whole row: the decision is the workgroup's)
   const float big = fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w)));
-  const bool fine = l > 0.0f && l < INFINITY && !__any(!(big < INFINITY) || o.x != o.x || o.y != o.y || o.z != o.z || o.w != o.w);
+  bool fine = l > 0.0f && l < INFINITY && !__any(!(big < INFINITY) || o.x != o.x || o.y != o.y || o.z != o.z || o.w != o.w);
+  // Rows whose outputs are all small are formed again: what is left subnormal of V (below), and of p 2^-34 whatever its
+  // size, is cut; beside a step of level 2, whose V are large, sooner.
+  if (fine) {
+    const float top = wave_max(big);
+    const bool high = __any((m0.y < 0.0f && f0 > 0.0f) || (m1.y < 0.0f && f1 > 0.0f));
+    fine = top == 0.0f ? !high : top >= l * (high ? 0x1p-9f : 0x1p-17f);
+  }
   bool empty = false;
   if (!fine) {
     empty = !tree_sees(a, i);
@@ -260,33 +268,29 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
 // all of its times 2^1, with one above 2^7 times 2^-7 (its level: 0, 1, 2), which keeps vh within fp16, and the outputs
 // are brought to the step's unit. vh and vl hold d * b exactly where the scaled d is exact: always at levels 0 and 1,
 // at level 2 from d = 2^-7 on. Smaller ones beside such large ones (16256 beside 1, in 32 neighbouring keys) leave NaN
-// in place of the range's sum, so that its rows are computed key by key; so do, at level 1, 8 keys of a lane whose scales
-// are all below 2^-15, whose products are subnormal (see below).
+// in place of the range's sum, so that its rows are computed key by key.
 // fp16 V is taken as it is, but for steps in which a lane's 8 keys have nothing but subnormals (and zeros) in some dim:
 // those are taken times 2^10 (level 1). The matrix cores align the products of a sum by their exponents, a subnormal's
-// taken as 2^-14, and lose what is 2^-22 below the largest: dims of 1e-7 beside ordinary ones came out 1e-4 off. Beside
-// values of 64 or more, which the factor would take past fp16, such a dim leaves NaN as a lost scale does. (A subnormal
-// beside a larger value in its own dim and 8 keys loses 2^-36 of the largest weight.) Looking for these dims takes 0 to
-// 2 % of the kernels' time, 4 % onto q8_0 K in blocks of 16 rows that read L2; all steps times 2^10 if their values
-// allow it took 2 to 14 %.
+// taken as 2^-14, and lose what is 2^-22 below the largest: dims of 1e-7 beside ordinary ones came out 1e-4 off. Looking
+// for these dims takes 0 to 2 % of the kernels' time, 4 % onto q8_0 K in blocks of 16 rows that read L2; all steps times
+// 2^10 if their values allow it took 2 to 14 %.
+// What is left subnormal loses up to 2^-36 of the largest weight: fp16 V beside a larger value in its own dim and 8 keys,
+// or beside values of 64 or more, which the factor would take past fp16; q8_0 V of scales below 2^-15 beside ones above
+// 1/2 (level 1).
 // the level of the largest of fp16 scales (bits, sign cleared): above 2^-1, above 2^7
 __device__ __forceinline__ int scale_level(uint32_t top) { return (top > 0x3800u) + (top > 0x5800u); }
-// whether a step of level 1 or 2 loses bits of what has these scales
-__device__ __forceinline__ bool scale_lost(int level, const uint32_t (&sc)[8]) {
-  bool some = false, all = true;
+// whether a step of level 2 loses bits of one of the scales
+__device__ __forceinline__ bool scale_lost(const uint32_t (&sc)[8]) {
+  bool lost = false;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t d = sc[j] & 0x7FFFu;
-    some |= level == 1 ? d > 0u : d - 1u < 0x1FFFu;   // (2^-7 is 0x2000)
-    all &= level == 2 || d < 0x200u;               // 2^-15
-  }
-  return __any(some && all);
+  for (int j = 0; j < 8; ++j) lost |= ((sc[j] & 0x7FFFu) - 1u) < 0x1FFFu;
+  return __any(lost);
 }
 constexpr int kLostBits = 4;                       // (beside the level)
 // V's operands are V * 2^(unit - step * level)
 constexpr int v_unit(int vf) { return vf ? 9 : 0; }
 constexpr int v_step(int vf) { return vf ? 8 : -10; }
-// the level of fp16 V of 8 keys and 2 W dims per lane, and kLostBits
+// the level of fp16 V of 8 keys and 2 W dims per lane
 template <int W>
 __device__ __forceinline__ int f16_level(const uint32_t (&r)[8][W]) {
   typedef uint16_t u2 __attribute__((ext_vector_type(2)));
@@ -312,7 +316,7 @@ __device__ __forceinline__ int f16_level(const uint32_t (&r)[8][W]) {
   for (int j = 0; j < 8; ++j)
 #pragma unroll
     for (int c = 0; c < W; ++c) sq = __builtin_amdgcn_fdot2(as_h2(r[j][c]), as_h2(r[j][c]), sq, false);
-  return __any(!(sq < 4096.0f)) ? kLostBits : 1;
+  return __any(!(sq < 4096.0f)) ? 0 : 1;
 }
 template <int W>
 __device__ __forceinline__ void f16_lift(uint32_t (&r)[8][W]) {
@@ -321,8 +325,10 @@ __device__ __forceinline__ void f16_lift(uint32_t (&r)[8][W]) {
 #pragma unroll
     for (int c = 0; c < W; ++c) r[j][c] = as_u(as_h2(r[j][c]) * h2{(_Float16)0x1p10f, (_Float16)0x1p10f});
 }
-// a range's sum of p as it is left for the join
-__device__ __forceinline__ float marked_sum(float l, uint32_t levels) { return levels & kLostBits ? __builtin_nanf("") : l; }
+// a range's sum of p as it is left for the join: below zero where a step of q8_0 V had level 2
+__device__ __forceinline__ float marked_sum(float l, uint32_t levels) {
+  return levels & kLostBits ? __builtin_nanf("") : levels & 2 ? -l : l;
+}
 
 // fp16 pair: the SEL-th byte of lo in the low half and of hi in the high one
 template <int SEL>
@@ -450,7 +456,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
   f4 o[16] = {};
   float m = -INFINITY, l = 0.0f;                   // m: the reference less kPScale
   int lv = 0;                                      // the outputs' level
-  uint32_t lv_any = 0;                             // kLostBits where a step lost something
+  uint32_t lv_any = 0;                             // all that were taken, or-ed
 
 #pragma unroll 1
   for (int t = t0; t < t1; ++t) {
@@ -537,7 +543,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
       }
       const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
       const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
-      if (level > 0 && scale_lost(level, sc)) lv_any = kLostBits;
+      if (level == 2) lv_any |= 2u | (scale_lost(sc) ? kLostBits : 0);
       if (level != lv) {
         const float x = __builtin_ldexpf(1.0f, 8 * (lv - level));
 #pragma unroll
@@ -575,11 +581,10 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
       }
       const int level = f16_level(r);
       if (level | lv) {
-        lv_any |= level & kLostBits;
-        const float x = __builtin_ldexpf(1.0f, v_step(VF) * (lv - (level & 1)));
+        const float x = __builtin_ldexpf(1.0f, v_step(VF) * (lv - level));
 #pragma unroll
         for (int dt = 0; dt < 16; ++dt) o[dt] *= x;
-        lv = level & 1;
+        lv = level;
         if (lv) f16_lift(r);
       }
 #pragma unroll
@@ -822,7 +827,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
       }
       const int level = __any(scale_level(top) != 0) ? (__any(scale_level(top) == 2) ? 2 : 1) : 0;
       const _Float16 f = level == 0 ? (_Float16)0x1p9f : level == 1 ? (_Float16)0x1p1f : (_Float16)0x1p-7f;
-      const int lost = level > 0 && scale_lost(level, sc) ? kLostBits : 0;
+      const int lost = level == 2 && scale_lost(sc) ? kLostBits : 0;
       if (lane == 0) vto[oLV + wk] = (uint8_t)(level | lost);
       h2 d[4];
 #pragma unroll
@@ -853,7 +858,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
       }
       const int level = f16_level(r);
       if (lane == 0) vto[oLV + wk] = (uint8_t)level;
-      if (level & 1) f16_lift(r);
+      if (level) f16_lift(r);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t ah[4];

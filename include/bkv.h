@@ -277,8 +277,8 @@ int bkv_tree_mask(const int32_t *parent, int n, uint64_t *mask, int32_t *depth);
  *   run in fp32 in no stated order (the result does not change from call to call): rows agree with
  *   bkv_attn_decode's to about the rounding of its fp16 probabilities. Beside fp32's roundings of the
  *   scores and of sum p |v| an output carries at most 2^-34 of sum |v|, and 2^-36 of the largest p for
- *   a position whose |v| is below 2^-14 (fp16, beside larger values of its dim in neighbouring positions)
- *   or whose scale is below 2^-15 (q8_0, beside scales above 1/2 there).
+ *   a position whose |v| is below 2^-14 (fp16, beside larger values of its dim or values of 64 or more in
+ *   neighbouring positions) or whose scale is below 2^-15 (q8_0, beside scales above 1/2 there).
  *   A row that sees nothing gets 0. Positions that a row does not see have no effect on it, whatever
  *   they hold (Inf and NaN included).
  *   out: [n_q][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)). Neither

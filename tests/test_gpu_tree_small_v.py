@@ -1,11 +1,13 @@
 """bkv_attn_tree with V of very different sizes in different dims, held to the formula in 64 bits dim by dim: a row's
 large outputs say nothing about its small ones."""
+import math
+
 import pytest
 import torch
 
 from tests.gpu_util import say
 from tests.test_gpu_tree import KERNELS, filled, rows
-from tests.tree_util import F16, HD, Q8, attention, check_rows, gen, rel, some_mask, tolerance
+from tests.tree_util import F16, HD, Q8, attention, check_rows, gen, rel, seen, some_mask, tolerance, values
 
 pytestmark = pytest.mark.gpu
 SMALL = {0: 1e-5, 9: 1e-6, 66: 1e-6, 130: 1e-7, 131: 2.0 ** -24, 250: 1e-7}   # dims and the size of their V
@@ -32,6 +34,32 @@ def check_dims(c, pos0, n, q, mask, dims):
     # scores being smaller here.
     assert worst < 4e-6
     return out, want
+
+
+def largest_weight(c, pos0, q, mask):
+    """The largest probability of each row, [n][nh][1], in 64 bits."""
+    n, group = q.shape[0], c.nh // c.nkv
+    k = values(c, "k", 0, 0, pos0 + n)
+    see = torch.cat([torch.ones(n, pos0, dtype=torch.bool, device="cuda"), seen(mask, n)], 1)
+    top = []
+    for h in range(c.nh):
+        s = (q[:, h].half().double() @ k[:, h // group].t().contiguous()) * c.scale
+        top.append(torch.softmax(s.masked_fill(~see, -math.inf), 1).max(1).values)
+    return torch.stack(top, 1)[..., None]
+
+
+def by_key(nk):
+    """What rows that are computed key by key add to a 2-norm: the sums of p and of p v are up to nk fp32 additions, one
+    after another, each off by 2^-24 of what the sum comes to."""
+    return 2 * nk * 2.0 ** -24
+
+
+def check_tiny(c, pos0, n, q, mask):
+    """Values that are left subnormal: up to 2^-36 of the largest weight for each position (bkv_attn_tree's bound)."""
+    out, _ = c.attn_tree(0, pos0, q, mask)
+    want, _, size = attention(c, 0, pos0, q, mask)
+    check_rows(out, want, tolerance(size, pos0 + n) + (pos0 + n) * 2.0 ** -36 * largest_weight(c, pos0, q, mask))
+    assert rel(out, want) < 4e-6
 
 
 @pytest.mark.parametrize("kf", [Q8, F16])
@@ -62,7 +90,7 @@ def test_dims_of_small_fp16_values_beside_large_ones(kf, n, pos0):
         small_dims(v)
         put_v(c, v.clamp(-6e4, 6e4))
         q, _ = rows(n, 16, 3, 0.5)
-        check_dims(c, pos0, n, q, some_mask("tree", n, 3), [d for d in SMALL])
+        check_tiny(c, pos0, n, q, some_mask("tree", n, 3))
 
 
 @pytest.mark.parametrize("kf", [Q8, F16])
@@ -100,7 +128,7 @@ def test_small_values_behind_a_zero_of_a_large_weight(vf, n, pos0):
     out, _ = c.attn_tree(0, pos0, q, mask)
     want, _, size = attention(c, 0, pos0, q, mask)
     check_rows(out, want, tolerance(size, pos0 + n))
-    assert float(want.min()) > 0 and rel(out, want) < 4e-6
+    assert float(want.min()) > 0 and rel(out, want) < 4e-6 + by_key(pos0 + n)
 
 
 def q8_rows(c, n, scales):
@@ -129,13 +157,36 @@ def test_blocks_of_small_q8_0_scales_beside_large_ones(kf, big, n, pos0):
         q8_rows(c, pos0 + n, sc)
         q, _ = rows(n, 16, 3, 0.5)
         mask = some_mask("tree", n, 3)
-        if some:
-            out, _ = c.attn_tree(0, pos0, q, mask)
-            want, _, size = attention(c, 0, pos0, q, mask)
-            check_rows(out, want, tolerance(size, pos0 + n))
-            assert rel(out, want) < 4e-6
+        check_tiny(c, pos0, n, q, mask)
+
+
+@pytest.mark.parametrize("vf", [F16, Q8])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_rows_that_are_small_as_a_whole(vf, n, pos0):
+    """V of 1e-6 in every dim beside one key of 100 that no row but its own sees, and V of 0.5 with next to no weight
+    beside keys of 1e-6: such rows are computed key by key where the products would be subnormal."""
+    for case in ("all", "some"):
+        c = filled(pos0 + n, F16, vf)
+        k = torch.randn(pos0 + n, 4, HD, generator=gen(7), device="cuda") * 0.01
+        v = torch.randn(pos0 + n, 4, HD, generator=gen(8), device="cuda") * (1e-6 if case == "all" else 0.5)
+        q = torch.randn(n, 16, HD, generator=gen(9), device="cuda") * 0.01
+        mask = some_mask("tree", n, 3)
+        if case == "all":
+            v[pos0 + 1] *= 1e8
+            mask[torch.arange(n, device="cuda") != 1, 0] &= ~2
         else:
-            check_dims(c, pos0, n, q, mask, list(range(32, 64, 5)) + list(range(160, 192, 5)) + [0, 70])
+            q[..., 0] = 4.0
+            k[3::20, :, 0] = 72.0 + 4 * torch.randn(k[3::20].shape[0], 4, generator=gen(10), device="cuda")   # scores about 18
+            v[3::20] *= 2e-6
+        c.append(0, 0, k, v)
+        if vf == F16:
+            put_v(c, v)
+        out, _ = c.attn_tree(0, pos0, q, mask)
+        want, _, size = attention(c, 0, pos0, q, mask)
+        check_rows(out, want, tolerance(size, pos0 + n) + size[0] * by_key(pos0 + n))
+        # (scores of 18 are off by 18 * 1.44 * 2^-23 = 3e-6 at most, each for itself)
+        others = torch.arange(n, device="cuda") != 1
+        assert rel(out[others], want[others]) < 4e-6 + by_key(pos0 + n)
 
 
 def test_v_of_zeros_is_zero():
