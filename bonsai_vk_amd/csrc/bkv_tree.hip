@@ -272,8 +272,7 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
 // fp16 V is taken as it is, but for steps in which a lane's 8 keys have nothing but subnormals (and zeros) in some dim:
 // those are taken times 2^10 (level 1). The matrix cores align the products of a sum by their exponents, a subnormal's
 // taken as 2^-14, and lose what is 2^-22 below the largest: dims of 1e-7 beside ordinary ones came out 1e-4 off. Looking
-// for these dims takes 0 to 2 % of the kernels' time, 4 % onto q8_0 K in blocks of 16 rows that read L2; all steps times
-// 2^10 if their values allow it took 2 to 14 %.
+// for these dims takes 0 to 2 % of the kernels' time; all steps times 2^10 if their values allow it took 2 to 14 %.
 // What is left subnormal loses up to 2^-36 of the largest weight: fp16 V beside a larger value in its own dim and 8 keys,
 // or beside values of 64 or more, which the factor would take past fp16; q8_0 V of scales below 2^-15 beside ones above
 // 1/2 (level 1).
@@ -302,7 +301,7 @@ __device__ __forceinline__ int f16_level(const uint32_t (&r)[8][W]) {
     x[c] = (r[0][c] | r[1][c] | r[2][c]) & 0x7FFF7FFFu;
     least = __builtin_elementwise_min(least, __builtin_bit_cast(u2, x[c]));
   }
-  if (!__any(least[0] < 0x400 || least[1] < 0x400)) return 0;
+  if (__builtin_expect(!__any(least[0] < 0x400 || least[1] < 0x400), 1)) return 0;
   bool some = false;                               // (dims of zeros need nothing)
 #pragma unroll
   for (int c = 0; c < W; ++c) {
@@ -340,7 +339,7 @@ __device__ __forceinline__ uint32_t pair_bytes(uint32_t lo, uint32_t hi) {
 // A workgroup holds 16 rows; each of its 4 waves streams a key range, 32 keys a step, without barriers until the
 // ranges are joined. A step's K is asked for as soon as the last one's has been read, its V likewise, so that a wave has
 // nearly a whole step (17 KB in q8_0) on its way into its own part of LDS at all times. Bound by the memory over long
-// contexts (4 rows of q8_0: 131072 keys 49 us, 5.8 TB/s; 32768 17.3 us, 4.1) and by latencies over short ones (600
+// contexts (4 rows of q8_0: 131072 keys 49 us, 5.8 TB/s; 32768 17.5 us, 4.1) and by latencies over short ones (600
 // keys: 7 us with 4 rows, 8.2 with 28, most of it the first step's). Loads into registers took 27.9 us where this took
 // 17.8; 8 waves a workgroup, for half the ranges to join, 18.9 (53 against 48 at 131072 keys); 32 rows a workgroup, which
 // read the cache once, 31.4 where two blocks of 16 take 28.4 and the second reads L2.
@@ -580,10 +579,16 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
         for (int c = 0; c < 4; ++c) r[j & 7][4 * (j >> 3) + c] = (&x.x)[c];
       }
       const int level = f16_level(r);
-      if (level | lv) {
+      if (__builtin_expect(level | lv, 0)) {
         const float x = __builtin_ldexpf(1.0f, v_step(VF) * (lv - level));
+        // (the outputs are accumulation registers; without the asm they are read ahead of the branch, 64 instructions a
+        // step: 25 tokens onto 8192 q8_0 K 27.1 us in place of 25.9)
 #pragma unroll
-        for (int dt = 0; dt < 16; ++dt) o[dt] *= x;
+        for (int dt = 0; dt < 16; ++dt) {
+          asm volatile("" : "+a"(o[dt]));
+          o[dt] *= x;
+          asm volatile("" : "+a"(o[dt]));
+        }
         lv = level;
         if (lv) f16_lift(r);
       }
@@ -658,7 +663,7 @@ __global__ __launch_bounds__(256, KF == BKV_Q8_0 && VF == BKV_Q8_0 ? 2 : 1) void
 // Bound by what two waves a SIMD can overlap: of a step's 7500 cycles (256 rows, q8_0) the matrix cores work 4096, the
 // vector unit (softmax, the scales of K's blocks, the operands) 4200, LDS about as many. q8_0 takes 4 products and fp16
 // 3 where the formula has 2. 1024 rows onto 32768 keys: 81 us (34 GFLOP, 0.42 PFLOP/s), 8192 onto 8192 164 us (71
-// GFLOP, 0.43), 1008 onto 65536 in fp16 113 us (68 GFLOP, 0.60). Of 81 us 25 are the rows' first bytes and the partial
+// GFLOP, 0.43), 1008 onto 65536 in fp16 112 us (68 GFLOP, 0.60). Of 81 us 25 are the rows' first bytes and the partial
 // results (67 MB written).
 //
 // LDS positions, in 16-byte pieces: K piece c of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
@@ -795,6 +800,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   uint32_t lv = 0, lv_any = 0;                     // the outputs' levels, a byte per 64 dims; all that were taken, or-ed
 
   // ---- the wave's bytes, landed, made into operands
+  uint32_t levels = 0;                             // fp16 V: those of the wave's 64 dims, the last step's first
   auto convert = [&](uint8_t *kto, uint8_t *vto) {
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -856,22 +862,31 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
         r[j][0] = x.x;
         r[j][1] = x.y;
       }
+      auto write = [&]() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t ah[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            ah[j] = __builtin_amdgcn_perm(r[2 * j + 1][e >> 1], r[2 * j][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+          *reinterpret_cast<uint4 *>(vto + v_piece(64 * wk + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+        }
+      };
+      write();                                     // (once more where they are to be lifted: the look waits for no write)
       const int level = f16_level(r);
-      if (lane == 0) vto[oLV + wk] = (uint8_t)level;
-      if (level) f16_lift(r);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t ah[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          ah[j] = __builtin_amdgcn_perm(r[2 * j + 1][e >> 1], r[2 * j][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-        *reinterpret_cast<uint4 *>(vto + v_piece(64 * wk + 4 * n + e, g)) = make_uint4(ah[0], ah[1], ah[2], ah[3]);
+      if (__builtin_expect(level, 0)) {
+        f16_lift(r);
+        write();
       }
+      // (the place's level is that of three steps ago)
+      if (__builtin_expect(level != (int)(levels >> 2 & 1u), 0) && lane == 0) vto[oLV + wk] = (uint8_t)level;
+      levels = levels << 1 | (uint32_t)level;
     }
   };
 
   h8 ph[MT], pl[MT];
-  auto scores = [&](int t, const uint8_t *kbuf) {
+  uint32_t now = 0;                                // the levels of the step whose products are next
+  auto scores = [&](int t, const uint8_t *kbuf, const uint8_t *vb) {
     const int64_t kb = (int64_t)t * kTreeKeys;
     // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
     const int g4 = 4 * (my_lane() >> 4);
@@ -896,9 +911,12 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
     auto s_at = [&](int ub) { return *reinterpret_cast<const h8 *>(sp + 256 * (ub >> 3) + 16 * ((ub & 7) >> 1)); };   // two blocks
     h8 kf[AK + 1], sc = {}, sn = {};
     f4 p[MT] = {};                                 // q8_0: the last block's products, still to be scaled and added
+    uint32_t mine = 0;                             // (fp16 V: there when K is; q8_0 V's are read with its products)
+    if constexpr (!VF) mine = *reinterpret_cast<const uint32_t *>(vb + oLV);
     if constexpr (KF) sn = s_at(0);
 #pragma unroll
     for (int j = 0; j < AK; ++j) kf[j] = k_at(j);
+    if constexpr (!VF) now = __builtin_amdgcn_readfirstlane(mine);
     auto add = [&](int ub) {                       // block ub's products (its pair's scales are in sc)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -964,8 +982,8 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   auto products = [&](const uint8_t *vb) {
     const int lane = my_lane(), n = lane & 15, g = lane >> 4;
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(vb + oLV));
-    if (now != lv) {
+    if constexpr (VF) now = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(vb + oLV));
+    if (__builtin_expect(now != lv, 0)) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float f = __builtin_ldexpf(1.0f, v_step(VF) * ((int)((lv >> (8 * c)) & 3u) - (int)((now >> (8 * c)) & 3u)));
@@ -1011,6 +1029,9 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
   const bool late = w >= 4, works = has_rows && RB * rb + 16 * MT * w < R;   // (a wave whose rows are all past the last only brings bytes)
   lds_barrier();                                   // (every wave has its rows)
   if (t0 < t1) {
+    if constexpr (!VF) {
+      if (does_v && lane < 3) sm[kVB * lane + oLV + wk] = 0;
+    }
     convert(sm + oK + kKB, sm);
     look_up(min(t0 + 1, t1 - 1));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1026,7 +1047,7 @@ __global__ __launch_bounds__(tree_tile_threads(MT), MT == 1 ? 3 : 2) void tree_t
     if (works && late && t > t0) products(sm + v_last);
     __builtin_amdgcn_s_setprio(2);
     __builtin_amdgcn_sched_barrier(0);
-    if (works) scores(t, sm + oK + kKB * b);
+    if (works) scores(t, sm + oK + kKB * b, sm + v_now);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
     if (works && !late) products(sm + v_now);
