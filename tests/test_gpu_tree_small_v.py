@@ -1,6 +1,7 @@
 """bkv_attn_tree with V of very different sizes in different dims, held to the formula in 64 bits dim by dim: a row's
 large outputs say nothing about its small ones."""
 import math
+import random
 
 import pytest
 import torch
@@ -91,6 +92,28 @@ def test_dims_of_small_fp16_values_beside_large_ones(kf, n, pos0):
         put_v(c, v.clamp(-6e4, 6e4))
         q, _ = rows(n, 16, 3, 0.5)
         check_tiny(c, pos0, n, q, some_mask("tree", n, 3))
+
+
+@pytest.mark.parametrize("kf", [Q8, F16])
+@pytest.mark.parametrize("page", [0, 48])
+@pytest.mark.parametrize("n,pos0", KERNELS)
+def test_dims_that_are_small_in_some_steps(kf, page, n, pos0):
+    """Runs of 1 to 5 steps of 32 keys whose small dims come and go, in each quarter of the dims by itself: the outputs
+    change their unit back and forth."""
+    c = filled(pos0 + n, kf, F16, page=page)
+    nk = pos0 + n
+    v = torch.randn(nk, 4, HD, generator=gen(6), device="cuda") * 0.5
+    r = random.Random(n)
+    for quarter in range(4):
+        at, on = 0, False
+        while at < nk:
+            end = at + 32 * r.randint(1, 5)
+            if on:
+                v[at:end, :, 64 * quarter + 5:64 * quarter + 64:13] *= 1e-7 / 0.5
+            at, on = end, not on
+    put_v(c, v) if not page else c.append(0, 0, torch.randn(nk, 4, HD, generator=gen(7), device="cuda"), v)
+    q, _ = rows(n, 16, 3, 0.5)
+    check_dims(c, pos0, n, q, some_mask("tree", n, 3), range(5, HD, 13))
 
 
 @pytest.mark.parametrize("kf", [Q8, F16])
