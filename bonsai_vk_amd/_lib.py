@@ -8,13 +8,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 # per-phase timestamps for profiling); the default is the in-tree libbkv.so
 LIB_PATH = os.environ.get("BKV_LIBRARY") or os.path.join(HERE, "libbkv.so")
 
-BKV_F16, BKV_Q8_0 = 0, 1
+BKV_F16, BKV_Q8_0, BKV_Q4_0 = 0, 1, 2
 BKV_OP_DECODE, BKV_OP_PREFILL, BKV_OP_TREE = 0, 1, 2
 BKV_PREFILL_MAX_Q = 4096
 BKV_TREE_MAX_Q = 1024
 BKV_ROPE_HALF, BKV_ROPE_INTERLEAVED = 0, 1
 BKV_ROPE_PLAIN, BKV_ROPE_LINEAR, BKV_ROPE_NTK, BKV_ROPE_YARN = 0, 1, 2, 3
 BKV_OUT_F32, BKV_OUT_F16, BKV_OUT_BF16 = 0, 1, 2
+BKV_SEQS_MAX, BKV_ROPE_MAX_AXES = 1024, 8
+BKV_AXES_BLOCKS, BKV_AXES_DEALT = 0, 1
 
 ERRORS = {
     0: "BKV_OK", -1: "BKV_EINVAL", -2: "BKV_ESHAPE", -3: "BKV_ECAP", -4: "BKV_EALIGN",
@@ -30,6 +32,8 @@ EXPORTS = [
     "bkv_workspace_error", "bkv_error_words", "bkv_decode_step_static", "bkv_static_scratch_bytes",
     "bkv_static_error", "bkv_static_reset", "bkv_static_debug_address",
     "bkv_tree_mask", "bkv_attn_tree", "bkv_rope_init", "bkv_rope_append", "bkv_kv_read", "bkv_kv_commit",
+    "bkv_rope_axes_init", "bkv_seqs_rope_append", "bkv_seqs_read", "bkv_seqs_workspace_bytes", "bkv_seqs_attn",
+    "bkv_pages_workspace_bytes", "bkv_pages_fork", "bkv_pages_extend", "bkv_pages_compact",
 ]
 
 
@@ -58,6 +62,17 @@ class BkvRope(ctypes.Structure):
                 ("reserved", ctypes.c_int32), ("turns", ctypes.c_double * 128)]
 
 
+class BkvSeqs(ctypes.Structure):
+    """Mirror of struct bkv_seqs."""
+    _fields_ = [("n_seq", ctypes.c_int32), ("n_tok", ctypes.c_int32), ("max_q", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("q_start", ctypes.c_void_p), ("len", ctypes.c_void_p), ("tables", ctypes.c_void_p)]
+
+
+class BkvRopeAxes(ctypes.Structure):
+    """Mirror of struct bkv_rope_axes."""
+    _fields_ = [("n_axes", ctypes.c_int32), ("n_pairs", ctypes.c_int32), ("axis", ctypes.c_uint8 * 128)]
+
+
 class BkvError(RuntimeError):
     def __init__(self, code, where=""):
         self.code = code
@@ -80,6 +95,7 @@ def lib():
                           "(there is no CPU fallback for the KV-cache path)")
     L = ctypes.CDLL(LIB_PATH)
     P, D, i32, u32, sz = ctypes.c_void_p, ctypes.POINTER(BkvCacheDesc), ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t
+    S, X = ctypes.POINTER(BkvSeqs), ctypes.POINTER(BkvRopeAxes)
     R, O, i64, f64 = ctypes.POINTER(BkvRows), ctypes.POINTER(BkvRope), ctypes.c_int64, ctypes.c_double
     sig = {
         "bkv_geom_check": (i32, [D]),
@@ -115,6 +131,15 @@ def lib():
         "bkv_rope_append": (i32, [D, i32, u32, i32, O, R, R, R, P, P, ctypes.c_float, P, P, P]),
         "bkv_kv_read": (i32, [D, i32, u32, i32, i32, P, P, i64, i64, P]),
         "bkv_kv_commit": (i32, [D, u32, i32, i32, P, P]),
+        "bkv_rope_axes_init": (i32, [X, i32, P, i32]),
+        "bkv_seqs_rope_append": (i32, [D, i32, S, O, X, R, R, R, P, P, ctypes.c_float, P, P, P]),
+        "bkv_seqs_read": (i32, [D, i32, S, i32, P, P, i64, i64, P]),
+        "bkv_seqs_workspace_bytes": (sz, [D, i32, i32]),
+        "bkv_seqs_attn": (i32, [D, i32, S, R, R, P, P, P, sz, P]),
+        "bkv_pages_workspace_bytes": (sz, [D]),
+        "bkv_pages_fork": (i32, [D, i32, P, P, P, P, P]),
+        "bkv_pages_extend": (i32, [D, i32, P, P, P, P, P, P, sz, P]),
+        "bkv_pages_compact": (i32, [D, i32, P, P, P, P, P, sz, P]),
         "bkv_qk_norm_rope_append": (i32, [D, i32, u32, i32, P, P, P, P, P, i32, ctypes.c_float,
                                           ctypes.c_float, P, P]),
     }

@@ -13,7 +13,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbkv.so")
 LIB_TS = os.path.join(HERE, "libbkv_ts.so")
 SOURCES = ["bkv_api.cpp", "bkv_decode.hip", "bkv_resident.hip", "bkv_stream.hip", "bkv_prefill.hip", "bkv_norm_rope.hip", "bkv_static.hip",
-           "bkv_short.hip", "bkv_tree.hip", "bkv_rope.hip", "bkv_read.hip"]
+           "bkv_short.hip", "bkv_tree.hip", "bkv_rope.hip", "bkv_read.hip", "bkv_seqs.hip", "bkv_seqs_attn.hip",
+           "bkv_pages.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -11,7 +11,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import (BKV_F16, BKV_OP_DECODE, BKV_OP_PREFILL, BKV_OP_TREE, BKV_OUT_BF16, BKV_OUT_F16, BKV_OUT_F32, BKV_Q8_0,
+from ._lib import (BKV_F16, BKV_OP_DECODE, BKV_OP_PREFILL, BKV_OP_TREE, BKV_OUT_BF16, BKV_OUT_F16, BKV_OUT_F32, BKV_Q4_0, BKV_Q8_0,
                    BkvCacheDesc, BkvRope, BkvRows, check, lib)
 
 
@@ -120,12 +120,12 @@ class KvCache:
         self.geom = geom
 
         def alloc(fmt, scales):
-            if scales and fmt != BKV_Q8_0:
+            if scales and fmt == BKV_F16:
                 return None
             if scales:
                 row = nkv * (hd // 32) * 2
             else:
-                row = nkv * hd * (2 if fmt == BKV_F16 else 1)
+                row = nkv * hd * 2 if fmt == BKV_F16 else nkv * hd // (2 if fmt == BKV_Q4_0 else 1)
             return torch.zeros((n_layers, cap, row), dtype=torch.uint8, device=self.device)
 
         self.k_data = alloc(k_fmt, False)
@@ -157,6 +157,8 @@ class KvCache:
         self.max_ctx = max_ctx or self.max_positions
         ws = lib().bkv_workspace_bytes(ctypes.byref(d), BKV_OP_DECODE, self.max_ctx)
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=self.device)
+        if ws == 0:                                # (a 4-bit cache: KvSeqs.attn's workspace is its own)
+            return
         check(lib().bkv_workspace_init(ctypes.byref(d), self.workspace.data_ptr(), ws, self._stream()),
               "bkv_workspace_init")
 

@@ -221,16 +221,18 @@ static uint64_t slot_bytes(const bkv_cache_desc *d, int which) {
   const int fmt = which < 2 ? d->k_fmt : d->v_fmt;
   const uint64_t hd = (uint64_t)d->hd, nkv = (uint64_t)d->nkv;
   switch (which) {
-    case 0: case 2: return fmt == BKV_F16 ? nkv * hd * 2 : nkv * hd;
+    case 0: case 2: return fmt == BKV_F16 ? nkv * hd * 2 : fmt == BKV_Q4_0 ? nkv * hd / 2 : nkv * hd;
     default: return fmt == BKV_F16 ? 0 : nkv * (hd / 32) * 2;
   }
 }
 
-static int check(const bkv_cache_desc *d) {
+static bool known(int fmt) { return fmt == BKV_F16 || fmt == BKV_Q8_0 || fmt == BKV_Q4_0; }
+
+// the geometry, of any format
+static int check_geom(const bkv_cache_desc *d) {
   if (!d) return BKV_EINVAL;
   if (d->n_layers < 1 || d->nkv < 1 || d->nh < 1 || d->hd < 1 || d->cap < 1) return BKV_EINVAL;
-  if ((d->k_fmt != BKV_F16 && d->k_fmt != BKV_Q8_0) || (d->v_fmt != BKV_F16 && d->v_fmt != BKV_Q8_0))
-    return BKV_EINVAL;
+  if (!known(d->k_fmt) || !known(d->v_fmt)) return BKV_EINVAL;
   // KvGeom::check (runtime_vk/kv_guard.h:103-113)
   if (d->hd % 4 || d->hd % 32 || (d->hd / 32) % 2) return BKV_ESHAPE;
   if (d->nh % d->nkv) return BKV_ESHAPE;
@@ -240,8 +242,8 @@ static int check(const bkv_cache_desc *d) {
     if (d->cap % d->page_tokens || d->max_pages < 1 || !d->block_table) return BKV_EINVAL;
   }
   if (!d->k_data || !d->v_data) return BKV_EINVAL;
-  if (d->k_fmt == BKV_Q8_0 && !d->k_scales) return BKV_EINVAL;
-  if (d->v_fmt == BKV_Q8_0 && !d->v_scales) return BKV_EINVAL;
+  if (d->k_fmt != BKV_F16 && !d->k_scales) return BKV_EINVAL;
+  if (d->v_fmt != BKV_F16 && !d->v_scales) return BKV_EINVAL;
   const void *ptrs[4] = {d->k_data, d->k_scales, d->v_data, d->v_scales};
   for (int i = 0; i < 4; ++i) {
     const uint64_t sb = slot_bytes(d, i);
@@ -251,6 +253,14 @@ static int check(const bkv_cache_desc *d) {
     if (d->layer_stride_bytes[i] % 16) return BKV_EALIGN;
   }
   return BKV_OK;
+}
+
+static bool any_q4(const bkv_cache_desc *d) { return d->k_fmt == BKV_Q4_0 || d->v_fmt == BKV_Q4_0; }
+
+// the geometry, and formats that every kernel takes (the 4-bit one has its own calls)
+static int check(const bkv_cache_desc *d) {
+  const int rc = check_geom(d);
+  return rc ? rc : any_q4(d) ? BKV_EUNSUPPORTED : BKV_OK;
 }
 
 // shapes the gfx950 kernels are specialised for: hd 256 and 4 query heads per KV head
@@ -378,7 +388,7 @@ using namespace bkv;
 
 extern "C" {
 
-int bkv_geom_check(const bkv_cache_desc *d) { return check(d); }
+int bkv_geom_check(const bkv_cache_desc *d) { return check_geom(d); }
 
 uint64_t bkv_slot_bytes(const bkv_cache_desc *d, int which) {
   if (!d || which < 0 || which > 3) return 0;
@@ -386,20 +396,54 @@ uint64_t bkv_slot_bytes(const bkv_cache_desc *d, int which) {
 }
 
 int64_t bkv_max_positions(const bkv_cache_desc *d) {
-  if (check(d)) return 0;
+  if (check_geom(d)) return 0;
   return max_positions(d);
+}
+
+// the single-sequence calls on a 4-bit cache: token t at position pos0 + t
+static SeqsView one_sequence(const bkv_cache_desc *d, const LayerView &L) {
+  SeqsView v{};
+  v.n_seq = 1;
+  v.tables = L.bt;
+  v.page = L.page;
+  v.pool_pages = d->page_tokens > 0 ? d->cap / d->page_tokens : 0;
+  v.max_pos = max_positions(d);
+  return v;
+}
+static hipError_t append_q4(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok, const bkv_rope &rope, Rows q, Rows k,
+                            Rows v, const float *qn_w, const float *kn_w, float eps, const int32_t *positions, float *q_out,
+                            hipStream_t stream) {
+  SeqsRowArgs a{};
+  a.L = view(d, layer);
+  a.v = one_sequence(d, a.L);
+  a.one = true;
+  a.pos0 = pos0;
+  a.nkv = d->nkv; a.nh = d->nh; a.n_tok = n_tok;
+  a.q = q; a.k = k; a.v_rows = v;
+  a.qn_w = qn_w; a.kn_w = kn_w;
+  a.eps = eps;
+  a.positions = positions;
+  a.q_out = q_out;
+  a.rope = rope;
+  return launch_seqs_rope_append(a, d->k_fmt, d->v_fmt, stream);
 }
 
 int bkv_kv_append(const bkv_cache_desc *d, int layer, uint32_t pos, int n_tok, const float *k,
                   const float *v, hipStream_t stream) {
-  int rc = check(d);
+  int rc = check_geom(d);
   if (rc) return rc;
-  if ((rc = check_kernels(d))) return rc;
+  if ((rc = any_q4(d) ? (d->hd == kHd ? BKV_OK : BKV_EUNSUPPORTED) : check_kernels(d))) return rc;
   if (layer < 0 || layer >= d->n_layers || n_tok < 0) return BKV_EINVAL;
   if (n_tok == 0) return BKV_OK;
   if ((int64_t)pos + n_tok > max_positions(d)) return BKV_ECAP;
   if (!k || !v) return BKV_EINVAL;
   if (!aligned16(k) || !aligned16(v)) return BKV_EALIGN;
+  if (any_q4(d)) {
+    const bkv_rope none{0, BKV_ROPE_HALF, 1.0f, 0, {}};
+    const int64_t tok = (int64_t)d->nkv * kHd;
+    return hip_fail(append_q4(d, layer, pos, n_tok, none, Rows{}, Rows{k, tok, kHd}, Rows{v, tok, kHd}, nullptr, nullptr, 0.0f,
+                              nullptr, nullptr, stream));
+  }
   AppendArgs a{};
   a.L = view(d, layer);
   a.nkv = d->nkv;
@@ -771,18 +815,23 @@ int bkv_rope_init(bkv_rope *r, int nrot, int layout, double freq_base, int scali
   return BKV_OK;
 }
 
+static bool rope_fine(const bkv_rope *rope) {
+  if (rope->nrot < 0 || rope->nrot > kHd || (rope->nrot & 1) || !std::isfinite(rope->mscale)) return false;
+  if (rope->layout != BKV_ROPE_HALF && rope->layout != BKV_ROPE_INTERLEAVED) return false;
+  for (int p = 0; p < rope->nrot / 2; ++p)
+    if (!std::isfinite(rope->turns[p])) return false;
+  return true;
+}
+
 int bkv_rope_append(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok, const bkv_rope *rope,
                     const bkv_rows *q, const bkv_rows *k, const bkv_rows *v, const float *qn_w,
                     const float *kn_w, float eps, const int32_t *positions, float *q_out,
                     hipStream_t stream) {
-  int rc = check(d);
+  int rc = check_geom(d);
   if (rc) return rc;
   if ((rc = check_hd(d))) return rc;
   if (layer < 0 || layer >= d->n_layers || n_tok < 0 || !rope) return BKV_EINVAL;
-  if (rope->nrot < 0 || rope->nrot > kHd || (rope->nrot & 1) || !std::isfinite(rope->mscale)) return BKV_EINVAL;
-  if (rope->layout != BKV_ROPE_HALF && rope->layout != BKV_ROPE_INTERLEAVED) return BKV_EINVAL;
-  for (int p = 0; p < rope->nrot / 2; ++p)
-    if (!std::isfinite(rope->turns[p])) return BKV_EINVAL;
+  if (!rope_fine(rope)) return BKV_EINVAL;
   if ((qn_w == nullptr) != (kn_w == nullptr) || (qn_w && !(eps >= 0.0f))) return BKV_EINVAL;
   if ((q == nullptr) != (q_out == nullptr)) return BKV_EINVAL;
   if (n_tok == 0) return BKV_OK;
@@ -791,6 +840,9 @@ int bkv_rope_append(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok
   if ((rc = check_rows(k)) || (rc = check_rows(v))) return rc;
   if ((q_out && !aligned16(q_out)) || (qn_w && (!aligned16(qn_w) || !aligned16(kn_w))) || ((uintptr_t)positions & 3u) != 0)
     return BKV_EALIGN;
+  if (any_q4(d))
+    return hip_fail(append_q4(d, layer, pos0, n_tok, *rope, rows_of(q), rows_of(k), rows_of(v), qn_w, kn_w, eps, positions, q_out,
+                              stream));
   RopeArgs a{};
   a.L = view(d, layer);
   a.pool_pages = pool_pages(d);
@@ -805,9 +857,21 @@ int bkv_rope_append(const bkv_cache_desc *d, int layer, uint32_t pos0, int n_tok
   return hip_fail(launch_rope_append(a, d->k_fmt, d->v_fmt, n_tok, stream));
 }
 
+// where values are written: rows that lie apart, whole tokens after one another or whole heads
+static int check_out_rows(const bkv_cache_desc *d, int n, int out_type, const void *k_out, const void *v_out, int64_t tok_stride,
+                          int64_t head_stride) {
+  const bool tokens = tok_stride >= (__int128)(d->nkv - 1) * head_stride + kHd && head_stride >= kHd;
+  const bool heads = head_stride >= (__int128)(n - 1) * tok_stride + kHd && tok_stride >= kHd;
+  if (n > 1 && d->nkv > 1 ? !(tokens || heads) : (n > 1 && tok_stride < kHd) || (d->nkv > 1 && head_stride < kHd)) return BKV_EINVAL;
+  const int64_t unit = out_type == BKV_OUT_F32 ? 4 : 8;
+  if ((k_out && !aligned16(k_out)) || (v_out && !aligned16(v_out)) || (n > 1 && tok_stride % unit) || (d->nkv > 1 && head_stride % unit))
+    return BKV_EALIGN;
+  return BKV_OK;
+}
+
 int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int out_type, void *k_out,
                 void *v_out, int64_t tok_stride, int64_t head_stride, hipStream_t stream) {
-  int rc = check(d);
+  int rc = check_geom(d);
   if (rc) return rc;
   if ((rc = check_hd(d))) return rc;
   if (layer < 0 || layer >= d->n_layers || n < 0) return BKV_EINVAL;
@@ -815,13 +879,19 @@ int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int ou
   if (n == 0) return BKV_OK;
   if (outside(d, pos0, n)) return BKV_ECAP;
   if (!k_out && !v_out) return BKV_EINVAL;
-  // rows lie apart: whole tokens after one another, or whole heads
-  const bool tokens = tok_stride >= (__int128)(d->nkv - 1) * head_stride + kHd && head_stride >= kHd;
-  const bool heads = head_stride >= (__int128)(n - 1) * tok_stride + kHd && tok_stride >= kHd;
-  if (n > 1 && d->nkv > 1 ? !(tokens || heads) : (n > 1 && tok_stride < kHd) || (d->nkv > 1 && head_stride < kHd)) return BKV_EINVAL;
-  const int64_t unit = out_type == BKV_OUT_F32 ? 4 : 8;
-  if ((k_out && !aligned16(k_out)) || (v_out && !aligned16(v_out)) || (n > 1 && tok_stride % unit) || (d->nkv > 1 && head_stride % unit))
-    return BKV_EALIGN;
+  if ((rc = check_out_rows(d, n, out_type, k_out, v_out, tok_stride, head_stride))) return rc;
+  if (any_q4(d)) {
+    SeqsReadArgs s{};
+    s.L = view(d, layer);
+    s.v = one_sequence(d, s.L);
+    s.one = true;
+    s.pos0 = pos0;
+    s.nkv = d->nkv;
+    s.n_tok = n;
+    s.k_out = k_out; s.v_out = v_out;
+    s.tok = tok_stride; s.head = head_stride;
+    return hip_fail(launch_seqs_read(s, d->k_fmt, d->v_fmt, out_type, stream));
+  }
   ReadArgs a{};
   a.L = view(d, layer);
   a.pool_pages = pool_pages(d);
@@ -835,7 +905,7 @@ int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int ou
 
 int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_keep, const int32_t *idx,
                   hipStream_t stream) {
-  int rc = check(d);
+  int rc = check_geom(d);
   if (rc) return rc;
   if ((rc = check_hd(d))) return rc;
   if (n_draft < 0 || n_draft > BKV_TREE_MAX_Q || n_keep < 0 || n_keep > n_draft) return BKV_EINVAL;
@@ -863,6 +933,234 @@ int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_kee
   return hip_fail(launch_kv_commit(a, d->n_layers, stream));
 }
 
+// ------------------------------------------------------------------ several sequences
+static int check_seqs(const bkv_cache_desc *d, const bkv_seqs *s) {
+  if (!s || s->n_seq < 0 || s->n_seq > BKV_SEQS_MAX || s->n_tok < 0 || s->max_q < 0 || s->reserved != 0) return BKV_EINVAL;
+  if (s->n_seq == 0 || s->n_tok == 0) return BKV_OK;
+  if (!s->len || (!s->q_start && s->n_tok < s->n_seq)) return BKV_EINVAL;
+  if (d->page_tokens > 0 ? !s->tables : s->n_seq > 1) return BKV_EINVAL;
+  if (((uintptr_t)s->q_start | (uintptr_t)s->len | (uintptr_t)s->tables) & 3u) return BKV_EALIGN;
+  // (rows and grids are counted in 31 bits, a step's bytes in 32)
+  if ((int64_t)s->n_tok * d->nh > INT32_MAX / 2 || d->nkv > 65536) return BKV_EUNSUPPORTED;
+  return BKV_OK;
+}
+static SeqsView seqs_view(const bkv_cache_desc *d, int layer, const bkv_seqs *s) {
+  SeqsView v{};
+  v.n_seq = s->n_seq;
+  v.n_tok = s->n_tok;
+  v.q_start = s->q_start;
+  v.len = s->len;
+  v.page = d->page_tokens > 0 ? d->page_tokens : 0;
+  v.pool_pages = pool_pages(d);
+  v.tables = v.page ? s->tables + (int64_t)layer * d->max_pages : nullptr;
+  v.table_stride = (int64_t)d->n_layers * d->max_pages;
+  v.max_pos = std::min<int64_t>(max_positions(d), INT32_MAX - 64);
+  return v;
+}
+
+int bkv_rope_axes_init(bkv_rope_axes *x, int n_axes, const int32_t *pairs, int order) {
+  if (!x || !pairs || n_axes < 1 || n_axes > BKV_ROPE_MAX_AXES) return BKV_EINVAL;
+  if (order != BKV_AXES_BLOCKS && order != BKV_AXES_DEALT) return BKV_EINVAL;
+  int left[BKV_ROPE_MAX_AXES], total = 0;
+  for (int i = 0; i < n_axes; ++i) {
+    if (pairs[i] < 0 || pairs[i] > kHd / 2 - total) return BKV_EINVAL;
+    total += left[i] = pairs[i];
+  }
+  std::memset(x, 0, sizeof *x);
+  x->n_axes = n_axes;
+  x->n_pairs = total;
+  for (int p = 0, i = 0; p < total; ++p) {
+    while (left[i] == 0) i = (i + 1) % n_axes;
+    x->axis[p] = (uint8_t)i;
+    --left[i];
+    if (order == BKV_AXES_DEALT) i = (i + 1) % n_axes;
+  }
+  return BKV_OK;
+}
+
+int bkv_seqs_rope_append(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, const bkv_rope *rope, const bkv_rope_axes *axes,
+                         const bkv_rows *q, const bkv_rows *k, const bkv_rows *v, const float *qn_w, const float *kn_w, float eps,
+                         const int32_t *positions, float *q_out, hipStream_t stream) {
+  int rc = check_geom(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (layer < 0 || layer >= d->n_layers || !rope || !rope_fine(rope)) return BKV_EINVAL;
+  if (axes) {
+    if (axes->n_axes < 1 || axes->n_axes > BKV_ROPE_MAX_AXES || axes->n_pairs != rope->nrot / 2 || (axes->n_axes > 1 && !positions))
+      return BKV_EINVAL;
+    for (int p = 0; p < axes->n_pairs; ++p)
+      if (axes->axis[p] >= axes->n_axes) return BKV_EINVAL;
+  }
+  if ((qn_w == nullptr) != (kn_w == nullptr) || (qn_w && !(eps >= 0.0f))) return BKV_EINVAL;
+  if ((q == nullptr) != (q_out == nullptr)) return BKV_EINVAL;
+  if ((rc = check_seqs(d, seqs))) return rc;
+  if (seqs->n_seq == 0 || seqs->n_tok == 0) return BKV_OK;
+  if (q && (rc = check_rows(q))) return rc;
+  if ((rc = check_rows(k)) || (rc = check_rows(v))) return rc;
+  if ((q_out && !aligned16(q_out)) || (qn_w && (!aligned16(qn_w) || !aligned16(kn_w))) || ((uintptr_t)positions & 3u) != 0)
+    return BKV_EALIGN;
+  SeqsRowArgs a{};
+  a.L = view(d, layer);
+  a.v = seqs_view(d, layer, seqs);
+  a.nkv = d->nkv; a.nh = d->nh; a.n_tok = seqs->n_tok;
+  a.q = rows_of(q); a.k = rows_of(k); a.v_rows = rows_of(v);
+  a.qn_w = qn_w; a.kn_w = kn_w;
+  a.eps = eps;
+  a.positions = positions;
+  a.q_out = q_out;
+  a.rope = *rope;
+  if (axes) std::memcpy(a.axis, axes->axis, sizeof a.axis);
+  return hip_fail(launch_seqs_rope_append(a, d->k_fmt, d->v_fmt, stream));
+}
+
+int bkv_seqs_read(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, int out_type, void *k_out, void *v_out,
+                  int64_t tok_stride, int64_t head_stride, hipStream_t stream) {
+  int rc = check_geom(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (layer < 0 || layer >= d->n_layers || out_type < BKV_OUT_F32 || out_type > BKV_OUT_BF16) return BKV_EINVAL;
+  if ((rc = check_seqs(d, seqs))) return rc;
+  if (seqs->n_seq == 0 || seqs->n_tok == 0) return BKV_OK;
+  if (!k_out && !v_out) return BKV_EINVAL;
+  if ((rc = check_out_rows(d, seqs->n_tok, out_type, k_out, v_out, tok_stride, head_stride))) return rc;
+  SeqsReadArgs a{};
+  a.L = view(d, layer);
+  a.v = seqs_view(d, layer, seqs);
+  a.nkv = d->nkv;
+  a.n_tok = seqs->n_tok;
+  a.k_out = k_out; a.v_out = v_out;
+  a.tok = tok_stride; a.head = head_stride;
+  return hip_fail(launch_seqs_read(a, d->k_fmt, d->v_fmt, out_type, stream));
+}
+
+size_t bkv_seqs_workspace_bytes(const bkv_cache_desc *d, int n_seq, int n_tok) {
+  if (check_geom(d) || n_seq < 1 || n_seq > BKV_SEQS_MAX || n_tok < 1 || (int64_t)n_tok * d->nh > INT32_MAX / 2 || d->nkv > 65536) return 0;
+  return plan_seqs_attn(d->nh, d->nkv, n_seq, n_tok).total;
+}
+
+int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, const bkv_rows *q, const bkv_rows *gate, float *out,
+                  float *out_gated, void *workspace, size_t ws_bytes, hipStream_t stream) {
+  int rc = check_geom(d);
+  if (rc) return rc;
+  if ((rc = check_hd(d))) return rc;
+  if (d->k_fmt != BKV_Q4_0 || d->v_fmt != BKV_Q4_0) return BKV_EUNSUPPORTED;
+  if (layer < 0 || layer >= d->n_layers) return BKV_EINVAL;
+  if ((rc = check_seqs(d, seqs))) return rc;
+  if (seqs->n_seq == 0 || seqs->n_tok == 0) return BKV_OK;
+  if ((rc = check_rows(q))) return rc;
+  if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
+  if (gate && (rc = check_rows(gate))) return rc;
+  if (!aligned16(out) || (out_gated && !aligned16(out_gated))) return BKV_EALIGN;
+  if (!workspace) return BKV_EWORKSPACE;
+  if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
+  const SeqsAttnPlan p = plan_seqs_attn(d->nh, d->nkv, seqs->n_seq, seqs->n_tok);
+  if (ws_bytes < p.total) return BKV_EWORKSPACE;
+  char *w = (char *)workspace;
+  SeqsAttnArgs a{};
+  a.L = view(d, layer);
+  a.v = seqs_view(d, layer, seqs);
+  a.nkv = d->nkv; a.nh = d->nh; a.grp = d->nh / d->nkv;
+  a.scale2 = (float)((double)d->scale * 1.4426950408889634);
+  a.q = rows_of(q);
+  a.gate = rows_of(gate);
+  a.out = out;
+  a.out_gated = out_gated;
+  a.lanes = p.lanes;
+  a.least = p.least;
+  a.part_rows = p.part_rows;
+  a.info = (uint4 *)w;
+  a.ml = (float2 *)(w + p.off_ml);
+  a.part = (float *)(w + p.off_part);
+  return hip_fail(launch_seqs_attn(a, p, stream));
+}
+
+// ------------------------------------------------------------------ pages
+static int check_pages(const bkv_cache_desc *d, int n_seq, const void *tables, const void *refs) {
+  if (n_seq < 0 || n_seq > BKV_SEQS_MAX || d->page_tokens <= 0 || !tables || !refs) return BKV_EINVAL;
+  if (((uintptr_t)tables | (uintptr_t)refs) & 3u) return BKV_EALIGN;
+  if ((int64_t)n_seq * d->max_pages > (1 << 30) || d->n_layers > 65535) return BKV_EUNSUPPORTED;   // (counts in 31 bits; a grid's rows)
+  return BKV_OK;
+}
+static PagesArgs pages_args(const bkv_cache_desc *d, int n_seq) {
+  PagesArgs a{};
+  void *bases[4] = {d->k_data, d->k_scales, d->v_data, d->v_scales};
+  for (int i = 0; i < 4; ++i) {
+    a.slot[i] = slot_bytes(d, i);
+    a.base[i] = a.slot[i] ? (uint8_t *)bases[i] : nullptr;
+    a.stride[i] = d->layer_stride_bytes[i];
+  }
+  a.n_layers = d->n_layers;
+  a.n_seq = n_seq;
+  a.page = d->page_tokens;
+  a.pool_pages = pool_pages(d);
+  a.max_pages = d->max_pages;
+  return a;
+}
+// a page's pieces are counted in 31 bits
+static bool page_too_large(const bkv_cache_desc *d) {
+  uint64_t most = 0;
+  for (int i = 0; i < 4; ++i) most = std::max<uint64_t>(most, slot_bytes(d, i) * (uint64_t)d->page_tokens);
+  return most > (uint64_t(1) << 40);
+}
+
+size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d) {
+  if (check_geom(d) || d->page_tokens <= 0) return 0;
+  return pages_workspace(d->n_layers, pool_pages(d));
+}
+
+int bkv_pages_fork(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t *refs, int32_t *len, const int32_t *parent,
+                   hipStream_t stream) {
+  int rc = check_geom(d);
+  if (rc) return rc;
+  if ((rc = check_pages(d, n_seq, tables, refs))) return rc;
+  if (n_seq == 0) return BKV_OK;
+  if (!parent) return BKV_EINVAL;
+  if (((uintptr_t)parent | (uintptr_t)len) & 3u) return BKV_EALIGN;
+  PagesArgs a = pages_args(d, n_seq);
+  a.tables = a.tables_out = tables;
+  a.refs = a.refs_out = refs;
+  a.len = len;
+  a.parent = parent;
+  return hip_fail(launch_pages_fork(a, stream));
+}
+
+int bkv_pages_extend(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t *refs, const int32_t *len, const int32_t *n_new,
+                     int32_t *lack, void *workspace, size_t ws_bytes, hipStream_t stream) {
+  int rc = check_geom(d);
+  if (rc) return rc;
+  if ((rc = check_pages(d, n_seq, tables, refs))) return rc;
+  if (!len || !n_new || !lack) return BKV_EINVAL;
+  if (((uintptr_t)len | (uintptr_t)n_new | (uintptr_t)lack) & 3u) return BKV_EALIGN;
+  if (page_too_large(d)) return BKV_EUNSUPPORTED;
+  if (!workspace || ws_bytes < pages_workspace(d->n_layers, pool_pages(d))) return BKV_EWORKSPACE;
+  if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
+  PagesArgs a = pages_args(d, n_seq);
+  a.tables = a.tables_out = tables;
+  a.refs = a.refs_out = refs;
+  a.len = const_cast<int32_t *>(len);
+  a.n_new = n_new;
+  a.lack = lack;
+  a.ws = (int32_t *)workspace;
+  return hip_fail(launch_pages_extend(a, stream));
+}
+
+int bkv_pages_compact(const bkv_cache_desc *d, int n_seq, const int32_t *tables, const int32_t *refs, int32_t *tables_out,
+                      int32_t *refs_out, void *workspace, size_t ws_bytes, hipStream_t stream) {
+  int rc = check_geom(d);
+  if (rc) return rc;
+  if ((rc = check_pages(d, n_seq, tables, refs)) || (rc = check_pages(d, n_seq, tables_out, refs_out))) return rc;
+  if (page_too_large(d)) return BKV_EUNSUPPORTED;
+  if (!workspace || ws_bytes < pages_workspace(d->n_layers, pool_pages(d))) return BKV_EWORKSPACE;
+  if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
+  PagesArgs a = pages_args(d, n_seq);
+  a.tables = tables;
+  a.refs = refs;
+  a.tables_out = tables_out;
+  a.refs_out = refs_out;
+  a.ws = (int32_t *)workspace;
+  return hip_fail(launch_pages_compact(a, stream));
+}
+
 size_t bkv_workspace_bytes(const bkv_cache_desc *d, int op, uint32_t max_ctx) {
   if (check(d) || max_ctx == 0) return 0;
   if (op == BKV_OP_TREE) return tree_workspace_bound(d->nh, prefill_base(d));
@@ -883,7 +1181,7 @@ const char *bkv_strerror(int err) {
     case BKV_EWORKSPACE: return "workspace missing or smaller than bkv_workspace_bytes()";
     case BKV_ESCRATCH: return "decode plan larger than the static scratch (bkv_static_scratch_bytes())";
     case BKV_EHIP: return "HIP runtime error (see bkv_last_hip_error)";
-    case BKV_EUNSUPPORTED: return "shape not supported by the gfx950 kernels (hd 256, nh = 4*nkv)";
+    case BKV_EUNSUPPORTED: return "shape or format not supported by this call (hd 256, nh = 4*nkv, the cache's formats)";
     case BKV_ETIMEOUT: return "a decode kernel's workgroup wait timed out (its output is not valid)";
     default: return "unknown error";
   }
@@ -954,17 +1252,15 @@ int bkv_workspace_init(const bkv_cache_desc *d, void *workspace, size_t ws_bytes
 }
 
 int bkv_kv_fill_synthetic(const bkv_cache_desc *d, hipStream_t stream) {
-  const int rc = check(d);
+  const int rc = check_geom(d);
   if (rc) return rc;
-  const size_t slots = (size_t)d->cap * d->nkv;
-  const size_t rows[4] = {slots * (size_t)row_bytes(d->k_fmt), slots * kScaleRowBytes,
-                          slots * (size_t)row_bytes(d->v_fmt), slots * kScaleRowBytes};
   void *bases[4] = {d->k_data, d->k_scales, d->v_data, d->v_scales};
   for (int i = 0; i < 4; ++i) {
     if (!bases[i]) continue;
     for (int l = 0; l < d->n_layers; ++l) {
       unsigned *p = (unsigned *)((char *)bases[i] + (uint64_t)l * d->layer_stride_bytes[i]);
-      const hipError_t e = launch_fill_words(p, rows[i] / 4, 0x3C003C00u, stream);
+      const size_t bytes = (size_t)d->cap * (i & 1 ? (size_t)d->nkv * kScaleRowBytes : slot_bytes(d, i));
+      const hipError_t e = launch_fill_words(p, bytes / 4, 0x3C003C00u, stream);
       if (e != hipSuccess) return hip_fail(e);
     }
   }

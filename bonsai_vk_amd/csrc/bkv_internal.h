@@ -7,6 +7,7 @@
 
 #include "../../include/bkv.h"
 #include "bkv_common.h"
+#include "bkv_q4.h"
 
 namespace bkv {
 
@@ -299,6 +300,73 @@ struct CommitArgs {
   const int32_t *idx;
 };
 hipError_t launch_kv_commit(const CommitArgs &a, int n_layers, hipStream_t st);
+
+// ------------------------------------------------------------------ several sequences
+struct SeqsRowArgs {
+  LayerView L;
+  SeqsView v;
+  bool one;                      // one sequence: token t is position pos0 + t (v.q_start and v.len are not read)
+  uint32_t pos0;
+  int nkv, nh, n_tok;
+  Rows q, k, v_rows;             // q.p null: K and V only
+  const float *qn_w, *kn_w;      // null: no norm
+  float eps;
+  const int32_t *positions;      // [axes][n_tok], null: the cache's positions
+  float *q_out;
+  bkv_rope rope;
+  uint8_t axis[kHd / 2];         // of each pair
+};
+hipError_t launch_seqs_rope_append(const SeqsRowArgs &a, int kf, int vf, hipStream_t st);
+
+struct SeqsReadArgs {
+  LayerView L;
+  SeqsView v;
+  bool one;
+  uint32_t pos0;
+  int nkv, n_tok;
+  void *k_out, *v_out;           // (one may be null)
+  int64_t tok, head;             // strides in elements
+};
+hipError_t launch_seqs_read(const SeqsReadArgs &a, int kf, int vf, int out_type, hipStream_t st);
+
+struct SeqsAttnArgs {
+  LayerView L;
+  SeqsView v;
+  int nkv, nh, grp;              // grp = nh / nkv query heads per KV head
+  float scale2;                  // softmax scale times log2(e)
+  Rows q, gate;                  // gate.p null: none
+  float *out, *out_gated;
+  int lanes, least;              // pieces that the line of steps is cut into at most, steps of each at least
+  uint64_t part_rows;            // rows of part
+  float *part;                   // unnormalised partial outputs [..][hd]
+  float2 *ml;                    // their reference (log2) and sum
+  uint4 *info;                   // per output row: its first partial result, the distance of the next, how many (1: none)
+};
+struct SeqsAttnPlan {
+  int lanes, least;
+  uint64_t part_rows;
+  size_t off_ml, off_part, total;
+};
+SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok);
+hipError_t launch_seqs_attn(const SeqsAttnArgs &a, const SeqsAttnPlan &p, hipStream_t st);
+
+// ------------------------------------------------------------------ pages
+struct PagesArgs {
+  uint8_t *base[4];              // layer 0's arrays (null: absent)
+  uint64_t stride[4];            // bytes from a layer to the next
+  uint64_t slot[4];              // bytes of a slot
+  int n_layers, n_seq, page, pool_pages, max_pages;
+  const int32_t *tables, *refs;
+  int32_t *tables_out, *refs_out;
+  int32_t *len;                  // fork: in and out (may be null); extend: in
+  const int32_t *parent, *n_new;
+  int32_t *lack;                 // [n_layers]
+  int32_t *ws;                   // see bkv_pages.hip
+};
+hipError_t launch_pages_fork(const PagesArgs &a, hipStream_t st);
+hipError_t launch_pages_extend(const PagesArgs &a, hipStream_t st);
+hipError_t launch_pages_compact(const PagesArgs &a, hipStream_t st);
+size_t pages_workspace(int n_layers, int pool_pages);
 
 #define BKV_FMT_SWITCH(KF, VF, ...)                                                    \
   do {                                                                                \

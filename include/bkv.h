@@ -34,8 +34,18 @@ typedef struct ihipStream_t *hipStream_t;
 /* ------------------------------------------------------------------ formats and errors */
 enum bkv_fmt {
   BKV_F16  = 0,   /* [slot][nkv][hd/2] u32, element 2w in the low half of word w (RNE packed)  */
-  BKV_Q8_0 = 1    /* data [slot][nkv][hd/4] u32 (element e = byte e%4 of word e/4, int8) plus   */
+  BKV_Q8_0 = 1,   /* data [slot][nkv][hd/4] u32 (element e = byte e%4 of word e/4, int8) plus   */
                   /* scales [slot][nkv][hd/64] u32 (fp16 scale of block 2i low, 2i+1 high)      */
+  BKV_Q4_0 = 2    /* 4 bits a value (no counterpart in the reference): data [slot][nkv][hd/8] u32, element */
+                  /* 8w+i of a head row as q+8 in 4 bits of word w, i = 2s+h at bit 16h+4s; scales as  */
+                  /* BKV_Q8_0's. A block of 32 has a scale d, value = d*q, q = -8 .. 7. Written: d is the */
+                  /* value furthest from 0 (of two as far the positive one) times -1/8, rounded to fp16, */
+                  /* then to that number's upper 13 bits, |d| at most 2048; q = clamp(rne(x*(1/d)), -8, 7), */
+                  /* 0 for a NaN. Read: a scale's low 3 bits do not count, and a magnitude past 2048 is  */
+                  /* 2048 (Inf and NaN patterns too), so every value is a finite, exact fp16 number.   */
+                  /* Taken by: bkv_kv_append, bkv_rope_append, bkv_kv_read, bkv_kv_commit,             */
+                  /* bkv_kv_fill_synthetic and the calls for several sequences (below). The others, whose */
+                  /* results are the reference's bit for bit, answer BKV_EUNSUPPORTED.                 */
 };
 
 enum bkv_err {
@@ -338,6 +348,93 @@ int bkv_kv_read(const bkv_cache_desc *d, int layer, uint32_t pos0, int n, int ou
  * outside 0 .. n_draft-1 leaves its position as it is. n_keep <= n_draft <= BKV_TREE_MAX_Q. */
 int bkv_kv_commit(const bkv_cache_desc *d, uint32_t pos0, int n_draft, int n_keep, const int32_t *idx,
                   hipStream_t stream);
+
+/* ------------------------------------------------------------------ several sequences
+ * A server's step over many sequences that share one pool of pages (no counterpart in the reference, which runs one
+ * sequence): bkv_pages_extend gives each the pages for its new tokens, bkv_seqs_rope_append writes them, bkv_seqs_attn
+ * attends, and bkv_pages_fork and bkv_pages_compact rearrange who has which pages. head_dim 256, any nh that is a multiple
+ * of nkv. What says how the step is shared out (starts, lengths, tables) is device memory, read by the kernels: a captured
+ * call serves other lengths at its next replay. No value in it makes a call reach outside the arrays it was given; a
+ * token whose position is not in the cache, or whose page is not in the pool, is not written and not seen.              */
+#define BKV_SEQS_MAX 1024
+
+/* The tokens of a call, those of each sequence one after another: sequence s has rows q_start[s] .. q_start[s+1]-1 of q, k,
+ * v and the outputs (none: it takes no part), and they are the last of the len[s] positions it has in the cache: row
+ * q_start[s]+i is position len[s] - n + i. Rows before q_start[0] and from q_start[n_seq] on are left as they are. */
+typedef struct bkv_seqs {
+  int32_t n_seq;              /* 0 .. BKV_SEQS_MAX                                                       */
+  int32_t n_tok;              /* rows that there are                                                     */
+  int32_t max_q;              /* tokens that no sequence has more of, which bkv_seqs_attn chooses its kernels */
+                              /* by, or 0: not known (a wrong one costs time, and nothing else)          */
+  int32_t reserved;           /* 0                                                                       */
+  const int32_t *q_start;     /* device [n_seq+1], ascending, 0 .. n_tok; NULL: one token each, s = row  */
+  const int32_t *len;         /* device [n_seq], this call's tokens among them                           */
+  const int32_t *tables;      /* device [n_seq][n_layers][max_pages], in the place of the descriptor's   */
+                              /* block table (paged); NULL for a contiguous cache, n_seq <= 1            */
+} bkv_seqs;
+
+/* Which axis' position turns each pair (time, height and width of a picture's tokens). */
+#define BKV_ROPE_MAX_AXES 8
+enum bkv_axes_order { BKV_AXES_BLOCKS = 0,   /* the first axis' pairs, then the second's, ..                 */
+                      BKV_AXES_DEALT = 1 };  /* dealt out in turn to the axes that still want some           */
+typedef struct bkv_rope_axes {
+  int32_t n_axes, n_pairs;
+  uint8_t axis[128];
+} bkv_rope_axes;
+
+/* Host side, no GPU: fill *x for n_axes (1 .. BKV_ROPE_MAX_AXES) axes of pairs[i] >= 0 pairs, nrot/2 in all. */
+int bkv_rope_axes_init(bkv_rope_axes *x, int n_axes, const int32_t *pairs, int order);
+
+/* bkv_rope_append of several sequences' tokens, any format, with positions of several axes: pair p is turned by the angle
+ * 2*pi * positions[axis[p]][t] * turns[p]. positions: device int32 [n_axes][n_tok], or NULL (one axis: the position in the
+ * cache); axes NULL: one. Every row of q that is a sequence's is rotated; K and V are written where the position is one.
+ * (The norm's sum and the angle are formed in fp64.) */
+int bkv_seqs_rope_append(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, const bkv_rope *rope, const bkv_rope_axes *axes,
+                         const bkv_rows *q, const bkv_rows *k, const bkv_rows *v, const float *qn_w, const float *kn_w,
+                         float eps, const int32_t *positions, float *q_out, hipStream_t stream);
+
+/* bkv_kv_read of the call's tokens: row t takes the values of its sequence's position (0 where that is not in the cache),
+ * any format. With q_start the lengths' sums it packs whole sequences one after another. */
+int bkv_seqs_read(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, int out_type, void *k_out, void *v_out,
+                  int64_t tok_stride, int64_t head_stride, hipStream_t stream);
+
+/* Attention over a 4-bit cache (K and V BKV_Q4_0): row i of a sequence of n tokens sees its positions 0 .. len - n + i.
+ *   Per head row: score = scale * (q16 . k) with q rounded to fp16, p = softmax over them, out = sum p * v, sums in fp32 in no
+ *   stated order (the result does not change from call to call). Beside fp32's roundings an output carries at most 2^-22
+ *   of sum p |v|, 2^-34 of sum |v|, and 2^-36 of the largest p for a position whose |v| is below 2^-14. A row that sees
+ *   nothing gets 0. Positions that a row does not see have no effect on it.
+ *   out: [n_tok][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)). Neither may overlap the inputs
+ *   or the other.
+ * Workspace: bkv_seqs_workspace_bytes(d, n_seq, n_tok), which grows with both; it needs no initialisation. Calls (and replays
+ * of captured ones) that share one must not overlap in time. */
+size_t bkv_seqs_workspace_bytes(const bkv_cache_desc *d, int n_seq, int n_tok);
+int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, const bkv_rows *q, const bkv_rows *gate, float *out,
+                  float *out_gated, void *workspace, size_t ws_bytes, hipStream_t stream);
+
+/* Pages (d paged, any format and head_dim; d->block_table is not read). tables: device [n_seq][n_layers][max_pages], the page
+ * of each sequence's positions, an entry outside the pool (-1) where there is none. refs: device [n_layers][cap /
+ * page_tokens], how many entries of all tables name a page; 0: it is free. Each layer has pages of its own.
+ *
+ * fork: row s of the tables becomes what row parent[s] (device [n_seq]) was, as if all were read before any is written, and
+ * refs follow: a new sequence goes on from another's positions, beams are put in order, and parent[s] outside 0 .. n_seq-1
+ * gives a sequence's pages back. len (device [n_seq], or NULL) is rearranged with them, 0 for the last kind. */
+int bkv_pages_fork(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t *refs, int32_t *len, const int32_t *parent,
+                   hipStream_t stream);
+
+/* extend: n_new[s] more positions of a sequence that has len[s] (both device [n_seq]): every page that these lie in becomes
+ * the sequence's own. Where there is none it gets a free one; where others have it too, it gets a free one with the
+ * positions below len[s] copied, but the last sequence keeps a page that nobody else would. Free pages are given
+ * lowest first, in the order of sequences and positions. lack: device [n_layers], the pages that a layer is short of (free
+ * ones, or places in a table's row); where any is, nothing is changed in any layer. */
+size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d);   /* of extend and compact; needs no initialisation */
+int bkv_pages_extend(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t *refs, const int32_t *len, const int32_t *n_new,
+                     int32_t *lack, void *workspace, size_t ws_bytes, hipStream_t stream);
+
+/* compact: with U pages in use in a layer, the i-th of them numbered U or more moves to the i-th free one below U. The new
+ * tables and counts go to tables_out and refs_out (which may be tables and refs). Entries outside the pool stay. The pages
+ * moved from keep their bytes until they are given out again. */
+int bkv_pages_compact(const bkv_cache_desc *d, int n_seq, const int32_t *tables, const int32_t *refs, int32_t *tables_out,
+                      int32_t *refs_out, void *workspace, size_t ws_bytes, hipStream_t stream);
 
 /* Human-readable text of an enum bkv_err value (static storage). */
 const char *bkv_strerror(int err);
