@@ -1035,7 +1035,7 @@ int bkv_seqs_read(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, int 
 
 size_t bkv_seqs_workspace_bytes(const bkv_cache_desc *d, int n_seq, int n_tok) {
   if (check_geom(d) || n_seq < 1 || n_seq > BKV_SEQS_MAX || n_tok < 1 || (int64_t)n_tok * d->nh > INT32_MAX / 2 || d->nkv > 65536) return 0;
-  return plan_seqs_attn(d->nh, d->nkv, n_seq, n_tok).total;
+  return plan_seqs_attn(d->nh, d->nkv, n_seq, n_tok, 0).total;
 }
 
 int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, const bkv_rows *q, const bkv_rows *gate, float *out,
@@ -1047,13 +1047,16 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
   if (layer < 0 || layer >= d->n_layers) return BKV_EINVAL;
   if ((rc = check_seqs(d, seqs))) return rc;
   if (seqs->n_seq == 0 || seqs->n_tok == 0) return BKV_OK;
+  // (row blocks of 16 times steps of 32 positions are counted in 31 bits)
+  const int64_t blocks = (int64_t)seqs->n_tok * (d->nh / d->nkv) / 16 + seqs->n_seq;
+  if (blocks > INT32_MAX / (std::min<int64_t>(max_positions(d), INT32_MAX) / 32 + 1)) return BKV_EUNSUPPORTED;
   if ((rc = check_rows(q))) return rc;
   if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
   if (gate && (rc = check_rows(gate))) return rc;
   if (!aligned16(out) || (out_gated && !aligned16(out_gated))) return BKV_EALIGN;
   if (!workspace) return BKV_EWORKSPACE;
   if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
-  const SeqsAttnPlan p = plan_seqs_attn(d->nh, d->nkv, seqs->n_seq, seqs->n_tok);
+  const SeqsAttnPlan p = plan_seqs_attn(d->nh, d->nkv, seqs->n_seq, seqs->n_tok, seqs->max_q);
   if (ws_bytes < p.total) return BKV_EWORKSPACE;
   char *w = (char *)workspace;
   SeqsAttnArgs a{};
@@ -1066,9 +1069,18 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
   a.out = out;
   a.out_gated = out_gated;
   a.lanes = p.lanes;
-  a.least = p.least;
-  a.part_rows = p.part_rows;
-  a.info = (uint4 *)w;
+  a.by_nkv = ByConst(d->nkv);
+  a.by_grp = ByConst(a.grp);
+  a.by_lanes = ByConst(p.lanes);
+  a.by_page = ByConst(std::max(1, d->page_tokens));
+  a.count = (unsigned *)w;
+  a.few = p.few;
+  a.tile_lanes = p.tile_lanes;
+  a.by_tile_lanes = ByConst(p.tile_lanes);
+  a.tile_part_rows = p.tile_part_rows;
+  a.info = (uint4 *)(w + p.off_info);
+  a.tile_ml = (float2 *)(w + p.off_tile_ml);
+  a.tile_part = (float *)(w + p.off_tile_part);
   a.ml = (float2 *)(w + p.off_ml);
   a.part = (float *)(w + p.off_part);
   return hip_fail(launch_seqs_attn(a, p, stream));
@@ -1241,11 +1253,11 @@ int bkv_debug_layout(const bkv_cache_desc *d, uint32_t nfill, uint64_t out[6]) {
 }
 
 int bkv_workspace_init(const bkv_cache_desc *d, void *workspace, size_t ws_bytes, hipStream_t stream) {
-  const int rc = check(d);
+  const int rc = check_geom(d);
   if (rc) return rc;
   if (!workspace) return BKV_EWORKSPACE;
   if (((uintptr_t)workspace & 255u) != 0) return BKV_EALIGN;
-  if (ws_bytes < kSyncBytes) return BKV_EWORKSPACE;
+  if (!any_q4(d) && ws_bytes < kSyncBytes) return BKV_EWORKSPACE;
   // the whole workspace: the sync words, and the tagged partials of the resident path (a tag is
   // the call generation, which starts at 1)
   return hip_fail(launch_workspace_init((unsigned *)workspace, ws_bytes / sizeof(unsigned), stream));

@@ -122,6 +122,15 @@ __device__ __forceinline__ void load_to_lds(const void *src, uint32_t dst) {
 __device__ __forceinline__ void load_to_lds(const void *base, uint32_t off, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
 }
+// (to dst + AT; a base that a vector instruction has just written, a v_readlane, needs five wait states)
+template <int AT>
+__device__ __forceinline__ void load_to_lds_at(const void *base, uint32_t off, uint32_t dst) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst), "i"(AT) : "memory", "m0", "scc");
+}
+template <int AT>
+__device__ __forceinline__ void load_to_lds_at(const void *src, uint32_t dst) {
+  asm volatile("s_add_u32 m0, %1, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst), "i"(AT) : "memory", "m0", "scc");
+}
 __device__ __forceinline__ void load4_to_lds(const void *src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
 }

@@ -336,18 +336,26 @@ struct SeqsAttnArgs {
   float scale2;                  // softmax scale times log2(e)
   Rows q, gate;                  // gate.p null: none
   float *out, *out_gated;
-  int lanes, least;              // pieces that the line of steps is cut into at most, steps of each at least
-  uint64_t part_rows;            // rows of part
-  float *part;                   // unnormalised partial outputs [..][hd]
+  int lanes;                     // pieces that the line of steps is cut into at most
+  ByConst by_nkv, by_grp, by_lanes, by_page;
+  unsigned *count;               // pieces of a row block that are done (all 0 between calls)
+  float *part;                   // [2 lanes][nkv][16] unnormalised partial outputs of hd
   float2 *ml;                    // their reference (log2) and sum
-  uint4 *info;                   // per output row: its first partial result, the distance of the next, how many (1: none)
+  int few;                       // sequences of more rows than this go by tiles
+  int tile_lanes;                // the same of the tiles
+  ByConst by_tile_lanes;
+  uint64_t tile_part_rows;
+  float *tile_part;
+  float2 *tile_ml;
+  uint4 *info;                   // per output row of a tile: its first partial result, the distance of the next, how many (1: none)
 };
 struct SeqsAttnPlan {
-  int lanes, least;
-  uint64_t part_rows;
-  size_t off_ml, off_part, total;
+  int lanes, tile_lanes, few;
+  bool blocks, tiles;            // which kernels run
+  uint64_t tile_part_rows;
+  size_t off_ml, off_part, off_info, off_tile_ml, off_tile_part, total;
 };
-SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok);
+SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q);
 hipError_t launch_seqs_attn(const SeqsAttnArgs &a, const SeqsAttnPlan &p, hipStream_t st);
 
 // ------------------------------------------------------------------ pages

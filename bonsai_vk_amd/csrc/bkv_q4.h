@@ -49,6 +49,21 @@ __device__ __forceinline__ uint32_t q4_scales(uint32_t two) {
   return __builtin_bit_cast(uint32_t, m) | (two & 0x80008000u);
 }
 
+// Division of 0 .. 2^31 - 1 by a number that the host knows: x / d = x * m >> (32 + s) with m = ceil(2^(32 + s) / d) and 2^s
+// < d <= 2^(s + 1): m d is less than d past 2^(32 + s), so that x (m d - 2^(32 + s)) < 2^(32 + s): the quotient is exact.
+// (d = 1 has m = 0 and adds x.)
+struct ByConst {
+  uint32_t m, one;
+  int s;
+  ByConst() = default;
+  explicit ByConst(uint32_t d) : m(0), one(d == 1 ? ~0u : 0u), s(0) {
+    while ((uint64_t(2) << s) < d) ++s;
+    if (d > 1) m = (uint32_t)(((uint64_t(1) << (32 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int div(uint32_t x) const { return (int)((__umulhi(x, m) + (x & one)) >> s); }
+  __device__ __forceinline__ uint32_t rest(uint32_t x, uint32_t d) const { return x - (uint32_t)div(x) * d; }
+};
+
 // ------------------------------------------------------------------ several sequences
 // Sequence s has the tokens q_begin(s) .. q_begin(s + 1) - 1 of a call and length(s) positions, its tokens' the last. What
 // is read from device memory is held against the call's sizes: whatever it says, no access leaves them.

@@ -15,6 +15,7 @@
 // partial results, which seqs_merge_kernel joins; a row block that lies in one piece is written as it is.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bkv_device.h"
 #include "bkv_internal.h"
@@ -27,20 +28,29 @@ constexpr float kLift = 6.0f;          // a score this far (in powers of two) ab
 constexpr float kPScale = 9.0f;        // log2 of the factor on p: 2^(kLift + kPScale) is within fp16
 constexpr int kSeqKeys = 32;           // keys of a step
 constexpr int kSeqBlock = 16;          // rows of a row block
+constexpr int kSeqLeast = 8;           // steps of a piece at least
 
 __device__ __forceinline__ int cdiv_d(int a, int b) { return (a + b - 1) / b; }
 
 // 4 h2 (8 elements in order) of a word of codes: 0x4C00 | q << 6 is the fp16 number 16 + q, and (16 + q + 8 - 24) * d, in one
 // fused step, is exact: both 24 d and the result have 11 bits at most.
-template <int S>
-__device__ __forceinline__ h2 q4_pair(uint32_t w, h2 d, h2 c) {
-  const uint32_t x = S == 0 ? w << 6 : S == 1 ? w << 2 : S == 2 ? w >> 2 : w >> 6;
-  return __builtin_elementwise_fma(as_h2((x & 0x03C003C0u) | 0x4C004C00u), d, c);
-}
+// (the constants in registers, one scalar and one vector, so that taking the bits and the or is one instruction)
+struct Q4Bits {
+  uint32_t mask = 0x03C003C0u, ones = 0x4C004C00u;
+  __device__ __forceinline__ Q4Bits() {
+    asm volatile("" : "+s"(mask));
+    asm volatile("" : "+v"(ones));
+  }
+  template <int S>
+  __device__ __forceinline__ h2 pair(uint32_t w, h2 d, h2 c) const {
+    const uint32_t x = S == 0 ? w << 6 : S == 1 ? w << 2 : S == 2 ? w >> 2 : w >> 6;
+    return __builtin_elementwise_fma(as_h2((x & mask) | ones), d, c);
+  }
+  __device__ __forceinline__ h8 eight(uint32_t w, h2 d, h2 c) const {
+    return __builtin_bit_cast(h8, make_uint4(as_u(pair<0>(w, d, c)), as_u(pair<1>(w, d, c)), as_u(pair<2>(w, d, c)), as_u(pair<3>(w, d, c))));
+  }
+};
 __device__ __forceinline__ h2 q4_offset(h2 d) { return d * h2{(_Float16)-24.0f, (_Float16)-24.0f}; }
-__device__ __forceinline__ h8 q4_eight(uint32_t w, h2 d, h2 c) {
-  return __builtin_bit_cast(h8, make_uint4(as_u(q4_pair<0>(w, d, c)), as_u(q4_pair<1>(w, d, c)), as_u(q4_pair<2>(w, d, c)), as_u(q4_pair<3>(w, d, c))));
-}
 
 // 8 probabilities as ph + pl: ph cut to fp16 (two in one instruction), pl the rest, rounded
 __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
@@ -54,162 +64,316 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
   for (int j = 0; j < 8; ++j) pl[j] = (_Float16)__builtin_fmaf((float)ph[j], -1.0f, p[j]);
 }
 
-// ------------------------------------------------------------------ the line of steps
-// A sequence's row blocks, and the steps of each (one at least, so that rows that see nothing are written too)
-__device__ __forceinline__ int blocks_of(const SeqsAttnArgs &a, int s) { return cdiv_d(a.v.tokens(s) * a.grp, kSeqBlock); }
-__device__ __forceinline__ int steps_of(const SeqsAttnArgs &a, int s) { return max(1, (a.v.length(s) + kSeqKeys - 1) / kSeqKeys); }
-
-// the line's length for one KV head (by every wave alike)
-__device__ __forceinline__ int64_t line_length(const SeqsAttnArgs &a) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int s0 = 0; s0 < a.v.n_seq; s0 += 64) {
-    const int s = s0 + lane;
-    int64_t v = s < a.v.n_seq ? (int64_t)blocks_of(a, s) * steps_of(a, s) : 0;
+// the kernel's arguments (its first and only one), read anew
+template <typename T>
+__device__ __forceinline__ T arguments_again() {
+  uint32_t raw[sizeof(T) / 4];
+#ifdef __HIP_DEVICE_COMPILE__
+  const __attribute__((address_space(4))) uint32_t *p = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    total += v;
-  }
-  return total;
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) raw[i] = p[i];
+#endif
+  return __builtin_bit_cast(T, raw);
 }
+
+// ------------------------------------------------------------------ the line of steps
+// inclusive sums over the wave
+__device__ __forceinline__ int wave_sums(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+__device__ __forceinline__ int of_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+
+// Lane l's of 64 sequences: where its rows begin, how many tokens and positions it has, its row blocks and the steps of
+// each (one at least, so that rows that see nothing are written too)
+struct SeqLanes {
+  int q0, nt, len, steps, blocks;
+  bool bad;                                        // some sequence's rows begin behind the next one's
+  __device__ __forceinline__ SeqLanes(const SeqsAttnArgs &a, int s0) {
+    const int s = s0 + (int)(threadIdx.x & 63), in = min(s, a.v.n_seq - 1);
+    int e = in + 1;
+    q0 = in;
+    if (a.v.q_start) {
+      q0 = a.v.q_start[in];
+      e = a.v.q_start[in + 1];
+    }
+    bad = __any(e < q0);
+    len = a.v.length(in);
+    q0 = min(max(q0, 0), a.v.n_tok);
+    nt = s < a.v.n_seq ? max(min(max(e, 0), a.v.n_tok) - q0, 0) : 0;
+    steps = max(1, (int)((uint32_t)(len + kSeqKeys - 1) / kSeqKeys));
+    blocks = (int)((uint32_t)(nt * a.grp + kSeqBlock - 1) / kSeqBlock);
+  }
+  // (of the sequences of few rows)
+  __device__ __forceinline__ int line(const SeqsAttnArgs &a) const { return nt * a.grp <= a.few ? blocks * steps : 0; }
+};
+
 // how the line is cut: nl pieces of share steps, the first spare of one more
 struct Cut {
-  int64_t share, spare;
-  int nl;
-  __device__ __forceinline__ Cut(int64_t total, int lanes, int least) {
-    nl = (int)min((int64_t)lanes, max((int64_t)1, total / least));
-    share = total / nl;
+  int share, spare, nl;
+  __device__ __forceinline__ Cut(int total, int lanes, const ByConst &by_lanes, int least) {
+    const int most = max(1, (int)((uint32_t)(total + least - 1) / (uint32_t)least));
+    nl = min(lanes, most);
+    share = nl == lanes ? by_lanes.div(total) : (int)((uint32_t)total / (uint32_t)nl);
     spare = total - share * nl;
   }
-  __device__ __forceinline__ int64_t begin(int i) const { return i * share + min((int64_t)i, spare); }
-  __device__ __forceinline__ int piece_of(int64_t x) const {
-    const int64_t longer = spare * (share + 1);
-    return (int)(x < longer ? x / (share + 1) : spare + (x - longer) / share);
+  __device__ __forceinline__ int begin(int i) const { return i * share + min(i, spare); }
+  __device__ __forceinline__ int piece_of(int x) const {
+    const int longer = spare * (share + 1);
+    return x < longer ? (int)((uint32_t)x / (uint32_t)(share + 1)) : spare + (int)((uint32_t)(x - longer) / (uint32_t)share);
   }
 };
 
 // ------------------------------------------------------------------ few rows a block
-// A workgroup of 4 waves takes its piece of the line for one KV head; of each row block in it the waves take a quarter of
+// A workgroup of 8 waves takes its piece of the line for one KV head; of each row block in it the waves take an eighth of
 // the steps each and meet in LDS. Scores are computed transposed, S^T = K Q^T: lane (n, g) = (lane % 16, lane / 16) holds
 // keys 4 g .. 4 g + 3 of a 16-key tile for row n, which is P^T's operand of O^T = V^T P^T as it stands if slot (g, j) of the
 // 32-key contraction stands for key 4 g + j (j < 4) or 16 + 4 g + j - 4, for both operands. Product c of the scores takes
 // word 8 g + c of a key, dims 64 g + 8 c .., so that a lane's 8 words are 32 bytes; product dt of the outputs dim 16 m + dt,
 // so that a lane's dims of a key are 8 bytes.
+//
+// A row block cut into several pieces: each leaves its partial results in memory, past the caches of its XCD, and counts
+// itself; the last of every 8 pieces joins theirs, and the last of those joins these.
 // PG: 0 a contiguous cache; 1 pages of whole steps (a multiple of 32 tokens); 2 any pages
+constexpr int kSeqWaves = 8;
+constexpr int kSeqFill = 256;          // pieces of all KV heads: a workgroup a CU
+constexpr int kJoin = 8;               // partial results that are joined at a time
+constexpr int kJoinLevels = 3;         // counters: of each level, a piece's two row blocks
+static_assert(kJoin * kJoin * kJoin >= kSeqFill, "levels of joins");
+
+__device__ __forceinline__ void st_part(float *p, float4 v) {
+  st_agent(reinterpret_cast<unsigned long long *>(p), __builtin_bit_cast(unsigned long long, make_float2(v.x, v.y)));
+  st_agent(reinterpret_cast<unsigned long long *>(p) + 1, __builtin_bit_cast(unsigned long long, make_float2(v.z, v.w)));
+}
+__device__ __forceinline__ float4 ld_part(const float *p) {
+  const float2 a = __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(p)));
+  const float2 b = __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(p) + 1));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+__device__ __forceinline__ void write_out(const SeqsAttnArgs &a, int t, int h, int col, float4 v, float l) {
+  const float by = l > 0.0f || l != l ? l : 1.0f;
+  const int64_t at = ((int64_t)t * a.nh + h) * kHd + col;
+  v = make_float4(v.x / by, v.y / by, v.z / by, v.w / by);
+  *reinterpret_cast<float4 *>(a.out + at) = v;
+  if (a.gate.p) {
+    const float4 g = *reinterpret_cast<const float4 *>(a.gate.at(t, h) + col);
+    *reinterpret_cast<float4 *>(a.out_gated + at) =
+        make_float4(v.x / (1.0f + expf(-g.x)), v.y / (1.0f + expf(-g.y)), v.z / (1.0f + expf(-g.z)), v.w / (1.0f + expf(-g.w)));
+  }
+}
+
 template <int PG>
-__global__ __launch_bounds__(256, 2) void seqs_attn_kernel(SeqsAttnArgs a) {
+__global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnArgs a) {
+  constexpr int NT = 64 * kSeqWaves;
+  // a wave's two steps: K and V rows of 128 bytes, then their scales, 16 bytes a key; later its rows of the join
+  constexpr uint32_t oV = kSeqKeys * kQ4RowBytes, oKS = 2 * oV, oVS = oKS + 512, kStep = oVS + 512, kWave = 2 * kStep;
   constexpr int kOS = kHd + 4;                     // a row of the join
-  __shared__ __attribute__((aligned(16))) float s_o[4 * kSeqBlock * kOS];
-  __shared__ float s_m[4][kSeqBlock], s_l[4][kSeqBlock];
+  static_assert(kSeqBlock * kOS * 4 <= kWave && 2 * 1024 <= kStep, "the join's rows and two rows of Q in the steps' place");
+  __shared__ __attribute__((aligned(128))) uint8_t sm[kSeqWaves * kWave];
+  __shared__ int32_t s_tab[PG ? 2 * kSeqWaves : 1][64];   // table entries of a wave's steps
+  __shared__ float s_m[kSeqWaves][kSeqBlock], s_l[kSeqWaves][kSeqBlock];
+  __shared__ int s_last;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const Q4Bits bits;
   // pieces 8 apart on the same XCD; a piece's KV heads next to one another there, whose scales share lines
-  const int at8 = (int)(blockIdx.x >> 3), hk = at8 % a.nkv, piece = at8 / a.nkv * 8 + (int)(blockIdx.x & 7);
-  const int64_t total = line_length(a);
-  const Cut cut(total, a.lanes, a.least);
+  const int at8 = (int)(blockIdx.x >> 3), round = a.by_nkv.div(at8), hk = at8 - round * a.nkv, piece = 8 * round + (int)(blockIdx.x & 7);
+  // the line, by every wave alike: 64 sequences at a time
+  SeqLanes my(a, 0);
+  int inc = wave_sums(my.line(a)), total = of_lane(inc, 63);
+  bool bad = my.bad;
+  for (int s0 = 64; s0 < a.v.n_seq; s0 += 64) {
+    const SeqLanes more(a, s0);
+    total += of_lane(wave_sums(more.line(a)), 63);
+    bad |= more.bad;
+  }
+  if (bad) return;                                 // (starts that go back: their sums would have no bound)
+  const Cut cut(total, a.lanes, a.by_lanes, kSeqLeast);
   if (piece >= cut.nl) return;
-  int64_t at = cut.begin(piece);
-  const int64_t end = cut.begin(piece + 1);
-  // the sequence that position `at` of the line lies in, and what lies before that
-  int seq = 0, tile0 = 0;
-  int64_t line0 = 0;
-  for (int s0 = 0; s0 < a.v.n_seq; s0 += 64) {
-    const int s = s0 + lane;
-    const int nb = s < a.v.n_seq ? blocks_of(a, s) : 0;
-    const int64_t v = s < a.v.n_seq ? (int64_t)nb * steps_of(a, s) : 0;
-    const int64_t inc = wave_incl_scan(v, lane);
-    const int binc = wave_incl_scan(nb, lane);
+  int at = cut.begin(piece);
+  const int end = cut.begin(piece + 1);
+  // the sequence that step `at` of the line lies in, and where that begins
+  int s0 = 0, in64 = 0, line0 = 0;
+  for (;;) {
     const uint64_t past = __ballot(line0 + inc > at);
     if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      seq = s0 + l;
-      line0 += __shfl(inc - v, l);
-      tile0 += __shfl(binc - nb, l);
+      in64 = __ffsll((unsigned long long)past) - 1;
+      line0 += of_lane(inc - my.line(a), in64);
       break;
     }
-    line0 += __shfl(inc, 63);
-    tile0 += __shfl(binc, 63);
+    line0 += of_lane(inc, 63);
+    s0 += 64;
+    if (s0 >= a.v.n_seq) return;
+    my = SeqLanes(a, s0);
+    inc = wave_sums(my.line(a));
   }
-  seq = __builtin_amdgcn_readfirstlane(seq);
 
   const uint32_t krow = (uint32_t)a.nkv * kQ4RowBytes, srow = (uint32_t)a.nkv * kScaleRowBytes;
   const uint8_t *kd = a.L.kd + (size_t)hk * kQ4RowBytes, *vd = a.L.vd + (size_t)hk * kQ4RowBytes;
   const uint8_t *ksc = a.L.ks + (size_t)hk * kScaleRowBytes, *vsc = a.L.vs + (size_t)hk * kScaleRowBytes;
+  uint8_t *const mine = sm + kWave * w;
+  const uint32_t mine0 = lds_addr(sm) + kWave * w;
+  // A lane's 16 bytes of the 8 keys that a load brings: key lane / 8, piece lane % 8 of V's row, that ^ key % 8 of K's (so
+  // that 8 keys' pieces of one number lie in different banks)
+  const uint32_t key8 = (uint32_t)lane >> 3, vcol = 16u * (lane & 7), kcol = 16u * ((lane & 7) ^ key8);
+  const uint8_t *const scales = lane < 32 ? ksc : vsc;      // the scales' load: K's keys by the lower lanes, V's by the others
 
-  while (at < end && seq < a.v.n_seq) {
+  while (at < end) {
     // ---- the piece's part of one row block
-    const int q0 = a.v.q_begin(seq), nt = a.v.tokens(seq), len = a.v.length(seq), steps = steps_of(a, seq);
-    if (nt == 0) { ++seq; continue; }              // (there is a sequence with rows: at < end)
-    const int R = nt * a.grp, rb = (int)((at - line0) / steps), st0 = (int)(at - line0 - (int64_t)rb * steps);
-    const int st1 = (int)min((int64_t)steps, st0 + (end - at)), m4 = st1 - st0;
-    const int t0 = st0 + m4 * w / 4, t1 = st0 + m4 * (w + 1) / 4;
+    const int q0 = of_lane(my.q0, in64), nt = of_lane(my.nt, in64), len = of_lane(my.len, in64), steps = of_lane(my.steps, in64);
+    const int blocks = nt * a.grp <= a.few ? of_lane(my.blocks, in64) : 0, seq = s0 + in64;
+    if (at - line0 >= blocks * steps) {            // the next sequence
+      line0 += blocks * steps;
+      if (++in64 == 64) {
+        in64 = 0;
+        s0 += 64;
+        if (s0 >= a.v.n_seq) break;
+        my = SeqLanes(a, s0);
+      } else if (s0 + in64 >= a.v.n_seq) {
+        break;
+      }
+      continue;
+    }
+    const int R = nt * a.grp, rb = blocks == 1 ? 0 : (at - line0) / steps, st0 = at - line0 - rb * steps;
+    const int st1 = min(steps, st0 + (end - at)), m4 = st1 - st0;
+    const int t0 = st0 + (int)((uint32_t)(m4 * w) / kSeqWaves), t1 = st0 + (int)((uint32_t)(m4 * (w + 1)) / kSeqWaves);
     const int last = max(len - 1, 0);              // (the last key that there are bytes of)
-    const int r0 = kSeqBlock * rb, row = min(r0 + n, R - 1), tok = row / a.grp;
+    // Blocks of 8 rows or fewer: columns n and n + 8 of the products are the same row, and one product of the outputs takes ph in
+    // the one and pl in the other, whose sum the join forms
+    const int r0 = kSeqBlock * rb, real = min(R - r0, kSeqBlock);
+    const bool halves = real <= kSeqBlock / 2;
+    const int col = halves ? n & 7 : n, row = min(r0 + col, R - 1), tok = a.by_grp.div(row);
     const int lim = len - nt + tok + 1;            // keys below it are seen
-    const int lim_all = len - nt + r0 / a.grp + 1; // by all rows of the block
+    const int lim_all = len - nt + a.by_grp.div(r0) + 1;   // by all rows of the block
 
+    // ---- a step's bytes on their way: 9 loads straight into LDS, and before them, in pages, the next step's table entries (a
+    // load into a register would be waited for with everything that is on its way)
+    constexpr int NL = PG ? 10 : 9;
     uint32_t there = ~0u, there_next = ~0u;        // keys whose pages are in the pool: this step's, the next's
-    int sl = 0;                                    // PG 2: the slot of key lane % 32
-    size_t s0 = 0;
-    auto look_up = [&](int t) {
-      const uint32_t kb = (uint32_t)t * kSeqKeys;
-      s0 = kb;
-      if constexpr (PG == 1) {
-        const int first = __builtin_amdgcn_readfirstlane(a.v.slot(seq, min(kb, (uint32_t)last)));
-        there_next = first >= 0 ? ~0u : 0u;
-        s0 = (size_t)max(first, 0);
+    const int32_t *const table = PG ? a.v.tables + (int64_t)seq * a.v.table_stride : nullptr;
+    auto ask_entries = [&](int t) {
+      const uint32_t key = PG == 2 ? min((uint32_t)t * kSeqKeys + ((uint32_t)lane & 31), (uint32_t)last) : (uint32_t)t * kSeqKeys;
+      load4_to_lds(reinterpret_cast<const uint8_t *>(table + a.by_page.div(key)), __builtin_amdgcn_readfirstlane(lds_addr(s_tab[2 * w + (t & 1)])));
+    };
+    auto request = [&](int t) {                    // (of its entries, asked for before)
+      const uint32_t kb = (uint32_t)t * kSeqKeys, dst = mine0 + kStep * (t & 1), left = (uint32_t)last - kb;
+      uint32_t entry = 0;
+      if constexpr (PG != 0) {
+        if (t != t0) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");   // (what was asked for since its entries: a step)
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        entry = (uint32_t)s_tab[2 * w + (t & 1)][lane];
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(entry)::"memory");
+        ask_entries(min(t + 1, t1 - 1));           // (always one, for the counts of what is on its way)
       }
       if constexpr (PG == 2) {
-        sl = a.v.slot(seq, min(kb + ((uint32_t)lane & 31), (uint32_t)last));
+        const uint32_t key = min(kb + ((uint32_t)lane & 31), (uint32_t)last);
+        const int sl = entry < (uint32_t)a.v.pool_pages ? (int)(entry * (uint32_t)a.v.page + a.by_page.rest(key, a.v.page)) : -1;
         there_next = (uint32_t)__ballot(sl >= 0);
-      }
-    };
-    // a lane's bytes of a key, `stride` from a key to the next
-    auto from = [&](const uint8_t *base, int t, int key, uint32_t stride) -> const uint8_t * {
-      if constexpr (PG == 2) return base + (size_t)max(__shfl(sl, key), 0) * stride;
-      else return base + s0 * stride + min((uint32_t)key, (uint32_t)last - (uint32_t)t * kSeqKeys) * stride;
-    };
-    uint4 kr[2][2];
-    uint32_t ks[2];
-    uint2 vr[8];
-    uint32_t vs[8];
-    auto key_of = [&](int j) { return (j & 4) * 4 + 4 * g + (j & 3); };
-    auto load_k = [&](int t) {
+        size_t slot[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(from(kd, t, 16 * u + n, krow) + 32 * g);
-        kr[u][0] = p[0];
-        kr[u][1] = p[1];
-        ks[u] = *reinterpret_cast<const uint32_t *>(from(ksc, t, 16 * u + n, srow) + 4 * g);
-      }
-    };
-    auto load_v = [&](int t) {
+        for (int u = 0; u < 4; ++u) slot[u] = (size_t)max(__shfl(sl, 8 * u + (int)key8), 0);
+        load_to_lds_at<0>(kd + slot[0] * krow + kcol, dst);
+        load_to_lds_at<1024>(kd + slot[1] * krow + kcol, dst);
+        load_to_lds_at<2048>(kd + slot[2] * krow + kcol, dst);
+        load_to_lds_at<3072>(kd + slot[3] * krow + kcol, dst);
+        load_to_lds_at<oKS>(scales + (size_t)max(sl, 0) * srow, dst);
+        load_to_lds_at<oV>(vd + slot[0] * krow + vcol, dst);
+        load_to_lds_at<oV + 1024>(vd + slot[1] * krow + vcol, dst);
+        load_to_lds_at<oV + 2048>(vd + slot[2] * krow + vcol, dst);
+        load_to_lds_at<oV + 3072>(vd + slot[3] * krow + vcol, dst);
+      } else {
+        uint32_t base = kb;
+        if constexpr (PG == 1) {
+          const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane((int)entry);
+          there_next = b < (uint32_t)a.v.pool_pages ? ~0u : 0u;
+          base = there_next ? b * (uint32_t)a.v.page + a.by_page.rest(kb, a.v.page) : 0;
+        }
+        const uint8_t *const kp = kd + (uint64_t)base * krow, *const vp = vd + (uint64_t)base * krow;
+        uint32_t at[4] = {key8, key8 + 8, key8 + 16, key8 + 24}, sk = lane & 31;
+        if (left < kSeqKeys - 1) {                 // (the last step: keys past the end take the last one's bytes)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        vr[j] = *reinterpret_cast<const uint2 *>(from(vd, t, key_of(j), krow) + 8 * n);
-        vs[j] = *reinterpret_cast<const uint16_t *>(from(vsc, t, key_of(j), srow) + 2 * (n >> 1));
+          for (int u = 0; u < 4; ++u) at[u] = min(at[u], left);
+          sk = min(sk, left);
+        }
+        load_to_lds_at<0>(kp, at[0] * krow + kcol, dst);
+        load_to_lds_at<1024>(kp, at[1] * krow + kcol, dst);
+        load_to_lds_at<2048>(kp, at[2] * krow + kcol, dst);
+        load_to_lds_at<3072>(kp, at[3] * krow + kcol, dst);
+        load_to_lds_at<oKS>(scales + (uint64_t)(base + sk) * srow, dst);
+        load_to_lds_at<oV>(vp, at[0] * krow + vcol, dst);
+        load_to_lds_at<oV + 1024>(vp, at[1] * krow + vcol, dst);
+        load_to_lds_at<oV + 2048>(vp, at[2] * krow + vcol, dst);
+        load_to_lds_at<oV + 3072>(vp, at[3] * krow + vcol, dst);
       }
     };
-    if (t0 < t1) {
-      look_up(t0);
-      load_k(t0);
-      load_v(t0);
+    // ---- the block's rows of Q, two by each wave, whole rows at a time (a lane's pieces of a row would ask for each line
+    // four times, in every wave), into the place of the second step; piece c of row r at c ^ r % 8
+    const uint32_t q_at = kStep * ((t0 & 1) ^ 1);
+    if (PG && t0 < t1) ask_entries(t0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = min(r0 + 2 * w + j, R - 1), ti = a.by_grp.div(r);
+      load_to_lds(reinterpret_cast<const uint8_t *>(a.q.at(q0 + ti, hk * a.grp + r - ti * a.grp)) + 16 * (lane ^ ((2 * w + j) & 7)),
+                  __builtin_amdgcn_readfirstlane(mine0 + q_at + 1024 * j));
     }
+    if (t0 < t1) {
+      request(t0);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(9) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    lds_barrier();
     h8 qh[8];                                      // row n, dims 64 g + 8 c ..
     {
-      const float4 *q = reinterpret_cast<const float4 *>(a.q.at(q0 + tok, hk * a.grp + row - tok * a.grp)) + 16 * g;
+      // (row col lies with wave col / 2, whose second step's place is its own)
+      const int wt0 = st0 + (int)((uint32_t)(m4 * (col >> 1)) / kSeqWaves);
+      const uint8_t *q = sm + kWave * (col >> 1) + kStep * ((wt0 & 1) ^ 1) + 1024 * (col & 1);
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const float4 x = q[2 * c], y = q[2 * c + 1];
+        const float4 x = *reinterpret_cast<const float4 *>(q + 16 * ((16 * g + 2 * c) ^ (col & 7))), y = *reinterpret_cast<const float4 *>(q + 16 * ((16 * g + 2 * c + 1) ^ (col & 7)));
         qh[c] = h8{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w, (_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
       }
     }
+    lds_barrier();
     f4 o[16] = {};
     float m = -INFINITY, l = 0.0f;                 // m: the reference less kPScale
 
+    auto sweep = [&](auto in_halves) {
+    constexpr bool HALVES = decltype(in_halves)::value;
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
       const int kb = t * kSeqKeys;
+      const uint8_t *const at_k = mine + kStep * (t & 1), *const at_v = at_k + oV;
       there = there_next;
+      if (t + 1 < t1) {
+        request(t + 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      // all of the step's bytes to registers at once: its LDS latency once
+      auto key_of = [&](int j) { return (j & 4) * 4 + 4 * g + (j & 3); };
+      uint4 kr[2][2];
+      uint32_t ks[2];
+      uint2 vr[8];
+      uint32_t vs[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        ks[u] = *reinterpret_cast<const uint32_t *>(at_k + oKS + 16 * (16 * u + n) + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) kr[u][i] = *reinterpret_cast<const uint4 *>(at_k + kQ4RowBytes * (16 * u + n) + 16 * ((2 * g + i) ^ (n & 7)));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vr[j] = *reinterpret_cast<const uint2 *>(at_v + kQ4RowBytes * key_of(j) + 8 * n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vs[j] = *reinterpret_cast<const uint16_t *>(at_k + oVS + 16 * key_of(j) + 2 * (n >> 1));
+      __builtin_amdgcn_sched_barrier(0);
       // which keys the rows see: lane (n, g)'s bit i is key 4 g + i, bit 16 + i key 16 + 4 g + i
       const bool whole = kb + kSeqKeys <= lim_all && (!PG || there == ~0u);
       uint32_t win = there;
@@ -226,11 +390,7 @@ __global__ __launch_bounds__(256, 2) void seqs_attn_kernel(SeqsAttnArgs a) {
         const h2 d[2] = {h2{two[0], two[0]}, h2{two[1], two[1]}};
         const h2 c[2] = {q4_offset(d[0]), q4_offset(d[1])};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[u] = mfma16(q4_eight((&kr[u][i >> 2].x)[i & 3], d[i >> 2], c[i >> 2]), qh[i], s[u]);
-      }
-      if (t + 1 < t1) {
-        look_up(t + 1);
-        load_k(t + 1);
+        for (int i = 0; i < 8; ++i) s[u] = mfma16(bits.eight((&kr[u][i >> 2].x)[i & 3], d[i >> 2], c[i >> 2]), qh[i], s[u]);
       }
       // ---- probabilities
       if (!whole) {
@@ -243,7 +403,7 @@ __global__ __launch_bounds__(256, 2) void seqs_attn_kernel(SeqsAttnArgs a) {
       if (__any(top > m + (kLift + kPScale))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m, top - kPScale);
+        const float mn = top > m + (kLift + kPScale) ? top - kPScale : m;   // (by the row alone: others leave it as it is)
         const float f = mn == m ? 1.0f : exp2f(m - mn);
         m = mn;
         l *= f;
@@ -261,6 +421,8 @@ __global__ __launch_bounds__(256, 2) void seqs_attn_kernel(SeqsAttnArgs a) {
       l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       h8 ph, pl;
       split_p(p, ph, pl);
+      if (HALVES) ph = n < 8 ? ph : pl;
+      __builtin_amdgcn_s_setprio(0);               // (the other wave's scores go first: the two take turns)
       // ---- P V
       h2 d[4], c[4];
 #pragma unroll
@@ -269,95 +431,557 @@ __global__ __launch_bounds__(256, 2) void seqs_attn_kernel(SeqsAttnArgs a) {
         c[j] = q4_offset(d[j]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {                // the 16-bit halves of the lane's two words: dims 8 (e / 2) + e % 2 + 0, 2, 4, 6
+      for (int e = 0; e < 4; ++e) {                // a 16-bit half of the lane's two words: dims 8 (e / 2) + e % 2 + 0, 2, 4, 6
         uint32_t x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           x[j] = __builtin_amdgcn_perm(e & 2 ? vr[2 * j + 1].y : vr[2 * j + 1].x, e & 2 ? vr[2 * j].y : vr[2 * j].x, e & 1 ? 0x07060302u : 0x05040100u);
-        auto product = [&](const h2 (&v)[4], int i) {
+        // (two products' small parts, then their large ones: a product does not wait for the one before it)
+        auto products = [&](const h2 (&v)[4], const h2 (&z)[4], int i) {
           const int dt = 8 * (e >> 1) + 2 * i + (e & 1);
           const h8 vh = __builtin_bit_cast(h8, make_uint4(as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3])));
-          o[dt] = mfma16(vh, pl, o[dt]);
+          const h8 zh = __builtin_bit_cast(h8, make_uint4(as_u(z[0]), as_u(z[1]), as_u(z[2]), as_u(z[3])));
+          if constexpr (!HALVES) {
+            o[dt] = mfma16(vh, pl, o[dt]);
+            o[dt + 2] = mfma16(zh, pl, o[dt + 2]);
+          }
           o[dt] = mfma16(vh, ph, o[dt]);
+          o[dt + 2] = mfma16(zh, ph, o[dt + 2]);
         };
-        const h2 v0[4] = {q4_pair<0>(x[0], d[0], c[0]), q4_pair<0>(x[1], d[1], c[1]), q4_pair<0>(x[2], d[2], c[2]), q4_pair<0>(x[3], d[3], c[3])};
-        const h2 v1[4] = {q4_pair<1>(x[0], d[0], c[0]), q4_pair<1>(x[1], d[1], c[1]), q4_pair<1>(x[2], d[2], c[2]), q4_pair<1>(x[3], d[3], c[3])};
-        const h2 v2[4] = {q4_pair<2>(x[0], d[0], c[0]), q4_pair<2>(x[1], d[1], c[1]), q4_pair<2>(x[2], d[2], c[2]), q4_pair<2>(x[3], d[3], c[3])};
-        const h2 v3[4] = {q4_pair<3>(x[0], d[0], c[0]), q4_pair<3>(x[1], d[1], c[1]), q4_pair<3>(x[2], d[2], c[2]), q4_pair<3>(x[3], d[3], c[3])};
-        product(v0, 0);
-        product(v1, 1);
-        product(v2, 2);
-        product(v3, 3);
+        const h2 v0[4] = {bits.pair<0>(x[0], d[0], c[0]), bits.pair<0>(x[1], d[1], c[1]), bits.pair<0>(x[2], d[2], c[2]), bits.pair<0>(x[3], d[3], c[3])};
+        const h2 v1[4] = {bits.pair<1>(x[0], d[0], c[0]), bits.pair<1>(x[1], d[1], c[1]), bits.pair<1>(x[2], d[2], c[2]), bits.pair<1>(x[3], d[3], c[3])};
+        products(v0, v1, 0);
+        const h2 v2[4] = {bits.pair<2>(x[0], d[0], c[0]), bits.pair<2>(x[1], d[1], c[1]), bits.pair<2>(x[2], d[2], c[2]), bits.pair<2>(x[3], d[3], c[3])};
+        const h2 v3[4] = {bits.pair<3>(x[0], d[0], c[0]), bits.pair<3>(x[1], d[1], c[1]), bits.pair<3>(x[2], d[2], c[2]), bits.pair<3>(x[3], d[3], c[3])};
+        products(v2, v3, 2);
       }
-      if (t + 1 < t1) load_v(t + 1);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the step's place is the next request's)
+      __builtin_amdgcn_s_setprio(1);
     }
+    };
+    if (halves) sweep(std::true_type{});
+    else sweep(std::false_type{});
 
-    // ---- the 4 waves' parts joined
+    // (what only the end needs is read here, and holds no register before)
+    const SeqsAttnArgs z = arguments_again<SeqsAttnArgs>();
+    // ---- the waves' parts joined
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (g == 0) { s_m[w][n] = m; s_l[w][n] = l; }
     __syncthreads();
-    const float mm = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
-    const float f = m == -INFINITY ? 0.0f : exp2f(m - mm);
+    float *const s_o = reinterpret_cast<float *>(sm);
+    constexpr int kWF = kWave / 4;                 // (a wave's rows in the place of its steps)
+    if (col < real) {
+      float mm = s_m[0][n];
 #pragma unroll
-    for (int dt = 0; dt < 16; dt += 4)             // (4 products' dims are neighbours)
+      for (int j = 1; j < kSeqWaves; ++j) mm = fmaxf(mm, s_m[j][n]);
+      const float f = m == -INFINITY ? 0.0f : exp2f(m - mm);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4 *>(&s_o[(kSeqBlock * w + n) * kOS + 16 * (4 * g + i) + dt]) =
-            make_float4(o[dt][i] * f, o[dt + 1][i] * f, o[dt + 2][i] * f, o[dt + 3][i] * f);
+      for (int dt = 0; dt < 16; dt += 4)           // (4 products' dims are neighbours)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4 *>(&s_o[kWF * w + n * kOS + 16 * (4 * g + i) + dt]) =
+              make_float4(o[dt][i] * f, o[dt + 1][i] * f, o[dt + 2][i] * f, o[dt + 3][i] * f);
+    }
     __syncthreads();
-    const int jr = threadIdx.x >> 4, c = threadIdx.x & 15, r = r0 + jr;
-    if (r < R) {
-      const int ti = r / a.grp, h = hk * a.grp + r - ti * a.grp;
-      const float mr = fmaxf(fmaxf(s_m[0][jr], s_m[1][jr]), fmaxf(s_m[2][jr], s_m[3][jr]));
-      float lr = 0.0f;
+    const bool alone = m4 == steps;
+    // the row block's pieces, this one among them, and where partial results of piece i lie
+    const int tile_line = line0 + rb * steps;
+    const int first = alone ? piece : cut.piece_of(tile_line), count = alone ? 1 : cut.piece_of(tile_line + steps - 1) - first + 1;
+    // (a piece is the first of one cut row block, whose beginning it holds the last of, and a later one of one other)
+    auto part_of = [&](int i) { return (uint32_t)((2 * (first + i) + (i == 0)) * z.nkv + hk); };
+    for (int x = threadIdx.x; x < real * (kHd / 4); x += NT) {
+      const int jr = x / (kHd / 4), col = 4 * (x % (kHd / 4));
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float mr = s_m[0][jr], lr = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) lr += s_m[j][jr] == -INFINITY ? 0.0f : s_l[j][jr] * exp2f(s_m[j][jr] - mr);
-      const bool alone = m4 == steps;
-      const float inv = lr > 0.0f || lr != lr ? lr : 1.0f;
-      const uint32_t part = ((uint32_t)(piece + tile0 + rb) * a.nkv + hk) * kSeqBlock + jr;
-      const int64_t dst = (int64_t)(q0 + ti) * a.nh + h;
+      for (int j = 1; j < kSeqWaves; ++j) mr = fmaxf(mr, s_m[j][jr]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 x = *reinterpret_cast<const float4 *>(&s_o[(kSeqBlock * j + jr) * kOS + 4 * c + 64 * k]);
-          v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      for (int j = 0; j < kSeqWaves; ++j) {
+        const float4 y = *reinterpret_cast<const float4 *>(&s_o[kWF * j + jr * kOS + col]);
+        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+        if (halves) {
+          const float4 x8 = *reinterpret_cast<const float4 *>(&s_o[kWF * j + (jr + 8) * kOS + col]);
+          v.x += x8.x; v.y += x8.y; v.z += x8.z; v.w += x8.w;
         }
-        const int col = 4 * c + 64 * k;
-        if (alone) {
-          v = make_float4(v.x / inv, v.y / inv, v.z / inv, v.w / inv);
-          *reinterpret_cast<float4 *>(a.out + dst * kHd + col) = v;
-          if (a.gate.p) {
-            const float4 gt = *reinterpret_cast<const float4 *>(a.gate.at(q0 + ti, h) + col);
-            *reinterpret_cast<float4 *>(a.out_gated + dst * kHd + col) =
-                make_float4(v.x / (1.0f + expf(-gt.x)), v.y / (1.0f + expf(-gt.y)), v.z / (1.0f + expf(-gt.z)), v.w / (1.0f + expf(-gt.w)));
-          }
-        } else if (part < a.part_rows) {
-          *reinterpret_cast<float4 *>(a.part + (int64_t)part * kHd + col) = v;
-        }
+        lr += s_m[j][jr] == -INFINITY ? 0.0f : s_l[j][jr] * exp2f(s_m[j][jr] - mr);
       }
-      if (c == 0) {
-        if (!alone && part < a.part_rows) a.ml[part] = make_float2(mr, lr);
-        if (st0 == 0) {
-          const int count = cut.piece_of(line0 + (int64_t)(rb + 1) * steps - 1) - piece + 1;
-          a.info[dst] = make_uint4(part, (uint32_t)a.nkv * kSeqBlock, (uint32_t)count, 0);
+      if (alone) {
+        const int ti = z.by_grp.div(r0 + jr);
+        write_out(z, q0 + ti, hk * z.grp + r0 + jr - ti * z.grp, col, v, lr);
+      } else {
+        const uint32_t p = part_of(piece - first) * kSeqBlock + jr;
+        st_part(z.part + (int64_t)p * kHd + col, v);
+        if (col == 0) st_agent(reinterpret_cast<unsigned long long *>(z.ml + p), __builtin_bit_cast(unsigned long long, make_float2(mr, lr)));
+      }
+    }
+    // ---- the pieces joined: 8 at a time, then those
+    if (!alone) {
+      int mine = piece - first, groups = count, unit = 1;   // this one among the results of a level; pieces that one stands for
+      for (unsigned *counters = z.count;; counters += 2 * kSeqFill) {
+        const int g0 = mine / kJoin * kJoin, size = min(kJoin, groups - g0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // (the results are in memory)
+        __syncthreads();
+        unsigned *const counter = counters + part_of(g0 * unit);
+        if (threadIdx.x == 0) s_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)size - 1;
+        __syncthreads();
+        if (!s_last) break;
+        if (threadIdx.x == 0) st_agent(counter, 0u);        // (for the next call)
+        const bool done = size == groups;
+        for (int x = threadIdx.x; x < real * (kHd / 4); x += NT) {
+          const int jr = x / (kHd / 4), col = 4 * (x % (kHd / 4));
+          float4 v[kJoin], o4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          float2 ml[kJoin];
+#pragma unroll
+          for (int j = 0; j < kJoin; ++j) {
+            const uint32_t p = part_of((g0 + min(j, size - 1)) * unit) * kSeqBlock + jr;
+            ml[j] = __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(z.ml + p)));
+            v[j] = ld_part(z.part + (int64_t)p * kHd + col);
+          }
+          float mr = ml[0].x, lr = 0.0f;
+#pragma unroll
+          for (int j = 1; j < kJoin; ++j) mr = fmaxf(mr, ml[j].x);
+#pragma unroll
+          for (int j = 0; j < kJoin; ++j) {
+            const float f = j >= size || ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - mr);
+            if (j < size) {
+              lr = fmaf(ml[j].y, f, lr);
+              o4.x = fmaf(v[j].x, f, o4.x); o4.y = fmaf(v[j].y, f, o4.y); o4.z = fmaf(v[j].z, f, o4.z); o4.w = fmaf(v[j].w, f, o4.w);
+            }
+          }
+          if (done) {
+            const int ti = z.by_grp.div(r0 + jr);
+            write_out(z, q0 + ti, hk * z.grp + r0 + jr - ti * z.grp, col, o4, lr);
+          } else {                                 // in the place of its first: what a thread writes it alone has read,
+            const uint32_t p = part_of(g0 * unit) * kSeqBlock + jr;
+            st_part(z.part + (int64_t)p * kHd + col, o4);
+            s_o[2 * jr] = mr;                      // but for the reference and the sum, written behind a barrier
+            s_o[2 * jr + 1] = lr;
+          }
         }
+        if (done) break;
+        __syncthreads();
+        if (threadIdx.x < real)
+          st_agent(reinterpret_cast<unsigned long long *>(z.ml + part_of(g0 * unit) * kSeqBlock + threadIdx.x),
+                   __builtin_bit_cast(unsigned long long, make_float2(s_o[2 * threadIdx.x], s_o[2 * threadIdx.x + 1])));
+        mine /= kJoin;
+        groups = (groups + kJoin - 1) / kJoin;
+        unit *= kJoin;
       }
     }
     __syncthreads();                               // (LDS is the next part's)
     at += m4;
-    if (rb + 1 == blocks_of(a, seq) && st1 == steps) {
-      line0 += (int64_t)(rb + 1) * steps;
-      tile0 += rb + 1;
-      ++seq;
+  }
+}
+
+// ------------------------------------------------------------------ many rows: key tiles in LDS
+// 4 waves hold 32 rows each, with all 256 outputs of a row in registers, and step through the workgroup's piece 32 keys at a
+// time; two workgroups a CU fill one another's waits. A step's cache bytes are loaded straight into LDS two steps ahead and
+// turned once into the products' operands for all 128 rows, the step before they are wanted: K as it is, V transposed, so
+// that a lane's 8 keys of one dim are 16 bytes. S^T and O^T are formed as in the kernel above, P never leaves its lane.
+//
+// LDS positions, in 16-byte pieces: K piece c (8 dims) of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
+// and 16 + 4 g .. 16 + 4 g + 3) at 4 d + (g ^ vx(d)); both so that 8 neighbouring lanes' reads and writes lie in different banks.
+constexpr int kTileRows = 128, kTileWaves = 4, kTileLeast = 8;
+__device__ __forceinline__ uint32_t v_piece(int d, int g) { return (uint32_t)(64 * d + 16 * (g ^ (((d >> 1) ^ (d >> 3)) & 3))); }
+
+// tiles of a sequence, and steps of tile rb: up to its last row's last key (one at least)
+struct Tiles {
+  int nt, len, grp;
+  __device__ __forceinline__ int count() const { return (int)((uint32_t)(nt * grp + kTileRows - 1) / kTileRows); }
+  __device__ __forceinline__ int steps(const ByConst &by_grp, int rb) const {
+    const int toks = min(nt, by_grp.div((uint32_t)(kTileRows * (rb + 1) + grp - 1)));
+    return (int)((uint32_t)(max(len - nt + toks, 1) + kSeqKeys - 1) / kSeqKeys);
+  }
+};
+
+template <int PG>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnArgs a) {
+  constexpr uint32_t kOp = kSeqKeys * 2 * kHd;     // an operand: 32 keys of 256 fp16
+  // two steps' operands of K and of V; behind them the bytes as they came, each wave's own: 8 keys' rows of K, 64 dims of V,
+  // 8 keys' scales of K, 2 blocks' scales of V
+  constexpr uint32_t oVop = 2 * kOp, oRaw = 4 * kOp, kRawV = 1024, kRawKS = 2048, kRawVS = 2176, kRaw = 2304;
+  __shared__ __attribute__((aligned(128))) uint8_t sm[oRaw + kTileWaves * kRaw];
+  __shared__ int32_t s_tab[PG ? kTileWaves : 1][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const Q4Bits bits;
+  // (the lane's number, opaque where addresses are formed from it: kept from step to step they would take the registers that
+  // the outputs need)
+  auto my_lane = [&]() {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  const int at8 = (int)(blockIdx.x >> 3), round = a.by_nkv.div(at8), hk = at8 - round * a.nkv, piece = 8 * round + (int)(blockIdx.x & 7);
+  // ---- the line: all tiles' steps, 64 sequences at a time
+  auto line_of = [&](const SeqLanes &s) {
+    const Tiles t{s.nt, s.len, a.grp};
+    int sum = 0;
+    if (s.nt * a.grp > a.few)
+      for (int rb = 0; rb < t.count(); ++rb) sum += t.steps(a.by_grp, rb);
+    return sum;
+  };
+  auto tiles_of = [&](const SeqLanes &s) { return s.nt * a.grp > a.few ? Tiles{s.nt, s.len, a.grp}.count() : 0; };
+  SeqLanes my(a, 0);
+  int mine_line = line_of(my), inc = wave_sums(mine_line), total = of_lane(inc, 63);
+  bool bad = my.bad;
+  for (int s0 = 64; s0 < a.v.n_seq; s0 += 64) {
+    const SeqLanes more(a, s0);
+    total += of_lane(wave_sums(line_of(more)), 63);
+    bad |= more.bad;
+  }
+  if (bad || total == 0) return;
+  const Cut cut(total, a.tile_lanes, a.by_tile_lanes, kTileLeast);
+  if (piece >= cut.nl) return;
+  int at = cut.begin(piece);
+  const int end = cut.begin(piece + 1);
+  int s0 = 0, in64 = 0, line0 = 0, tile0 = 0;      // the sequence that `at` lies in, where that begins, tiles before it
+  for (;;) {
+    const int nb = tiles_of(my), binc = wave_sums(nb);
+    const uint64_t past = __ballot(line0 + inc > at);
+    if (past) {
+      in64 = __ffsll((unsigned long long)past) - 1;
+      line0 += of_lane(inc - mine_line, in64);
+      tile0 += of_lane(binc - nb, in64);
+      break;
+    }
+    line0 += of_lane(inc, 63);
+    tile0 += of_lane(binc, 63);
+    s0 += 64;
+    if (s0 >= a.v.n_seq) return;
+    my = SeqLanes(a, s0);
+    mine_line = line_of(my);
+    inc = wave_sums(mine_line);
+  }
+  // the tile of that sequence: 64 at a time
+  int rb = 0;
+  {
+    const Tiles t{of_lane(my.nt, in64), of_lane(my.len, in64), a.grp};
+    for (;;) {
+      const int i = rb + lane, st = i < t.count() ? t.steps(a.by_grp, i) : 0, tinc = wave_sums(st);
+      const uint64_t past = __ballot(line0 + tinc > at);
+      if (past) {
+        const int l = __ffsll((unsigned long long)past) - 1;
+        line0 += of_lane(tinc - st, l);
+        rb += l;
+        break;
+      }
+      line0 += of_lane(tinc, 63);
+      rb += 64;
+      if (rb >= t.count()) return;
+    }
+  }
+  tile0 += rb;
+
+  const uint32_t krow = (uint32_t)a.nkv * kQ4RowBytes, srow = (uint32_t)a.nkv * kScaleRowBytes;
+  const uint8_t *kd = a.L.kd + (size_t)hk * kQ4RowBytes, *vd = a.L.vd + (size_t)hk * kQ4RowBytes;
+  const uint8_t *ksc = a.L.ks + (size_t)hk * kScaleRowBytes, *vsc = a.L.vs + (size_t)hk * kScaleRowBytes;
+  uint8_t *const raw = sm + oRaw + kRaw * w;
+  const uint32_t raw0 = lds_addr(sm) + oRaw + kRaw * w;
+
+  while (at < end) {
+    // ---- the piece's part of one tile
+    const int q0 = of_lane(my.q0, in64), nt = of_lane(my.nt, in64), len = of_lane(my.len, in64), seq = s0 + in64;
+    const Tiles tiles{nt, len, a.grp};
+    if (nt * a.grp <= a.few || rb == tiles.count()) {   // the next sequence
+      rb = 0;
+      if (++in64 == 64) {
+        in64 = 0;
+        s0 += 64;
+        if (s0 >= a.v.n_seq) break;
+        my = SeqLanes(a, s0);
+      } else if (s0 + in64 >= a.v.n_seq) {
+        break;
+      }
+      continue;
+    }
+    const int R = nt * a.grp, steps = tiles.steps(a.by_grp, rb), t0 = at - line0, t1 = min(steps, t0 + (end - at));
+    const int last = max(len - 1, 0), r0 = kTileRows * rb, rw = r0 + 32 * w;
+    const bool works = rw < R;                     // (a wave whose rows are all past the last only brings bytes)
+    // keys below lim are seen: by a row of the lane's, by all of the wave's, by any
+    auto lim_of = [&](int mt) { return len - nt + a.by_grp.div((uint32_t)min(rw + 16 * mt + (my_lane() & 15), R - 1)) + 1; };
+    const int lim_all = len - nt + a.by_grp.div((uint32_t)min(rw, R - 1)) + 1, lim_any = len - nt + a.by_grp.div((uint32_t)min(rw + 31, R - 1)) + 1;
+
+    // ---- bytes on their way: the wave's own, of step t
+    uint32_t there = ~0u, there_next = ~0u;        // keys whose pages are in the pool: this step's, the next's
+    const int32_t *const table = PG ? a.v.tables + (int64_t)seq * a.v.table_stride : nullptr;
+    auto ask_entries = [&](int t) {
+      const int lane = my_lane();
+      const uint32_t key = PG == 2 ? min((uint32_t)t * kSeqKeys + ((uint32_t)lane & 31), (uint32_t)last) : min((uint32_t)t * kSeqKeys, (uint32_t)last);
+      load4_to_lds(reinterpret_cast<const uint8_t *>(table + a.by_page.div(key)), __builtin_amdgcn_readfirstlane(lds_addr(s_tab[PG ? w : 0])));
+    };
+    // V's keys lie in the order of the contraction's slots: place 4 j + g is slot (g, j), so that the 4 groups' reads of one j
+    // are neighbours
+    auto key_of = [](int p) { return (p & 16) + 4 * (p & 3) + ((p >> 2) & 3); };
+    uint32_t there_after = ~0u;
+    auto request = [&](int t) {                    // (of its entries, landed)
+      const int lane = my_lane();
+      const uint32_t kb = (uint32_t)t * kSeqKeys, left = (uint32_t)last - min(kb, (uint32_t)last);
+      const int kk = 8 * w + (lane >> 3), kv = key_of(lane >> 1), ksk = (8 * w + lane) & 31, kvs = key_of(lane & 31);
+      if constexpr (PG == 2) {
+        const uint32_t key = min(kb + ((uint32_t)lane & 31), (uint32_t)last), e = (uint32_t)s_tab[w][lane];
+        const int sl = e < (uint32_t)a.v.pool_pages ? (int)(e * (uint32_t)a.v.page + a.by_page.rest(key, a.v.page)) : -1;
+        there_after = (uint32_t)__ballot(sl >= 0);
+        const size_t sk = (size_t)max(__shfl(sl, kk), 0), sv = (size_t)max(__shfl(sl, kv), 0), s1 = (size_t)max(__shfl(sl, ksk), 0), s2 = (size_t)max(__shfl(sl, kvs), 0);
+        load_to_lds_at<0>(kd + sk * krow + 16 * ((lane ^ (lane >> 3)) & 7), raw0);
+        load_to_lds_at<kRawV>(vd + sv * krow + 32 * w + 16 * (lane & 1), raw0);
+        if (lane < 8) load_to_lds_at<kRawKS>(ksc + s1 * srow, raw0);
+        if (lane < 32) load4_to_lds(vsc + s2 * srow + 4 * w, __builtin_amdgcn_readfirstlane(raw0 + kRawVS));
+      } else {
+        uint32_t base = min(kb, (uint32_t)last);
+        if constexpr (PG == 1) {
+          const uint32_t e = (uint32_t)__builtin_amdgcn_readfirstlane(s_tab[w][lane]);
+          there_after = e < (uint32_t)a.v.pool_pages ? ~0u : 0u;
+          base = there_after ? e * (uint32_t)a.v.page + a.by_page.rest(base, a.v.page) : 0;
+        }
+        const uint64_t off = (uint64_t)base * krow, soff = (uint64_t)base * srow;
+        load_to_lds_at<0>(kd + off, min((uint32_t)kk, left) * krow + 16 * ((lane ^ (lane >> 3)) & 7), raw0);
+        load_to_lds_at<kRawV>(vd + off, min((uint32_t)kv, left) * krow + 32 * w + 16 * (lane & 1), raw0);
+        if (lane < 8) load_to_lds_at<kRawKS>(ksc + soff, min((uint32_t)ksk, left) * srow, raw0);
+        if (lane < 32) load4_to_lds(vsc + soff + min((uint32_t)kvs, left) * srow + 4 * w, __builtin_amdgcn_readfirstlane(raw0 + kRawVS));
+      }
+    };
+    // ---- the wave's bytes, landed, made into operands
+    auto convert = [&](int buf) {
+      const int lane = my_lane(), n = lane & 15, g = lane >> 4;
+      uint8_t *const kto = sm + kOp * buf, *const vto = sm + oVop + kOp * buf;
+      {                                            // K: words i, i + 8, .. of key lane / 8
+        const int k = lane >> 3, i = lane & 7, key = 8 * w + k;
+        uint32_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint32_t *>(raw + 128 * k + 16 * (((i >> 2) + 2 * j) ^ k) + 4 * (i & 3));
+        const uint4 sc = *reinterpret_cast<const uint4 *>(raw + kRawKS + 16 * k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {              // (word i + 8 j: block 2 j + i / 4)
+          const h2 two = as_h2(q4_scales((&sc.x)[j]));
+          const h2 d = i & 4 ? h2{two[1], two[1]} : h2{two[0], two[0]};
+          *reinterpret_cast<h8 *>(kto + 512 * key + 16 * ((i + 8 * j) ^ (key & 15))) = bits.eight(x[j], d, q4_offset(d));
+        }
+      }
+      {                                            // V: 4 dims of 8 keys: a half of word n / 2 of the wave's 8
+        uint32_t x[4];
+        h2 d[4], c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = *reinterpret_cast<const uint16_t *>(raw + kRawV + 32 * (8 * j + g) + 2 * n), hi = *reinterpret_cast<const uint16_t *>(raw + kRawV + 32 * (8 * j + 4 + g) + 2 * n);
+          const uint32_t sl = *reinterpret_cast<const uint16_t *>(raw + kRawVS + 4 * (8 * j + g) + 2 * (n >> 3)), sh = *reinterpret_cast<const uint16_t *>(raw + kRawVS + 4 * (8 * j + 4 + g) + 2 * (n >> 3));
+          x[j] = lo | (hi << 16);
+          d[j] = as_h2(q4_scales(sl | (sh << 16)));
+          c[j] = q4_offset(d[j]);
+        }
+        const int d0 = 64 * w + 8 * (n >> 1) + (n & 1);
+        auto put = [&](int s, const h2 (&v)[4]) {
+          *reinterpret_cast<uint4 *>(vto + v_piece(d0 + 2 * s, g)) = make_uint4(as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3]));
+        };
+        put(0, {bits.pair<0>(x[0], d[0], c[0]), bits.pair<0>(x[1], d[1], c[1]), bits.pair<0>(x[2], d[2], c[2]), bits.pair<0>(x[3], d[3], c[3])});
+        put(1, {bits.pair<1>(x[0], d[0], c[0]), bits.pair<1>(x[1], d[1], c[1]), bits.pair<1>(x[2], d[2], c[2]), bits.pair<1>(x[3], d[3], c[3])});
+        put(2, {bits.pair<2>(x[0], d[0], c[0]), bits.pair<2>(x[1], d[1], c[1]), bits.pair<2>(x[2], d[2], c[2]), bits.pair<2>(x[3], d[3], c[3])});
+        put(3, {bits.pair<3>(x[0], d[0], c[0]), bits.pair<3>(x[1], d[1], c[1]), bits.pair<3>(x[2], d[2], c[2]), bits.pair<3>(x[3], d[3], c[3])});
+      }
+    };
+
+    // ---- Q, 32 rows a wave, through LDS (the operands' place, 16 rows of fp16 a wave at a time), piece c of row r at c ^ r
+    if (PG) ask_entries(t0);
+    h8 qh[2][8];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      float4 x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int r = min(rw + 16 * mt + j, R - 1), ti = a.by_grp.div((uint32_t)r);
+        x[j] = reinterpret_cast<const float4 *>(a.q.at(q0 + ti, hk * a.grp + r - ti * a.grp))[lane];
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const h2 lo = {(_Float16)x[j].x, (_Float16)x[j].y}, hi = {(_Float16)x[j].z, (_Float16)x[j].w};
+        *reinterpret_cast<uint2 *>(sm + 8192 * w + 512 * j + 16 * ((lane >> 1) ^ j) + 8 * (lane & 1)) = make_uint2(as_u(lo), as_u(hi));
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int b = 0; b < 8; ++b) qh[mt][b] = *reinterpret_cast<const h8 *>(sm + 8192 * w + 512 * n + 16 * ((4 * b + g) ^ n));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    request(t0);
+    there_next = there_after;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (PG) ask_entries(min(t0 + 1, t1 - 1));
+    f4 o[2][16] = {};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();                                 // (every wave has its rows)
+    convert(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t0 + 1 < t1) {
+      request(t0 + 1);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (PG) ask_entries(min(t0 + 2, t1 - 1));
+    }
+    lds_barrier();
+
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {                // (the same count in the whole workgroup)
+      const int kb = t * kSeqKeys, buf = (t - t0) & 1;
+      there = there_next;
+      there_next = there_after;
+      if (works && kb < lim_any) {
+        const int lane = my_lane(), n = lane & 15, g = lane >> 4;
+        const uint8_t *const kop = sm + kOp * buf + 512 * n, *const vop = sm + oVop + kOp * buf + 64 * n;
+        const uint32_t kx = 16 * (g ^ n);          // piece 4 b + g at (4 b + g) ^ n
+        const uint32_t vx[2] = {v_piece(n, g) - 64 * n, v_piece(16 + n, g) - 64 * (16 + n)};
+        auto k_at = [&](int ub) { return *reinterpret_cast<const h8 *>(kop + (kx ^ (64u * (ub & 3))) + 8192 * (ub >> 3) + 256 * ((ub & 7) >> 2)); };
+        auto v_at = [&](int dt) { return *reinterpret_cast<const h8 *>(vop + vx[dt & 1] + 1024 * dt); };
+        const bool whole = kb + kSeqKeys <= lim_all && (!PG || there == ~0u);
+        // ---- scores
+        // (the operands of product ub + AK are asked for before product ub, and no further ahead: the registers hold no more)
+        constexpr int AK = 3;
+        f4 s[2][2] = {};
+        h8 kf[AK + 1];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < AK; ++j) kf[j] = k_at(j);
+#pragma unroll
+        for (int ub = 0; ub < 16; ++ub) {
+          if (ub + AK < 16) kf[(ub + AK) % (AK + 1)] = k_at(ub + AK);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) s[mt][ub >> 3] = mfma16(kf[ub % (AK + 1)], qh[mt][ub & 7], s[mt][ub >> 3]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // ---- probabilities
+        h8 ph[2], pl[2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t win = ~0u;
+          if (!whole) {
+            const int seen = lim_of(mt) - kb;
+            win = there & (seen <= 0 ? 0u : seen >= 32 ? ~0u : (1u << seen) - 1u);
+            win >>= 4 * g;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (!((win >> ((j & 4) * 4 + (j & 3))) & 1u)) s[mt][j >> 2][j & 3] = -INFINITY;
+          }
+          float top = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
+                            fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3]))) * a.scale2;
+          if (__any(top > m[mt] + (kLift + kPScale))) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float mn = top > m[mt] + (kLift + kPScale) ? top - kPScale : m[mt];   // (by the row alone: others leave it as it is)
+            const float f = mn == m[mt] ? 1.0f : exp2f(m[mt] - mn);
+            m[mt] = mn;
+            l[mt] *= f;
+#pragma unroll
+            for (int dt = 0; dt < 16; ++dt) o[mt][dt] *= f;
+          }
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][j >> 2][j & 3], a.scale2, -m[mt]));
+          if (!whole) {                            // (where nothing was seen yet, -Inf - -Inf)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (!((win >> ((j & 4) * 4 + (j & 3))) & 1u)) p[j] = 0.0f;
+          }
+          l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+          split_p(p, ph[mt], pl[mt]);
+        }
+        // ---- P V
+        constexpr int AV = 3;
+        h8 vf[AV + 1];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < AV; ++j) vf[j] = v_at(j);
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) {
+          if (dt + AV < 16) vf[(dt + AV) % (AV + 1)] = v_at(dt + AV);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) o[mt][dt] = mfma16(vf[dt % (AV + 1)], pl[mt], o[mt][dt]);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) o[mt][dt] = mfma16(vf[dt % (AV + 1)], ph[mt], o[mt][dt]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (t + 1 < t1) {
+        // the next step's operands, in places whose readers have passed the barrier; then, with the wave's bytes used,
+        // those of the step after it
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        convert(buf ^ 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t + 2 < t1) {
+          request(t + 2);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (PG) ask_entries(min(t + 3, t1 - 1));
+        }
+      }
+      lds_barrier();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    const SeqsAttnArgs z = arguments_again<SeqsAttnArgs>();
+    // ---- the outputs, or a partial result for each row of a tile that several pieces share
+    const bool alone = t1 - t0 == steps;
+    const uint32_t part0 = ((uint32_t)(piece + tile0) * z.nkv + hk) * kTileRows + 32 * w;
+    if (works) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        float sum = l[mt];
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const int r = rw + 16 * mt + n, ti = z.by_grp.div((uint32_t)min(r, R - 1));
+        const int64_t dst = (int64_t)(q0 + ti) * z.nh + hk * z.grp + min(r, R - 1) - ti * z.grp;
+        const uint32_t part = part0 + 16 * mt + n;
+        const float by = !alone ? 1.0f : sum > 0.0f || sum != sum ? sum : 1.0f;
+        if (r < R && g == 0) {
+          if (t0 == 0) {
+            const int count = alone ? 1 : cut.piece_of(line0 + steps - 1) - piece + 1;
+            z.info[dst] = make_uint4(part, (uint32_t)z.nkv * kTileRows, (uint32_t)count, 0);
+          }
+          if (!alone) z.tile_ml[part] = make_float2(m[mt], sum);
+        }
+        // lanes n and n ^ 1 exchange halves of two products, so that a store reaches 8 rows' whole lines
+        const bool odd = n & 1;
+        float *const mine = r < R ? (alone ? z.out + dst * kHd : z.tile_part + (int64_t)part * kHd) : nullptr;
+        const uint64_t other = __shfl_xor((unsigned long long)(uintptr_t)mine, 1);
+        float *const even_row = odd ? (float *)(uintptr_t)other : mine, *const odd_row = odd ? mine : (float *)(uintptr_t)other;
+        const float by2 = __shfl_xor(by, 1), by_even = odd ? by2 : by, by_odd = odd ? by : by2;
+        const float *const gate = z.gate.p && alone && r < R ? z.gate.at(q0 + ti, hk * z.grp + min(r, R - 1) - ti * z.grp) : nullptr;
+        const uint64_t gother = __shfl_xor((unsigned long long)(uintptr_t)gate, 1);
+        const float *const even_gate = odd ? (const float *)(uintptr_t)gother : gate, *const odd_gate = odd ? gate : (const float *)(uintptr_t)gother;
+#pragma unroll
+        for (int dt = 0; dt < 16; dt += 2) {
+          f4 e, d;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = dpp<0xB1>(odd ? o[mt][dt][i] : o[mt][dt + 1][i]);      // the other row's half
+            e[i] = (odd ? x : o[mt][dt][i]) / by_even;
+            d[i] = (odd ? o[mt][dt + 1][i] : x) / by_odd;
+          }
+          const int col = 16 * (dt + (odd ? 1 : 0)) + 4 * g;
+          auto write = [&](float *row, const float *gt, f4 v) {
+            if (!row) return;
+            *reinterpret_cast<f4 *>(row + col) = v;
+            if (gt) {
+              const f4 x = *reinterpret_cast<const f4 *>(gt + col);
+              f4 y;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[i] = v[i] / (1.0f + expf(-x[i]));
+              *reinterpret_cast<f4 *>(z.out_gated + (row - z.out) + col) = y;
+            }
+          };
+          write(even_row, even_gate, e);
+          write(odd_row, odd_gate, d);
+        }
+      }
+    }
+    at += t1 - t0;
+    if (t1 == steps) {
+      line0 += steps;
+      ++rb;
+      ++tile0;
     }
   }
 }
 
-// ------------------------------------------------------------------ the join
-// One workgroup of NWV waves per row: wave w sums the partial results w, w + NWV, .. (a lane 4 dims, 8 of them requested
+// ------------------------------------------------------------------ the join of the tiles' partial results
+// A workgroup of NWV waves per row: wave w sums the partial results w, w + NWV, .. (a lane 4 dims, 8 of them requested
 // together), then the waves' sums meet in LDS.
 template <int NWV>
 __global__ __launch_bounds__(64 * NWV) void seqs_merge_kernel(SeqsAttnArgs a) {
@@ -366,15 +990,16 @@ __global__ __launch_bounds__(64 * NWV) void seqs_merge_kernel(SeqsAttnArgs a) {
   const int t = (int)(r / a.nh), h = (int)(r - (int64_t)t * a.nh);
   __shared__ __attribute__((aligned(16))) float s_o[NWV * kHd];
   const uint4 in = a.info[r];
-  if (a.v.sequence_of<64>(t) < 0) return;          // (no sequence's row: nothing was left for it)
+  const int s = a.v.sequence_of<64>(t);
+  if (s < 0 || a.v.tokens(s) * a.grp <= a.few) return;     // (no row of a tile: nothing was left for it)
   const uint32_t first = in.x, stride = in.y, count = in.z;
-  if (count <= 1 || (uint64_t)first + (uint64_t)stride * (count - 1) >= a.part_rows) return;
+  if (count <= 1 || (uint64_t)first + (uint64_t)stride * (count - 1) >= a.tile_part_rows) return;
   float mm = -INFINITY;
-  for (uint32_t i = lane; i < count; i += 64) mm = fmaxf(mm, a.ml[first + i * stride].x);
+  for (uint32_t i = lane; i < count; i += 64) mm = fmaxf(mm, a.tile_ml[first + i * stride].x);
   mm = wave_max(mm);
   float l = 0.0f;
   for (uint32_t i = lane; i < count; i += 64) {
-    const float2 x = a.ml[first + i * stride];
+    const float2 x = a.tile_ml[first + i * stride];
     l += x.x == -INFINITY ? 0.0f : x.y * exp2f(x.x - mm);
   }
   l = wave_sum(l);
@@ -384,8 +1009,8 @@ __global__ __launch_bounds__(64 * NWV) void seqs_merge_kernel(SeqsAttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t i = min(i0 + j * NWV, count - 1);
-      x[j] = reinterpret_cast<const float4 *>(a.part + (int64_t)(first + i * stride) * kHd)[lane];
-      m8[j] = a.ml[first + i * stride].x;
+      x[j] = reinterpret_cast<const float4 *>(a.tile_part + (int64_t)(first + i * stride) * kHd)[lane];
+      m8[j] = a.tile_ml[first + i * stride].x;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -394,54 +1019,69 @@ __global__ __launch_bounds__(64 * NWV) void seqs_merge_kernel(SeqsAttnArgs a) {
       o.x = fmaf(x[j].x, f, o.x); o.y = fmaf(x[j].y, f, o.y); o.z = fmaf(x[j].z, f, o.z); o.w = fmaf(x[j].w, f, o.w);
     }
   }
-  reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = o;
-  __syncthreads();
-  if (w != 0) return;
-  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if constexpr (NWV > 1) {
+    reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = o;
+    __syncthreads();
+    if (w != 0) return;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int j = 0; j < NWV; ++j) {
-    const float4 y = reinterpret_cast<const float4 *>(s_o + j * kHd)[lane];
-    o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+    for (int j = 0; j < NWV; ++j) {
+      const float4 y = reinterpret_cast<const float4 *>(s_o + j * kHd)[lane];
+      o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+    }
   }
-  const float inv = l > 0.0f || l != l ? l : 1.0f;
-  const float4 v = make_float4(o.x / inv, o.y / inv, o.z / inv, o.w / inv);
-  reinterpret_cast<float4 *>(a.out + r * kHd)[lane] = v;
-  if (a.gate.p) {
-    const float4 gt = reinterpret_cast<const float4 *>(a.gate.at(t, h))[lane];
-    reinterpret_cast<float4 *>(a.out_gated + r * kHd)[lane] =
-        make_float4(v.x / (1.0f + expf(-gt.x)), v.y / (1.0f + expf(-gt.y)), v.z / (1.0f + expf(-gt.z)), v.w / (1.0f + expf(-gt.w)));
-  }
+  write_out(a, t, h, 4 * lane, o, l);
 }
 
 // ------------------------------------------------------------------ host side
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
-constexpr int kSeqFill = 512;          // workgroups of all KV heads that the line is cut for
-constexpr int kSeqLeast = 4;           // steps of a piece at least
+constexpr int kTileFill = 512;         // pieces of all KV heads: two workgroups a CU
+// rows of a sequence from which on it goes by tiles
+constexpr int kFewRows = 16;
 
-SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok) {
+SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   SeqsAttnPlan p{};
+  const int grp = nh / nkv;
   p.lanes = std::max(1, kSeqFill / nkv);
-  p.least = kSeqLeast;
-  // a partial result's number is its piece plus its row block, both counted from 0
-  const uint64_t tiles = (uint64_t)n_tok * (nh / nkv) / kSeqBlock + n_seq;
-  p.part_rows = (p.lanes + tiles) * nkv * kSeqBlock;
-  p.off_ml = up256((size_t)n_tok * nh * sizeof(uint4));
-  p.off_part = up256(p.off_ml + p.part_rows * sizeof(float2));
-  p.total = up256(p.off_part + p.part_rows * kHd * sizeof(float));
+  const size_t parts = (size_t)2 * p.lanes * nkv * kSeqBlock;
+  p.off_ml = up256((size_t)kJoinLevels * 2 * kSeqFill * sizeof(unsigned));
+  p.off_part = up256(p.off_ml + parts * sizeof(float2));
+  p.total = up256(p.off_part + parts * kHd * sizeof(float));
+  // Both kernels where there may be sequences of both kinds; of a single one's only the size that it may have is known here,
+  // and either kernel takes it whatever it has.
+  const int most = max_q > 0 ? std::min(max_q, n_tok) : n_tok;
+  p.tiles = (int64_t)most * grp > kFewRows;
+  p.blocks = !p.tiles || n_seq > 1;
+  p.few = !p.tiles ? INT32_MAX : p.blocks ? kFewRows : 0;
+  p.tile_lanes = std::max(1, kTileFill / nkv);
+  if ((int64_t)n_tok * grp > kFewRows) {           // (whatever max_q says: one workspace for all of a size)
+    const uint64_t tiles = (uint64_t)n_tok * grp / kTileRows + n_seq;
+    p.tile_part_rows = (p.tile_lanes + tiles) * nkv * kTileRows;
+    p.off_info = p.total;
+    p.off_tile_ml = up256(p.off_info + (size_t)n_tok * nh * sizeof(uint4));
+    p.off_tile_part = up256(p.off_tile_ml + p.tile_part_rows * sizeof(float2));
+    p.total = up256(p.off_tile_part + p.tile_part_rows * kHd * sizeof(float));
+  }
   return p;
 }
 
+template <int PG>
+static hipError_t launch_seqs_attn_pg(const SeqsAttnArgs &a, const SeqsAttnPlan &p, hipStream_t st) {
+  if (p.tiles) {
+    hipLaunchKernelGGL((seqs_tile_kernel<PG>), dim3((unsigned)((p.tile_lanes + 7) / 8 * 8 * a.nkv)), dim3(64 * kTileWaves), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (p.blocks) hipLaunchKernelGGL((seqs_attn_kernel<PG>), dim3((unsigned)((p.lanes + 7) / 8 * 8 * a.nkv)), dim3(64 * kSeqWaves), 0, st, a);
+  return hipGetLastError();
+}
+
 hipError_t launch_seqs_attn(const SeqsAttnArgs &a, const SeqsAttnPlan &p, hipStream_t st) {
-  const dim3 grid((unsigned)((p.lanes + 7) / 8 * 8 * a.nkv));
-  if (a.v.page == 0) hipLaunchKernelGGL((seqs_attn_kernel<0>), grid, dim3(256), 0, st, a);
-  else if (a.v.page % kSeqKeys == 0) hipLaunchKernelGGL((seqs_attn_kernel<1>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((seqs_attn_kernel<2>), grid, dim3(256), 0, st, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  const hipError_t e = a.v.page == 0 ? launch_seqs_attn_pg<0>(a, p, st) : a.v.page % kSeqKeys == 0 ? launch_seqs_attn_pg<1>(a, p, st) : launch_seqs_attn_pg<2>(a, p, st);
+  if (e != hipSuccess || !p.tiles) return e;
   const dim3 rows((unsigned)((int64_t)a.v.n_tok * a.nh));
   if (rows.x > 2048) hipLaunchKernelGGL((seqs_merge_kernel<1>), rows, dim3(64), 0, st, a);
-  else if (rows.x > 256) hipLaunchKernelGGL((seqs_merge_kernel<4>), rows, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((seqs_merge_kernel<16>), rows, dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((seqs_merge_kernel<4>), rows, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -90,6 +90,7 @@ class KvSeqs:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call workspace(n_tok) before the capture: memory of a graph's own pool would not outlive it")
             self._ws, self._ws_bytes = torch.empty(need, dtype=torch.uint8, device=self._dev), need
+            check(lib().bkv_workspace_init(self.desc, self._ws.data_ptr(), need, self.cache._my_stream()), "bkv_workspace_init")
         return self._ws
 
     # ---------------------------------------------------------------- pages

@@ -367,7 +367,8 @@ typedef struct bkv_seqs {
   int32_t max_q;              /* tokens that no sequence has more of, which bkv_seqs_attn chooses its kernels */
                               /* by, or 0: not known (a wrong one costs time, and nothing else)          */
   int32_t reserved;           /* 0                                                                       */
-  const int32_t *q_start;     /* device [n_seq+1], ascending, 0 .. n_tok; NULL: one token each, s = row  */
+  const int32_t *q_start;     /* device [n_seq+1], ascending, 0 .. n_tok (where it goes back, nothing    */
+                              /* is said of the outputs); NULL: one token each, s = row                  */
   const int32_t *len;         /* device [n_seq], this call's tokens among them                           */
   const int32_t *tables;      /* device [n_seq][n_layers][max_pages], in the place of the descriptor's   */
                               /* block table (paged); NULL for a contiguous cache, n_seq <= 1            */
@@ -405,8 +406,9 @@ int bkv_seqs_read(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, int 
  *   nothing gets 0. Positions that a row does not see have no effect on it.
  *   out: [n_tok][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)). Neither may overlap the inputs
  *   or the other.
- * Workspace: bkv_seqs_workspace_bytes(d, n_seq, n_tok), which grows with both; it needs no initialisation. Calls (and replays
- * of captured ones) that share one must not overlap in time. */
+ * Workspace: bkv_seqs_workspace_bytes(d, n_seq, n_tok), which grows with both, made ready by bkv_workspace_init once and
+ * written by nothing else from then on; it serves calls of any sizes that it is large enough for. Calls (and replays of
+ * captured ones) that share one must not overlap in time. */
 size_t bkv_seqs_workspace_bytes(const bkv_cache_desc *d, int n_seq, int n_tok);
 int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, const bkv_rows *q, const bkv_rows *gate, float *out,
                   float *out_gated, void *workspace, size_t ws_bytes, hipStream_t stream);
