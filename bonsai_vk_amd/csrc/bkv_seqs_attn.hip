@@ -52,8 +52,11 @@ struct Q4Bits {
 };
 __device__ __forceinline__ h2 q4_offset(h2 d) { return d * h2{(_Float16)-24.0f, (_Float16)-24.0f}; }
 
-// 8 probabilities as ph + pl: ph cut to fp16 (two in one instruction), pl the rest, rounded
+// 8 probabilities as ph + pl: ph cut to fp16 (two in one instruction), pl the rest, rounded (one mixed-precision instruction
+// each, if the compiler does not see that the factor is -1)
 __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
+  float minus = -1.0f;
+  asm volatile("" : "+s"(minus));
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     const auto c = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
@@ -61,7 +64,7 @@ __device__ __forceinline__ void split_p(const float (&p)[8], h8 &ph, h8 &pl) {
     ph[j + 1] = (_Float16)c[1];
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) pl[j] = (_Float16)__builtin_fmaf((float)ph[j], -1.0f, p[j]);
+  for (int j = 0; j < 8; ++j) pl[j] = (_Float16)__builtin_fmaf((float)ph[j], minus, p[j]);
 }
 
 // the kernel's arguments (its first and only one), read anew
@@ -575,14 +578,17 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
 }
 
 // ------------------------------------------------------------------ many rows: key tiles in LDS
-// 4 waves hold 32 rows each, with all 256 outputs of a row in registers, and step through the workgroup's piece 32 keys at a
-// time; two workgroups a CU fill one another's waits. A step's cache bytes are loaded straight into LDS two steps ahead and
-// turned once into the products' operands for all 128 rows, the step before they are wanted: K as it is, V transposed, so
-// that a lane's 8 keys of one dim are 16 bytes. S^T and O^T are formed as in the kernel above, P never leaves its lane.
+// 4 waves hold 32 rows each, with all 256 outputs of a row in registers, and step through the even 32-key steps of the
+// workgroup's piece; 4 more waves have the same rows and the odd steps, and the two halves of the outputs meet in LDS at the
+// end. (As two workgroups, each a piece of its own, they read Q and write partial results twice.) A step's cache bytes are
+// loaded straight into LDS two rounds ahead and turned once into the products' operands for all 128 rows, the round before
+// they are wanted: K as it is, V transposed, so that a lane's 8 keys of one dim are 16 bytes. The one four turn bytes at a
+// round's beginning, the other at its end: while the matrix cores work for one, the vector unit works for the other. S^T and
+// O^T are formed as in the kernel above, P never leaves its lane.
 //
 // LDS positions, in 16-byte pieces: K piece c (8 dims) of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
 // and 16 + 4 g .. 16 + 4 g + 3) at 4 d + (g ^ vx(d)); both so that 8 neighbouring lanes' reads and writes lie in different banks.
-constexpr int kTileRows = 128, kTileWaves = 4, kTileLeast = 8;
+constexpr int kTileRows = 128, kTileWaves = 8, kTileLeast = 16;
 __device__ __forceinline__ uint32_t v_piece(int d, int g) { return (uint32_t)(64 * d + 16 * (g ^ (((d >> 1) ^ (d >> 3)) & 3))); }
 
 // tiles of a sequence, and steps of tile rb: up to its last row's last key (one at least)
@@ -600,10 +606,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   constexpr uint32_t kOp = kSeqKeys * 2 * kHd;     // an operand: 32 keys of 256 fp16
   // two steps' operands of K and of V; behind them the bytes as they came, each wave's own: 8 keys' rows of K, 64 dims of V,
   // 8 keys' scales of K, 2 blocks' scales of V
-  constexpr uint32_t oVop = 2 * kOp, oRaw = 4 * kOp, kRawV = 1024, kRawKS = 2048, kRawVS = 2176, kRaw = 2304;
-  __shared__ __attribute__((aligned(128))) uint8_t sm[oRaw + kTileWaves * kRaw];
+  constexpr uint32_t oVop = 2 * kOp, oRaw = 4 * kOp, kRawV = 1024, kRawKS = 2048, kRawVS = 2176, kRaw = 2304, kFour = oRaw + 4 * kRaw;
+  __shared__ __attribute__((aligned(128))) uint8_t all[2 * kFour];   // (of each four waves)
+  __shared__ float s_m[2][kTileRows], s_l[2][kTileRows];
+  __shared__ int s_seq[3][64];                     // rows' beginnings, tokens and lengths of the 64 sequences at hand
   __shared__ int32_t s_tab[PG ? kTileWaves : 1][64];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = w8 & 3, odd = w8 >> 2, n = lane & 15, g = lane >> 4;
+  uint8_t *const sm = all + kFour * odd;
   const Q4Bits bits;
   // (the lane's number, opaque where addresses are formed from it: kept from step to step they would take the registers that
   // the outputs need)
@@ -633,8 +642,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   if (bad || total == 0) return;
   const Cut cut(total, a.tile_lanes, a.by_tile_lanes, kTileLeast);
   if (piece >= cut.nl) return;
-  int at = cut.begin(piece);
-  const int end = cut.begin(piece + 1);
+  // A piece that would begin or end a little inside a tile begins or ends at the tile's own end: its rows' way in and out costs
+  // as much as near steps.
+  const int near = cut.share / 8;
+  auto last_piece = [&](int begin, int steps) {    // of a tile
+    const int p = cut.piece_of(begin + steps - 1), b = cut.begin(p);
+    return b > begin && b - begin > near && begin + steps - b <= near ? p - 1 : p;
+  };
+  int at = cut.begin(piece), end = cut.begin(piece + 1);
   int s0 = 0, in64 = 0, line0 = 0, tile0 = 0;      // the sequence that `at` lies in, where that begins, tiles before it
   for (;;) {
     const int nb = tiles_of(my), binc = wave_sums(nb);
@@ -672,16 +687,31 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     }
   }
   tile0 += rb;
+  bool first = true;
+  auto keep = [&](const SeqLanes &x) {             // (by every wave alike)
+    s_seq[0][lane] = x.q0;
+    s_seq[1][lane] = x.nt;
+    s_seq[2][lane] = x.len;
+  };
+  keep(my);
+  lds_barrier();
 
   const uint32_t krow = (uint32_t)a.nkv * kQ4RowBytes, srow = (uint32_t)a.nkv * kScaleRowBytes;
   const uint8_t *kd = a.L.kd + (size_t)hk * kQ4RowBytes, *vd = a.L.vd + (size_t)hk * kQ4RowBytes;
   const uint8_t *ksc = a.L.ks + (size_t)hk * kScaleRowBytes, *vsc = a.L.vs + (size_t)hk * kScaleRowBytes;
   uint8_t *const raw = sm + oRaw + kRaw * w;
   const uint32_t raw0 = lds_addr(sm) + oRaw + kRaw * w;
+  // Where the lane finds its bytes and puts its operands. K: words i + 8 j of key 8 w + k lie in raw piece (i / 4 + 2 j) ^ k and go
+  // to piece (i + 8 j) ^ key % 16: the number j changes bits by itself. V: dims d0 + 2 s, whose piece's place s changes likewise.
+  const int lk = lane >> 3, li = lane & 7;
+  const uint32_t k_raw = 128 * lk + 16 * ((li >> 2) ^ lk) + 4 * (li & 3);
+  const uint32_t k_op = 512 * (8 * w + lk) + 16 * (li ^ lk) + 128 * (w & 1);
+  const uint32_t v_raw = kRawV + 32 * g + 2 * n;
+  const uint32_t v_op = 64 * (64 * w + 8 * (n >> 1) + (n & 1)) + 16 * (g ^ ((n >> 1) & 3));
 
   while (at < end) {
     // ---- the piece's part of one tile
-    const int q0 = of_lane(my.q0, in64), nt = of_lane(my.nt, in64), len = of_lane(my.len, in64), seq = s0 + in64;
+    const int q0 = __builtin_amdgcn_readfirstlane(s_seq[0][in64]), nt = __builtin_amdgcn_readfirstlane(s_seq[1][in64]), len = __builtin_amdgcn_readfirstlane(s_seq[2][in64]), seq = s0 + in64;
     const Tiles tiles{nt, len, a.grp};
     if (nt * a.grp <= a.few || rb == tiles.count()) {   // the next sequence
       rb = 0;
@@ -689,13 +719,28 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
         in64 = 0;
         s0 += 64;
         if (s0 >= a.v.n_seq) break;
-        my = SeqLanes(a, s0);
+        lds_barrier();
+        keep(SeqLanes(a, s0));
+        lds_barrier();
       } else if (s0 + in64 >= a.v.n_seq) {
         break;
       }
       continue;
     }
-    const int R = nt * a.grp, steps = tiles.steps(a.by_grp, rb), t0 = at - line0, t1 = min(steps, t0 + (end - at));
+    const int R = nt * a.grp, steps = tiles.steps(a.by_grp, rb);
+    // (the boundaries moved: of a piece's beginning in the first tile that it meets, of its end in the last)
+    auto moved = [&](int x) { return x - line0 <= near ? line0 : line0 + steps - x <= near ? line0 + steps : x; };
+    if (first && piece > 0) at = moved(at);
+    first = false;
+    const int stop = end < line0 + steps && piece + 1 < cut.nl ? moved(end) : end;
+    if (at >= line0 + steps) {                     // (all of it is the piece's before)
+      line0 += steps;
+      ++rb;
+      ++tile0;
+      continue;
+    }
+    if (stop <= at) break;                         // (what is left of it is the next piece's)
+    const int t0 = __builtin_amdgcn_readfirstlane(at - line0), t1 = __builtin_amdgcn_readfirstlane(min(steps, t0 + (stop - at)));
     const int last = max(len - 1, 0), r0 = kTileRows * rb, rw = r0 + 32 * w;
     const bool works = rw < R;                     // (a wave whose rows are all past the last only brings bytes)
     // keys below lim are seen: by a row of the lane's, by all of the wave's, by any
@@ -708,7 +753,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     auto ask_entries = [&](int t) {
       const int lane = my_lane();
       const uint32_t key = PG == 2 ? min((uint32_t)t * kSeqKeys + ((uint32_t)lane & 31), (uint32_t)last) : min((uint32_t)t * kSeqKeys, (uint32_t)last);
-      load4_to_lds(reinterpret_cast<const uint8_t *>(table + a.by_page.div(key)), __builtin_amdgcn_readfirstlane(lds_addr(s_tab[PG ? w : 0])));
+      load4_to_lds(reinterpret_cast<const uint8_t *>(table + a.by_page.div(key)), __builtin_amdgcn_readfirstlane(lds_addr(s_tab[PG ? w8 : 0])));
     };
     // V's keys lie in the order of the contraction's slots: place 4 j + g is slot (g, j), so that the 4 groups' reads of one j
     // are neighbours
@@ -719,7 +764,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       const uint32_t kb = (uint32_t)t * kSeqKeys, left = (uint32_t)last - min(kb, (uint32_t)last);
       const int kk = 8 * w + (lane >> 3), kv = key_of(lane >> 1), ksk = (8 * w + lane) & 31, kvs = key_of(lane & 31);
       if constexpr (PG == 2) {
-        const uint32_t key = min(kb + ((uint32_t)lane & 31), (uint32_t)last), e = (uint32_t)s_tab[w][lane];
+        const uint32_t key = min(kb + ((uint32_t)lane & 31), (uint32_t)last), e = (uint32_t)s_tab[w8][lane];
         const int sl = e < (uint32_t)a.v.pool_pages ? (int)(e * (uint32_t)a.v.page + a.by_page.rest(key, a.v.page)) : -1;
         there_after = (uint32_t)__ballot(sl >= 0);
         const size_t sk = (size_t)max(__shfl(sl, kk), 0), sv = (size_t)max(__shfl(sl, kv), 0), s1 = (size_t)max(__shfl(sl, ksk), 0), s2 = (size_t)max(__shfl(sl, kvs), 0);
@@ -730,7 +775,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       } else {
         uint32_t base = min(kb, (uint32_t)last);
         if constexpr (PG == 1) {
-          const uint32_t e = (uint32_t)__builtin_amdgcn_readfirstlane(s_tab[w][lane]);
+          const uint32_t e = (uint32_t)__builtin_amdgcn_readfirstlane(s_tab[w8][lane]);
           there_after = e < (uint32_t)a.v.pool_pages ? ~0u : 0u;
           base = there_after ? e * (uint32_t)a.v.page + a.by_page.rest(base, a.v.page) : 0;
         }
@@ -743,19 +788,22 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     };
     // ---- the wave's bytes, landed, made into operands
     auto convert = [&](int buf) {
-      const int lane = my_lane(), n = lane & 15, g = lane >> 4;
-      uint8_t *const kto = sm + kOp * buf, *const vto = sm + oVop + kOp * buf;
-      {                                            // K: words i, i + 8, .. of key lane / 8
-        const int k = lane >> 3, i = lane & 7, key = 8 * w + k;
+      typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+      uint32_t k_raw_ = k_raw, k_op_ = k_op, v_op_ = v_op;   // (opaque: their variants are formed here, not kept)
+      asm volatile("" : "+v"(k_raw_), "+v"(k_op_), "+v"(v_op_));
+      const int lane = my_lane();
+      const uint32_t ks_raw = kRawKS + 16 * (lane >> 3), k_half = lane & 4 ? 0x03020302u : 0x01000100u, vs_raw = kRawVS + 4 * (lane >> 4) + 2 * ((lane >> 3) & 1);
+      {                                            // K: words i, i + 8, .. of key lane / 8 (word i + 8 j: block 2 j + i / 4)
         uint32_t x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint32_t *>(raw + 128 * k + 16 * (((i >> 2) + 2 * j) ^ k) + 4 * (i & 3));
-        const uint4 sc = *reinterpret_cast<const uint4 *>(raw + kRawKS + 16 * k);
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint32_t *>(raw + (k_raw_ ^ (32u * j)));
+        const uint4 sc = *reinterpret_cast<const uint4 *>(raw + ks_raw);
+        uint8_t *const to = sm + kOp * buf;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {              // (word i + 8 j: block 2 j + i / 4)
-          const h2 two = as_h2(q4_scales((&sc.x)[j]));
-          const h2 d = i & 4 ? h2{two[1], two[1]} : h2{two[0], two[0]};
-          *reinterpret_cast<h8 *>(kto + 512 * key + 16 * ((i + 8 * j) ^ (key & 15))) = bits.eight(x[j], d, q4_offset(d));
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t two = q4_scales((&sc.x)[j]);
+          const h2 d = as_h2(__builtin_amdgcn_perm(two, two, k_half));
+          *reinterpret_cast<h8 *>(to + (k_op_ ^ (128u * (j & 1))) + 256 * (j >> 1)) = bits.eight(x[j], d, q4_offset(d));
         }
       }
       {                                            // V: 4 dims of 8 keys: a half of word n / 2 of the wave's 8
@@ -763,15 +811,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
         h2 d[4], c[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = *reinterpret_cast<const uint16_t *>(raw + kRawV + 32 * (8 * j + g) + 2 * n), hi = *reinterpret_cast<const uint16_t *>(raw + kRawV + 32 * (8 * j + 4 + g) + 2 * n);
-          const uint32_t sl = *reinterpret_cast<const uint16_t *>(raw + kRawVS + 4 * (8 * j + g) + 2 * (n >> 3)), sh = *reinterpret_cast<const uint16_t *>(raw + kRawVS + 4 * (8 * j + 4 + g) + 2 * (n >> 3));
-          x[j] = lo | (hi << 16);
-          d[j] = as_h2(q4_scales(sl | (sh << 16)));
+          const uint8_t *const p = raw + v_raw + 256 * j, *const q = raw + vs_raw + 32 * j;
+          x[j] = __builtin_bit_cast(uint32_t, u2{*reinterpret_cast<const uint16_t *>(p), *reinterpret_cast<const uint16_t *>(p + 128)});
+          d[j] = as_h2(q4_scales(__builtin_bit_cast(uint32_t, u2{*reinterpret_cast<const uint16_t *>(q), *reinterpret_cast<const uint16_t *>(q + 16)})));
           c[j] = q4_offset(d[j]);
         }
-        const int d0 = 64 * w + 8 * (n >> 1) + (n & 1);
+        uint8_t *const to = sm + oVop + kOp * buf;
         auto put = [&](int s, const h2 (&v)[4]) {
-          *reinterpret_cast<uint4 *>(vto + v_piece(d0 + 2 * s, g)) = make_uint4(as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3]));
+          *reinterpret_cast<uint4 *>(to + (v_op_ ^ (16u * s)) + 128 * s) = make_uint4(as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3]));
         };
         put(0, {bits.pair<0>(x[0], d[0], c[0]), bits.pair<0>(x[1], d[1], c[1]), bits.pair<0>(x[2], d[2], c[2]), bits.pair<0>(x[3], d[3], c[3])});
         put(1, {bits.pair<1>(x[0], d[0], c[0]), bits.pair<1>(x[1], d[1], c[1]), bits.pair<1>(x[2], d[2], c[2]), bits.pair<1>(x[3], d[3], c[3])});
@@ -780,51 +827,66 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       }
     };
 
-    // ---- Q, 32 rows a wave, through LDS (the operands' place, 16 rows of fp16 a wave at a time), piece c of row r at c ^ r
-    if (PG) ask_entries(t0);
+    // ---- Q: 16 rows by each wave, to fp16 and through LDS (the operands' place), piece c of row r at c ^ r % 16
+    if (PG) ask_entries(min(t0 + odd, t1 - 1));
     h8 qh[2][8];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    {
       float4 x[16];
+      const int first = r0 + 16 * w8;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const int r = min(rw + 16 * mt + j, R - 1), ti = a.by_grp.div((uint32_t)r);
+        const int r = min(first + j, R - 1), ti = a.by_grp.div((uint32_t)r);
         x[j] = reinterpret_cast<const float4 *>(a.q.at(q0 + ti, hk * a.grp + r - ti * a.grp))[lane];
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const h2 lo = {(_Float16)x[j].x, (_Float16)x[j].y}, hi = {(_Float16)x[j].z, (_Float16)x[j].w};
-        *reinterpret_cast<uint2 *>(sm + 8192 * w + 512 * j + 16 * ((lane >> 1) ^ j) + 8 * (lane & 1)) = make_uint2(as_u(lo), as_u(hi));
+        *reinterpret_cast<uint2 *>(all + 8192 * w8 + 512 * j + 16 * ((lane >> 1) ^ j) + 8 * (lane & 1)) = make_uint2(as_u(lo), as_u(hi));
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-      for (int b = 0; b < 8; ++b) qh[mt][b] = *reinterpret_cast<const h8 *>(sm + 8192 * w + 512 * n + 16 * ((4 * b + g) ^ n));
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    request(t0);
+    request(t0 + odd);
     there_next = there_after;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (PG) ask_entries(min(t0 + 1, t1 - 1));
+    if (PG) ask_entries(min(t0 + 2 + odd, t1 - 1));
+    lds_barrier();                                 // (the rows are there)
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int b = 0; b < 8; ++b) qh[mt][b] = *reinterpret_cast<const h8 *>(all + 8192 * (2 * w + mt) + 512 * n + 16 * ((4 * b + g) ^ n));
+    static_assert(8 * 8192 <= oRaw, "the rows end before the bytes that are on their way");
     f4 o[2][16] = {};
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();                                 // (every wave has its rows)
     convert(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (t0 + 1 < t1) {
-      request(t0 + 1);
+    auto ask = [&](int t) {                        // the bytes of step t, where there is one, and the entries of the one after it
+      if (t >= t1) return;
+      request(t);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (PG) ask_entries(min(t0 + 2, t1 - 1));
-    }
+      if (PG) ask_entries(min(t + 2, t1 - 1));
+    };
+    ask(t0 + 2 + odd);
     lds_barrier();
 
+    // the next round's operands, in places whose readers have passed the barrier; then, with the wave's bytes used, those of
+    // the round after it
+    auto bring = [&](int t, int buf) {
+      if (t + 2 < t1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        convert(buf ^ 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        ask(t + 4);
+      }
+    };
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t) {                // (the same count in the whole workgroup)
-      const int kb = t * kSeqKeys, buf = (t - t0) & 1;
+    for (int tt = t0; tt < t1; tt += 2) {          // (the same count in the whole workgroup)
+      const int t = tt + odd, kb = t * kSeqKeys, buf = ((tt - t0) >> 1) & 1;
       there = there_next;
       there_next = there_after;
-      if (works && kb < lim_any) {
+      if (odd) bring(t, buf);
+      if (works && t < t1 && kb < lim_any) {
         const int lane = my_lane(), n = lane & 15, g = lane >> 4;
         const uint8_t *const kop = sm + kOp * buf + 512 * n, *const vop = sm + oVop + kOp * buf + 64 * n;
         const uint32_t kx = 16 * (g ^ n);          // piece 4 b + g at (4 b + g) ^ n
@@ -834,7 +896,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
         const bool whole = kb + kSeqKeys <= lim_all && (!PG || there == ~0u);
         // ---- scores
         // (the operands of product ub + AK are asked for before product ub, and no further ahead: the registers hold no more)
-        constexpr int AK = 3;
+        constexpr int AK = 2;
         f4 s[2][2] = {};
         h8 kf[AK + 1];
         __builtin_amdgcn_sched_barrier(0);
@@ -884,7 +946,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
           split_p(p, ph[mt], pl[mt]);
         }
         // ---- P V
-        constexpr int AV = 3;
+        constexpr int AV = 2;
         h8 vf[AV + 1];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -899,62 +961,75 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (t + 1 < t1) {
-        // the next step's operands, in places whose readers have passed the barrier; then, with the wave's bytes used,
-        // those of the step after it
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        convert(buf ^ 1);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (t + 2 < t1) {
-          request(t + 2);
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (PG) ask_entries(min(t + 3, t1 - 1));
-        }
-      }
+      if (!odd) bring(t, buf);
       lds_barrier();
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     const SeqsAttnArgs z = arguments_again<SeqsAttnArgs>();
+    // ---- the two fours' outputs joined: each sends the half of the dims that the other finishes
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      l[mt] += __shfl_xor(l[mt], 16);
+      l[mt] += __shfl_xor(l[mt], 32);
+      if (g == 0) { s_m[odd][32 * w + 16 * mt + n] = m[mt]; s_l[odd][32 * w + 16 * mt + n] = l[mt]; }
+    }
+    lds_barrier();
+    float f[2], by[2];                             // of the wave's own outputs; the sums
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const float mo = s_m[odd ^ 1][32 * w + 16 * mt + n], mm = fmaxf(m[mt], mo), fo = mo == -INFINITY ? 0.0f : exp2f(mo - mm);
+      f[mt] = m[mt] == -INFINITY ? 0.0f : exp2f(m[mt] - mm);
+      by[mt] = (m[mt] == -INFINITY && l[mt] == 0.0f ? 0.0f : l[mt] * f[mt]) + (mo == -INFINITY ? 0.0f : s_l[odd ^ 1][32 * w + 16 * mt + n] * fo);
+      m[mt] = mm;
+    }
+    auto send = [&](auto from) {                   // 16 bytes a lane and product, one after another
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+          *reinterpret_cast<f4 *>(all + 65536 * odd + 16384 * w + 1024 * (8 * mt + dt) + 16 * lane) = o[mt][decltype(from)::value + dt] * f[mt];
+    };
+    if (odd) send(std::integral_constant<int, 0>{});
+    else send(std::integral_constant<int, 8>{});
+    lds_barrier();
+    static_assert(2 * 65536 <= 2 * kFour, "the outputs in the operands' place");
     // ---- the outputs, or a partial result for each row of a tile that several pieces share
     const bool alone = t1 - t0 == steps;
     const uint32_t part0 = ((uint32_t)(piece + tile0) * z.nkv + hk) * kTileRows + 32 * w;
-    if (works) {
+    auto finish = [&](auto from) {
+      constexpr int D0 = decltype(from)::value;
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        float sum = l[mt];
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        const int r = rw + 16 * mt + n, ti = z.by_grp.div((uint32_t)min(r, R - 1));
-        const int64_t dst = (int64_t)(q0 + ti) * z.nh + hk * z.grp + min(r, R - 1) - ti * z.grp;
+        const int r = rw + 16 * mt + n, ti = z.by_grp.div((uint32_t)min(r, R - 1)), h = hk * z.grp + min(r, R - 1) - ti * z.grp;
+        const int64_t dst = (int64_t)(q0 + ti) * z.nh + h;
         const uint32_t part = part0 + 16 * mt + n;
-        const float by = !alone ? 1.0f : sum > 0.0f || sum != sum ? sum : 1.0f;
-        if (r < R && g == 0) {
-          if (t0 == 0) {
-            const int count = alone ? 1 : cut.piece_of(line0 + steps - 1) - piece + 1;
-            z.info[dst] = make_uint4(part, (uint32_t)z.nkv * kTileRows, (uint32_t)count, 0);
-          }
+        const float sum = by[mt], div = !alone ? 1.0f : sum > 0.0f || sum != sum ? sum : 1.0f;
+        if (D0 == 0 && r < R && g == 0) {
+          if (t0 == 0) z.info[dst] = make_uint4(part, (uint32_t)z.nkv * kTileRows, (uint32_t)(alone ? 1 : last_piece(line0, steps) - piece + 1), 0);
           if (!alone) z.tile_ml[part] = make_float2(m[mt], sum);
         }
         // lanes n and n ^ 1 exchange halves of two products, so that a store reaches 8 rows' whole lines
-        const bool odd = n & 1;
+        const bool odd_n = n & 1;
         float *const mine = r < R ? (alone ? z.out + dst * kHd : z.tile_part + (int64_t)part * kHd) : nullptr;
         const uint64_t other = __shfl_xor((unsigned long long)(uintptr_t)mine, 1);
-        float *const even_row = odd ? (float *)(uintptr_t)other : mine, *const odd_row = odd ? mine : (float *)(uintptr_t)other;
-        const float by2 = __shfl_xor(by, 1), by_even = odd ? by2 : by, by_odd = odd ? by : by2;
-        const float *const gate = z.gate.p && alone && r < R ? z.gate.at(q0 + ti, hk * z.grp + min(r, R - 1) - ti * z.grp) : nullptr;
+        float *const even_row = odd_n ? (float *)(uintptr_t)other : mine, *const odd_row = odd_n ? mine : (float *)(uintptr_t)other;
+        const float *const gate = z.gate.p && alone && r < R ? z.gate.at(q0 + ti, h) : nullptr;
         const uint64_t gother = __shfl_xor((unsigned long long)(uintptr_t)gate, 1);
-        const float *const even_gate = odd ? (const float *)(uintptr_t)gother : gate, *const odd_gate = odd ? gate : (const float *)(uintptr_t)gother;
+        const float *const even_gate = odd_n ? (const float *)(uintptr_t)gother : gate, *const odd_gate = odd_n ? gate : (const float *)(uintptr_t)gother;
 #pragma unroll
-        for (int dt = 0; dt < 16; dt += 2) {
+        for (int dt = 0; dt < 8; dt += 2) {
+          const uint8_t *const in = all + 65536 * (odd ^ 1) + 16384 * w + 1024 * (8 * mt + dt) + 16 * lane;
+          f4 v0 = o[mt][D0 + dt] * f[mt] + *reinterpret_cast<const f4 *>(in), v1 = o[mt][D0 + dt + 1] * f[mt] + *reinterpret_cast<const f4 *>(in + 1024);
+          if (alone) { v0 /= div; v1 /= div; }
           f4 e, d;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float x = dpp<0xB1>(odd ? o[mt][dt][i] : o[mt][dt + 1][i]);      // the other row's half
-            e[i] = (odd ? x : o[mt][dt][i]) / by_even;
-            d[i] = (odd ? o[mt][dt + 1][i] : x) / by_odd;
+            const float x = dpp<0xB1>(odd_n ? v0[i] : v1[i]);      // the other row's half
+            e[i] = odd_n ? x : v0[i];
+            d[i] = odd_n ? v1[i] : x;
           }
-          const int col = 16 * (dt + (odd ? 1 : 0)) + 4 * g;
+          const int col = 16 * (D0 + dt + (odd_n ? 1 : 0)) + 4 * g;
           auto write = [&](float *row, const float *gt, f4 v) {
             if (!row) return;
             *reinterpret_cast<f4 *>(row + col) = v;
@@ -970,7 +1045,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
           write(odd_row, odd_gate, d);
         }
       }
+    };
+    if (works) {
+      if (odd) finish(std::integral_constant<int, 8>{});
+      else finish(std::integral_constant<int, 0>{});
     }
+    lds_barrier();                                 // (LDS is the next part's)
     at += t1 - t0;
     if (t1 == steps) {
       line0 += steps;
@@ -1035,7 +1115,7 @@ __global__ __launch_bounds__(64 * NWV) void seqs_merge_kernel(SeqsAttnArgs a) {
 
 // ------------------------------------------------------------------ host side
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
-constexpr int kTileFill = 512;         // pieces of all KV heads: two workgroups a CU
+constexpr int kTileFill = 256;         // pieces of all KV heads: a workgroup a CU
 // rows of a sequence from which on it goes by tiles
 constexpr int kFewRows = 16;
 
