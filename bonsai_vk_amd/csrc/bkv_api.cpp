@@ -1049,6 +1049,7 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
   if (seqs->n_seq == 0 || seqs->n_tok == 0) return BKV_OK;
   // (row blocks of 16 times steps of 32 positions are counted in 31 bits)
   const int64_t blocks = (int64_t)seqs->n_tok * (d->nh / d->nkv) / 16 + seqs->n_seq;
+  if ((int64_t)seqs->n_tok * d->nh > INT32_MAX / 2 || d->nkv > 65536) return BKV_EUNSUPPORTED;
   if (blocks > INT32_MAX / (std::min<int64_t>(max_positions(d), INT32_MAX) / 32 + 1)) return BKV_EUNSUPPORTED;
   if ((rc = check_rows(q))) return rc;
   if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
@@ -1069,6 +1070,7 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
   a.out = out;
   a.out_gated = out_gated;
   a.lanes = p.lanes;
+  a.by_nh = ByConst(d->nh);
   a.by_nkv = ByConst(d->nkv);
   a.by_grp = ByConst(a.grp);
   a.by_lanes = ByConst(p.lanes);

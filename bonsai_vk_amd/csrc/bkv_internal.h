@@ -337,7 +337,7 @@ struct SeqsAttnArgs {
   Rows q, gate;                  // gate.p null: none
   float *out, *out_gated;
   int lanes;                     // pieces that the line of steps is cut into at most
-  ByConst by_nkv, by_grp, by_lanes, by_page;
+  ByConst by_nh, by_nkv, by_grp, by_lanes, by_page;
   unsigned *count;               // pieces of a row block that are done (all 0 between calls)
   float *part;                   // [2 lanes][nkv][16] unnormalised partial outputs of hd
   float2 *ml;                    // their reference (log2) and sum

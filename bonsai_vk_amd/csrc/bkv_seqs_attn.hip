@@ -582,9 +582,9 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
 // workgroup's piece; 4 more waves have the same rows and the odd steps, and the two halves of the outputs meet in LDS at the
 // end. (As two workgroups, each a piece of its own, they read Q and write partial results twice.) A step's cache bytes are
 // loaded straight into LDS two rounds ahead and turned once into the products' operands for all 128 rows, the round before
-// they are wanted: K as it is, V transposed, so that a lane's 8 keys of one dim are 16 bytes. The one four turn bytes at a
-// round's beginning, the other at its end: while the matrix cores work for one, the vector unit works for the other. S^T and
-// O^T are formed as in the kernel above, P never leaves its lane.
+// they are wanted: K as it is, V transposed, so that a lane's 8 keys of one dim are 16 bytes. (Were the one four to turn bytes
+// at a round's beginning and the other at its end, pages of 48 tokens would take 120 us instead of 103, a round's bytes being
+// asked for later.) S^T and O^T are formed as in the kernel above, P never leaves its lane.
 //
 // LDS positions, in 16-byte pieces: K piece c (8 dims) of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
 // and 16 + 4 g .. 16 + 4 g + 3) at 4 d + (g ^ vx(d)); both so that 8 neighbouring lanes' reads and writes lie in different banks.
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     asm volatile("" : "+v"(x));
     return x;
   };
-  const int at8 = (int)(blockIdx.x >> 3), round = a.by_nkv.div(at8), hk = at8 - round * a.nkv, piece = 8 * round + (int)(blockIdx.x & 7);
+  const int at8 = (int)(blockIdx.x >> 3), round = a.by_nkv.div(at8), hk = at8 - round * a.nkv;
   // ---- the line: all tiles' steps, 64 sequences at a time
   auto line_of = [&](const SeqLanes &s) {
     const Tiles t{s.nt, s.len, a.grp};
@@ -641,7 +641,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   }
   if (bad || total == 0) return;
   const Cut cut(total, a.tile_lanes, a.by_tile_lanes, kTileLeast);
-  if (piece >= cut.nl) return;
+  // an XCD has neighbouring pieces: those of one tile read the same rows of Q, each of which comes to its L2 once
+  const int rounds = (cut.nl + 7) / 8, piece = rounds * (int)(blockIdx.x & 7) + round;
+  if (round >= rounds || piece >= cut.nl) return;
   // A piece that would begin or end a little inside a tile begins or ends at the tile's own end: its rows' way in and out costs
   // as much as near steps.
   const int near = cut.share / 8;
@@ -885,7 +887,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       const int t = tt + odd, kb = t * kSeqKeys, buf = ((tt - t0) >> 1) & 1;
       there = there_next;
       there_next = there_after;
-      if (odd) bring(t, buf);
       if (works && t < t1 && kb < lim_any) {
         const int lane = my_lane(), n = lane & 15, g = lane >> 4;
         const uint8_t *const kop = sm + kOp * buf + 512 * n, *const vop = sm + oVop + kOp * buf + 64 * n;
@@ -961,7 +962,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (!odd) bring(t, buf);
+      bring(t, buf);
       lds_barrier();
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1061,51 +1062,56 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
 }
 
 // ------------------------------------------------------------------ the join of the tiles' partial results
-// A workgroup of NWV waves per row: wave w sums the partial results w, w + NWV, .. (a lane 4 dims, 8 of them requested
-// together), then the waves' sums meet in LDS.
-template <int NWV>
-__global__ __launch_bounds__(64 * NWV) void seqs_merge_kernel(SeqsAttnArgs a) {
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t r = blockIdx.x;
-  const int t = (int)(r / a.nh), h = (int)(r - (int64_t)t * a.nh);
-  __shared__ __attribute__((aligned(16))) float s_o[NWV * kHd];
+// A row by SW waves: wave w of them sums the partial results w, w + SW, .. (a lane 4 dims, 8 of them requested together), then
+// the waves' sums meet in LDS.
+constexpr int kMergeWaves = 4;
+template <int SW>
+__global__ __launch_bounds__(64 * kMergeWaves) void seqs_merge_kernel(SeqsAttnArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % SW;
+  const int64_t r = (int64_t)blockIdx.x * (kMergeWaves / SW) + wave / SW;
+  if (r >= (int64_t)a.v.n_tok * a.nh) return;      // (all SW waves of it)
+  const int t = a.by_nh.div((uint32_t)r), h = (int)r - t * a.nh;
+  __shared__ __attribute__((aligned(16))) float s_o[SW > 1 ? SW * kHd : 4];
   const uint4 in = a.info[r];
   const int s = a.v.sequence_of<64>(t);
   if (s < 0 || a.v.tokens(s) * a.grp <= a.few) return;     // (no row of a tile: nothing was left for it)
   const uint32_t first = in.x, stride = in.y, count = in.z;
   if (count <= 1 || (uint64_t)first + (uint64_t)stride * (count - 1) >= a.tile_part_rows) return;
-  float mm = -INFINITY;
-  for (uint32_t i = lane; i < count; i += 64) mm = fmaxf(mm, a.tile_ml[first + i * stride].x);
+  auto part = [&](uint32_t i) { return reinterpret_cast<const float4 *>(a.tile_part + (int64_t)(first + i * stride) * kHd)[lane]; };
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = part(min((uint32_t)(w + j * SW), count - 1));
+  float2 ml = a.tile_ml[first + min((uint32_t)lane, count - 1) * stride];
+  float mm = ml.x;
+  for (uint32_t i = 64 + lane; i < count; i += 64) mm = fmaxf(mm, a.tile_ml[first + i * stride].x);
   mm = wave_max(mm);
   float l = 0.0f;
-  for (uint32_t i = lane; i < count; i += 64) {
-    const float2 x = a.tile_ml[first + i * stride];
-    l += x.x == -INFINITY ? 0.0f : x.y * exp2f(x.x - mm);
+  for (uint32_t i0 = 0; i0 < count; i0 += 64) {    // 64 partial results' weights at a time
+    if (i0) ml = a.tile_ml[first + min(i0 + lane, count - 1) * stride];
+    const float f = i0 + lane >= count || ml.x == -INFINITY ? 0.0f : exp2f(ml.x - mm);
+    l += i0 + lane >= count || ml.x == -INFINITY ? 0.0f : ml.y * f;
+    const uint32_t n64 = min(count - i0, 64u);
+    for (uint32_t i = w; i < n64; i += 8 * SW) {
+      if (i0 + i >= 8 * SW) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = part(min(i0 + i + j * SW, count - 1));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (i + j * SW >= n64) break;
+        const float fj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (int)(i + j * SW)));
+        o.x = fmaf(x[j].x, fj, o.x); o.y = fmaf(x[j].y, fj, o.y); o.z = fmaf(x[j].z, fj, o.z); o.w = fmaf(x[j].w, fj, o.w);
+      }
+    }
   }
   l = wave_sum(l);
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x[8];
-  for (uint32_t i0 = w; i0 < count; i0 += 8 * NWV) {
-    float m8[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t i = min(i0 + j * NWV, count - 1);
-      x[j] = reinterpret_cast<const float4 *>(a.tile_part + (int64_t)(first + i * stride) * kHd)[lane];
-      m8[j] = a.tile_ml[first + i * stride].x;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (i0 + j * NWV >= count) break;
-      const float f = m8[j] == -INFINITY ? 0.0f : exp2f(m8[j] - mm);
-      o.x = fmaf(x[j].x, f, o.x); o.y = fmaf(x[j].y, f, o.y); o.z = fmaf(x[j].z, f, o.z); o.w = fmaf(x[j].w, f, o.w);
-    }
-  }
-  if constexpr (NWV > 1) {
+  if constexpr (SW > 1) {
     reinterpret_cast<float4 *>(s_o + w * kHd)[lane] = o;
     __syncthreads();
     if (w != 0) return;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < NWV; ++j) {
+    for (int j = 0; j < SW; ++j) {
       const float4 y = reinterpret_cast<const float4 *>(s_o + j * kHd)[lane];
       o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
     }
@@ -1159,9 +1165,9 @@ static hipError_t launch_seqs_attn_pg(const SeqsAttnArgs &a, const SeqsAttnPlan 
 hipError_t launch_seqs_attn(const SeqsAttnArgs &a, const SeqsAttnPlan &p, hipStream_t st) {
   const hipError_t e = a.v.page == 0 ? launch_seqs_attn_pg<0>(a, p, st) : a.v.page % kSeqKeys == 0 ? launch_seqs_attn_pg<1>(a, p, st) : launch_seqs_attn_pg<2>(a, p, st);
   if (e != hipSuccess || !p.tiles) return e;
-  const dim3 rows((unsigned)((int64_t)a.v.n_tok * a.nh));
-  if (rows.x > 2048) hipLaunchKernelGGL((seqs_merge_kernel<1>), rows, dim3(64), 0, st, a);
-  else hipLaunchKernelGGL((seqs_merge_kernel<4>), rows, dim3(256), 0, st, a);
+  const unsigned rows = (unsigned)((int64_t)a.v.n_tok * a.nh);
+  if (rows > 2048) hipLaunchKernelGGL((seqs_merge_kernel<1>), dim3((rows + kMergeWaves - 1) / kMergeWaves), dim3(64 * kMergeWaves), 0, st, a);
+  else hipLaunchKernelGGL((seqs_merge_kernel<kMergeWaves>), dim3(rows), dim3(64 * kMergeWaves), 0, st, a);
   return hipGetLastError();
 }
 
