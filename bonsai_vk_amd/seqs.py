@@ -173,7 +173,7 @@ class KvSeqs:
 
     def read(self, layer, q_start, n_tok, dtype=torch.float32):
         """bkv_seqs_read: (K, V) of the call's tokens as values, [n_tok][nkv][hd] of dtype (float32, float16 or bfloat16);
-        rows that are no sequence's are 0."""
+        rows that are no sequence's are not written."""
         c = self.cache
         if c._elsewhere():
             with torch.cuda.device(self._dev):

@@ -45,7 +45,7 @@ def q4_values(data, scales):
 
 
 # ------------------------------------------------------------------ caches
-def make(lens, page, nkv=4, grp=4, k="q4_0", v="q4_0", layers=1, spare=3, seed=0, cap=None, room=None):
+def make(lens, page, nkv=4, grp=4, k="q4_0", v="q4_0", layers=1, spare=3, seed=0, cap=None, room=None, hd=256):
     """(KvCache, KvSeqs) of sequences that have `lens` positions, their pages anywhere in the pool (every layer its own);
     room: positions that a sequence can have."""
     r = np.random.default_rng(seed)
@@ -53,7 +53,7 @@ def make(lens, page, nkv=4, grp=4, k="q4_0", v="q4_0", layers=1, spare=3, seed=0
         per = [-(-n // page) for n in lens]
         pool = sum(per) + spare if cap is None else cap // page
         most = max(1, -(-(room or max(lens)) // page), *per)
-        cache = KvCache(n_layers=layers, nh=nkv * grp, nkv=nkv, cap=pool * page, k_fmt=FMT[k], v_fmt=FMT[v], page_tokens=page,
+        cache = KvCache(n_layers=layers, nh=nkv * grp, nkv=nkv, hd=hd, cap=pool * page, k_fmt=FMT[k], v_fmt=FMT[v], page_tokens=page,
                         max_pages=most, block_table=torch.full((layers, most), -1))
     else:
         cache = KvCache(n_layers=layers, nh=nkv * grp, nkv=nkv, cap=cap or max(max(lens), 1), k_fmt=FMT[k], v_fmt=FMT[v])

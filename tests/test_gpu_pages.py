@@ -63,6 +63,26 @@ def test_a_life_of_sequences(k, v, page, nkv):
         assert np.array_equal(count(seqs), want.refs)
 
 
+@pytest.mark.parametrize("hd, nkv", [(64, 1), (64, 3), (128, 1), (192, 2)])
+@pytest.mark.parametrize("page", [3, 16])
+def test_rows_of_few_scales(hd, nkv, page):
+    """4, 12, 8 and 24 bytes of scales a position: what is held of a page ends inside 16 bytes, and so may a page begin."""
+    cache, seqs = make([0] * 4, page, nkv, 2, "q8_0", "q4_0", layers=2, cap=page * 40, room=10 * page, hd=hd)
+    random_bytes(cache, hd + page)
+    want = Pages(seqs)
+    for n in ([page - 1, 1, 2 * page + 2, 5], [1, 2, 3, 1]):
+        extend(seqs, n, want)
+        want.len += np.array(n, np.int32)
+        seqs.len += device_ints(n)
+        parent = [0, 0, 2, 2] if page == 3 else [3, 1, 3, 2]
+        seqs.fork(device_ints(parent))
+        want.fork(parent)
+        extend(seqs, [1, 1, 1, 1], want)
+        before = [a.clone() for a in arrays(cache)]
+        seqs.compact()
+        same(seqs, want, before, want.compact())
+
+
 def test_the_last_keeps_a_page_that_nobody_else_would():
     cache, seqs = make([0] * 4, 16, layers=2, cap=16 * 20, room=64)
     random_bytes(cache)
