@@ -423,6 +423,7 @@ static hipError_t append_q4(const bkv_cache_desc *d, int layer, uint32_t pos0, i
   a.qn_w = qn_w; a.kn_w = kn_w;
   a.eps = eps;
   a.positions = positions;
+  a.n_axes = 1;
   a.q_out = q_out;
   a.rope = rope;
   return launch_seqs_rope_append(a, d->k_fmt, d->v_fmt, stream);
@@ -1007,6 +1008,7 @@ int bkv_seqs_rope_append(const bkv_cache_desc *d, int layer, const bkv_seqs *seq
   a.qn_w = qn_w; a.kn_w = kn_w;
   a.eps = eps;
   a.positions = positions;
+  a.n_axes = axes ? axes->n_axes : 1;
   a.q_out = q_out;
   a.rope = *rope;
   if (axes) std::memcpy(a.axis, axes->axis, sizeof a.axis);

@@ -311,7 +311,9 @@ struct SeqsRowArgs {
   Rows q, k, v_rows;             // q.p null: K and V only
   const float *qn_w, *kn_w;      // null: no norm
   float eps;
-  const int32_t *positions;      // [axes][n_tok], null: the cache's positions
+  const int32_t *positions;      // [n_axes][n_tok], null: the cache's positions
+  int n_axes;
+  int rows_per;                  // rows of a workgroup (the launch's)
   float *q_out;
   bkv_rope rope;
   uint8_t axis[kHd / 2];         // of each pair
