@@ -349,7 +349,7 @@ struct SeqsAttnArgs {
   uint64_t tile_part_rows;
   float *tile_part;
   float2 *tile_ml;
-  uint4 *info;                   // per output row of a tile: its first partial result, the distance of the next, how many (1: none)
+  uint4 *info;                   // per output row of a tile: its first partial result, the distance of the later ones, how many (1: none)
 };
 struct SeqsAttnPlan {
   int lanes, tile_lanes, few;

@@ -630,7 +630,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       for (int rb = 0; rb < t.count(); ++rb) sum += t.steps(a.by_grp, rb);
     return sum;
   };
-  auto tiles_of = [&](const SeqLanes &s) { return s.nt * a.grp > a.few ? Tiles{s.nt, s.len, a.grp}.count() : 0; };
   SeqLanes my(a, 0);
   int mine_line = line_of(my), inc = wave_sums(mine_line), total = of_lane(inc, 63);
   bool bad = my.bad;
@@ -652,18 +651,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     return b > begin && b - begin > near && begin + steps - b <= near ? p - 1 : p;
   };
   int at = cut.begin(piece), end = cut.begin(piece + 1);
-  int s0 = 0, in64 = 0, line0 = 0, tile0 = 0;      // the sequence that `at` lies in, where that begins, tiles before it
+  int s0 = 0, in64 = 0, line0 = 0;                 // the sequence that `at` lies in, and where that begins
   for (;;) {
-    const int nb = tiles_of(my), binc = wave_sums(nb);
     const uint64_t past = __ballot(line0 + inc > at);
     if (past) {
       in64 = __ffsll((unsigned long long)past) - 1;
       line0 += of_lane(inc - mine_line, in64);
-      tile0 += of_lane(binc - nb, in64);
       break;
     }
     line0 += of_lane(inc, 63);
-    tile0 += of_lane(binc, 63);
     s0 += 64;
     if (s0 >= a.v.n_seq) return;
     my = SeqLanes(a, s0);
@@ -688,7 +684,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       if (rb >= t.count()) return;
     }
   }
-  tile0 += rb;
   bool first = true;
   auto keep = [&](const SeqLanes &x) {             // (by every wave alike)
     s_seq[0][lane] = x.q0;
@@ -738,7 +733,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     if (at >= line0 + steps) {                     // (all of it is the piece's before)
       line0 += steps;
       ++rb;
-      ++tile0;
       continue;
     }
     if (stop <= at) break;                         // (what is left of it is the next piece's)
@@ -997,7 +991,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     static_assert(2 * 65536 <= 2 * kFour, "the outputs in the operands' place");
     // ---- the outputs, or a partial result for each row of a tile that several pieces share
     const bool alone = t1 - t0 == steps;
-    const uint32_t part0 = ((uint32_t)(piece + tile0) * z.nkv + hk) * kTileRows + 32 * w;
+    // (a piece leaves partial results of two tiles at most: the one that it begins inside, and the one whose beginning it has
+    // but not its end)
+    const uint32_t part0 = ((uint32_t)(2 * piece + (t0 == 0)) * z.nkv + hk) * kTileRows + 32 * w;
     auto finish = [&](auto from) {
       constexpr int D0 = decltype(from)::value;
 #pragma unroll
@@ -1007,7 +1003,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
         const uint32_t part = part0 + 16 * mt + n;
         const float sum = by[mt], div = !alone ? 1.0f : sum > 0.0f || sum != sum ? sum : 1.0f;
         if (D0 == 0 && r < R && g == 0) {
-          if (t0 == 0) z.info[dst] = make_uint4(part, (uint32_t)z.nkv * kTileRows, (uint32_t)(alone ? 1 : last_piece(line0, steps) - piece + 1), 0);
+          if (t0 == 0) z.info[dst] = make_uint4(part, 2u * (uint32_t)z.nkv * kTileRows, (uint32_t)(alone ? 1 : last_piece(line0, steps) - piece + 1), 0);
           if (!alone) z.tile_ml[part] = make_float2(m[mt], sum);
         }
         // lanes n and n ^ 1 exchange halves of two products, so that a store reaches 8 rows' whole lines
@@ -1056,7 +1052,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     if (t1 == steps) {
       line0 += steps;
       ++rb;
-      ++tile0;
     }
   }
 }
@@ -1077,17 +1072,18 @@ __global__ __launch_bounds__(64 * kMergeWaves) void seqs_merge_kernel(SeqsAttnAr
   if (s < 0 || a.v.tokens(s) * a.grp <= a.few) return;     // (no row of a tile: nothing was left for it)
   const uint32_t first = in.x, stride = in.y, count = in.z;
   if (count <= 1 || (uint64_t)first + (uint64_t)stride * (count - 1) >= a.tile_part_rows) return;
-  auto part = [&](uint32_t i) { return reinterpret_cast<const float4 *>(a.tile_part + (int64_t)(first + i * stride) * kHd)[lane]; };
+  auto row_of = [&](uint32_t i) { return first + i * stride - (i ? stride / 2 : 0); };
+  auto part = [&](uint32_t i) { return reinterpret_cast<const float4 *>(a.tile_part + (int64_t)row_of(i) * kHd)[lane]; };
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = part(min((uint32_t)(w + j * SW), count - 1));
-  float2 ml = a.tile_ml[first + min((uint32_t)lane, count - 1) * stride];
+  float2 ml = a.tile_ml[row_of(min((uint32_t)lane, count - 1))];
   float mm = ml.x;
-  for (uint32_t i = 64 + lane; i < count; i += 64) mm = fmaxf(mm, a.tile_ml[first + i * stride].x);
+  for (uint32_t i = 64 + lane; i < count; i += 64) mm = fmaxf(mm, a.tile_ml[row_of(i)].x);
   mm = wave_max(mm);
   float l = 0.0f;
   for (uint32_t i0 = 0; i0 < count; i0 += 64) {    // 64 partial results' weights at a time
-    if (i0) ml = a.tile_ml[first + min(i0 + lane, count - 1) * stride];
+    if (i0) ml = a.tile_ml[row_of(min(i0 + lane, count - 1))];
     const float f = i0 + lane >= count || ml.x == -INFINITY ? 0.0f : exp2f(ml.x - mm);
     l += i0 + lane >= count || ml.x == -INFINITY ? 0.0f : ml.y * f;
     const uint32_t n64 = min(count - i0, 64u);
@@ -1141,8 +1137,7 @@ SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   p.few = !p.tiles ? INT32_MAX : p.blocks ? kFewRows : 0;
   p.tile_lanes = std::max(1, kTileFill / nkv);
   if ((int64_t)n_tok * grp > kFewRows) {           // (whatever max_q says: one workspace for all of a size)
-    const uint64_t tiles = (uint64_t)n_tok * grp / kTileRows + n_seq;
-    p.tile_part_rows = (p.tile_lanes + tiles) * nkv * kTileRows;
+    p.tile_part_rows = p.tile_lanes > 1 ? (uint64_t)2 * p.tile_lanes * nkv * kTileRows : 0;   // (a single piece shares no tile)
     p.off_info = p.total;
     p.off_tile_ml = up256(p.off_info + (size_t)n_tok * nh * sizeof(uint4));
     p.off_tile_part = up256(p.off_tile_ml + p.tile_part_rows * sizeof(float2));
