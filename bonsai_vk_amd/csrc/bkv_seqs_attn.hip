@@ -644,8 +644,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   const int rounds = (cut.nl + 7) / 8, piece = rounds * (int)(blockIdx.x & 7) + round;
   if (round >= rounds || piece >= cut.nl) return;
   // A piece that would begin or end a little inside a tile begins or ends at the tile's own end: its rows' way in and out costs
-  // as much as near steps.
-  const int near = cut.share / 8;
+  // as much as near steps (15 sequences with chunks among them: 92 us; with an eighth of a piece 101).
+  const int near = min(cut.share / 4, 8);
   auto last_piece = [&](int begin, int steps) {    // of a tile
     const int p = cut.piece_of(begin + steps - 1), b = cut.begin(p);
     return b > begin && b - begin > near && begin + steps - b <= near ? p - 1 : p;
@@ -824,7 +824,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     };
 
     // ---- Q: 16 rows by each wave, to fp16 and through LDS (the operands' place), piece c of row r at c ^ r % 16
-    if (PG) ask_entries(min(t0 + odd, t1 - 1));
+    if (PG) {
+      ask_entries(min(t0 + odd, t1 - 1));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    request(t0 + odd);
+    there_next = there_after;
     h8 qh[2][8];
     {
       float4 x[16];
@@ -840,9 +845,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
         *reinterpret_cast<uint2 *>(all + 8192 * w8 + 512 * j + 16 * ((lane >> 1) ^ j) + 8 * (lane & 1)) = make_uint2(as_u(lo), as_u(hi));
       }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    request(t0 + odd);
-    there_next = there_after;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (PG) ask_entries(min(t0 + 2 + odd, t1 - 1));
     lds_barrier();                                 // (the rows are there)
