@@ -1049,10 +1049,10 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
   if (layer < 0 || layer >= d->n_layers) return BKV_EINVAL;
   if ((rc = check_seqs(d, seqs))) return rc;
   if (seqs->n_seq == 0 || seqs->n_tok == 0) return BKV_OK;
-  // (row blocks of 16 times steps of 32 positions are counted in 31 bits)
+  // (row blocks of 16 times steps of 32 positions, and what a block's way in counts as, are counted in 31 bits)
   const int64_t blocks = (int64_t)seqs->n_tok * (d->nh / d->nkv) / 16 + seqs->n_seq;
   if ((int64_t)seqs->n_tok * d->nh > INT32_MAX / 2 || d->nkv > 65536) return BKV_EUNSUPPORTED;
-  if (blocks > INT32_MAX / (std::min<int64_t>(max_positions(d), INT32_MAX) / 32 + 1)) return BKV_EUNSUPPORTED;
+  if (blocks > INT32_MAX / (std::min<int64_t>(max_positions(d), INT32_MAX) / 32 + 1 + kSeqWayIn)) return BKV_EUNSUPPORTED;
   if ((rc = check_rows(q))) return rc;
   if (!out || (gate == nullptr) != (out_gated == nullptr)) return BKV_EINVAL;
   if (gate && (rc = check_rows(gate))) return rc;
@@ -1079,6 +1079,7 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
   a.by_page = ByConst(std::max(1, d->page_tokens));
   a.count = (unsigned *)w;
   a.few = p.few;
+  a.way_in = p.way_in;
   a.tile_lanes = p.tile_lanes;
   a.by_tile_lanes = ByConst(p.tile_lanes);
   a.tile_part_rows = p.tile_part_rows;

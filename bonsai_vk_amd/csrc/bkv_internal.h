@@ -331,6 +331,9 @@ struct SeqsReadArgs {
 };
 hipError_t launch_seqs_read(const SeqsReadArgs &a, int kf, int vf, int out_type, hipStream_t st);
 
+// steps that a row block's way in and out counts as where work is shared out, beside its own, in a line of several (29 sequences of
+// 40 to 12000 positions: 28 us; with 0, 8, 24 steps 42, 29, 30)
+constexpr int kSeqWayIn = 16;
 struct SeqsAttnArgs {
   LayerView L;
   SeqsView v;
@@ -344,6 +347,7 @@ struct SeqsAttnArgs {
   float *part;                   // [2 lanes][nkv][16] unnormalised partial outputs of hd
   float2 *ml;                    // their reference (log2) and sum
   int few;                       // sequences of more rows than this go by tiles
+  int way_in;                    // steps that a row block of the others counts as beside its own
   int tile_lanes;                // the same of the tiles
   ByConst by_tile_lanes;
   uint64_t tile_part_rows;
@@ -352,7 +356,7 @@ struct SeqsAttnArgs {
   uint4 *info;                   // per output row of a tile: its first partial result, the distance of the later ones, how many (1: none)
 };
 struct SeqsAttnPlan {
-  int lanes, tile_lanes, few;
+  int lanes, tile_lanes, few, way_in;
   bool blocks, tiles;            // which kernels run
   uint64_t tile_part_rows;
   size_t off_ml, off_part, off_info, off_tile_ml, off_tile_part, total;

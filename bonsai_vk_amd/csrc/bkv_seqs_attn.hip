@@ -114,7 +114,7 @@ struct SeqLanes {
     blocks = (int)((uint32_t)(nt * a.grp + kSeqBlock - 1) / kSeqBlock);
   }
   // (of the sequences of few rows)
-  __device__ __forceinline__ int line(const SeqsAttnArgs &a) const { return nt * a.grp <= a.few ? blocks * steps : 0; }
+  __device__ __forceinline__ int line(const SeqsAttnArgs &a) const { return nt * a.grp <= a.few ? blocks * (a.way_in + steps) : 0; }
 };
 
 // how the line is cut: nl pieces of share steps, the first spare of one more
@@ -150,25 +150,25 @@ constexpr int kJoin = 8;               // partial results that are joined at a t
 constexpr int kJoinLevels = 3;         // counters: of each level, a piece's two row blocks
 static_assert(kJoin * kJoin * kJoin >= kSeqFill, "levels of joins");
 
-__device__ __forceinline__ void st_part(float *p, float4 v) {
-  st_agent(reinterpret_cast<unsigned long long *>(p), __builtin_bit_cast(unsigned long long, make_float2(v.x, v.y)));
-  st_agent(reinterpret_cast<unsigned long long *>(p) + 1, __builtin_bit_cast(unsigned long long, make_float2(v.z, v.w)));
-}
-__device__ __forceinline__ float4 ld_part(const float *p) {
-  const float2 a = __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(p)));
-  const float2 b = __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(p) + 1));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
+__device__ __forceinline__ void st_part(void *p, float2 v) { st_agent(reinterpret_cast<unsigned long long *>(p), __builtin_bit_cast(unsigned long long, v)); }
+__device__ __forceinline__ float2 ld_part(const void *p) { return __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(p))); }
 
-__device__ __forceinline__ void write_out(const SeqsAttnArgs &a, int t, int h, int col, float4 v, float l) {
+// N outputs of a row, from dim col on
+template <int N>
+__device__ __forceinline__ void write_out(const SeqsAttnArgs &a, int t, int h, int col, const float (&v)[N], float l) {
+  typedef float V __attribute__((ext_vector_type(N)));
   const float by = l > 0.0f || l != l ? l : 1.0f;
   const int64_t at = ((int64_t)t * a.nh + h) * kHd + col;
-  v = make_float4(v.x / by, v.y / by, v.z / by, v.w / by);
-  *reinterpret_cast<float4 *>(a.out + at) = v;
+  V o;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = v[i] / by;
+  *reinterpret_cast<V *>(a.out + at) = o;
   if (a.gate.p) {
-    const float4 g = *reinterpret_cast<const float4 *>(a.gate.at(t, h) + col);
-    *reinterpret_cast<float4 *>(a.out_gated + at) =
-        make_float4(v.x / (1.0f + expf(-g.x)), v.y / (1.0f + expf(-g.y)), v.z / (1.0f + expf(-g.z)), v.w / (1.0f + expf(-g.w)));
+    const V g = *reinterpret_cast<const V *>(a.gate.at(t, h) + col);
+    V y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = o[i] / (1.0f + expf(-g[i]));
+    *reinterpret_cast<V *>(a.out_gated + at) = y;
   }
 }
 
@@ -231,8 +231,9 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
     // ---- the piece's part of one row block
     const int q0 = of_lane(my.q0, in64), nt = of_lane(my.nt, in64), len = of_lane(my.len, in64), steps = of_lane(my.steps, in64);
     const int blocks = nt * a.grp <= a.few ? of_lane(my.blocks, in64) : 0, seq = s0 + in64;
-    if (at - line0 >= blocks * steps) {            // the next sequence
-      line0 += blocks * steps;
+    const int way_in = a.way_in, long_steps = way_in + steps;
+    if (at - line0 >= blocks * long_steps) {       // the next sequence
+      line0 += blocks * long_steps;
       if (++in64 == 64) {
         in64 = 0;
         s0 += 64;
@@ -243,8 +244,10 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
       }
       continue;
     }
-    const int R = nt * a.grp, rb = blocks == 1 ? 0 : (at - line0) / steps, st0 = at - line0 - rb * steps;
-    const int st1 = min(steps, st0 + (end - at)), m4 = st1 - st0;
+    const int R = nt * a.grp, rb = blocks == 1 ? 0 : (at - line0) / long_steps, x0 = at - line0 - rb * long_steps;
+    const int x1 = min(long_steps, x0 + (end - at)), st0 = max(x0 - way_in, 0), st1 = max(x1 - way_in, 0), m4 = st1 - st0;
+    at += x1 - x0;
+    if (m4 == 0) continue;
     const int t0 = st0 + (int)((uint32_t)(m4 * w) / kSeqWaves), t1 = st0 + (int)((uint32_t)(m4 * (w + 1)) / kSeqWaves);
     const int last = max(len - 1, 0);              // (the last key that there are bytes of)
     // Blocks of 8 rows or fewer: columns n and n + 8 of the products are the same row, and one product of the outputs takes ph in
@@ -470,52 +473,61 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
     // ---- the waves' parts joined
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) { s_m[w][n] = m; s_l[w][n] = l; }
+    if (g == 0) s_m[w][n] = m;
     __syncthreads();
     float *const s_o = reinterpret_cast<float *>(sm);
     constexpr int kWF = kWave / 4;                 // (a wave's rows in the place of its steps)
-    if (col < real) {
+    {
       float mm = s_m[0][n];
 #pragma unroll
       for (int j = 1; j < kSeqWaves; ++j) mm = fmaxf(mm, s_m[j][n]);
       const float f = m == -INFINITY ? 0.0f : exp2f(m - mm);
+      if (g == 0) s_l[w][n] = l * f;
 #pragma unroll
-      for (int dt = 0; dt < 16; dt += 4)           // (4 products' dims are neighbours)
+      for (int dt = 0; dt < 16; ++dt) o[dt] *= f;
+      if (halves) {                                // (the large parts' sums and the small parts')
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float4 *>(&s_o[kWF * w + n * kOS + 16 * (4 * g + i) + dt]) =
-              make_float4(o[dt][i] * f, o[dt + 1][i] * f, o[dt + 2][i] * f, o[dt + 3][i] * f);
+        for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][i] += dpp<0x128>(o[dt][i]);
+      }
+      if (n < real) {
+#pragma unroll
+        for (int dt = 0; dt < 16; dt += 4)         // (4 products' dims are neighbours)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4 *>(&s_o[kWF * w + n * kOS + 16 * (4 * g + i) + dt]) = make_float4(o[dt][i], o[dt + 1][i], o[dt + 2][i], o[dt + 3][i]);
+      }
     }
     __syncthreads();
     const bool alone = m4 == steps;
     // the row block's pieces, this one among them, and where partial results of piece i lie
-    const int tile_line = line0 + rb * steps;
+    const int tile_line = line0 + rb * long_steps + way_in;
     const int first = alone ? piece : cut.piece_of(tile_line), count = alone ? 1 : cut.piece_of(tile_line + steps - 1) - first + 1;
     // (a piece is the first of one cut row block, whose beginning it holds the last of, and a later one of one other)
     auto part_of = [&](int i) { return (uint32_t)((2 * (first + i) + (i == 0)) * z.nkv + hk); };
-    for (int x = threadIdx.x; x < real * (kHd / 4); x += NT) {
-      const int jr = x / (kHd / 4), col = 4 * (x % (kHd / 4));
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float mr = s_m[0][jr], lr = 0.0f;
-#pragma unroll
-      for (int j = 1; j < kSeqWaves; ++j) mr = fmaxf(mr, s_m[j][jr]);
+    // (two dims a thread: 4 rows are the whole workgroup's)
+    for (int x = threadIdx.x; x < real * (kHd / 2); x += NT) {
+      const int jr = x / (kHd / 2), col = 2 * (x % (kHd / 2));
+      float v[2] = {}, lr = 0.0f;
 #pragma unroll
       for (int j = 0; j < kSeqWaves; ++j) {
-        const float4 y = *reinterpret_cast<const float4 *>(&s_o[kWF * j + jr * kOS + col]);
-        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-        if (halves) {
-          const float4 x8 = *reinterpret_cast<const float4 *>(&s_o[kWF * j + (jr + 8) * kOS + col]);
-          v.x += x8.x; v.y += x8.y; v.z += x8.z; v.w += x8.w;
-        }
-        lr += s_m[j][jr] == -INFINITY ? 0.0f : s_l[j][jr] * exp2f(s_m[j][jr] - mr);
+        const float2 y = *reinterpret_cast<const float2 *>(&s_o[kWF * j + jr * kOS + col]);
+        v[0] += y.x; v[1] += y.y;
+        lr += s_l[j][jr];
       }
       if (alone) {
         const int ti = z.by_grp.div(r0 + jr);
         write_out(z, q0 + ti, hk * z.grp + r0 + jr - ti * z.grp, col, v, lr);
       } else {
         const uint32_t p = part_of(piece - first) * kSeqBlock + jr;
-        st_part(z.part + (int64_t)p * kHd + col, v);
-        if (col == 0) st_agent(reinterpret_cast<unsigned long long *>(z.ml + p), __builtin_bit_cast(unsigned long long, make_float2(mr, lr)));
+        st_part(z.part + (int64_t)p * kHd + col, make_float2(v[0], v[1]));
+        if (col == 0) {
+          float mr = s_m[0][jr];
+#pragma unroll
+          for (int j = 1; j < kSeqWaves; ++j) mr = fmaxf(mr, s_m[j][jr]);
+          st_part(z.ml + p, make_float2(mr, lr));
+        }
       }
     }
     // ---- the pieces joined: 8 at a time, then those
@@ -531,14 +543,14 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
         if (!s_last) break;
         if (threadIdx.x == 0) st_agent(counter, 0u);        // (for the next call)
         const bool done = size == groups;
-        for (int x = threadIdx.x; x < real * (kHd / 4); x += NT) {
-          const int jr = x / (kHd / 4), col = 4 * (x % (kHd / 4));
-          float4 v[kJoin], o4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          float2 ml[kJoin];
+        for (int x = threadIdx.x; x < real * (kHd / 2); x += NT) {
+          const int jr = x / (kHd / 2), col = 2 * (x % (kHd / 2));
+          float2 v[kJoin], ml[kJoin];
+          float o2[2] = {};
 #pragma unroll
           for (int j = 0; j < kJoin; ++j) {
             const uint32_t p = part_of((g0 + min(j, size - 1)) * unit) * kSeqBlock + jr;
-            ml[j] = __builtin_bit_cast(float2, ld_agent(reinterpret_cast<const unsigned long long *>(z.ml + p)));
+            ml[j] = ld_part(z.ml + p);
             v[j] = ld_part(z.part + (int64_t)p * kHd + col);
           }
           float mr = ml[0].x, lr = 0.0f;
@@ -549,15 +561,16 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
             const float f = j >= size || ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - mr);
             if (j < size) {
               lr = fmaf(ml[j].y, f, lr);
-              o4.x = fmaf(v[j].x, f, o4.x); o4.y = fmaf(v[j].y, f, o4.y); o4.z = fmaf(v[j].z, f, o4.z); o4.w = fmaf(v[j].w, f, o4.w);
+              o2[0] = fmaf(v[j].x, f, o2[0]);
+              o2[1] = fmaf(v[j].y, f, o2[1]);
             }
           }
           if (done) {
             const int ti = z.by_grp.div(r0 + jr);
-            write_out(z, q0 + ti, hk * z.grp + r0 + jr - ti * z.grp, col, o4, lr);
+            write_out(z, q0 + ti, hk * z.grp + r0 + jr - ti * z.grp, col, o2, lr);
           } else {                                 // in the place of its first: what a thread writes it alone has read,
             const uint32_t p = part_of(g0 * unit) * kSeqBlock + jr;
-            st_part(z.part + (int64_t)p * kHd + col, o4);
+            st_part(z.part + (int64_t)p * kHd + col, make_float2(o2[0], o2[1]));
             s_o[2 * jr] = mr;                      // but for the reference and the sum, written behind a barrier
             s_o[2 * jr + 1] = lr;
           }
@@ -565,15 +578,13 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
         if (done) break;
         __syncthreads();
         if (threadIdx.x < real)
-          st_agent(reinterpret_cast<unsigned long long *>(z.ml + part_of(g0 * unit) * kSeqBlock + threadIdx.x),
-                   __builtin_bit_cast(unsigned long long, make_float2(s_o[2 * threadIdx.x], s_o[2 * threadIdx.x + 1])));
+          st_part(z.ml + part_of(g0 * unit) * kSeqBlock + threadIdx.x, make_float2(s_o[2 * threadIdx.x], s_o[2 * threadIdx.x + 1]));
         mine /= kJoin;
         groups = (groups + kJoin - 1) / kJoin;
         unit *= kJoin;
       }
     }
     __syncthreads();                               // (LDS is the next part's)
-    at += m4;
   }
 }
 
@@ -1114,7 +1125,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void seqs_merge_kernel(SeqsAttnAr
       o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
     }
   }
-  write_out(a, t, h, 4 * lane, o, l);
+  write_out(a, t, h, 4 * lane, {o.x, o.y, o.z, o.w}, l);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1137,6 +1148,7 @@ SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   p.tiles = (int64_t)most * grp > kFewRows;
   p.blocks = !p.tiles || n_seq > 1;
   p.few = !p.tiles ? INT32_MAX : p.blocks ? kFewRows : 0;
+  p.way_in = n_seq > 1 ? kSeqWayIn : 0;
   p.tile_lanes = std::max(1, kTileFill / nkv);
   if ((int64_t)n_tok * grp > kFewRows) {           // (whatever max_q says: one workspace for all of a size)
     p.tile_part_rows = p.tile_lanes > 1 ? (uint64_t)2 * p.tile_lanes * nkv * kTileRows : 0;   // (a single piece shares no tile)
