@@ -428,7 +428,8 @@ int bkv_pages_fork(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t 
  * positions below len[s] copied, but the last sequence keeps a page that nobody else would. Free pages are given
  * lowest first, in the order of sequences and positions. lack: device [n_layers], the pages that a layer is short of (free
  * ones, or places in a table's row); where any is, nothing is changed in any layer. */
-size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d);   /* of extend and compact; needs no initialisation */
+size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d);   /* of extend and compact, which must not overlap in time where */
+                                                             /* they share one; it needs no initialisation */
 int bkv_pages_extend(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t *refs, const int32_t *len, const int32_t *n_new,
                      int32_t *lack, void *workspace, size_t ws_bytes, hipStream_t stream);
 

@@ -156,6 +156,11 @@ def test_many_sequences_and_long_tables(n):
     want.fork(parent)
     same(seqs, want)
     extend(seqs, [1] * n, want)
+    for parent in ([n - 1] * n, [n - 1] * n, [-1] * (n - 1) + [0]):   # (all from one; nothing new; one is left)
+        seqs.fork(device_ints(parent))
+        want.fork(parent)
+        same(seqs, want)
+        extend(seqs, [2] * n, want)
     before = [a.clone() for a in arrays(cache)]
     seqs.compact()
     same(seqs, want, before, want.compact())

@@ -192,6 +192,64 @@ def test_axes(pairs, order, layout, norm):
         assert bool(((x.double() - y).abs() <= top / 8 * 1.05).all())
 
 
+@pytest.mark.parametrize("n_seq", [63, 64, 65, 200])
+def test_appends_of_many_sequences(n_seq):
+    """Some without tokens, some rows before the first and behind the last sequence: every token's codes and scales are its
+    row's, at its own position, and it reads back as them."""
+    r = np.random.default_rng(n_seq)
+    n = [int(x) for x in r.integers(0, 4, n_seq)]
+    lens = [m + int(x) for m, x in zip(n, r.integers(0, 40, n_seq))]
+    cache, seqs = make(lens, 16, 1, 2, room=64)
+    random_bytes(cache)
+    before = [a.clone() for a in arrays(cache)]
+    t, starts = sum(n) + 5, [x + 2 for x in starts_of(n)]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n_seq)
+    q, k, v = (torch.randn(t, h, 256, device="cuda", generator=g) for h in (2, 1, 1))
+    out = torch.full((t, 2, 256), 4.0, device="cuda")
+    seqs.rope_append(0, q, k, v, NONE, device_ints(starts), q_out=out)
+    end = starts[-1]
+    assert torch.equal(out[2:end], q[2:end]) and bool((out[:2] == 4.0).all()) and bool((out[end:] == 4.0).all())
+    got = seqs.read(0, device_ints(starts), t)
+    want = [a.cpu().numpy().reshape(cache.cap, -1).copy() for a in before]
+    for i, x in enumerate((k, v)):
+        c, d = q4_quantise(x.cpu().numpy()[:, 0])
+        values = q4_values(q4_pack(c), d)
+        assert np.array_equal(got[i][2:end, 0].cpu().numpy(), values[2:end].astype(np.float32))
+        for s in range(n_seq):
+            for j, slot in enumerate(slots(seqs, 0, s, lens[s])[lens[s] - n[s]:]):
+                want[2 * i][slot] = q4_pack(c[starts[s] + j])
+                want[2 * i + 1][slot] = d[starts[s] + j].view(np.uint8)
+    for a, b in zip(arrays(cache), want):
+        assert np.array_equal(a.cpu().numpy().reshape(cache.cap, -1), b)
+
+
+@pytest.mark.parametrize("nkv, grp", [(1, 1), (3, 1), (1, 9), (8, 8), (5, 3)])
+@pytest.mark.parametrize("t", [1, 300])
+def test_any_number_of_rows(nkv, grp, t):
+    """Row counts that do not divide into a workgroup's, with and without norms and queries: Q against the formula, K and V the
+    same bytes with Q beside them or not."""
+    cache, seqs = make([t], 64, nkv, grp)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(nkv)
+    q, k, v = (torch.randn(t, h, 256, device="cuda", generator=g) for h in (nkv * grp, nkv, nkv))
+    qw, kw = (torch.rand(256, device="cuda", generator=g) + 0.5 for _ in range(2))
+    rope, start = Rope(64), device_ints([0, t])
+    for a, b in ((None, None), (qw, kw)):
+        got = seqs.rope_append(0, q, k, v, rope, start, qn_w=a, kn_w=b)
+        want = plain_rope(q, rope, torch.zeros(32, dtype=torch.long, device="cuda"), torch.arange(t, device="cuda")[None], a)
+        assert float((got.double() - want).abs().max()) <= 8 * 2.0 ** -24 * 2 * float(want.abs().max())
+        with_q = seqs.read(0, start, t)
+        bytes_with_q = [x.clone() for x in arrays(cache)]
+        random_bytes(cache)
+        assert seqs.rope_append(0, None, k, v, rope, start, qn_w=a, kn_w=b) is None
+        for x, y in zip(with_q, seqs.read(0, start, t)):
+            assert torch.equal(x, y)
+        for x, y in zip(arrays(cache), bytes_with_q):
+            at = torch.from_numpy(slots(seqs, 0, 0, t)).cuda()
+            assert torch.equal(x[0].view(cache.cap, -1)[at], y[0].view(cache.cap, -1)[at])
+
+
 def test_tokens_without_a_place():
     """Rows of no sequence are left as they are; tokens of negative positions or of missing pages are rotated and not
     written; nothing else in the cache changes."""

@@ -76,6 +76,27 @@ def test_chunk(page, n, length):
     run([length], [n], page, gate=n == 33)
 
 
+def test_many_tiles():
+    """More tiles than pieces of a KV head, and pieces that have the ends of two tiles and whole ones between."""
+    run([1600], [1500], 64, nkv=1, grp=8)
+    run([700, 900, 650, 30], [640, 700, 650, 30], 48, nkv=2, grp=16)
+    run([40] * 90 + [3000], [33] * 90 + [40], 16, nkv=1, grp=4)
+
+
+def test_one_workspace_for_calls_of_all_sizes():
+    """It is as large as the largest call wants, and the calls before leave nothing in it that one after them would take."""
+    cache, seqs = make([2000, 600, 90], 32)
+    fill(cache)
+    seqs.workspace(700)
+    outs = []
+    for n in ([300, 1, 90], [1, 1, 1], [2, 300, 4], [1, 1, 1], [300, 1, 90], [0, 0, 1], [2, 300, 4]):
+        q = queries(sum(n), 16, sum(n))
+        out, _ = seqs.attn(0, q, device_ints(starts_of(n)))
+        check(seqs, q, n, [2000, 600, 90], out)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[4]) and torch.equal(outs[1], outs[3]) and torch.equal(outs[2], outs[6])
+
+
 def test_chunks_and_tokens_together():
     run([700, 3, 1200, 90, 400, 64], [90, 1, 1, 64, 200, 1], 48, gate=True)
 
