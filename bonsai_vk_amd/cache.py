@@ -17,6 +17,7 @@ from ._lib import (BKV_F16, BKV_OP_DECODE, BKV_OP_PREFILL, BKV_OP_TREE, BKV_OUT_
 
 # (private to torch, so not taken for granted)
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 @dataclass
@@ -130,6 +131,7 @@ class KvCache:
 
         self.k_data = alloc(k_fmt, False)
         self._dev = self.k_data.device             # (with its index, unlike self.device)
+        self._index = self.k_data.get_device()     # (compared with a tensor's in a third of a device's time)
         self.k_scales = alloc(k_fmt, True)
         self.v_data = alloc(v_fmt, False)
         self.v_scales = alloc(v_fmt, True)
@@ -170,7 +172,7 @@ class KvCache:
     def _f32(self, t, shape):
         # a tensor that is as the call needs it is taken as it is (as_tensor and contiguous would return
         # it too, 2 us later: a decode makes four such checks per layer)
-        if type(t) is not torch.Tensor or t.dtype is not torch.float32 or t.device != self._dev or not t.is_contiguous():
+        if type(t) is not torch.Tensor or t.dtype is not torch.float32 or t.get_device() != self._index or not t.is_contiguous():
             t = torch.as_tensor(t, dtype=torch.float32, device=self.device).contiguous()
         assert t.shape == shape, (tuple(t.shape), shape)
         return t
@@ -273,18 +275,18 @@ class KvCache:
     # needs it is taken with one look at each of its properties.
     def _elsewhere(self):
         """Whether another device than the cache's is current (its calls then run under torch.cuda.device)."""
-        return torch.cuda.current_device() != self._dev.index
+        return _CURRENT() != self._index
 
     def _my_stream(self):
         """The current stream of the cache's device."""
         if _RAW_STREAM is not None:
-            return _RAW_STREAM(self._dev.index)
+            return _RAW_STREAM(self._index)
         return torch.cuda.current_stream(self._dev).cuda_stream
 
     def _rows(self, t, heads, keep):
         """fp32 [n][heads][hd] on the cache's device as a BkvRows, in place where its rows are whole (element stride 1,
         token and head strides multiples of 4 floats); anything else is copied, and `keep` holds the copy."""
-        if type(t) is torch.Tensor and t.dtype is torch.float32 and t.device == self._dev and t.dim() == 3:
+        if type(t) is torch.Tensor and t.dtype is torch.float32 and t.get_device() == self._index and t.dim() == 3:
             (n, h, d), (tok, head, one), p = t.shape, t.stride(), t.data_ptr()
             if h == heads and d == self.hd and one == 1 and not (tok | head) & 3 and not p & 15:
                 return BkvRows(p, tok, head)
@@ -303,7 +305,7 @@ class KvCache:
             raise ValueError(f"positions are 32 bits, got {pos0}")
 
     def _on_device(self, t, dtype, shape):
-        if t.dtype is not dtype or t.device != self._dev or t.shape != shape or not t.is_contiguous():
+        if t.dtype is not dtype or t.get_device() != self._index or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"a contiguous {dtype} tensor of shape {tuple(shape)} on {self._dev} is wanted, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
         return t

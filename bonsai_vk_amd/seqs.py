@@ -52,6 +52,7 @@ class KvSeqs:
         if not cache.page_tokens and n_seq != 1:
             raise ValueError("a contiguous cache holds one sequence")
         self.cache, self.n_seq, self._dev = cache, n_seq, cache._dev
+        self._per, self._starts = torch.Size((n_seq,)), torch.Size((n_seq + 1,))
         self.len = torch.zeros(n_seq, dtype=torch.int32, device=self._dev)
         self.tables = self.refs = None
         self.desc = BkvCacheDesc()
@@ -71,11 +72,11 @@ class KvSeqs:
             raise ValueError("a contiguous cache has no pages")
 
     def _per_seq(self, t):
-        return self.cache._on_device(t, torch.int32, (self.n_seq,)).data_ptr()
+        return self.cache._on_device(t, torch.int32, self._per).data_ptr()
 
     def _seqs(self, n_tok, q_start, max_q=0):
         if q_start is not None:
-            q_start = self.cache._on_device(q_start, torch.int32, (self.n_seq + 1,)).data_ptr()
+            q_start = self.cache._on_device(q_start, torch.int32, self._starts).data_ptr()
         elif n_tok < self.n_seq:
             raise ValueError(f"a token of each of {self.n_seq} sequences is wanted without q_start, got {n_tok}")
         return BkvSeqs(self.n_seq, n_tok, 1 if q_start is None else max_q, 0, q_start, self._per_seq(self.len),
