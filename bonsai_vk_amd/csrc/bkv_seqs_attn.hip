@@ -80,6 +80,19 @@ __device__ __forceinline__ T arguments_again() {
   return __builtin_bit_cast(T, raw);
 }
 
+// The lines that the kernel's arguments lie in, asked for at once: where each use waits for its own, a launch's first
+// microseconds are such waits one after another.
+template <typename T>
+__device__ __forceinline__ void arguments_near() {
+#ifdef __HIP_DEVICE_COMPILE__
+  const __attribute__((address_space(4))) uint32_t *p = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+  uint32_t x = 0;
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; i += 16) x |= p[i];
+  asm volatile("" ::"s"(x));
+#endif
+}
+
 // ------------------------------------------------------------------ the line of steps
 // inclusive sums over the wave
 __device__ __forceinline__ int wave_sums(int v) {
@@ -183,6 +196,7 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
   __shared__ int32_t s_tab[PG ? 2 * kSeqWaves : 1][64];   // table entries of a wave's steps
   __shared__ float s_m[kSeqWaves][kSeqBlock], s_l[kSeqWaves][kSeqBlock];
   __shared__ int s_last;
+  arguments_near<SeqsAttnArgs>();
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const Q4Bits bits;
   // pieces 8 apart on the same XCD; a piece's KV heads next to one another there, whose scales share lines
@@ -622,6 +636,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   __shared__ float s_m[2][kTileRows], s_l[2][kTileRows];
   __shared__ int s_seq[3][64];                     // rows' beginnings, tokens and lengths of the 64 sequences at hand
   __shared__ int32_t s_tab[PG ? kTileWaves : 1][64];
+  arguments_near<SeqsAttnArgs>();
   const int lane = threadIdx.x & 63, w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = w8 & 3, odd = w8 >> 2, n = lane & 15, g = lane >> 4;
   uint8_t *const sm = all + kFour * odd;
   const Q4Bits bits;
