@@ -1146,8 +1146,9 @@ __global__ __launch_bounds__(64 * kMergeWaves) void seqs_merge_kernel(SeqsAttnAr
 // ------------------------------------------------------------------ host side
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 constexpr int kTileFill = 256;         // pieces of all KV heads: a workgroup a CU
-// rows of a sequence from which on it goes by tiles
-constexpr int kFewRows = 16;
+// A sequence of more rows goes by tiles. 64 rows in blocks of 16 / in a tile: 17 / 37 us at 1000 positions, 39 / 40 at 8000,
+// 53 / 46 at 32000, 16 sequences at 3000 49 / 71; 96 rows 17 / 38, 40 / 42, 61 / 49, 75 / 75.
+constexpr int kFewRows = 64;
 
 SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   SeqsAttnPlan p{};
@@ -1163,7 +1164,7 @@ SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   p.tiles = (int64_t)most * grp > kFewRows;
   p.blocks = !p.tiles || n_seq > 1;
   p.few = !p.tiles ? INT32_MAX : p.blocks ? kFewRows : 0;
-  p.way_in = n_seq > 1 ? kSeqWayIn : 0;
+  p.way_in = n_seq > 1 || (int64_t)most * grp > kSeqBlock ? kSeqWayIn : 0;
   p.tile_lanes = std::max(1, kTileFill / nkv);
   if ((int64_t)n_tok * grp > kFewRows) {           // (whatever max_q says: one workspace for all of a size)
     p.tile_part_rows = p.tile_lanes > 1 ? (uint64_t)2 * p.tile_lanes * nkv * kTileRows : 0;   // (a single piece shares no tile)
