@@ -1146,9 +1146,11 @@ __global__ __launch_bounds__(64 * kMergeWaves) void seqs_merge_kernel(SeqsAttnAr
 // ------------------------------------------------------------------ host side
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 constexpr int kTileFill = 256;         // pieces of all KV heads: a workgroup a CU
-// A sequence of more rows goes by tiles. 64 rows in blocks of 16 / in a tile: 17 / 37 us at 1000 positions, 39 / 40 at 8000,
-// 53 / 46 at 32000, 16 sequences at 3000 49 / 71; 96 rows 17 / 38, 40 / 42, 61 / 49, 75 / 75.
-constexpr int kFewRows = 64;
+// A sequence of more rows goes by tiles, where the call has more than kFewInAll (in fewer, no workgroup has much to do by
+// either, and a block's way in and out is the shorter). One sequence in blocks / in tiles: 128 rows 17 / 39 us at 1000
+// positions, 29 / 44 at 8000, 56 / 51 at 32000; 192 rows 19 / 40, 35 / 54, 80 / 82; 256 rows 20 / 41, 39 / 58, 92 / 84.
+// 16 sequences at 3000: 64 rows each 47 / 71, 96 77 / 78, 128 87 / 79, 192 127 / 97.
+constexpr int kFewRows = 96, kFewInAll = 192;
 
 SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   SeqsAttnPlan p{};
@@ -1161,12 +1163,13 @@ SeqsAttnPlan plan_seqs_attn(int nh, int nkv, int n_seq, int n_tok, int max_q) {
   // Both kernels where there may be sequences of both kinds; of a single one's only the size that it may have is known here,
   // and either kernel takes it whatever it has.
   const int most = max_q > 0 ? std::min(max_q, n_tok) : n_tok;
-  p.tiles = (int64_t)most * grp > kFewRows;
+  const int few = (int64_t)n_tok * grp <= kFewInAll ? kFewInAll : kFewRows;
+  p.tiles = (int64_t)most * grp > few;
   p.blocks = !p.tiles || n_seq > 1;
-  p.few = !p.tiles ? INT32_MAX : p.blocks ? kFewRows : 0;
+  p.few = !p.tiles ? INT32_MAX : p.blocks ? few : 0;
   p.way_in = n_seq > 1 || (int64_t)most * grp > kSeqBlock ? kSeqWayIn : 0;
   p.tile_lanes = std::max(1, kTileFill / nkv);
-  if ((int64_t)n_tok * grp > kFewRows) {           // (whatever max_q says: one workspace for all of a size)
+  if ((int64_t)n_tok * grp > few) {                // (whatever max_q says: one workspace for all of a size)
     p.tile_part_rows = p.tile_lanes > 1 ? (uint64_t)2 * p.tile_lanes * nkv * kTileRows : 0;   // (a single piece shares no tile)
     p.off_info = p.total;
     p.off_tile_ml = up256(p.off_info + (size_t)n_tok * nh * sizeof(uint4));
