@@ -614,6 +614,9 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
 // LDS positions, in 16-byte pieces: K piece c (8 dims) of key k at 32 k + (c ^ k % 16); V piece g of dim d (keys 4 g .. 4 g + 3
 // and 16 + 4 g .. 16 + 4 g + 3) at 4 d + (g ^ vx(d)); both so that 8 neighbouring lanes' reads and writes lie in different banks.
 constexpr int kTileRows = 128, kTileWaves = 8, kTileLeast = 16;
+constexpr int kTileFill = 256;         // pieces of all KV heads: a workgroup a CU
+constexpr int kTileShort = 4;          // steps of a piece of a tile at least, where tiles are cut
+constexpr int kTileWayIn = 8;          // steps that a tile's way in and out takes as long as
 __device__ __forceinline__ uint32_t v_piece(int d, int g) { return (uint32_t)(64 * d + 16 * (g ^ (((d >> 1) ^ (d >> 3)) & 3))); }
 
 // tiles of a sequence, and steps of tile rb: up to its last row's last key (one at least)
@@ -634,6 +637,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   constexpr uint32_t oVop = 2 * kOp, oRaw = 4 * kOp, kRawV = 1024, kRawKS = 2048, kRawVS = 2176, kRaw = 2304, kFour = oRaw + 4 * kRaw;
   __shared__ __attribute__((aligned(128))) uint8_t all[2 * kFour];   // (of each four waves)
   __shared__ float s_m[2][kTileRows], s_l[2][kTileRows];
+  __shared__ int s_tile[kTileFill], s_steps[kTileFill];   // of up to as many tiles as pieces: sequence and number in it; steps
   __shared__ int s_seq[3][64];                     // rows' beginnings, tokens and lengths of the 64 sequences at hand
   __shared__ int32_t s_tab[PG ? kTileWaves : 1][64];
   arguments_near<SeqsAttnArgs>();
@@ -656,58 +660,135 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       for (int rb = 0; rb < t.count(); ++rb) sum += t.steps(a.by_grp, rb);
     return sum;
   };
+  auto tiles_of = [&](const SeqLanes &s) { return s.nt * a.grp > a.few ? Tiles{s.nt, s.len, a.grp}.count() : 0; };
   SeqLanes my(a, 0);
-  int mine_line = line_of(my), inc = wave_sums(mine_line), total = of_lane(inc, 63);
+  int mine_line = line_of(my), inc = wave_sums(mine_line), total = of_lane(inc, 63), n_tiles = of_lane(wave_sums(tiles_of(my)), 63);
   bool bad = my.bad;
   for (int s0 = 64; s0 < a.v.n_seq; s0 += 64) {
     const SeqLanes more(a, s0);
     total += of_lane(wave_sums(line_of(more)), 63);
+    n_tiles += of_lane(wave_sums(tiles_of(more)), 63);
     bad |= more.bad;
   }
   if (bad || total == 0) return;
   const Cut cut(total, a.tile_lanes, a.by_tile_lanes, kTileLeast);
   // an XCD has neighbouring pieces: those of one tile read the same rows of Q, each of which comes to its L2 once
-  const int rounds = (cut.nl + 7) / 8, piece = rounds * (int)(blockIdx.x & 7) + round;
-  if (round >= rounds || piece >= cut.nl) return;
-  // A piece that would begin or end a little inside a tile begins or ends at the tile's own end: its rows' way in and out costs
+  int piece = 0;
+  auto none = [&](int nl) {
+    const int rounds = (nl + 7) / 8;
+    piece = rounds * (int)(blockIdx.x & 7) + round;
+    return round >= rounds || piece >= nl;
+  };
+  int at = 0, end = 0, s0 = 0, in64 = 0, line0 = 0, rb = 0;   // the sequence and tile that `at` lies in, and where that begins
+  // ---- Where there are no more tiles than pieces: each tile cut into equal pieces, the longest of which are as short as their
+  // number allows, so that a piece has one way in and out. (Unless the longest have more than another way in and out over an
+  // equal share.)
+  int parts = 0;                                   // of the tile, 0: the line is cut
+  if (n_tiles <= a.tile_lanes) {
+    if (w8 == 0) {
+      int before = 0;
+      for (int q = 0; q < a.v.n_seq; q += 64) {
+        const SeqLanes s(a, q);
+        const Tiles t{s.nt, s.len, a.grp};
+        const int c = tiles_of(s), c_inc = wave_sums(c);
+        for (int i = 0; i < c; ++i) {
+          s_tile[before + c_inc - c + i] = (q + lane) << 8 | i;
+          s_steps[before + c_inc - c + i] = t.steps(a.by_grp, i);
+        }
+        before += of_lane(c_inc, 63);
+      }
+    }
+    lds_barrier();
+    constexpr int NC = kTileFill / 64;
+    int st[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) st[j] = 64 * j + lane < n_tiles ? s_steps[64 * j + lane] : 0;
+    // pieces of x steps of s at most (s is no less than an equal share: the quotient is small, and its error less than 1)
+    auto pieces_of = [&](int x, int s) {
+      const int y = x + s - 1;
+      int n = (int)((float)y * (1.0f / (float)s));
+      n += (n + 1) * s <= y ? 1 : 0;
+      return n - (n * s > y ? 1 : 0);
+    };
+    auto in_all = [&](int s) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) n += pieces_of(st[j], s);
+      return of_lane(wave_sums(n), 63);
+    };
+    int lo = max(kTileShort, (int)((uint32_t)(total + a.tile_lanes - 1) / (uint32_t)a.tile_lanes)), hi = lo + kTileWayIn;
+    if (in_all(hi) <= a.tile_lanes) {
+      while (lo < hi) {                            // (the least that is enough: hi always is)
+        const int mid = (lo + hi) / 2;
+        if (in_all(mid) <= a.tile_lanes) hi = mid;
+        else lo = mid + 1;
+      }
+      if (none(in_all(hi))) return;
+      int before = 0, tile = 0, steps = 0;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int k = pieces_of(st[j], hi), k_inc = wave_sums(k);
+        const uint64_t past = __ballot(before + k_inc > piece);
+        if (parts == 0 && past) {
+          const int l = __ffsll((unsigned long long)past) - 1;
+          tile = 64 * j + l;
+          steps = of_lane(st[j], l);
+          parts = of_lane(k, l);
+          at = piece - (before + of_lane(k_inc - k, l));
+        }
+        before += of_lane(k_inc, 63);
+      }
+      const int each = steps / parts, longer = steps - each * parts, part = at;
+      at = part * each + min(part, longer);
+      end = at + each + (part < longer ? 1 : 0);
+      const int where = __builtin_amdgcn_readfirstlane(s_tile[tile]);
+      rb = where & 255;
+      in64 = (where >> 8) & 63;
+      s0 = (where >> 8) - in64;
+      if (s0) my = SeqLanes(a, s0);
+    }
+  }
+  // A piece of the line that would begin or end a little inside a tile begins or ends at the tile's own end: its rows' way in and out costs
   // as much as near steps (15 sequences with chunks among them: 92 us; with an eighth of a piece 101).
-  const int near = min(cut.share / 4, 8);
+  const int near = parts ? -1 : min(cut.share / 4, 8);
   auto last_piece = [&](int begin, int steps) {    // of a tile
     const int p = cut.piece_of(begin + steps - 1), b = cut.begin(p);
     return b > begin && b - begin > near && begin + steps - b <= near ? p - 1 : p;
   };
-  int at = cut.begin(piece), end = cut.begin(piece + 1);
-  int s0 = 0, in64 = 0, line0 = 0;                 // the sequence that `at` lies in, and where that begins
-  for (;;) {
-    const uint64_t past = __ballot(line0 + inc > at);
-    if (past) {
-      in64 = __ffsll((unsigned long long)past) - 1;
-      line0 += of_lane(inc - mine_line, in64);
-      break;
-    }
-    line0 += of_lane(inc, 63);
-    s0 += 64;
-    if (s0 >= a.v.n_seq) return;
-    my = SeqLanes(a, s0);
-    mine_line = line_of(my);
-    inc = wave_sums(mine_line);
-  }
-  // the tile of that sequence: 64 at a time
-  int rb = 0;
-  {
-    const Tiles t{of_lane(my.nt, in64), of_lane(my.len, in64), a.grp};
+  if (!parts) {
+    if (none(cut.nl)) return;
+    at = cut.begin(piece);
+    end = cut.begin(piece + 1);
     for (;;) {
-      const int i = rb + lane, st = i < t.count() ? t.steps(a.by_grp, i) : 0, tinc = wave_sums(st);
-      const uint64_t past = __ballot(line0 + tinc > at);
+      const uint64_t past = __ballot(line0 + inc > at);
       if (past) {
-        const int l = __ffsll((unsigned long long)past) - 1;
-        line0 += of_lane(tinc - st, l);
-        rb += l;
+        in64 = __ffsll((unsigned long long)past) - 1;
+        line0 += of_lane(inc - mine_line, in64);
         break;
       }
-      line0 += of_lane(tinc, 63);
-      rb += 64;
-      if (rb >= t.count()) return;
+      line0 += of_lane(inc, 63);
+      s0 += 64;
+      if (s0 >= a.v.n_seq) return;
+      my = SeqLanes(a, s0);
+      mine_line = line_of(my);
+      inc = wave_sums(mine_line);
+    }
+    // the tile of that sequence: 64 at a time
+    {
+      const Tiles t{of_lane(my.nt, in64), of_lane(my.len, in64), a.grp};
+      for (;;) {
+        const int i = rb + lane, st = i < t.count() ? t.steps(a.by_grp, i) : 0, tinc = wave_sums(st);
+        const uint64_t past = __ballot(line0 + tinc > at);
+        if (past) {
+          const int l = __ffsll((unsigned long long)past) - 1;
+          line0 += of_lane(tinc - st, l);
+          rb += l;
+          break;
+        }
+        line0 += of_lane(tinc, 63);
+        rb += 64;
+        if (rb >= t.count()) return;
+      }
     }
   }
   bool first = true;
@@ -1031,7 +1112,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
         const uint32_t part = part0 + 16 * mt + n;
         const float sum = by[mt], div = !alone ? 1.0f : sum > 0.0f || sum != sum ? sum : 1.0f;
         if (D0 == 0 && r < R && g == 0) {
-          if (t0 == 0) z.info[dst] = make_uint4(part, 2u * (uint32_t)z.nkv * kTileRows, (uint32_t)(alone ? 1 : last_piece(line0, steps) - piece + 1), 0);
+          if (t0 == 0) z.info[dst] = make_uint4(part, 2u * (uint32_t)z.nkv * kTileRows, (uint32_t)(alone ? 1 : parts ? parts : last_piece(line0, steps) - piece + 1), 0);
           if (!alone) z.tile_ml[part] = make_float2(m[mt], sum);
         }
         // lanes n and n ^ 1 exchange halves of two products, so that a store reaches 8 rows' whole lines
@@ -1145,7 +1226,6 @@ __global__ __launch_bounds__(64 * kMergeWaves) void seqs_merge_kernel(SeqsAttnAr
 
 // ------------------------------------------------------------------ host side
 static inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
-constexpr int kTileFill = 256;         // pieces of all KV heads: a workgroup a CU
 // A sequence of more rows goes by tiles, where the call has more than kFewInAll (in fewer, no workgroup has much to do by
 // either, and a block's way in and out is the shorter). One sequence in blocks / in tiles: 128 rows 17 / 39 us at 1000
 // positions, 29 / 44 at 8000, 56 / 51 at 32000; 192 rows 19 / 40, 35 / 54, 80 / 82; 256 rows 20 / 41, 39 / 58, 92 / 84.
