@@ -23,7 +23,8 @@ __device__ __forceinline__ int64_t table_at(const PagesArgs &a, int s, int layer
 // ------------------------------------------------------------------ fork
 // A workgroup has 8 columns of one layer's table in LDS, every sequence's: all are read before any is written. How many rows
 // come to name a sequence's page is counted in LDS and added to the page's count at once (200 samples of one prompt: an addition
-// a page, not 200), whole numbers by atomics, whose order does not show.
+// a page, not 200), whole numbers by atomics, whose order does not show. Three trips to memory one after another: 3.5 us for 8
+// sequences of 33 pages in 8 layers, 5.6 for 200 (14 where each row adds its own change).
 __global__ __launch_bounds__(256) void pages_fork_kernel(PagesArgs a) {
   // [n_seq][kForkCols] entries; rows that come to name each, two columns' in 16 bits each (1024 at most); the parents
   extern __shared__ int32_t s_tab[];
@@ -161,7 +162,8 @@ __device__ __forceinline__ void atomics_barrier() {
 
 // One workgroup a layer decides. L lanes take a sequence, as many as the most pages that one of them needs (64 at most): all
 // sequences of a step of single tokens at once. What the time goes to is trips to memory one after another; what a lane has read
-// of its first page (most often its only one) it keeps.
+// of its first page (most often its only one) it keeps. 7.5 us for 8 sequences in 8 layers, 10.2 for 200 (a wave a sequence,
+// nothing kept: 14.8 and 58.7).
 __global__ __launch_bounds__(kPlanThreads) void pages_extend_plan_kernel(PagesArgs a) {
   __shared__ int s_p0[BKV_SEQS_MAX], s_n[BKV_SEQS_MAX], s_len[BKV_SEQS_MAX], s_cnt[BKV_SEQS_MAX], s_scan[kPlanThreads / 64], s_over, s_most, s_any;
   const int layer = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
@@ -278,7 +280,8 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_plan_kernel(PagesAr
   });
 }
 
-// The k-th fresh page takes its table entry and what is held of the one before it.
+// The k-th fresh page takes its table entry and what is held of the one before it. 5.0 us for 56 pages, 7.6 for 1592 of 9 KB each
+// (24.5 where a workgroup goes through the arrays' pieces one by one, the empty ones too).
 template <class T>
 __global__ __launch_bounds__(256) void pages_extend_apply_kernel(PagesArgs a, int pieces) {
   const int layer = blockIdx.y;
@@ -317,7 +320,8 @@ hipError_t launch_pages_extend(const PagesArgs &a, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------ compact
-// U pages are used: the i-th used one from U on moves to the i-th free one below U. One workgroup a layer lists them.
+// U pages are used: the i-th used one from U on moves to the i-th free one below U. One workgroup a layer lists them: 5.1 us for
+// 77 pages, 6.7 for 2000.
 __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PagesArgs a) {
   __shared__ long long s_scan[kPlanThreads / 64];
   const int layer = blockIdx.x, tid = threadIdx.x;
@@ -366,6 +370,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PagesA
   for (int p = U + tid; p < a.pool_pages; p += kPlanThreads) out[p] = 0;
 }
 
+// Bound by memory: 449 pages of 74 KB in each of 8 layers, 539 MB, in 117 us (4.6 TB/s; a large copy has 4.9).
 template <class T>
 __global__ __launch_bounds__(256) void pages_compact_apply_kernel(PagesArgs a, int pieces) {
   const int layer = blockIdx.y;

@@ -85,7 +85,8 @@ __device__ __forceinline__ double rsqrt_f64(double x) {
 
 // What bounds it: 40 KB a token in and out of 16 Q and 8 KV rows, and nearly as much the vector unit, in rows that are normed. So
 // the four rows of a wave share a norm's reduction and root, a lane has its cosines and sines in registers for all its rows,
-// and the small loads, which wait for one another, are asked for before the rows.
+// and the small loads, which wait for one another, are asked for before the rows. One token 4.4 us (two trips to memory and the
+// sines), 1201 of a picture without norms 12.5 (3.8 TB/s), 1100 with norms 14.1.
 template <int KF, int VF>
 __global__ __launch_bounds__(256) void seqs_rope_append_kernel(SeqsRowArgs a) {
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);

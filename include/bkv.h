@@ -406,7 +406,7 @@ int bkv_seqs_read(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, int 
  *   nothing gets 0. Positions that a row does not see have no effect on it.
  *   out: [n_tok][nh][hd]; gate (or NULL) with out_gated: out_gated = out * 1/(1+exp(-gate)). Neither may overlap the inputs
  *   or the other.
- * Workspace: bkv_seqs_workspace_bytes(d, n_seq, n_tok), which grows with both, made ready by bkv_workspace_init once and
+ * Workspace: bkv_seqs_workspace_bytes(d, n_seq, n_tok), no less for more of either, made ready by bkv_workspace_init once and
  * written by nothing else from then on; it serves calls of any sizes that it is large enough for. Calls (and replays of
  * captured ones) that share one must not overlap in time. */
 size_t bkv_seqs_workspace_bytes(const bkv_cache_desc *d, int n_seq, int n_tok);
