@@ -306,12 +306,12 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
         load_to_lds_at<0>(kd + slot[0] * krow + kcol, dst);
         load_to_lds_at<1024>(kd + slot[1] * krow + kcol, dst);
         load_to_lds_at<2048>(kd + slot[2] * krow + kcol, dst);
-        load_to_lds_at<3072>(kd + slot[3] * krow + kcol, dst);
+        load_to_lds_at<3 * 1024>(kd + slot[3] * krow + kcol, dst);
         load_to_lds_at<oKS>(scales + (size_t)max(sl, 0) * srow, dst);
         load_to_lds_at<oV>(vd + slot[0] * krow + vcol, dst);
         load_to_lds_at<oV + 1024>(vd + slot[1] * krow + vcol, dst);
         load_to_lds_at<oV + 2048>(vd + slot[2] * krow + vcol, dst);
-        load_to_lds_at<oV + 3072>(vd + slot[3] * krow + vcol, dst);
+        load_to_lds_at<oV + 3 * 1024>(vd + slot[3] * krow + vcol, dst);
       } else {
         uint32_t base = kb;
         if constexpr (PG == 1) {
@@ -329,12 +329,12 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
         load_to_lds_at<0>(kp, at[0] * krow + kcol, dst);
         load_to_lds_at<1024>(kp, at[1] * krow + kcol, dst);
         load_to_lds_at<2048>(kp, at[2] * krow + kcol, dst);
-        load_to_lds_at<3072>(kp, at[3] * krow + kcol, dst);
+        load_to_lds_at<3 * 1024>(kp, at[3] * krow + kcol, dst);
         load_to_lds_at<oKS>(scales + (uint64_t)(base + sk) * srow, dst);
         load_to_lds_at<oV>(vp, at[0] * krow + vcol, dst);
         load_to_lds_at<oV + 1024>(vp, at[1] * krow + vcol, dst);
         load_to_lds_at<oV + 2048>(vp, at[2] * krow + vcol, dst);
-        load_to_lds_at<oV + 3072>(vp, at[3] * krow + vcol, dst);
+        load_to_lds_at<oV + 3 * 1024>(vp, at[3] * krow + vcol, dst);
       }
     };
     // ---- the block's rows of Q, two by each wave, whole rows at a time (a lane's pieces of a row would ask for each line
