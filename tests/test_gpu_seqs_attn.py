@@ -81,6 +81,17 @@ def test_many_tiles():
     run([1600], [1500], 64, nkv=1, grp=8)
     run([700, 900, 650, 30], [640, 700, 650, 30], 48, nkv=2, grp=16)
     run([40] * 90 + [3000], [33] * 90 + [40], 16, nkv=1, grp=4)
+    run([40] * 90 + [3000], [33] * 90 + [40], 16, nkv=4, grp=4)
+
+
+def test_tiles_that_equal_pieces_would_share_out_badly():
+    """5 x 8 tiles of a KV head for 64 pieces: whole ones would be twice as long as an equal share; 33 of which one is long."""
+    run([4000] * 5, [256] * 5, 64)
+    run([150] * 32 + [6000], [33] * 33, 48)
+
+
+def test_blocks_of_several_rows_and_tiles_of_more_than_64_sequences():
+    run([300] * 40 + [90] * 40, [1] * 20 + [9, 20, 24, 25] * 10 + [3] * 20, 32, nkv=2, grp=4)
 
 
 def test_one_workspace_for_calls_of_all_sizes():
