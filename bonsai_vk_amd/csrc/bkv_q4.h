@@ -78,7 +78,7 @@ struct SeqsView {
 
   __device__ __forceinline__ int q_begin(int s) const { return min(max(q_start ? q_start[s] : s, 0), n_tok); }
   __device__ __forceinline__ int tokens(int s) const { return max(q_begin(s + 1) - q_begin(s), 0); }
-  __device__ __forceinline__ int length(int s) const { return (int)min((int64_t)max(len[s], 0), max_pos); }
+  __device__ __forceinline__ int length(int s) const { return max(len[s], 0); }   // (it may be past max_pos: those tokens are not there)
   // the slot of a position (0 <= pos < max_pos), -1 where its page is not in the pool
   __device__ __forceinline__ int slot(int s, uint32_t pos) const {
     if (page == 0) return (int)pos;

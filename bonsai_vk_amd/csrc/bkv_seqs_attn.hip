@@ -1,9 +1,10 @@
 // bkv_seqs_attn.hip - attention of the tokens of several sequences over a 4-bit cache (bkv_seqs_attn).
 //
 // The rows of one KV head and sequence are its n * grp (token, query head) pairs; the row of token i sees the keys below
-// len - n + i + 1. With s = q16 . k and x = s * scale * log2(e): out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m) over the
-// visible j, for any m near the largest x_j. One pass over the keys: every wave keeps a reference m, a sum and 256
-// unnormalised outputs per row, and lifts m only when a row's score exceeds it by kLift.
+// len - n + i + 1 that the cache has room for (len may be past that). With s = q16 . k and x = s * scale * log2(e):
+// out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m) over the visible j, for any m near the largest x_j. One pass over the
+// keys: every wave keeps a reference m, a sum and 256 unnormalised outputs per row, and lifts m only when a row's score
+// exceeds it by kLift.
 //
 // Products on the fp16 matrix cores, summed in fp32: q and k are exact operands (bkv_q4.h), v too, and
 // 2^(x - m) * 2^9 = ph + pl, two fp16 (22 bits; the factor keeps pl normal down to p = 2^-14 of the largest). One product
@@ -31,6 +32,8 @@ constexpr int kSeqBlock = 16;          // rows of a row block
 constexpr int kSeqLeast = 8;           // steps of a piece at least
 
 __device__ __forceinline__ int cdiv_d(int a, int b) { return (a + b - 1) / b; }
+// the positions of a sequence that there are bytes of
+__device__ __forceinline__ int keys_of(const SeqsAttnArgs &a, int len) { return min(len, (int)a.v.max_pos); }
 
 // 4 h2 (8 elements in order) of a word of codes: 0x4C00 | q << 6 is the fp16 number 16 + q, and (16 + q + 8 - 24) * d, in one
 // fused step, is exact: both 24 d and the result have 11 bits at most.
@@ -123,7 +126,7 @@ struct SeqLanes {
     len = a.v.length(in);
     q0 = min(max(q0, 0), a.v.n_tok);
     nt = s < a.v.n_seq ? max(min(max(e, 0), a.v.n_tok) - q0, 0) : 0;
-    steps = max(1, (int)((uint32_t)(len + kSeqKeys - 1) / kSeqKeys));
+    steps = max(1, (int)((uint32_t)(keys_of(a, len) + kSeqKeys - 1) / kSeqKeys));
     blocks = (int)((uint32_t)(nt * a.grp + kSeqBlock - 1) / kSeqBlock);
   }
   // (of the sequences of few rows)
@@ -268,14 +271,14 @@ __global__ __launch_bounds__(64 * kSeqWaves, 2) void seqs_attn_kernel(SeqsAttnAr
     at += x1 - x0;
     if (m4 == 0) continue;
     const int t0 = st0 + (int)((uint32_t)(m4 * w) / kSeqWaves), t1 = st0 + (int)((uint32_t)(m4 * (w + 1)) / kSeqWaves);
-    const int last = max(len - 1, 0);              // (the last key that there are bytes of)
+    const int last = max(keys_of(a, len) - 1, 0), before = len - nt;   // (the last key that there are bytes of; none: len - nt + tok < 0)
     // Blocks of 8 rows or fewer: columns n and n + 8 of the products are the same row, and one product of the outputs takes ph in
     // the one and pl in the other, whose sum the join forms
     const int r0 = kSeqBlock * rb, real = min(R - r0, kSeqBlock);
     const bool halves = real <= kSeqBlock / 2;
     const int col = halves ? n & 7 : n, row = min(r0 + col, R - 1), tok = a.by_grp.div(row);
-    const int lim = len - nt + tok + 1;            // keys below it are seen
-    const int lim_all = len - nt + a.by_grp.div(r0) + 1;   // by all rows of the block
+    const int lim = min(before + tok, last) + 1;   // keys below it are seen
+    const int lim_all = min(before + a.by_grp.div(r0), last) + 1;   // by all rows of the block
 
     // ---- a step's bytes on their way: 9 loads straight into LDS, and before them, in pages, the next step's table entries (a
     // load into a register would be waited for with everything that is on its way)
@@ -631,11 +634,11 @@ __device__ __forceinline__ uint32_t v_piece(int d, int g) { return (uint32_t)(64
 
 // tiles of a sequence, and steps of tile rb: up to its last row's last key (one at least)
 struct Tiles {
-  int nt, len, grp;
+  int nt, len, grp, most;                          // most: positions that the cache has room for
   __device__ __forceinline__ int count() const { return (int)((uint32_t)(nt * grp + kTileRows - 1) / kTileRows); }
   __device__ __forceinline__ int steps(const ByConst &by_grp, int rb) const {
     const int toks = min(nt, by_grp.div((uint32_t)(kTileRows * (rb + 1) + grp - 1)));
-    return (int)((uint32_t)(max(len - nt + toks, 1) + kSeqKeys - 1) / kSeqKeys);
+    return (int)((uint32_t)(min(max(len - nt + toks, 1), most) + kSeqKeys - 1) / kSeqKeys);
   }
 };
 
@@ -664,13 +667,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   const int at8 = (int)(blockIdx.x >> 3), round = a.by_nkv.div(at8), hk = at8 - round * a.nkv;
   // ---- the line: all tiles' steps, 64 sequences at a time
   auto line_of = [&](const SeqLanes &s) {
-    const Tiles t{s.nt, s.len, a.grp};
+    const Tiles t{s.nt, s.len, a.grp, (int)a.v.max_pos};
     int sum = 0;
     if (s.nt * a.grp > a.few)
       for (int rb = 0; rb < t.count(); ++rb) sum += t.steps(a.by_grp, rb);
     return sum;
   };
-  auto tiles_of = [&](const SeqLanes &s) { return s.nt * a.grp > a.few ? Tiles{s.nt, s.len, a.grp}.count() : 0; };
+  auto tiles_of = [&](const SeqLanes &s) { return s.nt * a.grp > a.few ? Tiles{s.nt, s.len, a.grp, (int)a.v.max_pos}.count() : 0; };
   SeqLanes my(a, 0);
   int mine_line = line_of(my), inc = wave_sums(mine_line), total = of_lane(inc, 63), n_tiles = of_lane(wave_sums(tiles_of(my)), 63);
   bool bad = my.bad;
@@ -699,7 +702,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
       int before = 0;
       for (int q = 0; q < a.v.n_seq; q += 64) {
         const SeqLanes s(a, q);
-        const Tiles t{s.nt, s.len, a.grp};
+        const Tiles t{s.nt, s.len, a.grp, (int)a.v.max_pos};
         const int c = tiles_of(s), c_inc = wave_sums(c);
         for (int i = 0; i < c; ++i) {
           s_tile[before + c_inc - c + i] = (q + lane) << 8 | i;
@@ -785,7 +788,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     }
     // the tile of that sequence: 64 at a time
     {
-      const Tiles t{of_lane(my.nt, in64), of_lane(my.len, in64), a.grp};
+      const Tiles t{of_lane(my.nt, in64), of_lane(my.len, in64), a.grp, (int)a.v.max_pos};
       for (;;) {
         const int i = rb + lane, st = i < t.count() ? t.steps(a.by_grp, i) : 0, tinc = wave_sums(st);
         const uint64_t past = __ballot(line0 + tinc > at);
@@ -826,7 +829,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
   while (at < end) {
     // ---- the piece's part of one tile
     const int q0 = __builtin_amdgcn_readfirstlane(s_seq[0][in64]), nt = __builtin_amdgcn_readfirstlane(s_seq[1][in64]), len = __builtin_amdgcn_readfirstlane(s_seq[2][in64]), seq = s0 + in64;
-    const Tiles tiles{nt, len, a.grp};
+    const Tiles tiles{nt, len, a.grp, (int)a.v.max_pos};
     if (nt * a.grp <= a.few || rb == tiles.count()) {   // the next sequence
       rb = 0;
       if (++in64 == 64) {
@@ -854,11 +857,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void seqs_tile_kernel(SeqsAttnA
     }
     if (stop <= at) break;                         // (what is left of it is the next piece's)
     const int t0 = __builtin_amdgcn_readfirstlane(at - line0), t1 = __builtin_amdgcn_readfirstlane(min(steps, t0 + (stop - at)));
-    const int last = max(len - 1, 0), r0 = kTileRows * rb, rw = r0 + 32 * w;
+    const int last = max(keys_of(a, len) - 1, 0), before = len - nt, r0 = kTileRows * rb, rw = r0 + 32 * w;
     const bool works = rw < R;                     // (a wave whose rows are all past the last only brings bytes)
     // keys below lim are seen: by a row of the lane's, by all of the wave's, by any
-    auto lim_of = [&](int mt) { return len - nt + a.by_grp.div((uint32_t)min(rw + 16 * mt + (my_lane() & 15), R - 1)) + 1; };
-    const int lim_all = len - nt + a.by_grp.div((uint32_t)min(rw, R - 1)) + 1, lim_any = len - nt + a.by_grp.div((uint32_t)min(rw + 31, R - 1)) + 1;
+    auto lim_of = [&](int mt) { return min(before + a.by_grp.div((uint32_t)min(rw + 16 * mt + (my_lane() & 15), R - 1)), last) + 1; };
+    const int lim_all = min(before + a.by_grp.div((uint32_t)min(rw, R - 1)), last) + 1, lim_any = min(before + a.by_grp.div((uint32_t)min(rw + 31, R - 1)), last) + 1;
 
     // ---- bytes on their way: the wave's own, of step t
     uint32_t there = ~0u, there_next = ~0u;        // keys whose pages are in the pool: this step's, the next's

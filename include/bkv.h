@@ -369,7 +369,8 @@ typedef struct bkv_seqs {
   int32_t reserved;           /* 0                                                                       */
   const int32_t *q_start;     /* device [n_seq+1], ascending, 0 .. n_tok (where it goes back, nothing    */
                               /* is said of the outputs); NULL: one token each, s = row                  */
-  const int32_t *len;         /* device [n_seq], this call's tokens among them                           */
+  const int32_t *len;         /* device [n_seq], this call's tokens among them; it may be past what the  */
+                              /* cache holds (the tokens past it are then not there)                     */
   const int32_t *tables;      /* device [n_seq][n_layers][max_pages], in the place of the descriptor's   */
                               /* block table (paged); NULL for a contiguous cache, n_seq <= 1            */
 } bkv_seqs;
