@@ -64,7 +64,7 @@ class KvSeqs:
             need = lib().bkv_pages_workspace_bytes(ctypes.byref(self.desc))
             self._pws = torch.empty(need, dtype=torch.uint8, device=self._dev)
             self._pws_bytes = need
-        self._ws, self._ws_bytes = None, 0
+        self._ws, self._ws_bytes, self._held = None, 0, []
 
     # ---------------------------------------------------------------- helpers
     def _paged(self):
@@ -84,14 +84,18 @@ class KvSeqs:
 
     def workspace(self, n_tok):
         """The workspace of attn for n_tok rows, made where the one there is smaller; a program that captures that call into a
-        graph asks for it before. All of this object's attn calls share it: they run one after another, on one stream or on
-        streams that wait for one another."""
+        graph asks for it before. All of this object's attn calls (and replays) share it: they run one after another, on one
+        stream or on streams that wait for one another. One that was ever handed out lives as long as this object: captured
+        calls have its address, and a stream may still be at work in it."""
         need = lib().bkv_seqs_workspace_bytes(self.desc, self.n_seq, n_tok) if n_tok else 0
         if need > self._ws_bytes:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call workspace(n_tok) before the capture: memory of a graph's own pool would not outlive it")
-            self._ws, self._ws_bytes = torch.empty(need, dtype=torch.uint8, device=self._dev), need
-            check(lib().bkv_workspace_init(self.desc, self._ws.data_ptr(), need, self.cache._my_stream()), "bkv_workspace_init")
+            need = max(need, 2 * self._ws_bytes)   # (all that were outgrown together are no larger than the one there)
+            ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+            check(lib().bkv_workspace_init(self.desc, ws.data_ptr(), need, self.cache._my_stream()), "bkv_workspace_init")
+            self._held.append(ws)
+            self._ws, self._ws_bytes = ws, need
         return self._ws
 
     # ---------------------------------------------------------------- pages
