@@ -4,10 +4,15 @@
 
 A step of a server, everything on the device and nothing read back:
 
-    seqs.extend(n_new)                       # pages for the new tokens, copied where others share them
-    seqs.len += n_new
+    lack = seqs.extend(n_new)                # pages for the new tokens, copied where others share them
+    have = (lack == 0).all()                 # else nothing was changed, and the step must not happen:
+    seqs.len += n_new * have                 # no sequence gets longer,
+    q_start = starts * have                  # none has rows in this call
     q = seqs.rope_append(layer, q, k, v, rope, q_start, positions, axes)
     out, gated = seqs.attn(layer, q, q_start, gate)
+
+Without `have`, a pool that is exhausted would leave sequences that share a page all writing their new tokens into it. Whoever
+takes the step's results reads `have` with them; a server then gives up a sequence (fork) and takes the step again.
 """
 import ctypes
 
@@ -113,7 +118,9 @@ class KvSeqs:
 
     def extend(self, n_new, lack=None):
         """bkv_pages_extend: pages for n_new[s] (int32 [n_seq] on the cache's device) more positions than len[s]. Returns lack,
-        int32 [n_layers] on the device: the pages that each layer is short of; where any is, nothing was changed."""
+        int32 [n_layers] on the device: the pages that each layer is short of; where any is, nothing was changed, and the new
+        positions must not be written (a page there may still be several sequences'): len stays, and no sequence has rows in
+        the step's calls (a q_start of 0s)."""
         if self.cache._elsewhere():
             with torch.cuda.device(self._dev):
                 return self.extend(n_new, lack)

@@ -428,7 +428,9 @@ int bkv_pages_fork(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t 
  * the sequence's own. Where there is none it gets a free one; where others have it too, it gets a free one with the
  * positions below len[s] copied, but the last sequence keeps a page that nobody else would. Free pages are given
  * lowest first, in the order of sequences and positions. lack: device [n_layers], the pages that a layer is short of (free
- * ones, or places in a table's row); where any is, nothing is changed in any layer. */
+ * ones, or places in a table's row); where any is, nothing is changed in any layer. The new positions must then not be
+ * written, since a page there may still be several sequences': len stays as it is and the step's calls get a q_start of 0s (no
+ * sequence takes part), both of which a kernel of the caller's can see to, so that nothing is read back. */
 size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d);   /* of extend and compact, which must not overlap in time where */
                                                              /* they share one; it needs no initialisation */
 int bkv_pages_extend(const bkv_cache_desc *d, int n_seq, int32_t *tables, int32_t *refs, const int32_t *len, const int32_t *n_new,
