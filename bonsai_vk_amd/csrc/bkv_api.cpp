@@ -1273,10 +1273,10 @@ int bkv_kv_fill_synthetic(const bkv_cache_desc *d, hipStream_t stream) {
   if (rc) return rc;
   void *bases[4] = {d->k_data, d->k_scales, d->v_data, d->v_scales};
   for (int i = 0; i < 4; ++i) {
-    if (!bases[i]) continue;
+    const size_t bytes = (size_t)d->cap * slot_bytes(d, i);   // (0: the format has no such array)
+    if (!bytes) continue;
     for (int l = 0; l < d->n_layers; ++l) {
       unsigned *p = (unsigned *)((char *)bases[i] + (uint64_t)l * d->layer_stride_bytes[i]);
-      const size_t bytes = (size_t)d->cap * (i & 1 ? (size_t)d->nkv * kScaleRowBytes : slot_bytes(d, i));
       const hipError_t e = launch_fill_words(p, bytes / 4, 0x3C003C00u, stream);
       if (e != hipSuccess) return hip_fail(e);
     }
