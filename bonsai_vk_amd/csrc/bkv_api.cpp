@@ -1113,11 +1113,13 @@ static PagesArgs pages_args(const bkv_cache_desc *d, int n_seq) {
   a.max_pages = d->max_pages;
   return a;
 }
-// a page's pieces are counted in 31 bits
+// The chunks of a page, all its arrays' one after another, are counted in 32 bits, and a workgroup's next piece is up to
+// kPagePieces of kPagePiece of them further on: up to 2^31 chunks (32 GiB where positions go by 16 bytes, else 8).
+static_assert((uint64_t)kPagePieces * kPagePiece + kPagePiece <= uint64_t(1) << 31, "a page's chunks and the step behind them in 32 bits");
 static bool page_too_large(const bkv_cache_desc *d) {
-  uint64_t most = 0;
-  for (int i = 0; i < 4; ++i) most = std::max<uint64_t>(most, slot_bytes(d, i) * (uint64_t)d->page_tokens);
-  return most > (uint64_t(1) << 40);
+  __int128 bytes = 0;
+  for (int i = 0; i < 4; ++i) bytes += (__int128)slot_bytes(d, i) * d->page_tokens;
+  return bytes / pages_chunk(pages_args(d, 0)) > (__int128(1) << 31);
 }
 
 size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d) {

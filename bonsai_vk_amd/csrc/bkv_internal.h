@@ -381,6 +381,10 @@ hipError_t launch_pages_fork(const PagesArgs &a, hipStream_t st);
 hipError_t launch_pages_extend(const PagesArgs &a, hipStream_t st);
 hipError_t launch_pages_compact(const PagesArgs &a, hipStream_t st);
 size_t pages_workspace(int n_layers, int pool_pages);
+constexpr int kPagePiece = 1024;       // chunks of a page that a workgroup copies at a time
+constexpr int kPagePieces = 4096;      // pieces of a page that are shared out at most
+// bytes of a chunk: 16 where every position's arrays go by them (any of head_dim 256), else 4 (rows of 64 or 128 elements have few scales)
+inline int pages_chunk(const PagesArgs &a) { return (a.slot[0] | a.slot[1] | a.slot[2] | a.slot[3]) % 16 == 0 ? 16 : 4; }
 
 #define BKV_FMT_SWITCH(KF, VF, ...)                                                    \
   do {                                                                                \

@@ -14,7 +14,6 @@ namespace bkv {
 constexpr int kForkCols = 8;           // table columns of a fork workgroup
 constexpr int kPlanThreads = 1024;
 typedef uint32_t Four __attribute__((ext_vector_type(4)));
-constexpr int kPiece = 1024;           // chunks that a workgroup copies at a time
 
 __device__ __forceinline__ int64_t table_at(const PagesArgs &a, int s, int layer, int p) {
   return ((int64_t)s * a.n_layers + layer) * a.max_pages + p;
@@ -104,7 +103,7 @@ struct PagesWs {
 size_t pages_workspace(int n_layers, int pool_pages) { return (size_t)n_layers * PagesWs::words(pool_pages) * sizeof(int32_t); }
 
 // The first `held` positions of a page's arrays from -> to, those of the four arrays one after another, in chunks T: of the pieces
-// first, first + step, .. of 1024 chunks
+// first, first + step, .. of kPagePiece chunks. (All arrays' chunks are counted in 32 bits, 2^31 at most: the calls refuse larger pages.)
 template <class T>
 __device__ __forceinline__ void copy_page(const PagesArgs &a, int layer, int from, int to, int held, int first, int step) {
   struct Array { uint64_t src, dst; uint32_t end; };   // (less the chunks of the arrays before)
@@ -114,7 +113,7 @@ __device__ __forceinline__ void copy_page(const PagesArgs &a, int layer, int fro
   };
   const Array x0 = after(0, a.base[0], a.stride[0], a.slot[0]), x1 = after(x0.end, a.base[1], a.stride[1], a.slot[1]);
   const Array x2 = after(x1.end, a.base[2], a.stride[2], a.slot[2]), x3 = after(x2.end, a.base[3], a.stride[3], a.slot[3]);
-  for (uint32_t c0 = (uint32_t)first * kPiece; c0 < x3.end; c0 += (uint32_t)step * kPiece) {
+  for (uint32_t c0 = (uint32_t)first * kPagePiece; c0 < x3.end; c0 += (uint32_t)step * kPagePiece) {
     T v[4];
     uint64_t to_at[4];
 #pragma unroll
@@ -132,12 +131,10 @@ __device__ __forceinline__ void copy_page(const PagesArgs &a, int layer, int fro
       if (to_at[j]) *reinterpret_cast<T *>(to_at[j]) = v[j];
   }
 }
-// 16 bytes at a time where every position's do so (any of head_dim 256), else 4: rows of 64 or 128 elements have few scales
-static bool by_16(const PagesArgs &a) { return (a.slot[0] | a.slot[1] | a.slot[2] | a.slot[3]) % 16 == 0; }
 static uint32_t pieces_of(const PagesArgs &a) {
   uint64_t bytes = 0;
   for (int i = 0; i < 4; ++i) bytes += a.slot[i] * a.page;
-  return (uint32_t)std::min<uint64_t>((bytes / (by_16(a) ? 16 : 4) + kPiece - 1) / kPiece, 4096);
+  return (uint32_t)std::min<uint64_t>((bytes / pages_chunk(a) + kPagePiece - 1) / kPagePiece, kPagePieces);
 }
 // `count` pages shared out to the workgroups of a layer: `step` of them to a page, the workgroup's first of which is `k`
 struct Shares {
@@ -314,7 +311,7 @@ hipError_t launch_pages_extend(const PagesArgs &a, hipStream_t st) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid(copy_grid((int64_t)a.pool_pages * pieces, a.n_layers), a.n_layers);
-  if (by_16(a)) hipLaunchKernelGGL(pages_extend_apply_kernel<Four>, grid, dim3(256), 0, st, a, (int)pieces);
+  if (pages_chunk(a) == 16) hipLaunchKernelGGL(pages_extend_apply_kernel<Four>, grid, dim3(256), 0, st, a, (int)pieces);
   else hipLaunchKernelGGL(pages_extend_apply_kernel<uint32_t>, grid, dim3(256), 0, st, a, (int)pieces);
   return hipGetLastError();
 }
@@ -398,7 +395,7 @@ hipError_t launch_pages_compact(const PagesArgs &a, hipStream_t st) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid(copy_grid((int64_t)(a.pool_pages + 1) / 2 * pieces, a.n_layers), a.n_layers);
-  if (by_16(a)) hipLaunchKernelGGL(pages_compact_apply_kernel<Four>, grid, dim3(256), 0, st, a, (int)pieces);
+  if (pages_chunk(a) == 16) hipLaunchKernelGGL(pages_compact_apply_kernel<Four>, grid, dim3(256), 0, st, a, (int)pieces);
   else hipLaunchKernelGGL(pages_compact_apply_kernel<uint32_t>, grid, dim3(256), 0, st, a, (int)pieces);
   return hipGetLastError();
 }
