@@ -1095,7 +1095,8 @@ int bkv_seqs_attn(const bkv_cache_desc *d, int layer, const bkv_seqs *seqs, cons
 static int check_pages(const bkv_cache_desc *d, int n_seq, const void *tables, const void *refs) {
   if (n_seq < 0 || n_seq > BKV_SEQS_MAX || d->page_tokens <= 0 || !tables || !refs) return BKV_EINVAL;
   if (((uintptr_t)tables | (uintptr_t)refs) & 3u) return BKV_EALIGN;
-  if ((int64_t)n_seq * d->max_pages > (1 << 30) || d->n_layers > 65535) return BKV_EUNSUPPORTED;   // (counts in 31 bits; a grid's rows)
+  // (counts in 31 bits, pages by thousands at a time; a grid's rows)
+  if ((int64_t)n_seq * d->max_pages > (1 << 30) || pool_pages(d) > (1 << 30) || d->n_layers > 65535) return BKV_EUNSUPPORTED;
   return BKV_OK;
 }
 static PagesArgs pages_args(const bkv_cache_desc *d, int n_seq) {
@@ -1123,7 +1124,7 @@ static bool page_too_large(const bkv_cache_desc *d) {
 }
 
 size_t bkv_pages_workspace_bytes(const bkv_cache_desc *d) {
-  if (check_geom(d) || d->page_tokens <= 0) return 0;
+  if (check_geom(d) || d->page_tokens <= 0 || pool_pages(d) > (1 << 30)) return 0;
   return pages_workspace(d->n_layers, pool_pages(d));
 }
 

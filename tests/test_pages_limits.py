@@ -32,3 +32,14 @@ def test_a_page_of_more_chunks_than_are_counted(hd, nkv, k_fmt, v_fmt, chunks):
 
 def test_a_page_whose_bytes_pass_64_bits():
     assert answers(1 << 30, 1 << 30, BKV_F16, BKV_F16, 1 << 30) == {EUNSUPPORTED}
+
+
+def test_a_pool_of_more_pages_than_are_counted():
+    assert answers(64, 1, BKV_Q8_0, BKV_Q4_0, 1, 1 << 30) == {EWORKSPACE}
+    for pages in ((1 << 30) + 1, 2**31 - 1):
+        assert answers(64, 1, BKV_Q8_0, BKV_Q4_0, 1, pages) == {EUNSUPPORTED}
+    d = BkvCacheDesc()
+    d.n_layers, d.nh, d.nkv, d.hd, d.cap, d.scale, d.page_tokens, d.max_pages = 1, 1, 1, 64, 2**31 - 1, 0.0625, 1, 1
+    d.k_data = d.v_data = d.block_table = PTR
+    assert lib().bkv_pages_workspace_bytes(d) == 0
+    assert lib().bkv_pages_fork(d, 1, PTR, PTR, None, PTR, None) == EUNSUPPORTED
