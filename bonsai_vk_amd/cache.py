@@ -23,13 +23,15 @@ _CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 @dataclass
 class KvGeom:
     """Per-slot geometry in u32 words (kv_guard.h:118-130). k_q8 extends the reference (which never
-    compresses K) with the same q8_0 layout V uses."""
+    compresses K) with the same q8_0 layout V uses, k_q4 and v_q4 with BKV_Q4_0's: half its data words, the same scales."""
     nkv: int = 4
     hd: int = 256
     n_attn: int = 8
     blk: int = 32
     v_q8: int = 1
     k_q8: int = 0
+    v_q4: int = 0
+    k_q4: int = 0
 
     def check(self):
         """KvGeom::check (kv_guard.h:103-113): returns '' or the reason the geometry is refused."""
@@ -47,23 +49,23 @@ class KvGeom:
     def nblk_head(self):
         return self.hd // self.blk
 
-    def words(self, q8):
+    def words(self, q8, q4=0):
         """(data words, scale words) per slot per layer of one tensor."""
-        if q8:
-            return self.nkv * self.hd // 4, self.nkv * self.nblk_head // 2
+        if q8 or q4:
+            return self.nkv * self.hd // (8 if q4 else 4), self.nkv * self.nblk_head // 2
         return self.nkv * self.hd // 2, 0
 
     @property
     def w_k(self):
-        return sum(self.words(self.k_q8))
+        return sum(self.words(self.k_q8, self.k_q4))
 
     @property
     def w_vd(self):
-        return self.words(self.v_q8)[0]
+        return self.words(self.v_q8, self.v_q4)[0]
 
     @property
     def w_vs(self):
-        return self.words(self.v_q8)[1]
+        return self.words(self.v_q8, self.v_q4)[1]
 
     @property
     def w_layer(self):
@@ -114,7 +116,7 @@ class KvCache:
         self.device = torch.device(device)
         self.scale = float(scale if scale is not None else 1.0 / (hd ** 0.5))
         geom = KvGeom(nkv=nkv, hd=hd, n_attn=n_layers, v_q8=int(v_fmt == BKV_Q8_0),
-                      k_q8=int(k_fmt == BKV_Q8_0))
+                      k_q8=int(k_fmt == BKV_Q8_0), v_q4=int(v_fmt == BKV_Q4_0), k_q4=int(k_fmt == BKV_Q4_0))
         why = geom.check()
         if why:
             raise ValueError(why)
