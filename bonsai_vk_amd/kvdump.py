@@ -11,6 +11,7 @@ values printed as %.9g of the fp32 value. kk / kvd / kvs are u32 words per slot 
 scales (KvGeom, runtime_vk/kv_guard.h:118-130); per-layer = cap * (kk + kvd + kvs).
 A q8_0 K (which the reference never stores) prints its reconstructed values on the K lines, and the
 header then carries an extra "kks" field (K scale words per slot) before "per-layer".
+A cache with 4 bits (BKV_Q4_0) has no lines in this format and is refused (KvSeqs.read and KvCache.read give its values).
 """
 import numpy as np
 
@@ -21,10 +22,17 @@ def _fmt(x):
     return "%.9g" % float(x)
 
 
+def _check_formats(k_fmt, v_fmt):
+    for name, fmt in (("K", k_fmt), ("V", v_fmt)):
+        if fmt not in (F16, Q8_0):
+            raise ValueError(f"the dump's format has fp16 and q8_0, not {name}'s format {fmt}")
+
+
 def dump_lines(arrays, layer, nfill, cap, nkv=4, hd=256, k_fmt=F16, v_fmt=Q8_0, max_pos=None,
                block_table=None, page_tokens=0):
     """Lines (without newlines) of the dump of one layer. arrays: (k_data, k_scales, v_data,
     v_scales) as uint8 arrays [n_layers][cap][row bytes] (None where absent)."""
+    _check_formats(k_fmt, v_fmt)
     kd, ks, vd, vs = [None if a is None else np.asarray(a) for a in arrays]
     npos = nfill if max_pos is None else min(nfill, max_pos)
     kk = nkv * hd // (4 if k_fmt == Q8_0 else 2)
@@ -71,6 +79,7 @@ def dump_lines(arrays, layer, nfill, cap, nkv=4, hd=256, k_fmt=F16, v_fmt=Q8_0, 
 def dump_cache(cache, layer, nfill, path=None, max_pos=None):
     """Dump a bonsai_vk_amd.KvCache (device arrays are copied to the host) or an oracle.HostCache.
     Returns the lines; writes them to `path` when given."""
+    _check_formats(cache.k_fmt, cache.v_fmt)       # (before anything is copied)
     arrs = cache.host_arrays() if hasattr(cache, "host_arrays") else cache.arrays()
     arrs = [None if a is None else (a.numpy() if hasattr(a, "numpy") else a) for a in arrs]
     bt = getattr(cache, "block_table_host", None)
