@@ -49,6 +49,7 @@ class KvSeqs:
       len     int32 [n_seq]                        positions that each has; the caller's to advance
       tables  int32 [n_seq][n_layers][max_pages]   their pages, -1 where there is none (paged only)
       refs    int32 [n_layers][pages]              how many table entries name a page (paged only)
+    Others of the same kind may be put in their places (compact's, say); captured calls go on with those that were there.
     A contiguous cache has one sequence, and no pages to give out."""
 
     def __init__(self, cache, n_seq):
@@ -59,21 +60,41 @@ class KvSeqs:
         self.cache, self.n_seq, self._dev = cache, n_seq, cache._dev
         self._per, self._starts = torch.Size((n_seq,)), torch.Size((n_seq + 1,))
         self.len = torch.zeros(n_seq, dtype=torch.int32, device=self._dev)
-        self.tables = self.refs = None
+        self._tables = self._refs = None
         self.desc = BkvCacheDesc()
         ctypes.memmove(ctypes.byref(self.desc), ctypes.byref(cache.desc), ctypes.sizeof(BkvCacheDesc))
         if cache.page_tokens:
-            self.tables = torch.full((n_seq, cache.n_layers, cache.max_pages), -1, dtype=torch.int32, device=self._dev)
-            self.refs = torch.zeros((cache.n_layers, cache.cap // cache.page_tokens), dtype=torch.int32, device=self._dev)
-            self.desc.block_table = self.tables.data_ptr()
+            self._tables = torch.full((n_seq, cache.n_layers, cache.max_pages), -1, dtype=torch.int32, device=self._dev)
+            self._refs = torch.zeros((cache.n_layers, cache.cap // cache.page_tokens), dtype=torch.int32, device=self._dev)
+            self.desc.block_table = self._tables.data_ptr()
             need = lib().bkv_pages_workspace_bytes(ctypes.byref(self.desc))
             self._pws = torch.empty(need, dtype=torch.uint8, device=self._dev)
             self._pws_bytes = need
         self._ws, self._ws_bytes, self._held = None, 0, []
 
+    # (looked at when they are set: the calls hand their addresses on as they are)
+    @property
+    def tables(self):
+        return self._tables
+
+    @tables.setter
+    def tables(self, t):
+        self._paged()
+        self._tables = self.cache._on_device(t, torch.int32, self._tables.shape)
+        self.desc.block_table = t.data_ptr()
+
+    @property
+    def refs(self):
+        return self._refs
+
+    @refs.setter
+    def refs(self, t):
+        self._paged()
+        self._refs = self.cache._on_device(t, torch.int32, self._refs.shape)
+
     # ---------------------------------------------------------------- helpers
     def _paged(self):
-        if self.tables is None:
+        if self._tables is None:
             raise ValueError("a contiguous cache has no pages")
 
     def _per_seq(self, t):
@@ -85,7 +106,7 @@ class KvSeqs:
         elif n_tok < self.n_seq:
             raise ValueError(f"a token of each of {self.n_seq} sequences is wanted without q_start, got {n_tok}")
         return BkvSeqs(self.n_seq, n_tok, 1 if q_start is None else max_q, 0, q_start, self._per_seq(self.len),
-                       None if self.tables is None else self.tables.data_ptr())
+                       None if self._tables is None else self._tables.data_ptr())
 
     def workspace(self, n_tok):
         """The workspace of attn for n_tok rows, made where the one there is smaller; a program that captures that call into a
@@ -111,7 +132,7 @@ class KvSeqs:
             with torch.cuda.device(self._dev):
                 return self.fork(parent)
         self._paged()
-        rc = lib().bkv_pages_fork(self.desc, self.n_seq, self.tables.data_ptr(), self.refs.data_ptr(), self._per_seq(self.len),
+        rc = lib().bkv_pages_fork(self.desc, self.n_seq, self._tables.data_ptr(), self._refs.data_ptr(), self._per_seq(self.len),
                                   self._per_seq(parent), self.cache._my_stream())
         if rc:
             check(rc, "bkv_pages_fork")
@@ -129,7 +150,7 @@ class KvSeqs:
             lack = torch.empty(self.cache.n_layers, dtype=torch.int32, device=self._dev)
         else:
             self.cache._on_device(lack, torch.int32, (self.cache.n_layers,))
-        rc = lib().bkv_pages_extend(self.desc, self.n_seq, self.tables.data_ptr(), self.refs.data_ptr(), self._per_seq(self.len),
+        rc = lib().bkv_pages_extend(self.desc, self.n_seq, self._tables.data_ptr(), self._refs.data_ptr(), self._per_seq(self.len),
                                     self._per_seq(n_new), lack.data_ptr(), self._pws.data_ptr(), self._pws_bytes, self.cache._my_stream())
         if rc:
             check(rc, "bkv_pages_extend")
@@ -144,9 +165,9 @@ class KvSeqs:
         self._paged()
         if (tables is None) != (refs is None):
             raise ValueError("tables and refs, or neither")
-        tables = self.tables if tables is None else self.cache._on_device(tables, torch.int32, self.tables.shape)
-        refs = self.refs if refs is None else self.cache._on_device(refs, torch.int32, self.refs.shape)
-        rc = lib().bkv_pages_compact(self.desc, self.n_seq, self.tables.data_ptr(), self.refs.data_ptr(), tables.data_ptr(),
+        tables = self._tables if tables is None else self.cache._on_device(tables, torch.int32, self._tables.shape)
+        refs = self._refs if refs is None else self.cache._on_device(refs, torch.int32, self._refs.shape)
+        rc = lib().bkv_pages_compact(self.desc, self.n_seq, self._tables.data_ptr(), self._refs.data_ptr(), tables.data_ptr(),
                                      refs.data_ptr(), self._pws.data_ptr(), self._pws_bytes, self.cache._my_stream())
         if rc:
             check(rc, "bkv_pages_compact")
