@@ -159,6 +159,7 @@ class KvCache:
         check(lib().bkv_geom_check(ctypes.byref(d)), "bkv_geom_check")
         self.max_positions = lib().bkv_max_positions(ctypes.byref(d))
         self.max_ctx = max_ctx or self.max_positions
+        self._captured = []                        # (workspaces that graphs may hold)
         ws = lib().bkv_workspace_bytes(ctypes.byref(d), BKV_OP_DECODE, self.max_ctx)
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=self.device)
         if ws == 0:                                # (a 4-bit cache: KvSeqs.attn's workspace is its own)
@@ -429,11 +430,15 @@ class KvCache:
             check(rc, "bkv_kv_commit")
 
     def prefill_workspace(self, max_ctx):
+        """The workspace of the prefill calls, made where the one there is too small for max_ctx. One that a call was captured
+        with lives as long as this cache: the graph has its address."""
         need = lib().bkv_workspace_bytes(ctypes.byref(self.desc), BKV_OP_PREFILL, max_ctx)
         if getattr(self, "_pws", None) is None or self._pws.numel() < need:
             self._pws = torch.empty(need, dtype=torch.uint8, device=self.device)
             check(lib().bkv_workspace_init(ctypes.byref(self.desc), self._pws.data_ptr(), need,
                                            self._stream()), "bkv_workspace_init")
+        if torch.cuda.is_current_stream_capturing() and not any(ws is self._pws for ws in self._captured):
+            self._captured.append(self._pws)
         return self._pws
 
     def decode_window(self, layer, kstart, nfill, q, gate=None):

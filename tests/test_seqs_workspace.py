@@ -1,12 +1,13 @@
-"""The workspace of KvSeqs.attn as calls grow: what was handed out once stays, since a captured call has its address. (No
-counterpart in the reference.)"""
+"""Workspaces as calls grow: of KvSeqs.attn all that were handed out stay, of KvCache's prefills those that a call was captured
+with, since a captured call has its workspace's address. (No counterpart in the reference.)"""
 import weakref
 
 import pytest
 import torch
 
+import bonsai_vk_amd.cache as cache_module
 import bonsai_vk_amd.seqs as module
-from bonsai_vk_amd import BKV_Q4_0, BkvError, KvCache, KvSeqs
+from bonsai_vk_amd import BKV_Q4_0, BKV_Q8_0, BkvError, KvCache, KvSeqs
 from bonsai_vk_amd._lib import lib
 
 from seqs_util import device_ints, fill, make
@@ -65,6 +66,23 @@ def test_one_that_was_not_made_ready_is_not_used(host):
         seqs.workspace(3)
     host.answer = 0
     assert seqs.workspace(3).data_ptr() == host.made[-1][0] and len(host.made) == 2
+
+
+def test_a_prefill_workspace_that_was_captured_lives_on(monkeypatch):
+    capturing = [False]
+    monkeypatch.setattr(cache_module, "lib", lambda host=Host(): host)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(KvCache, "_stream", lambda self: 0)
+    cache = KvCache(n_layers=1, nh=16, nkv=4, cap=8192, k_fmt=BKV_Q8_0, v_fmt=BKV_Q8_0, device="cpu")
+    seen, sizes = [], (600, 2000, 4000)
+    for ctx in sizes:
+        seen.append(weakref.ref(cache.prefill_workspace(ctx)))
+        capturing[0] = ctx == 2000                 # (the call of that context captured, twice)
+        for _ in range(2):
+            assert cache.prefill_workspace(ctx) is seen[-1]()
+        capturing[0] = False
+    assert seen[0]() is None and seen[1]() is not None and seen[2]() is cache.prefill_workspace(600)
+    assert len(cache._captured) == 1
 
 
 @pytest.mark.gpu
