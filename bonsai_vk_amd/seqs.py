@@ -9,7 +9,7 @@ A step of a server, everything on the device and nothing read back:
     seqs.len += n_new * have                 # no sequence gets longer,
     q_start = starts * have                  # none has rows in this call
     q = seqs.rope_append(layer, q, k, v, rope, q_start, positions, axes)
-    out, gated = seqs.attn(layer, q, q_start, gate)
+    out, gated = seqs.attn(layer, q, q_start, gate, max_q=longest)   # (tokens of the sequence that has most)
 
 Without `have`, a pool that is exhausted would leave sequences that share a page all writing their new tokens into it. Whoever
 takes the step's results reads `have` with them; a server then gives up a sequence (fork) and takes the step again.
@@ -222,8 +222,8 @@ class KvSeqs:
 
     def attn(self, layer, q, q_start=None, gate=None, out=None, out_gated=None, max_q=0):
         """bkv_seqs_attn: attention of the tokens' queries (q [n_tok][nh][hd], rotated), each over its sequence's positions up to
-        its own. q and gate may be strided rows. max_q: tokens that no sequence has more of (0: not known), by which the
-        kernels are chosen. Returns (out, out_gated); out_gated is None without a gate. Rows that are no sequence's are left
+        its own, K and V both in 4 bits. q and gate may be strided rows. max_q: tokens that no sequence has more of (0: not
+        known), by which the kernels are chosen (64 single tokens at 1000 positions: 20.9 us, 25.1 without it). Returns (out, out_gated); out_gated is None without a gate. Rows that are no sequence's are left
         as they are."""
         c = self.cache
         if c._elsewhere():

@@ -365,7 +365,8 @@ typedef struct bkv_seqs {
   int32_t n_seq;              /* 0 .. BKV_SEQS_MAX                                                       */
   int32_t n_tok;              /* rows that there are                                                     */
   int32_t max_q;              /* tokens that no sequence has more of, which bkv_seqs_attn chooses its kernels */
-                              /* by, or 0: not known (a wrong one costs time, and nothing else)          */
+                              /* by, or 0: not known (a wrong one costs time, and nothing else: 64 single */
+                              /* tokens of 16 heads at 1000 positions 20.9 us, 25.1 with 0)              */
   int32_t reserved;           /* 0                                                                       */
   const int32_t *q_start;     /* device [n_seq+1], ascending, 0 .. n_tok (where it goes back, nothing    */
                               /* is said of the outputs); NULL: one token each, s = row                  */

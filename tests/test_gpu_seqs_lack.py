@@ -110,7 +110,7 @@ def test_the_documented_step():
     before = state(seqs)
     q, k, v = rows(4, 3)
     names = dict(seqs=seqs, layer=0, q=q, k=k, v=v, rope=Rope(32), positions=torch.zeros(2, 4, dtype=torch.int32, device="cuda"),
-                 axes=RopeAxes([8, 8]), gate=q.clone(), n_new=device_ints([1, 1, 1, 1]), starts=device_ints([0, 1, 2, 3, 4]))
+                 axes=RopeAxes([8, 8]), gate=q.clone(), longest=1, n_new=device_ints([1, 1, 1, 1]), starts=device_ints([0, 1, 2, 3, 4]))
     exec(example, names)
     for a, b in zip(state(seqs), before):
         assert torch.equal(a, b)
